@@ -1,0 +1,311 @@
+"""Timed cases of the policy-score, int8-product and 8-bit-checkpoint operators.
+
+Four kinds of pass:
+
+``scores``       log probability of the given action, entropy and the ``top`` best alternatives of every row of logits
+``scores_grad``  the same with its gradient: d(sum g_lp * log_prob + g_ent * entropy) / d logits
+``int8``         one dense layer in 8-bit integers: rows of x are coded in the call, the weight was coded once
+``restore``      a tensor saved as an 8-bit checkpoint and read back
+``grads``        a tensor saved as an 8-bit checkpoint, and the weight and bias gradients formed from it
+
+``own`` selects between the plain form (elementary torch operations) and the package's kernels.
+"""
+import math
+
+import torch
+
+own = False
+
+_TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+_BYTES = {"f32": 4, "bf16": 2, "f16": 2}
+_TINY = 2.0 ** -119  # a row whose largest magnitude is below this counts as zero
+
+
+def listed():
+    return [
+        # one move of 4096 Connect-Four games: the policy head's logits, some columns full (illegal)
+        {"name": "scores-games", "kind": "scores", "T": 4096, "V": 7, "top": 3, "dtype": "f32", "masked": True},
+        # one answer at a time over a large set of alternatives: latency
+        {"name": "scores-one-row", "kind": "scores", "T": 1, "V": 131072, "top": 5, "dtype": "bf16", "masked": False},
+        # a batch of answers with a list of alternatives each
+        {"name": "scores-batch", "kind": "scores", "T": 64, "V": 131072, "top": 20, "dtype": "f16", "masked": False},
+        # a long record scored at once; odd width, so rows start at every alignment
+        {"name": "scores-record", "kind": "scores", "T": 3001, "V": 50001, "top": 8, "dtype": "f32", "masked": False},
+        # a learner batch: 256 windows of 6 steps over 7 actions
+        {"name": "grad-windows", "kind": "scores_grad", "T": 1536, "V": 7, "top": 0, "dtype": "f32", "masked": True},
+        # a training step over a large set of alternatives
+        {"name": "grad-large", "kind": "scores_grad", "T": 4096, "V": 32768, "top": 0, "dtype": "bf16", "masked": False},
+        # one latent through a layer as wide as the towers' latent (256 * 6 * 6): weight-bound
+        {"name": "int8-one-row", "kind": "int8", "T": 1, "K": 9216, "N": 9216, "dtype": "f32", "act": "relu"},
+        # 256 games through the merge layer of the towers
+        {"name": "int8-merge", "kind": "int8", "T": 256, "K": 18432, "N": 9216, "dtype": "f32", "act": "relu"},
+        # a long batch: bound by the matrix cores
+        {"name": "int8-long", "kind": "int8", "T": 8192, "K": 4096, "N": 8192, "dtype": "bf16", "act": "none"},
+        # the merge layer's input kept for the backward pass of a step of 256 windows and read back
+        {"name": "restore-merge", "kind": "restore", "T": 1536, "K": 18432, "dtype": "f32"},
+        # first layer of the Connect-Four policy head, 256 windows: latency
+        {"name": "grads-windows", "kind": "grads", "T": 256, "K": 168, "N": 256, "dtype": "f32"},
+        # a long batch: bound by the matrix cores
+        {"name": "grads-long", "kind": "grads", "T": 8192, "K": 4096, "N": 8192, "dtype": "bf16"},
+    ]
+
+
+def _log_int(rng, lo, hi):
+    return max(lo, min(hi, int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))))
+
+
+def draw(rng):
+    kind = rng.choice(["scores", "scores_grad", "int8", "int8", "restore", "grads", "grads"])
+    dtype = rng.choice(["f32", "bf16", "f16"])
+    if kind in ("scores", "scores_grad"):
+        V = _log_int(rng, 2, 131072)
+        T = _log_int(rng, 1, min(65536, 134000000 // V))
+        top = 0 if kind == "scores_grad" else min(V, rng.randint(0, 20))
+        return {"kind": kind, "T": T, "V": V, "top": top, "dtype": dtype, "masked": rng.random() < 0.3}
+    K = _log_int(rng, 16, 18432)
+    if kind == "restore":
+        return {"kind": kind, "T": _log_int(rng, 1, min(16384, 28000000 // K)), "K": K, "dtype": dtype}
+    N = _log_int(rng, 1, 16384)
+    limit = 270000000000 // (K * N)
+    T = _log_int(rng, 1, max(1, min(8192, limit)))
+    case = {"kind": kind, "T": T, "K": K, "N": N, "dtype": dtype}
+    if kind == "int8":
+        case["act"] = rng.choice(["none", "relu", "tanh", "sigmoid"])
+    return case
+
+
+def _generator(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _logits(case, gen):
+    T, V = case["T"], case["V"]
+    z = torch.randn(T, V, generator=gen, device="cuda", dtype=torch.float32)
+    z = z.mul_(torch.rand(T, 1, generator=gen, device="cuda").mul_(3.0).add_(0.5))  # flat and peaked rows
+    actions = torch.randint(0, V, (T,), generator=gen, device="cuda")
+    z = z.to(_TYPES[case["dtype"]])
+    if case["masked"]:  # illegal alternatives; the given one is legal
+        illegal = torch.rand(T, V, generator=gen, device="cuda") < 0.25
+        illegal.scatter_(1, actions[:, None], False)
+        z = z.masked_fill_(illegal, float("-inf"))
+    return z, actions
+
+
+def _score_grads(case, gen):
+    """Gradients of the two scores: advantages, and a small reward for entropy.  A loss in half precision is scaled, as
+    its gradients would be lost below the type's range otherwise."""
+    T = case["T"]
+    loss_scale = 1024.0 if case["dtype"] == "f16" else 1.0
+    g_log_prob = torch.randn(T, generator=gen, device="cuda").mul_(loss_scale / T)
+    return g_log_prob, torch.full((T,), -0.01 * loss_scale / T, device="cuda")
+
+
+def _rows(T, K, dtype, gen):
+    """Activations as a dense layer meets them: channels of unlike size, half of them cut off at zero."""
+    x = torch.randn(T, K, generator=gen, device="cuda", dtype=torch.float32)
+    x.mul_(torch.randn(K, generator=gen, device="cuda").mul_(0.7).exp_())
+    half = K // 2
+    x[:, :half].clamp_(min=0.0)
+    return x.to(_TYPES[dtype])
+
+
+def _codes(x):
+    """Row codes, in 32 bits; the quotient that every code of a row goes by is formed in 64 and rounded once."""
+    x = x.to(torch.float32)
+    top = x.abs().amax(dim=1)
+    live = top >= _TINY
+    safe = torch.where(live, top, torch.ones_like(top)).to(torch.float64)
+    inverse = torch.where(live, (127.0 / safe).to(torch.float32), torch.zeros_like(top))
+    scale = torch.where(live, (safe / 127.0).to(torch.float32), torch.zeros_like(top))
+    return torch.round(x * inverse[:, None]), scale
+
+
+def prepare(case, seed):
+    gen = _generator(seed)
+    state = {"case": dict(case)}
+    kind = case["kind"]
+    if kind in ("scores", "scores_grad"):
+        state["logits"], state["actions"] = _logits(case, gen)
+        if kind == "scores_grad":
+            state["g_log_prob"], state["g_entropy"] = _score_grads(case, gen)
+            if own:
+                state["logits"].requires_grad_(True)
+        return state
+    state["x"] = _rows(case["T"], case["K"], case["dtype"], gen)
+    dtype = _TYPES[case["dtype"]]
+    if kind == "int8":
+        w = torch.randn(case["N"], case["K"], generator=gen, device="cuda") / math.sqrt(case["K"])
+        state["bias"] = torch.randn(case["N"], generator=gen, device="cuda").mul_(0.1)
+        if own:
+            from muzero_amd.quantized import quantize_rows
+            state["weight"] = quantize_rows(w)
+        else:
+            codes, scale = _codes(w)
+            state["weight"] = (codes.to(torch.int8), scale)
+    elif kind == "grads":
+        dz = torch.randn(case["T"], case["N"], generator=gen, device="cuda").mul_(1e-3)
+        dz[torch.rand(case["T"], generator=gen, device="cuda") < 0.1] = 0.0  # windows that carry no weight
+        state["dz"] = dz.to(dtype)
+    return state
+
+
+def _activate(y, act):
+    if act == "relu":
+        return y.clamp(min=0.0)
+    if act == "tanh":
+        return torch.tanh(y)
+    if act == "sigmoid":
+        return torch.sigmoid(y)
+    return y
+
+
+def _top(z, top):
+    """The ``top`` largest of every row, the lowest index first among equals: one whole-number key holds both."""
+    V = z.shape[1]
+    bits = (z + 0.0).view(torch.int32)
+    order = torch.where(bits < 0, bits ^ 0x7FFFFFFF, bits).to(torch.int64)
+    key = order * 4294967296 + (V - 1 - torch.arange(V, device=z.device))
+    best = torch.topk(key, top, dim=1).values
+    return V - 1 - (best & 0xFFFFFFFF)
+
+
+def _plain_scores(state):
+    case = state["case"]
+    z = state["logits"].to(torch.float32)
+    a = state["actions"][:, None]
+    m = z.amax(dim=1, keepdim=True)
+    e = torch.exp(z - m)
+    total = e.sum(dim=1, keepdim=True)
+    lp = z - (m + torch.log(total))
+    p = e / total
+    plogp = torch.where(p > 0, p * lp, torch.zeros_like(p))
+    entropy = -plogp.sum(dim=1)
+    log_prob = lp.gather(1, a)[:, 0]
+    if case["kind"] == "scores":
+        if case["top"] == 0:
+            return {"log_prob": log_prob, "entropy": entropy}
+        ids = _top(z, case["top"])
+        return {"log_prob": log_prob, "entropy": entropy, "top_actions": ids, "top_log_probs": lp.gather(1, ids)}
+    g_lp, g_ent = state["g_log_prob"][:, None], state["g_entropy"][:, None]
+    grad = -g_lp * p - g_ent * (plogp + p * entropy[:, None])
+    grad.scatter_add_(1, a, g_lp)
+    return {"log_prob": log_prob, "entropy": entropy, "grad": grad.to(state["logits"].dtype)}
+
+
+def _plain(state):
+    case = state["case"]
+    kind = case["kind"]
+    if kind in ("scores", "scores_grad"):
+        return _plain_scores(state)
+    x = state["x"]
+    codes, scale = _codes(x)
+    if kind == "restore":
+        return (codes * scale[:, None]).to(x.dtype)
+    if kind == "int8":
+        w, w_scale = state["weight"]
+        total = codes @ w.to(torch.float32).t()
+        y = total * (scale[:, None] * w_scale[None, :]) + state["bias"]
+        return _activate(y, case["act"]).to(x.dtype)
+    dz = state["dz"].to(torch.float32)
+    dw = dz.t() @ (codes * scale[:, None])
+    return {"weight": dw.to(x.dtype), "bias": dz.sum(dim=0).to(x.dtype)}
+
+
+def run(state):
+    if not own:
+        return _plain(state)
+    case = state["case"]
+    kind = case["kind"]
+    if kind in ("scores", "scores_grad"):
+        from muzero_amd.policy_scores import policy_scores
+        if kind == "scores":
+            s = policy_scores(state["logits"], state["actions"], top=case["top"])
+            out = {"log_prob": s.log_prob, "entropy": s.entropy}
+            if case["top"]:
+                out.update(top_actions=s.top_actions, top_log_probs=s.top_log_probs)
+            return out
+        s = policy_scores(state["logits"], state["actions"])
+        grad, = torch.autograd.grad((s.log_prob, s.entropy), state["logits"], (state["g_log_prob"], state["g_entropy"]))
+        return {"log_prob": s.log_prob.detach(), "entropy": s.entropy.detach(), "grad": grad}
+    if kind == "int8":
+        from muzero_amd.quantized import int8_linear
+        return int8_linear(state["x"], state["weight"], state["bias"], activation=case["act"])
+    from muzero_amd.checkpoints import save_activations, weight_grad
+    saved = save_activations(state["x"])
+    if kind == "restore":
+        return saved.dequantize()
+    dw, db = weight_grad(state["dz"], saved)
+    return {"weight": dw, "bias": db}
+
+
+def work(case):
+    T, b = case["T"], _BYTES[case["dtype"]]
+    kind = case["kind"]
+    if kind == "scores":
+        V = case["V"]
+        return {"bytes": T * (V * b + 16 + 12 * case["top"]), "flops": 5 * T * V}
+    if kind == "scores_grad":
+        V = case["V"]
+        return {"bytes": T * (2 * V * b + 24), "flops": 11 * T * V}
+    K = case["K"]
+    if kind == "restore":
+        return {"bytes": 2 * T * K * b, "flops": 4 * T * K}
+    N = case["N"]
+    if kind == "int8":
+        return {"bytes": T * K * b + N * K + 8 * N + T * N * b, "flops": 2 * T * N * K}
+    return {"bytes": T * (K + N) * b + N * (K + 1) * b, "flops": 2 * T * N * K}
+
+
+def _exact_codes(x):
+    """The codes and scales are defined by their 32-bit roundings; in 64 bits each of these is one rounding of an exact
+    or doubly precise value."""
+    x = x.to(torch.float64)
+    top = x.abs().max(dim=1).values
+    inverse, scale = torch.zeros_like(top), torch.zeros_like(top)
+    live = top >= _TINY
+    inverse[live] = (127.0 / top[live]).float().double()
+    scale[live] = (top[live] / 127.0).float().double()
+    return (x * inverse[:, None]).float().double().round(), scale
+
+
+def exact(case, seed):
+    kind = case["kind"]
+    if kind in ("scores", "scores_grad"):
+        gen = _generator(seed)
+        logits, actions = _logits(case, gen)
+        g_lp, g_ent = (g.double() for g in _score_grads(case, gen))
+        rows = max(1, 60000000 // case["V"])
+        parts = []
+        for lo in range(0, case["T"], rows):
+            z = logits[lo:lo + rows].to(torch.float64)
+            a = actions[lo:lo + rows]
+            lse = torch.logsumexp(z, dim=1, keepdim=True)
+            lp = z - lse
+            p = torch.exp(lp)
+            surprise = p * lp.clamp(min=-1e300)
+            ent = -surprise.sum(dim=1)
+            part = {"log_prob": lp.gather(1, a[:, None]).squeeze(1), "entropy": ent}
+            if kind == "scores" and case["top"]:
+                ids = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :case["top"]]
+                part.update(top_actions=ids, top_log_probs=lp.gather(1, ids))
+            if kind == "scores_grad":
+                gl, ge = g_lp[lo:lo + rows, None], g_ent[lo:lo + rows, None]
+                grad = -gl * p - ge * (surprise + p * ent[:, None])
+                grad[torch.arange(a.numel(), device="cuda"), a] += gl[:, 0]
+                part["grad"] = grad
+            parts.append(part)
+        return {k: torch.cat([q[k] for q in parts]) for k in parts[0]}
+    gen = _generator(seed)
+    x = _rows(case["T"], case["K"], case["dtype"], gen)
+    q, s = _exact_codes(x)
+    if kind == "restore":
+        return q * s[:, None]
+    if kind == "int8":
+        w = torch.randn(case["N"], case["K"], generator=gen, device="cuda") / math.sqrt(case["K"])
+        bias = torch.randn(case["N"], generator=gen, device="cuda").mul_(0.1).double()
+        wq, ws = _exact_codes(w)
+        return _activate((q @ wq.t()) * s[:, None] * ws + bias, case["act"])
+    dz = torch.randn(case["T"], case["N"], generator=gen, device="cuda").mul_(1e-3)
+    dz[torch.rand(case["T"], generator=gen, device="cuda") < 0.1] = 0.0
+    dz = dz.to(_TYPES[case["dtype"]]).double()
+    return {"weight": dz.t().contiguous() @ (q * s[:, None]), "bias": dz.sum(dim=0)}
