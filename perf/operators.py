@@ -109,15 +109,20 @@ def _rows(T, K, dtype, gen):
     return x.to(_TYPES[dtype])
 
 
-def _codes(x):
-    """Row codes, in 32 bits; the quotient that every code of a row goes by is formed in 64 and rounded once."""
+def _codes(x, short_scale):
+    """Row codes, in 32 bits; the quotients that every code of a row goes by are formed in 64 and rounded once.  A
+    checkpoint's scale is rounded up to three significant bits (1, 1.25, 1.5, 1.75 times a power of two)."""
     x = x.to(torch.float32)
     top = x.abs().amax(dim=1)
     live = top >= _TINY
     safe = torch.where(live, top, torch.ones_like(top)).to(torch.float64)
-    inverse = torch.where(live, (127.0 / safe).to(torch.float32), torch.zeros_like(top))
-    scale = torch.where(live, (safe / 127.0).to(torch.float32), torch.zeros_like(top))
-    return torch.round(x * inverse[:, None]), scale
+    scale = (safe / 127.0).to(torch.float32)
+    inverse = (127.0 / safe).to(torch.float32)
+    if short_scale:
+        scale = ((scale.view(torch.int32) + 0x1FFFFF) & ~0x1FFFFF).view(torch.float32)
+        inverse = (1.0 / scale.to(torch.float64)).to(torch.float32)
+    zero = torch.zeros_like(top)
+    return torch.round(x * torch.where(live, inverse, zero)[:, None]), torch.where(live, scale, zero)
 
 
 def prepare(case, seed):
@@ -140,7 +145,7 @@ def prepare(case, seed):
             from muzero_amd.quantized import quantize_rows
             state["weight"] = quantize_rows(w)
         else:
-            codes, scale = _codes(w)
+            codes, scale = _codes(w, False)
             state["weight"] = (codes.to(torch.int8), scale)
     elif kind == "grads":
         dz = torch.randn(case["T"], case["N"], generator=gen, device="cuda").mul_(1e-3)
@@ -198,7 +203,7 @@ def _plain(state):
     if kind in ("scores", "scores_grad"):
         return _plain_scores(state)
     x = state["x"]
-    codes, scale = _codes(x)
+    codes, scale = _codes(x, kind != "int8")
     if kind == "restore":
         return (codes * scale[:, None]).to(x.dtype)
     if kind == "int8":
@@ -256,15 +261,19 @@ def work(case):
     return {"bytes": T * (K + N) * b + N * (K + 1) * b, "flops": 2 * T * N * K}
 
 
-def _exact_codes(x):
+def _exact_codes(x, short_scale):
     """The codes and scales are defined by their 32-bit roundings; in 64 bits each of these is one rounding of an exact
     or doubly precise value."""
     x = x.to(torch.float64)
     top = x.abs().max(dim=1).values
     inverse, scale = torch.zeros_like(top), torch.zeros_like(top)
     live = top >= _TINY
-    inverse[live] = (127.0 / top[live]).float().double()
     scale[live] = (top[live] / 127.0).float().double()
+    inverse[live] = (127.0 / top[live]).float().double()
+    if short_scale:
+        mantissa, exponent = torch.frexp(scale[live])
+        scale[live] = torch.ldexp(torch.ceil(mantissa * 8.0) / 8.0, exponent)
+        inverse[live] = (1.0 / scale[live]).float().double()
     return (x * inverse[:, None]).float().double().round(), scale
 
 
@@ -297,13 +306,13 @@ def exact(case, seed):
         return {k: torch.cat([q[k] for q in parts]) for k in parts[0]}
     gen = _generator(seed)
     x = _rows(case["T"], case["K"], case["dtype"], gen)
-    q, s = _exact_codes(x)
+    q, s = _exact_codes(x, kind != "int8")
     if kind == "restore":
         return q * s[:, None]
     if kind == "int8":
         w = torch.randn(case["N"], case["K"], generator=gen, device="cuda") / math.sqrt(case["K"])
         bias = torch.randn(case["N"], generator=gen, device="cuda").mul_(0.1).double()
-        wq, ws = _exact_codes(w)
+        wq, ws = _exact_codes(w, False)
         return _activate((q @ wq.t()) * s[:, None] * ws + bias, case["act"])
     dz = torch.randn(case["T"], case["N"], generator=gen, device="cuda").mul_(1e-3)
     dz[torch.rand(case["T"], generator=gen, device="cuda") < 0.1] = 0.0
