@@ -764,6 +764,78 @@ int mz_action_table(const float *embedding, const float *merge_weight, const flo
 int mz_policy_post(const float *policy_in, int32_t B, int32_t A, int32_t softmax_times,
                    float *policy_out, int32_t *argmax, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Scores of the policy head, dense layers in 8-bit integers, 8-bit activation checkpoints.
+ * Element types of the matrices that come in or go out:
+ * ------------------------------------------------------------------------------------ */
+#define MZ_TYPE_F32 0
+#define MZ_TYPE_BF16 1
+#define MZ_TYPE_F16 2
+
+/* Log probability of a given action, entropy and the best alternatives of T rows of V logits (the input of
+ * policy_mlp's softmax, src/neural_networks/neural_network.py:227-262; row stride ld elements):
+ *   log_prob f32[T]   log softmax(row)[action]; actions i64[T] or NULL.  A negative action scores 0 (no action), one of
+ *                     V or more NaN;
+ *   entropy f32[T]    -sum p log p;
+ *   stats f32[T][2]   row maximum and log of the sum of exponentials relative to it (what the backward call needs);
+ *   top_actions i64[T][top], top_log_probs f32[T][top]   the `top` (0..32, at most V) largest logits, the lowest index
+ *                     first among equals, NaN before everything; their log probabilities.
+ * A logit of -inf is an illegal action (probability 0).  A row of nothing else has log probabilities -inf, entropy 0
+ * and gradient 0.  A NaN or +inf makes its row's results NaN.  workspace: mz_policy_scores_workspace bytes
+ * (may be 0), 16-byte aligned. */
+int64_t mz_policy_scores_workspace(int32_t type, int64_t T, int32_t V, int32_t top);
+int mz_policy_scores(const void *logits, int32_t type, int64_t ld, const int64_t *actions, int64_t T, int32_t V,
+                     int32_t top, float *log_prob, float *entropy, float *stats, int64_t *top_actions,
+                     float *top_log_probs, void *workspace, int64_t workspace_bytes, void *stream);
+/* grad[T][V] (type and shape of the logits, row stride ld_grad; it must not overlap them) =
+ * d(sum g_log_prob log_prob + g_entropy entropy + g_top top_log_probs) / d logits; each g f32 and may be NULL. */
+int mz_policy_scores_backward(const void *logits, int32_t type, int64_t ld, const int64_t *actions, int64_t T,
+                              int32_t V, int32_t top, const float *stats, const float *entropy,
+                              const int64_t *top_actions, const float *g_log_prob, const float *g_entropy,
+                              const float *g_top, void *grad, int64_t ld_grad, void *stream);
+
+/* Row codes: q i8[rows][ldc] and scales f32[rows] with x_rk about scales[r] * q_rk, q in -127..127 (round half to even).
+ * scale_bits 24: scale = fl(max |row| / 127), q = rne(x * fl(127 / max)); scale_bits 3: that scale rounded up to three
+ * significant bits, q = rne(x * fl(1 / scale)) (what mz_ckpt8_weight_grad multiplies exactly with bfloat16 gradients).
+ * A row whose largest magnitude is below 2^-119 gets zeros and scale 0, a row with an infinity or a NaN zeros and
+ * scale NaN.  ldc: a multiple of 16, at least K; columns K..ldc-1 are set to zero. */
+int mz_quant8_rows(const void *x, int32_t type, int64_t ldx, int64_t rows, int32_t K, int32_t scale_bits,
+                   int8_t *codes, int64_t ldc, float *scales, void *stream);
+/* x = scales * q, rounded once to the type. */
+int mz_dequant8_rows(const int8_t *codes, int64_t ldc, const float *scales, int64_t rows, int32_t K, void *x,
+                     int32_t type, int64_t ldx, void *stream);
+
+/* y = act(x W^T + bias) in 8-bit integers: rows of x (type x_type, row stride ldx) are coded in the call, W is
+ * w_codes i8[N][ldw] / w_scales f32[N] of mz_quant8_rows(..., 24, ...); sums are exact 32-bit integers (K <= 131072),
+ * bias f32[N] or NULL, activation none / relu / tanh / sigmoid, y of any type.  ldw: a multiple of 128 (the columns
+ * behind K zero).  The int8 form of nn.Linear + activation (build_mlp, src/neural_networks/network_builder.py:183-205).
+ * mz_int8_forward_codes takes rows that are coded already (heads that share an input).
+ * workspace: mz_int8_workspace / mz_int8_codes_workspace bytes (may be 0 for the latter), 16-byte aligned. */
+int64_t mz_int8_workspace(int32_t rows, int32_t K, int32_t N);
+int64_t mz_int8_codes_workspace(int32_t rows, int32_t K, int32_t N);
+int mz_int8_forward(const void *x, int32_t x_type, int64_t ldx, int32_t rows, int32_t K, const int8_t *w_codes,
+                    int64_t ldw, const float *w_scales, int32_t N, const float *bias, int32_t activation, void *y,
+                    int32_t type, int64_t ldy, void *workspace, int64_t workspace_bytes, void *stream);
+int mz_int8_forward_codes(const int8_t *x_codes, int64_t ldxc, const float *x_scales, int32_t rows, int32_t K,
+                          const int8_t *w_codes, int64_t ldw, const float *w_scales, int32_t N, const float *bias,
+                          int32_t activation, void *y, int32_t type, int64_t ldy, void *workspace,
+                          int64_t workspace_bytes, void *stream);
+
+/* 8-bit activation checkpoints.  A dense layer's input is kept as row codes (mz_quant8_rows with scale_bits 3); what its
+ * activation's derivative needs is kept as one bit per value (relu) or a code of 8 bits (tanh, sigmoid):
+ * mz_ckpt8_act_bytes(N, activation) bytes per row.  dz may be dy itself (same stride).
+ * mz_ckpt8_weight_grad: dw[N][K] = dz^T x and db[N] = column sums of dz (db may be NULL) from dz[rows][N] and the codes
+ * of x[rows][K]; dz, dw and db share the type, sums are held in float32 with dz to 22 bits or exact. */
+int64_t mz_ckpt8_act_bytes(int32_t N, int32_t activation);
+int mz_ckpt8_act_save(const void *y, int32_t type, int64_t ldy, int64_t rows, int32_t N, int32_t activation,
+                      uint8_t *saved, void *stream);
+int mz_ckpt8_act_grad(const void *dy, int32_t type, int64_t ldy, const uint8_t *saved, int64_t rows, int32_t N,
+                      int32_t activation, void *dz, int64_t ldz, void *stream);
+int64_t mz_ckpt8_workspace(int32_t type, int32_t scale_bits, int32_t rows, int32_t N, int32_t K);
+int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows, int32_t N, const int8_t *codes,
+                         int64_t ldc, const float *scales, int32_t scale_bits, int32_t K, void *dw, int64_t ldw,
+                         void *db, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

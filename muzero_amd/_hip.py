@@ -74,6 +74,7 @@ class SearchParams(C.Structure):
                 ("stamps", C.c_void_p), ("z_pool", C.c_void_p)]
 
 
+TYPE_F32, TYPE_BF16, TYPE_F16 = 0, 1, 2
 MAX_BLOCKS = 4
 
 
@@ -195,6 +196,25 @@ _SIGS = {
                                    _P, C.c_int64, C.c_int32, C.c_int32, _P]),
     "mz_action_table": (C.c_int, [_P, _P, _P, C.c_int32, C.c_int32, _P, _P]),
     "mz_policy_post": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P]),
+    "mz_policy_scores_workspace": (C.c_int64, [C.c_int32, C.c_int64, C.c_int32, C.c_int32]),
+    "mz_policy_scores": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P, C.c_int64,
+                                   _P]),
+    "mz_policy_scores_backward": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P,
+                                            _P, C.c_int64, _P]),
+    "mz_quant8_rows": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P]),
+    "mz_dequant8_rows": (C.c_int, [_P, C.c_int64, _P, C.c_int64, C.c_int32, _P, C.c_int32, C.c_int64, _P]),
+    "mz_int8_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
+    "mz_int8_codes_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),
+    "mz_int8_forward": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, _P, C.c_int32, _P, C.c_int32, _P,
+                                  C.c_int32, C.c_int64, _P, C.c_int64, _P]),
+    "mz_int8_forward_codes": (C.c_int, [_P, C.c_int64, _P, C.c_int32, C.c_int32, _P, C.c_int64, _P, C.c_int32, _P, C.c_int32, _P,
+                                        C.c_int32, C.c_int64, _P, C.c_int64, _P]),
+    "mz_ckpt8_act_bytes": (C.c_int64, [C.c_int32, C.c_int32]),
+    "mz_ckpt8_act_save": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, _P]),
+    "mz_ckpt8_act_grad": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, _P]),
+    "mz_ckpt8_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32]),
+    "mz_ckpt8_weight_grad": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, _P, C.c_int32, C.c_int32, _P,
+                                       C.c_int64, _P, _P, C.c_int64, _P]),
 }
 
 

@@ -1,0 +1,54 @@
+"""What the row operators (policy scores, 8-bit codes, products and checkpoints) share on the host side: element
+types, two-dimensional views of their arguments, the stream and device a call belongs to."""
+from __future__ import annotations
+
+import contextlib
+
+import torch
+
+from muzero_amd import _hip
+
+TYPE = {torch.float32: _hip.TYPE_F32, torch.bfloat16: _hip.TYPE_BF16, torch.float16: _hip.TYPE_F16}
+_NULL = contextlib.nullcontext()
+
+
+def check_tensor(t: torch.Tensor, what: str) -> None:
+    """A float32 / bfloat16 / float16 tensor on the GPU, or a TypeError / HipError that says which."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{what} must be a tensor, not {type(t).__name__}")
+    if t.dtype not in TYPE:
+        raise TypeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+    if not t.is_cuda:
+        raise _hip.HipError(f"{what} must be on the GPU (there is no CPU fallback for the kernels)")
+
+
+def rows_of(t: torch.Tensor) -> torch.Tensor:
+    """t as [rows, columns] with adjacent columns and rows that do not overlap: a view where its strides allow one, else
+    a copy."""
+    cols = t.shape[-1]
+    if t.dim() != 2:
+        t = t.reshape(-1, cols) if cols else t.reshape(t.shape[:-1].numel(), 0)
+    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+        t = t.contiguous()
+    return t
+
+
+def row_stride(t: torch.Tensor) -> int:
+    """Elements from one row of rows_of's result to the next (a single row may carry any stride)."""
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def on_device(t: torch.Tensor):
+    """Context in which t's device is the current one."""
+    return _NULL if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def stream_of(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def workspace(nbytes: int, t: torch.Tensor) -> torch.Tensor | None:
+    """Scratch memory of one call, from torch's allocator: it belongs to the stream the call runs on."""
+    if nbytes < 0:
+        raise _hip.HipError("bad workspace size")
+    return torch.empty(nbytes, dtype=torch.uint8, device=t.device) if nbytes > 0 else None

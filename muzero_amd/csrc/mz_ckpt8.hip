@@ -1,0 +1,218 @@
+// Weight gradients from 8-bit activation checkpoints (gfx950): a dense layer z = x W^T + b keeps its input as row codes
+// (mz_quant8_rows: x_rk about s_r q_rk), and its backward pass forms
+//     dW_nk = sum_r dz_rn s_r q_rk,     db_n = sum_r dz_rn
+// without writing x out again.
+//
+// The product runs on the fp16 matrix instruction.  Codes are whole numbers up to 127: exact in fp16.  The row scale lies
+// along the reduction, so it goes to the other side: v_rn = dz_rn s_r, which fp16 cannot hold as it is.  Each output row n
+// is first brought into range by a power of two c_n (the largest |v_rn c_n| lies in 2^14 .. 2^15) and then held as
+//     one plane   hi = fp16(v c)                       bfloat16 dz with scales of 3 significant bits: 8 + 3 = 11 bits,
+//                                                      which is what fp16 has -- exact
+//     two planes  hi = fp16(v c), lo = fp16(v c - hi)  everything else: 22 bits
+// (values below 2^-16 of their row's largest lose bits of the second plane, values below 2^-28 of the first one: an
+// absolute error of at most 2^-25 c_n^-1 then, 2^-39 of the largest).  The two planes' products go to one float32
+// accumulator, and 1 / c_n is applied at the end, exact.
+//   k_col_stats   per column of dz: largest |v| and sum of dz, for chunks of rows
+//   k_split       dz -> planes, transposed to [n][plane][r]; db and 1 / c_n from the chunks
+//   k_codes_t     codes -> fp16, transposed to [k][r]
+//   k_weight_grad the product
+#include "mz_tile.h"
+
+namespace {
+
+using namespace mze;
+using namespace mzt8;
+
+constexpr int kCT = 256;
+constexpr int kMaxChunks = 64;
+
+int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+template <class T>
+__global__ void __launch_bounds__(kCT)
+k_col_stats(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int chunk_rows,
+            unsigned *__restrict__ part_max, float *__restrict__ part_sum) {
+    const int n = blockIdx.x * kCT + threadIdx.x, chunk = blockIdx.y;
+    if (n >= N) return;
+    unsigned m = 0;
+    float s = 0.0f;
+    for (int r = chunk * chunk_rows; r < min(R, (chunk + 1) * chunk_rows); ++r) {
+        const float g = (float)dz[r * ldz + n];
+        m = max(m, __float_as_uint(g * scales[r]) & 0x7FFFFFFFu);
+        s += g;
+    }
+    part_max[(int64_t)chunk * N + n] = m;
+    part_sum[(int64_t)chunk * N + n] = s;
+}
+
+// The power of two that brings a column with largest magnitude `bits` to 2^14 .. 2^15, and its inverse; NaN for a column
+// with an infinity or a NaN.
+__device__ __forceinline__ float column_factor(unsigned bits, float *inverse) {
+    if (bits >= 0x7F800000u) {
+        *inverse = __uint_as_float(0x7FC00000u);
+        return *inverse;
+    }
+    int e = 14 - (max((int)(bits >> 23), 1) - 127);  // ilogb of the largest (subnormal ones count as 2^-126)
+    e = min(max(e, -126), 126);
+    *inverse = __uint_as_float((unsigned)(127 - e) << 23);
+    return __uint_as_float((unsigned)(127 + e) << 23);
+}
+
+// 64 x 64 values per workgroup, transposed through LDS; rows behind the last one become zeros.
+template <class T, int PLANES>
+__global__ void __launch_bounds__(kCT)
+k_split(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int64_t Rp, int chunks,
+        const unsigned *__restrict__ part_max, const float *__restrict__ part_sum, f16 *__restrict__ planes,
+        float *__restrict__ inverse, T *__restrict__ db) {
+    __shared__ float tile[64][65];
+    __shared__ float factor[64];
+    const int n0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
+    if (threadIdx.x < 64) {
+        const int n = n0 + threadIdx.x;
+        unsigned m = 0;
+        float s = 0.0f;
+        if (n < N)
+            for (int c = 0; c < chunks; ++c) {
+                m = max(m, part_max[(int64_t)c * N + n]);
+                s += part_sum[(int64_t)c * N + n];
+            }
+        float inv;
+        factor[threadIdx.x] = column_factor(m, &inv);
+        if (n < N && blockIdx.y == 0) {
+            inverse[n] = inv;
+            if (db) db[n] = (T)s;
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 64; i += kCT) {
+        const int r = i >> 6, n = i & 63;
+        float v = 0.0f;
+        if (r0 + r < R && n0 + n < N) v = ((float)dz[(r0 + r) * ldz + n0 + n] * scales[r0 + r]) * factor[n];
+        tile[r][n] = v;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 64; i += kCT) {
+        const int n = i >> 6, r = i & 63;
+        if (n0 + n >= N) continue;
+        const float v = tile[r][n];
+        const f16 hi = (f16)v;
+        f16 *row = planes + (int64_t)(n0 + n) * PLANES * Rp;
+        row[r0 + r] = hi;
+        if (PLANES == 2) row[Rp + r0 + r] = (f16)(v - (float)hi);
+    }
+}
+
+__global__ void __launch_bounds__(kCT)
+k_codes_t(const int8_t *__restrict__ codes, int64_t ldc, int R, int K, int64_t Rp, f16 *__restrict__ out) {
+    __shared__ int8_t tile[64][68];
+    const int k0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
+    for (int i = threadIdx.x; i < 64 * 64; i += kCT) {
+        const int r = i >> 6, k = i & 63;
+        tile[r][k] = r0 + r < R && k0 + k < K ? codes[(r0 + r) * ldc + k0 + k] : (int8_t)0;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * 64; i += kCT) {
+        const int k = i >> 6, r = i & 63;
+        if (k0 + k < K) out[(k0 + k) * Rp + r0 + r] = (f16)(float)tile[r][k];
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads)
+k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, const float *__restrict__ inverse, int K, int N,
+              int64_t Rp, int n_planes, T *__restrict__ dw, int64_t ldw) {
+    __shared__ __align__(16) uint8_t lds[2 * kTile * kStep];
+    const int tiles_k = (K + kTile - 1) / kTile;
+    const int k0 = (blockIdx.x % tiles_k) * kTile, n0 = (blockIdx.x / tiles_k) * kTile;
+    const Operand inner{(const uint8_t *)codes_t, 2 * Rp, K, (int)(2 * Rp)};
+    const Operand outer{(const uint8_t *)planes, 2 * Rp * n_planes, N, (int)(2 * Rp * n_planes)};
+    f32x4 acc[4][4];
+    tile_product<OpF16>(inner, k0, outer, n0, (int)(2 * Rp * n_planes), lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave & 1) * 64, wo = (wave >> 1) * 64;
+    for (int b = 0; b < 4; ++b) {
+        const int n = n0 + wo + 16 * b + (lane & 15);
+        if (n >= N) continue;
+        const float inv = inverse[n];
+        for (int a = 0; a < 4; ++a)
+            for (int e = 0; e < 4; ++e) {
+                const int k = k0 + wi + 16 * a + 4 * (lane >> 4) + e;
+                if (k < K) dw[n * ldw + k] = (T)(acc[a][b][e] * inv);
+            }
+    }
+}
+
+struct Layout {
+    int planes, chunks, chunk_rows;
+    int64_t Rp, off_sum, off_inverse, off_planes, off_codes, bytes;
+};
+
+Layout layout(int32_t type, int32_t scale_bits, int64_t R, int64_t N, int64_t K) {
+    Layout l;
+    l.planes = type == MZ_TYPE_BF16 && scale_bits == 3 ? 1 : 2;
+    l.Rp = round_up(R, 64);
+    l.chunks = (int)(R < 32 * kMaxChunks ? (R + 31) / 32 : kMaxChunks);
+    l.chunk_rows = (int)((R + l.chunks - 1) / l.chunks);
+    const int64_t stat = round_up((int64_t)l.chunks * N * 4, 128);
+    l.off_sum = stat;
+    l.off_inverse = 2 * stat;
+    l.off_planes = l.off_inverse + round_up(N * 4, 128);
+    l.off_codes = l.off_planes + N * l.planes * l.Rp * 2;
+    l.bytes = l.off_codes + K * l.Rp * 2;
+    return l;
+}
+
+constexpr int64_t kMaxRows = 1 << 28;  // two planes of fp16 in 31 bits of bytes
+
+}  // namespace
+
+extern "C" {
+
+int64_t mz_ckpt8_workspace(int32_t type, int32_t scale_bits, int32_t rows, int32_t N, int32_t K) {
+    if (rows <= 0 || N <= 0 || K <= 0 || rows > kMaxRows) return 0;
+    return layout(type, scale_bits, rows, N, K).bytes;
+}
+
+int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows, int32_t N, const int8_t *codes, int64_t ldc,
+                         const float *scales, int32_t scale_bits, int32_t K, void *dw, int64_t ldw, void *db, void *workspace,
+                         int64_t workspace_bytes, void *stream) {
+    if (rows <= 0 || N <= 0 || K <= 0 || rows > kMaxRows)
+        return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: bad dimensions rows=%d N=%d K=%d", rows, N, K);
+    if (!type_ok(type)) return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: unknown element type %d", type);
+    if (scale_bits != 24 && scale_bits != 3)
+        return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: scale_bits must be 24 or 3, not %d", scale_bits);
+    if (!dz || !codes || !scales || !dw) return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: NULL argument");
+    if (ldz < N || ldw < K || ldc < K || ldc % 16 != 0 || ((uintptr_t)codes & 15) != 0 ||
+        (((uintptr_t)dz | (uintptr_t)dw | (uintptr_t)db) & (type_bytes(type) - 1)) != 0)
+        return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: bad stride or alignment (ldz=%lld ldw=%lld ldc=%lld)", (long long)ldz,
+                        (long long)ldw, (long long)ldc);
+    const Layout l = layout(type, scale_bits, rows, N, K);
+    if (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 15) != 0)
+        return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: needs a 16-byte aligned workspace of %lld bytes (got %lld)",
+                        (long long)l.bytes, (long long)workspace_bytes);
+    const int64_t tiles = (round_up(N, kTile) / kTile) * (round_up(K, kTile) / kTile);
+    if (tiles > (1 << 23) || l.Rp / 64 > 65535)
+        return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: rows=%d N=%d K=%d is too large for one call", rows, N, K);
+    uint8_t *ws = (uint8_t *)workspace;
+    unsigned *part_max = (unsigned *)ws;
+    float *part_sum = (float *)(ws + l.off_sum), *inverse = (float *)(ws + l.off_inverse);
+    f16 *planes = (f16 *)(ws + l.off_planes), *codes_t = (f16 *)(ws + l.off_codes);
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 split_grid((unsigned)((N + 63) / 64), (unsigned)(l.Rp / 64)), codes_grid((unsigned)((K + 63) / 64), (unsigned)(l.Rp / 64));
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL(k_col_stats<T>, dim3((unsigned)((N + kCT - 1) / kCT), (unsigned)l.chunks), dim3(kCT), 0, st, (const T *)dz,
+                           ldz, scales, rows, N, l.chunk_rows, part_max, part_sum);
+        if (l.planes == 1)
+            hipLaunchKernelGGL((k_split<T, 1>), split_grid, dim3(kCT), 0, st, (const T *)dz, ldz, scales, rows, N, l.Rp, l.chunks,
+                               part_max, part_sum, planes, inverse, (T *)db);
+        else
+            hipLaunchKernelGGL((k_split<T, 2>), split_grid, dim3(kCT), 0, st, (const T *)dz, ldz, scales, rows, N, l.Rp, l.chunks,
+                               part_max, part_sum, planes, inverse, (T *)db);
+        hipLaunchKernelGGL(k_codes_t, codes_grid, dim3(kCT), 0, st, codes, ldc, rows, K, l.Rp, codes_t);
+        hipLaunchKernelGGL(k_weight_grad<T>, dim3((unsigned)tiles), dim3(kThreads), 0, st, codes_t, planes, inverse, K, N, l.Rp,
+                           l.planes, (T *)dw, ldw);
+    });
+    return mz::check_launch("mz_ckpt8_weight_grad");
+}
+
+}  // extern "C"

@@ -1,0 +1,129 @@
+// Dense layers in 8-bit integers (gfx950): y = act(x W^T + b) with a scale for each row of x and each row of W
+// (mz_quant8_rows with full scales),
+//     y_rn = act(fl(sum_k q_rk w_nk) (s_r t_n) + b_n),
+// the sum in 32-bit integers, which K <= 131072 keeps exact.
+#include <cmath>
+
+#include "mz_tile.h"
+
+namespace {
+
+using namespace mze;
+using namespace mzt8;
+
+constexpr int kMaxK = 131072;
+
+__device__ __forceinline__ float activate(float v, int act) {
+    switch (act) {
+        case MZ_ACT_RELU: return v > 0.0f || v != v ? v : 0.0f;
+        case MZ_ACT_TANH: return tanhf(v);
+        case MZ_ACT_SIGMOID: return 1.0f / (1.0f + expf(-v));
+        default: return v;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kThreads)
+k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs, int rows, const int8_t *__restrict__ wc,
+       int64_t ldw, const float *__restrict__ ws, int N, int kbytes, const float *__restrict__ bias, int act, T *__restrict__ y,
+       int64_t ldy) {
+    __shared__ __align__(16) uint8_t lds[2 * kTile * kStep];
+    const int tiles_n = (N + kTile - 1) / kTile;
+    const int n0 = (blockIdx.x % tiles_n) * kTile, r0 = (blockIdx.x / tiles_n) * kTile;
+    const Operand inner{(const uint8_t *)wc, ldw, N, kbytes}, outer{(const uint8_t *)xc, ldxc, rows, kbytes};
+    i32x4 acc[4][4];
+    tile_product<OpI8>(inner, n0, outer, r0, kbytes, lds, acc);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave & 1) * 64, wo = (wave >> 1) * 64;
+    for (int b = 0; b < 4; ++b) {
+        const int r = r0 + wo + 16 * b + (lane & 15);
+        if (r >= rows) continue;
+        const float s = xs[r];
+        for (int a = 0; a < 4; ++a)
+            for (int e = 0; e < 4; ++e) {
+                const int n = n0 + wi + 16 * a + 4 * (lane >> 4) + e;
+                if (n < N) y[r * ldy + n] = (T)activate((float)acc[a][b][e] * (s * ws[n]) + (bias ? bias[n] : 0.0f), act);
+            }
+    }
+}
+
+int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+int check_code_rows(const char *what, const int8_t *codes, int64_t ldc, const float *scales, int32_t K) {
+    if (!codes || !scales) return mz::fail(MZ_ERR_ARG, "%s: NULL argument", what);
+    if (ldc < K || ldc % 128 != 0 || ((uintptr_t)codes & 15) != 0)
+        return mz::fail(MZ_ERR_ARG, "%s: codes need 16-byte aligned rows of a multiple of 128 bytes, zero behind K=%d (row stride %lld)",
+                        what, K, (long long)ldc);
+    return MZ_OK;
+}
+
+int check_int8(int32_t rows, int32_t K, const int8_t *w_codes, int64_t ldw, const float *w_scales, int32_t N, int32_t activation,
+               const void *y, int32_t type, int64_t ldy) {
+    if (rows < 0 || K <= 0 || N <= 0) return mz::fail(MZ_ERR_ARG, "mz_int8_forward: bad dimensions rows=%d K=%d N=%d", rows, K, N);
+    if (K > kMaxK) return mz::fail(MZ_ERR_ARG, "mz_int8_forward: K=%d above %d would overflow the 32-bit sums", K, kMaxK);
+    if (!type_ok(type)) return mz::fail(MZ_ERR_ARG, "mz_int8_forward: unknown element type %d", type);
+    if (activation < MZ_ACT_NONE || activation > MZ_ACT_SIGMOID)
+        return mz::fail(MZ_ERR_ARG, "mz_int8_forward: activation %d is not element-wise", activation);
+    MZ_TRY(check_code_rows("mz_int8_forward", w_codes, ldw, w_scales, K));
+    if (rows > 0 && !y) return mz::fail(MZ_ERR_ARG, "mz_int8_forward: NULL argument");
+    if (ldy < N || ((uintptr_t)y & (type_bytes(type) - 1)) != 0)
+        return mz::fail(MZ_ERR_ARG, "mz_int8_forward: bad output stride %lld or alignment for N=%d", (long long)ldy, N);
+    if ((round_up(N, kTile) / kTile) * (round_up(rows, kTile) / kTile) > (1 << 23))
+        return mz::fail(MZ_ERR_ARG, "mz_int8_forward: output of %d x %d is too large for one call", rows, N);
+    return MZ_OK;
+}
+
+int launch_codes(const int8_t *x_codes, int64_t ldxc, const float *x_scales, int32_t rows, int32_t K, const int8_t *w_codes,
+                 int64_t ldw, const float *w_scales, int32_t N, const float *bias, int32_t activation, void *y, int32_t type,
+                 int64_t ldy, hipStream_t stream) {
+    const int64_t tiles = (round_up(N, kTile) / kTile) * (round_up(rows, kTile) / kTile);
+    with_type(type, [&](auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL(k_int8<T>, dim3((unsigned)tiles), dim3(kThreads), 0, stream, x_codes, ldxc, x_scales, rows, w_codes, ldw,
+                           w_scales, N, (int)round_up(K, 128), bias, activation, (T *)y, ldy);
+    });
+    return mz::check_launch("k_int8");
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t mz_int8_codes_workspace(int32_t rows, int32_t K, int32_t N) {
+    (void)rows, (void)K, (void)N;
+    return 0;
+}
+
+int mz_int8_forward_codes(const int8_t *x_codes, int64_t ldxc, const float *x_scales, int32_t rows, int32_t K,
+                          const int8_t *w_codes, int64_t ldw, const float *w_scales, int32_t N, const float *bias,
+                          int32_t activation, void *y, int32_t type, int64_t ldy, void *workspace, int64_t workspace_bytes,
+                          void *stream) {
+    MZ_TRY(check_int8(rows, K, w_codes, ldw, w_scales, N, activation, y, type, ldy));
+    if (rows == 0) return MZ_OK;
+    MZ_TRY(check_code_rows("mz_int8_forward", x_codes, ldxc, x_scales, K));
+    (void)workspace, (void)workspace_bytes;
+    return launch_codes(x_codes, ldxc, x_scales, rows, K, w_codes, ldw, w_scales, N, bias, activation, y, type, ldy,
+                        (hipStream_t)stream);
+}
+
+int64_t mz_int8_workspace(int32_t rows, int32_t K, int32_t N) {
+    if (rows <= 0 || K <= 0 || N <= 0) return 0;
+    return round_up((int64_t)rows * 4, 128) + (int64_t)rows * round_up(K, 128);
+}
+
+int mz_int8_forward(const void *x, int32_t x_type, int64_t ldx, int32_t rows, int32_t K, const int8_t *w_codes, int64_t ldw,
+                    const float *w_scales, int32_t N, const float *bias, int32_t activation, void *y, int32_t type, int64_t ldy,
+                    void *workspace, int64_t workspace_bytes, void *stream) {
+    MZ_TRY(check_int8(rows, K, w_codes, ldw, w_scales, N, activation, y, type, ldy));
+    const int64_t need = mz_int8_workspace(rows, K, N);
+    if (rows > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
+        return mz::fail(MZ_ERR_ARG, "mz_int8_forward: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
+                        (long long)workspace_bytes);
+    float *scales = (float *)workspace;
+    int8_t *codes = (int8_t *)workspace + round_up((int64_t)rows * 4, 128);
+    const int64_t ldc = round_up(K, 128);
+    MZ_TRY(mz_quant8_rows(x, x_type, ldx, rows, K, 24, codes, ldc, scales, stream));
+    if (rows == 0) return MZ_OK;
+    return launch_codes(codes, ldc, scales, rows, K, w_codes, ldw, w_scales, N, bias, activation, y, type, ldy, (hipStream_t)stream);
+}
+
+}  // extern "C"

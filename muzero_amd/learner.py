@@ -14,13 +14,16 @@ cross entropy with the already-softmaxed policy used as logits.
 """
 from __future__ import annotations
 
+import contextlib
 from dataclasses import dataclass
 
 import numpy as np
 import torch
 import torch.nn.functional as F
 
+from muzero_amd.checkpoints import eight_bit_checkpoints
 from muzero_amd.neural_networks.per_call import per_call_statistics
+from muzero_amd.policy_scores import PolicyScores, score_actions
 from muzero_amd.ring_buffer import Frame, FrameRingBuffer, make_history_tensor
 
 
@@ -67,15 +70,18 @@ def windows_to_batch(windows, z_targets: np.ndarray, rewards: np.ndarray, is_wei
                        torch.as_tensor(np.asarray(is_weights, dtype=np.float64), dtype=torch.float32))
 
 
-def batched_unroll_loss(repr_net, dyn_net, pred_net, batch: WindowBatch, roll_ahead: int, coeff=(1.0, 1.0, 1.0), latent=None):
+def batched_unroll_loss(repr_net, dyn_net, pred_net, batch: WindowBatch, roll_ahead: int, coeff=(1.0, 1.0, 1.0), latent=None,
+                        checkpoints8: bool = False):
     """Returns (weighted_sum, per_window_loss[B], (policy_sum, value_sum, reward_sum)).
 
     weighted_sum = sum_b is_weights[b] * loss_b, NOT yet divided by sum(is_weights): the caller
     normalises (a data-parallel caller after summing over ranks).  Networks with BatchNorm layers
     are evaluated with per-window statistics: the reference unrolls one window per call.
-    `latent`: the root latents when the caller has evaluated repr_net itself (it is not called then)."""
+    `latent`: the root latents when the caller has evaluated repr_net itself (it is not called then).
+    `checkpoints8`: the dense layers keep what their backward pass needs in 8 bits (muzero_amd.checkpoints)."""
     cp, cv, cr = coeff
-    with per_call_statistics(repr_net), per_call_statistics(dyn_net), per_call_statistics(pred_net):
+    kept = eight_bit_checkpoints(repr_net, dyn_net, pred_net) if checkpoints8 else contextlib.nullcontext()
+    with per_call_statistics(repr_net), per_call_statistics(dyn_net), per_call_statistics(pred_net), kept:
         return _unroll(repr_net, dyn_net, pred_net, batch, roll_ahead, cp, cv, cr, latent)
 
 
@@ -173,7 +179,10 @@ class DataParallelLearner:
     in one flat buffer (a single collective of n_params + 1 floats, ~1 MB for c4_mlp: one
     message per step suits point-to-point xGMI links better than per-tensor calls)."""
 
-    def __init__(self, repr_net, dyn_net, pred_net, optimizer, roll_ahead: int, coeff=(1.0, 1.0, 1.0), dist=None):
+    def __init__(self, repr_net, dyn_net, pred_net, optimizer, roll_ahead: int, coeff=(1.0, 1.0, 1.0), dist=None,
+                 checkpoints8: bool = False):
+        """checkpoints8: the dense layers of the unroll keep their inputs in 8 bits for the backward pass."""
+        self.checkpoints8 = checkpoints8
         self.nets = (repr_net, dyn_net, pred_net)
         self.params = [p for n in self.nets for p in n.parameters()]
         self.optimizer, self.roll_ahead, self.coeff, self.dist = optimizer, roll_ahead, coeff, dist
@@ -230,7 +239,7 @@ class DataParallelLearner:
         multi = self.world > 1
         if local is not None and len(local) > 0:
             local = local.to(dev)
-            wsum, per_window, _ = batched_unroll_loss(*self.nets, local, self.roll_ahead, self.coeff)
+            wsum, per_window, _ = batched_unroll_loss(*self.nets, local, self.roll_ahead, self.coeff, checkpoints8=self.checkpoints8)
             flat_extra[0] = local.is_weights.sum()
             flat_extra[1] = wsum.detach()
             ready = [False] * len(buckets)
@@ -360,7 +369,8 @@ class DataParallelLearner:
         lat0 = representation_latents(self.nets[0], self._rec_batch)
         self._rec_lat0 = lat0
         lat = lat0.detach().requires_grad_(lat0.requires_grad)
-        wsum, per_window, _ = batched_unroll_loss(*self.nets, self._rec_batch, self.roll_ahead, self.coeff, latent=lat)
+        wsum, per_window, _ = batched_unroll_loss(*self.nets, self._rec_batch, self.roll_ahead, self.coeff, latent=lat,
+                                                  checkpoints8=self.checkpoints8)
         wsum.backward()
         self._rec_lat_grad = lat.grad
         n = self._rec_split - 2
@@ -445,6 +455,15 @@ class DataParallelLearner:
         with torch.cuda.graph(self._rec_update, pool=self._rec_backward.pool()):
             self._update_from_flat()
         self._rec_shapes = shapes
+
+    @torch.no_grad()
+    def policy_report(self, batch: WindowBatch, top: int = 3) -> PolicyScores:
+        """How the current networks judge the recorded moves at the windows' first step: log probability of each, entropy
+        of the policy, its `top` preferred actions."""
+        batch = batch.to(self.params[0].device)
+        latent = representation_latents(self.nets[0], batch)
+        with per_call_statistics(self.nets[2]):
+            return score_actions(self.nets[2], latent, batch.actions[:, 0], top)
 
     def broadcast_weights(self, src: int = 0):
         """Learner -> actors: one flat broadcast; actors re-pack their MFMA weight blob afterwards

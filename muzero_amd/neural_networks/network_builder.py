@@ -110,3 +110,21 @@ def build_mlp(layers_config: list[DenseLayerConfig], input_dim: int) -> tuple[nn
         mods += [nn.Linear(width, cfg.out_features), get_activation(cfg.activation)]
         width = cfg.out_features
     return nn.Sequential(*mods), width
+
+
+_DENSE_ACTIVATIONS = {nn.Identity: "none", nn.ReLU: "relu", nn.Tanh: "tanh", nn.Sigmoid: "sigmoid", nn.Softmax: "softmax"}
+
+
+def is_dense_sequence(module: nn.Module) -> bool:
+    """True for what build_mlp makes: Linear and activation in turn."""
+    mods = list(module) if isinstance(module, nn.Sequential) else []
+    return len(mods) > 0 and len(mods) % 2 == 0 and all(
+        isinstance(m, nn.Linear) if i % 2 == 0 else type(m) in _DENSE_ACTIVATIONS for i, m in enumerate(mods))
+
+
+def dense_pairs(seq: nn.Sequential) -> list[tuple[nn.Linear, str]]:
+    """(Linear, activation name) pairs of a build_mlp sequence."""
+    if not is_dense_sequence(seq):
+        raise ValueError("expected a sequence of Linear layers, each followed by its activation")
+    mods = list(seq)
+    return [(lin, _DENSE_ACTIVATIONS[type(act)]) for lin, act in zip(mods[::2], mods[1::2])]

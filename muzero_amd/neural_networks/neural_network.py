@@ -75,10 +75,13 @@ class DynamicsNetwork(nn.Module):
         head = list(config.reward_net) + [DenseLayerConfig(out_features=1, activation="linear")]
         self.reward_mlp, _ = build_mlp(head, input_dim=d)
 
+    def merge(self, merged: torch.Tensor) -> torch.Tensor:
+        return F.relu(self.fc_merge(merged))
+
     def forward(self, latent_state: torch.Tensor, action: torch.Tensor):
         b, c, h, w = latent_state.shape
         merged = torch.cat([latent_state.view(b, -1), self.action_embedding(action)], dim=1)
-        x = F.relu(self.fc_merge(merged)).view(b, c, h, w)
+        x = self.merge(merged).view(b, c, h, w)
         for block in self.res_blocks:
             x = block(x)
         next_latent = self.res_final(x)
@@ -99,16 +102,23 @@ class PredictionNetwork(nn.Module):
         p_head = list(config.policy_net) + [DenseLayerConfig(out_features=num_actions, activation="softmax")]
         self.policy_mlp, _ = build_mlp(p_head, input_dim=d)
 
-    def forward(self, latent_state: torch.Tensor):
+    def _flat(self, latent_state: torch.Tensor) -> torch.Tensor:
         b, c, h, w = latent_state.shape
         assert (c, h, w) == tuple(self.latent_shape), "Latent shape mismatch."
         x = latent_state
         for block in self.res_blocks:
             x = block(x)
-        flat = self.res_final(x).view(b, -1)
+        return self.res_final(x).view(b, -1)
+
+    def forward(self, latent_state: torch.Tensor):
+        flat = self._flat(latent_state)
         value = self.value_mlp(flat)
         policy = self.policy_mlp(flat)  # already softmaxed (last activation is Softmax)
         return policy, value
+
+    def policy_logits(self, latent_state: torch.Tensor) -> torch.Tensor:
+        """The policy in front of its softmax (what muzero_amd.policy_scores reads)."""
+        return self.policy_mlp[:-1](self._flat(latent_state))
 
 
 def load_networks(model_folder_path: str, config=None, observation_space=None, num_actions=None):

@@ -1,0 +1,113 @@
+"""Scores of actions under a policy head's logits: log probability, entropy and the best alternatives, with gradient.
+
+The reference reads its policy head through `torch.softmax` and `argmax` alone (src/search/expansion.py:26-27,
+src/search/simulation.py:36); a learner or a report that asks how likely the recorded moves are, how sure the network
+is and what it would rather play needs these values for every row, in one pass over the logits:
+
+    scores = policy_scores(logits, actions, top=3)
+    scores.log_prob, scores.entropy              # [...]        differentiable
+    scores.top_actions, scores.top_log_probs     # [..., top]   the latter differentiable
+
+`logits` are the values in front of the head's softmax (`PredictionNetwork.policy_logits`), float32, bfloat16 or
+float16, of any leading shape; illegal actions carry -inf.  Results are float32.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from muzero_amd import _hip
+from muzero_amd._hip import ptr
+from muzero_amd._rows import TYPE, check_tensor, on_device, row_stride, rows_of, stream_of, workspace
+
+MAX_TOP = 32
+
+
+class PolicyScores(NamedTuple):
+    log_prob: Optional[torch.Tensor]       # f32[...]       log p(action), None without actions
+    entropy: torch.Tensor                  # f32[...]       -sum p log p
+    top_actions: torch.Tensor              # i64[..., top]  largest logits first, the lowest index among equals
+    top_log_probs: torch.Tensor            # f32[..., top]
+
+
+def _forward(logits: torch.Tensor, actions: Optional[torch.Tensor], top: int):
+    T, V = logits.shape
+    f32 = dict(dtype=torch.float32, device=logits.device)
+    log_prob = torch.empty(T, **f32) if actions is not None else None
+    entropy, stats = torch.empty(T, **f32), torch.empty((T, 2), **f32)
+    top_actions = torch.empty((T, top), dtype=torch.int64, device=logits.device)
+    top_log_probs = torch.empty((T, top), **f32)
+    if T > 0:
+        lib, kind = _hip.lib(), TYPE[logits.dtype]
+        with on_device(logits):
+            need = lib.mz_policy_scores_workspace(kind, T, V, top)
+            ws = workspace(need, logits)
+            _hip.check(lib.mz_policy_scores(ptr(logits), kind, row_stride(logits), ptr(actions), T, V, top, ptr(log_prob),
+                                            ptr(entropy), ptr(stats), ptr(top_actions), ptr(top_log_probs), ptr(ws), need,
+                                            stream_of(logits)), "mz_policy_scores")
+    return log_prob, entropy, stats, top_actions, top_log_probs
+
+
+class _PolicyScores(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, actions, top):
+        log_prob, entropy, stats, top_actions, top_log_probs = _forward(logits, actions, top)
+        ctx.save_for_backward(logits, actions, stats, entropy, top_actions)
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(top_actions)
+        return log_prob, entropy, top_actions, top_log_probs
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_log_prob, g_entropy, _g_actions, g_top):
+        logits, actions, stats, entropy, top_actions = ctx.saved_tensors
+        T, V = logits.shape
+        grad = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
+        if T > 0:
+            g_log_prob, g_entropy, g_top = (g if g is None else g.contiguous() for g in (g_log_prob, g_entropy, g_top))
+            with on_device(logits):
+                _hip.check(_hip.lib().mz_policy_scores_backward(
+                    ptr(logits), TYPE[logits.dtype], row_stride(logits), ptr(actions), T, V, top_actions.shape[1], ptr(stats),
+                    ptr(entropy), ptr(top_actions), ptr(g_log_prob), ptr(g_entropy), ptr(g_top), ptr(grad), V,
+                    stream_of(logits)), "mz_policy_scores_backward")
+        return grad, None, None
+
+
+def policy_scores(logits: torch.Tensor, actions: Optional[torch.Tensor] = None, top: int = 0) -> PolicyScores:
+    """Scores of every row of `logits` [..., V].  `actions` (whole numbers, shape [...]): a negative one scores 0 and
+    takes no gradient (no action was played there), one of V or more scores NaN.  `top`: 0..32 alternatives.
+
+    A row with nothing but -inf has log probabilities -inf, entropy 0 and no gradient; NaN or +inf make their row NaN."""
+    check_tensor(logits, "logits")
+    if logits.dim() < 1 or logits.shape[-1] < 1:
+        raise ValueError(f"logits need at least one action in their last dimension, not shape {tuple(logits.shape)}")
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    if V > 0x7FFFFFFF:
+        raise ValueError(f"{V} actions are more than a call takes")
+    if not 0 <= top <= min(MAX_TOP, V):
+        raise ValueError(f"top={top} must lie in 0..{MAX_TOP} and not exceed the {V} actions")
+    if actions is not None:
+        if not isinstance(actions, torch.Tensor) or actions.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8,
+                                                                          torch.uint8):
+            raise TypeError("actions must be a tensor of whole numbers")
+        if actions.shape != lead:
+            raise ValueError(f"actions of shape {tuple(actions.shape)} do not match logits of shape {tuple(logits.shape)}")
+        if actions.device != logits.device:
+            raise ValueError(f"actions are on {actions.device}, logits on {logits.device}")
+        actions = actions.reshape(-1).to(torch.int64).contiguous()
+    rows = rows_of(logits)
+    if torch.is_grad_enabled() and rows.requires_grad:
+        log_prob, entropy, top_actions, top_log_probs = _PolicyScores.apply(rows, actions, top)
+    else:
+        log_prob, entropy, _, top_actions, top_log_probs = _forward(rows, actions, top)
+    if len(lead) != 1:
+        log_prob = log_prob if log_prob is None else log_prob.reshape(lead)
+        entropy, top_actions, top_log_probs = entropy.reshape(lead), top_actions.reshape(*lead, top), top_log_probs.reshape(*lead, top)
+    return PolicyScores(log_prob, entropy, top_actions, top_log_probs)
+
+
+def score_actions(pred_net, latent: torch.Tensor, actions: Optional[torch.Tensor] = None, top: int = 0) -> PolicyScores:
+    """policy_scores of a PredictionNetwork's policy for latents [B, c, h, w]."""
+    return policy_scores(pred_net.policy_logits(latent), actions, top)

@@ -1,0 +1,162 @@
+"""Dense layers in 8-bit integers: rows with a scale each, and products of them.
+
+    weight = quantize_rows(linear.weight)                 # one scale per output channel, once per weight update
+    y = int8_linear(x, weight, linear.bias, "relu")       # rows of x are coded in the call, one scale per row
+    heads = Int8MLP(pred_net.policy_mlp)                  # a whole build_mlp sequence
+
+The int8 form of nn.Linear + activation (`build_mlp`, src/neural_networks/network_builder.py:183-205) for networks that
+answer with trained weights: a quarter of the weight bytes of float32, the matrix cores' int8 rate.  Values are off by
+the two roundings to 127 steps of the largest value of a row, which is NOT the float32 accuracy of the search's own
+networks (muzero_amd.engine): choose it where that is enough.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from muzero_amd import _hip
+from muzero_amd._hip import ptr
+from muzero_amd._rows import TYPE, check_tensor, on_device, row_stride, rows_of, stream_of, workspace
+
+MAX_K = 131072  # sums of K products of codes stay exact in 32 bits
+ACTIVATIONS = ("none", "linear", "relu", "tanh", "sigmoid")
+
+
+@dataclass(frozen=True)
+class QuantizedRows:
+    """Rows in 8 bits: x[r, k] is about scales[r] * codes[r, k].  `codes` is padded with zeros to a row stride of a
+    multiple of 128 bytes."""
+    codes: torch.Tensor        # i8[rows, ldc]
+    scales: torch.Tensor       # f32[rows]
+    shape: torch.Size          # of the tensor that was coded
+    dtype: torch.dtype         # of the tensor that was coded
+    scale_bits: int            # significant bits of the scales: 24 or 3
+
+    @property
+    def rows(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def columns(self) -> int:
+        return self.shape[-1]
+
+    def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+        """scales * codes in the shape and (by default) the type of the tensor that was coded."""
+        dtype = self.dtype if dtype is None else dtype
+        if dtype not in TYPE:
+            raise TypeError(f"rows can be read back as float32, bfloat16 or float16, not {dtype}")
+        out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
+        if self.rows > 0:
+            with on_device(out):
+                _hip.check(_hip.lib().mz_dequant8_rows(ptr(self.codes), self.codes.stride(0), ptr(self.scales), self.rows, self.columns,
+                                                       ptr(out), TYPE[dtype], self.columns, stream_of(out)), "mz_dequant8_rows")
+        return out
+
+
+def quantize_rows(x: torch.Tensor, scale_bits: int = 24) -> QuantizedRows:
+    """Codes of x [..., K], one scale per row.  scale_bits=3 rounds the scale up to 1, 1.25, 1.5 or 1.75 times a power of
+    two (what muzero_amd.checkpoints keeps)."""
+    check_tensor(x, "x")
+    if scale_bits not in (24, 3):
+        raise ValueError(f"scale_bits must be 24 or 3, not {scale_bits}")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x needs at least one value in a row, not shape {tuple(x.shape)}")
+    rows = rows_of(x.detach())
+    R, K = rows.shape
+    codes = torch.empty((R, (K + 127) // 128 * 128), dtype=torch.int8, device=x.device)
+    scales = torch.empty(R, dtype=torch.float32, device=x.device)
+    if R > 0:
+        with on_device(rows):
+            _hip.check(_hip.lib().mz_quant8_rows(ptr(rows), TYPE[rows.dtype], row_stride(rows), R, K, scale_bits, ptr(codes),
+                                                 codes.stride(0), ptr(scales), stream_of(rows)), "mz_quant8_rows")
+    return QuantizedRows(codes, scales, x.shape, x.dtype, scale_bits)
+
+
+def _check_weight(weight: QuantizedRows, K: int) -> int:
+    if not isinstance(weight, QuantizedRows):
+        raise TypeError("weight must be the QuantizedRows of a [N, K] matrix (quantize_rows)")
+    if len(weight.shape) != 2:
+        raise ValueError(f"weight must be a matrix, not of shape {tuple(weight.shape)}")
+    if weight.columns != K:
+        raise ValueError(f"rows of {K} values do not match a weight of {weight.columns} input features")
+    if K > MAX_K:
+        raise ValueError(f"{K} input features are more than the {MAX_K} whose sums stay exact in 32 bits")
+    return weight.rows
+
+
+def int8_linear(x, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, activation: str = "none",
+                out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """act(x W^T + bias) for x [..., K] (a tensor, or QuantizedRows when several layers read the same rows).  The result
+    has x's type unless `out_dtype` says otherwise.  There is no gradient: training goes through float weights
+    (muzero_amd.checkpoints keeps their inputs in 8 bits)."""
+    coded = isinstance(x, QuantizedRows)
+    if not coded:
+        check_tensor(x, "x")
+        if x.dim() < 1:
+            raise ValueError("x needs at least one dimension")
+        if torch.is_grad_enabled() and x.requires_grad:
+            raise RuntimeError("int8_linear has no gradient; call it under torch.no_grad() or on a detached tensor")
+    N = _check_weight(weight, x.shape[-1])
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {ACTIVATIONS}, not {activation!r}")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if out_dtype not in TYPE:
+        raise TypeError(f"out_dtype must be float32, bfloat16 or float16, not {out_dtype}")
+    dev = weight.codes.device
+    if (x.codes if coded else x).device != dev:
+        raise ValueError("x and weight are on different devices")
+    if bias is not None:
+        if bias.shape != (N,) or bias.device != dev:
+            raise ValueError(f"bias must be {N} values on {dev}")
+        bias = bias.detach().to(torch.float32).contiguous()
+    K = weight.columns
+    y = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype, device=dev)
+    if y.numel() == 0:
+        return y
+    lib, act = _hip.lib(), _hip.ACT[activation]
+    with on_device(y):
+        if coded:
+            need = lib.mz_int8_codes_workspace(x.rows, K, N)
+            ws = workspace(need, y)
+            _hip.check(lib.mz_int8_forward_codes(ptr(x.codes), x.codes.stride(0), ptr(x.scales), x.rows, K, ptr(weight.codes),
+                                                 weight.codes.stride(0), ptr(weight.scales), N, ptr(bias), act, ptr(y), TYPE[out_dtype],
+                                                 N, ptr(ws), need, stream_of(y)), "mz_int8_forward_codes")
+        else:
+            rows = rows_of(x.detach())
+            need = lib.mz_int8_workspace(rows.shape[0], K, N)
+            ws = workspace(need, y)
+            _hip.check(lib.mz_int8_forward(ptr(rows), TYPE[rows.dtype], row_stride(rows), rows.shape[0], K, ptr(weight.codes),
+                                           weight.codes.stride(0), ptr(weight.scales), N, ptr(bias), act, ptr(y), TYPE[out_dtype], N,
+                                           ptr(ws), need, stream_of(y)), "mz_int8_forward")
+    return y
+
+
+class Int8MLP:
+    """A build_mlp sequence (Linear + activation pairs) with its weights in 8 bits.  Call `refresh()` after the weights
+    change.  `logits(x)` stops in front of a final softmax."""
+
+    def __init__(self, seq: torch.nn.Sequential, device="cuda"):
+        self.seq, self.device = seq, torch.device(device)
+        self.refresh()
+
+    def refresh(self) -> None:
+        from muzero_amd.neural_networks.network_builder import dense_pairs
+        self.layers, self.softmax = [], False
+        for lin, act in dense_pairs(self.seq):
+            if self.softmax:
+                raise ValueError("softmax is supported as the last activation only")
+            self.softmax = act == "softmax"
+            w = quantize_rows(lin.weight.detach().to(self.device))
+            b = None if lin.bias is None else lin.bias.detach().to(self.device, torch.float32).clone()
+            self.layers.append((w, b, "none" if self.softmax else act))
+
+    def logits(self, x) -> torch.Tensor:
+        for w, b, act in self.layers:
+            x = int8_linear(x, w, b, act)
+        return x
+
+    def __call__(self, x) -> torch.Tensor:
+        y = self.logits(x)
+        return torch.softmax(y, dim=-1) if self.softmax else y

@@ -1,0 +1,467 @@
+"""Row codes, dense layers in 8-bit integers and 8-bit activation checkpoints against their definitions in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.float32: 0.0, torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+SHORT = np.arange(4, 9) / 8.0   # mantissas of a short scale in [1/2, 1]
+
+
+def _codes64(x, bits=24):
+    """Codes and scales by the definition: float32 roundings, each of one value that float64 holds well enough."""
+    x = x.detach().cpu().to(torch.float32).double().numpy()
+    a = np.abs(x).max(1)
+    f = lambda v: v.astype(np.float32).astype(np.float64)  # noqa: E731
+    with np.errstate(all="ignore"):
+        s, i = f(a / 127), f(127 / a)
+        if bits == 3:
+            m, e = np.frexp(s)
+            s = np.ldexp(np.ceil(m * 8) / 8, e)
+            i = f(1 / s)
+        q = np.rint(f(x * i[:, None]))
+    q[a < 2.0 ** -119], s[a < 2.0 ** -119] = 0, 0
+    bad = ~np.isfinite(a)
+    q[bad], s[bad] = 0, np.nan
+    return q, s
+
+
+def _act64(v, name):
+    return {"none": lambda v: v, "relu": lambda v: np.maximum(v, 0), "tanh": np.tanh, "sigmoid": lambda v: 1 / (1 + np.exp(-v))}[name](v)
+
+
+def _x(R, K, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(R, K, generator=g) * torch.exp(torch.randn(K, generator=g)) * torch.exp(2 * torch.randn(R, 1, generator=g))
+    x[:, : K // 2].clamp_(min=0)
+    return x.to(dtype).cuda()
+
+
+def _within(got, want, tol):
+    # rounding to nearest takes a float16 of 65504 + half a step (32 / 2) or more to infinity: right where the value may be one
+    inf = got.dtype == torch.float16
+    got = got.detach().cpu().double().numpy()
+    ok = (got == want) | (np.isnan(got) & np.isnan(want)) | (np.abs(got - want) <= tol)
+    if inf:
+        ok |= np.isinf(got) & (np.sign(got) == np.sign(want)) & (np.abs(want) + tol >= 65520.0)
+    assert ok.all(), (int((~ok).sum()), got[~ok][:5], want[~ok][:5], np.broadcast_to(tol, got.shape)[~ok][:5])
+
+
+@pytest.mark.parametrize("bits", [24, 3])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,K", [(1, 1), (3, 2), (5, 16), (64, 168), (7, 127), (2, 129), (33, 1000), (4, 4096), (3, 9217), (2, 18432), (2, 70001)])
+def test_codes_are_the_definitions(R, K, dtype, bits):
+    from muzero_amd.quantized import quantize_rows
+    x = _x(R, K, dtype, seed=K)
+    c = quantize_rows(x, scale_bits=bits)
+    q, s = _codes64(x, bits)
+    assert c.codes.shape[1] % 128 == 0 and (c.codes[:, K:] == 0).all()
+    np.testing.assert_array_equal(c.codes[:, :K].cpu().numpy(), q)
+    np.testing.assert_array_equal(c.scales.cpu().double().numpy(), s)
+    if bits == 3:
+        assert set(np.frexp(s[s > 0])[0]) <= set(SHORT)
+    back = c.dequantize()
+    assert back.dtype == dtype and back.shape == x.shape
+    np.testing.assert_array_equal(back.cpu().float().numpy(), torch.from_numpy((q * s[:, None]).astype(np.float32)).to(dtype).float().numpy())
+
+
+@pytest.mark.parametrize("bits", [24, 3])
+def test_hard_rows(bits):
+    from muzero_amd.quantized import quantize_rows
+    x = torch.randn(12, 300)
+    x[0] = 0.0
+    x[1] = 1e-40                                   # below float32's normal range
+    x[2] *= 2.0 ** -121                            # below the smallest scale
+    x[3] *= 2.0 ** -116
+    x[4] = torch.finfo(torch.float32).max
+    x[5, 17] = torch.inf
+    x[6, 299] = torch.nan
+    x[7] = 0.0
+    x[7, 1] = -3.0
+    x[8] = torch.arange(300) % 128 / 127.0         # every code, on the step
+    x[9] = (torch.arange(300) % 254 + 0.5) / 254   # halfway between steps
+    x[10] = -x[9]
+    x[11, 0] = torch.finfo(torch.float32).max
+    c = quantize_rows(x.cuda(), scale_bits=bits)
+    q, s = _codes64(x, bits)
+    np.testing.assert_array_equal(c.codes[:, :300].cpu().numpy(), q)
+    np.testing.assert_array_equal(c.scales.cpu().double().numpy(), s)
+    assert np.abs(q).max() <= 127 and c.dequantize()[5:7].isnan().all()
+
+
+def _int8_reference(x, w, b, act, bits=24):
+    (q, s), (t, v) = _codes64(x), _codes64(w)
+    lin = (q @ t.T) * s[:, None] * v[None, :]
+    bias = 0.0 if b is None else b.cpu().double().numpy()[None, :]
+    pre = lin + bias
+    # sum -> float32, scale product, product, bias: four roundings; every activation's slope is at most 1, its own
+    # evaluation costs a few units of its result
+    return _act64(pre, act), 4 * U * (np.abs(lin) + np.abs(pre)) + 8 * U * np.abs(_act64(pre, act)) + 1e-37
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,K,N,act", [(1, 1, 1, "none"), (1, 16, 7, "relu"), (3, 168, 256, "relu"), (1, 168, 256, "tanh"), (256, 256, 7, "none"),
+                                       (5, 129, 33, "sigmoid"), (16, 1000, 100, "none"), (17, 512, 130, "relu"), (64, 640, 64, "none"),
+                                       (65, 127, 127, "tanh"), (128, 128, 128, "none"), (130, 300, 257, "sigmoid"), (1, 9216, 300, "relu"),
+                                       (2, 18432, 65, "none"), (300, 4097, 190, "relu"), (8, 4096, 1024, "none"), (520, 260, 520, "none"),
+                                       (33, 2048, 2, "none"), (1030, 64, 1, "none"), (48, 8192, 1000, "relu"), (700, 1200, 900, "none")])
+def test_int8_linear(R, K, N, act, dtype):
+    from muzero_amd.quantized import int8_linear, quantize_rows
+    x = _x(R, K, dtype, seed=R + K)
+    w = torch.randn(N, K, generator=torch.Generator().manual_seed(N)) / K ** 0.5
+    b = torch.randn(N, generator=torch.Generator().manual_seed(1)) if N % 2 else None
+    qw = quantize_rows(w.cuda())
+    want, tol = _int8_reference(x, w, b, act)
+    y = int8_linear(x, qw, None if b is None else b.cuda(), act)
+    assert y.dtype == dtype and y.shape == (R, N)
+    _within(y, want, tol + HALF[dtype] * (np.abs(want) + tol) + TINY[dtype])
+    coded = int8_linear(quantize_rows(x), qw, None if b is None else b.cuda(), act)
+    assert torch.equal(coded, y)                       # rows coded beforehand: the same numbers
+    y32 = int8_linear(x, qw, None if b is None else b.cuda(), act, out_dtype=torch.float32)
+    _within(y32, want, tol + U * np.abs(want))
+
+
+@pytest.mark.parametrize("R", [1, 9, 100, 400])
+def test_int8_rows_are_independent_and_nan_is_loud(R):
+    from muzero_amd.quantized import int8_linear, quantize_rows
+    K, N = 500, 140
+    x, w = _x(R, K, torch.float32), torch.randn(N, K).cuda()
+    w[3, 4] = torch.nan
+    qw = quantize_rows(w)
+    y = int8_linear(x, qw, activation="relu")
+    assert y[:, 3].isnan().all()
+    keep = [n for n in range(N) if n != 3]
+    assert y[:, keep].isfinite().all()
+    x2 = x.clone()
+    x2[R // 2, 7] = torch.inf
+    y2 = int8_linear(x2, qw, activation="relu")
+    assert y2[R // 2].isnan().all()
+    rest = [r for r in range(R) if r != R // 2]
+    assert torch.equal(y2[rest][:, keep], y[rest][:, keep])
+
+
+def test_largest_sum_stays_exact():
+    from muzero_amd.quantized import int8_linear, quantize_rows
+    K = 131072
+    for R, N in ((1, 3), (200, 150)):
+        x, w = torch.ones(R, K, device="cuda"), torch.ones(N, K, device="cuda")
+        w[1] = -1.0
+        y = int8_linear(x, quantize_rows(w))
+        s = float(quantize_rows(x).scales[0])
+        want = np.float64(127 * 127 * K) * s * s
+        got = y.cpu().double().numpy()
+        assert np.abs(got[:, 0] - want).max() <= 4 * U * want and np.abs(got[:, 1] + want).max() <= 4 * U * want
+    with pytest.raises(ValueError):
+        int8_linear(torch.ones(1, K + 1, device="cuda"), quantize_rows(torch.ones(1, K + 1, device="cuda")))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_int8_shapes_strides_and_alignment(dtype):
+    from muzero_amd.quantized import int8_linear, quantize_rows
+    big = _x(40, 700, dtype)
+    w = torch.randn(90, 333).cuda()
+    qw, qv = quantize_rows(w), quantize_rows(torch.cat([w, w], 1)[:, :333])
+    assert torch.equal(qw.codes, qv.codes)
+    for view in (big[:, :333], big[:, 1:334], big[::3, 5:338], big.t()[:333].t(), big[:, : 2 * 333 : 2], big[3:4, 7:340],
+                 big[:1, :333].expand(40, 333), big[:, :333].reshape(2, 5, 4, 333), big[0, :333]):
+        want = int8_linear(view.contiguous().clone(), qw)
+        assert torch.equal(int8_linear(view, qw), want) and want.shape == view.shape[:-1] + (90,)
+        c, d = quantize_rows(view), quantize_rows(view.contiguous().clone())
+        assert torch.equal(c.codes, d.codes) and torch.equal(c.scales, d.scales)
+    assert int8_linear(big[:0, :333], qw).shape == (0, 90)
+
+
+def _grad_reference(dz, x, bits=3):
+    q, s = _codes64(x, bits)
+    g = dz.detach().cpu().double().numpy()
+    v = g * s[:, None]
+    mag = np.abs(v).T @ np.abs(q)
+    # v is rounded once and held to 22 bits (2^-39 of its column's largest at least); products are exact; a float32 sum
+    # of R terms in any order is off by at most R u of the magnitudes
+    tol = (2.0 ** -21 + (g.shape[0] + 8) * U) * mag + 2.0 ** -39 * np.abs(v).max(0, initial=0)[:, None] * np.abs(q).sum(0)[None, :]
+    return v.T @ q, tol + 1e-37, g.sum(0), (g.shape[0] + 4) * U * np.abs(g).sum(0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,K,N", [(1, 1, 1), (1, 168, 7), (2, 16, 300), (31, 129, 5), (64, 64, 64), (65, 168, 256), (256, 336, 168), (300, 100, 130),
+                                   (1000, 257, 33), (2049, 40, 50), (5000, 128, 128), (256, 1152, 640), (130, 2000, 700)])
+def test_weight_gradient(R, K, N, dtype):
+    from muzero_amd.checkpoints import save_activations, weight_grad
+    x = _x(R, K, dtype, seed=R)
+    g = torch.Generator().manual_seed(K)
+    dz = (torch.randn(R, N, generator=g) * torch.exp(3 * torch.randn(N, generator=g)) * 1e-2)
+    dz[torch.rand(R, generator=g) < 0.2] = 0.0
+    dz = dz.to(dtype).cuda()
+    saved = save_activations(x)
+    want, tol, want_b, tol_b = _grad_reference(dz, x)
+    dw, db = weight_grad(dz, saved)
+    assert dw.dtype == db.dtype == dtype and dw.shape == (N, K)
+    _within(dw, want, tol + HALF[dtype] * (np.abs(want) + tol) + TINY[dtype])
+    _within(db, want_b, tol_b + HALF[dtype] * (np.abs(want_b) + tol_b) + TINY[dtype])
+    again, none = weight_grad(dz, saved, want_bias=False)
+    assert none is None and torch.equal(again, dw)
+
+
+def test_weight_gradient_holds_columns_of_any_size():
+    """Each output row has a range of its own; within one, values down to 2^-16 of the largest keep 22 bits."""
+    from muzero_amd.checkpoints import save_activations, weight_grad
+    R, K, N = 200, 96, 60
+    x = _x(R, K, torch.float32)
+    dz = torch.randn(R, N) * torch.logspace(-33, 30, N)[None, :]
+    dz[:, 5] = 0.0
+    dz[:, 6] = 1e-42
+    dz[:, 7] *= torch.logspace(0, -8, R)                # a wide range inside one column
+    dz = dz.cuda()
+    want, tol, _, _ = _grad_reference(dz, x)
+    dw, _ = weight_grad(dz, save_activations(x))
+    _within(dw, want, tol + 2 * U * np.abs(want) + 1e-40)
+    assert (dw[5] == 0).all()
+    dz[3, 8], dz[4, 9] = torch.inf, torch.nan
+    dw2, db2 = weight_grad(dz, save_activations(x))
+    assert dw2[8].isnan().all() and dw2[9].isnan().all() and db2[8].isinf() and db2[9].isnan()
+    keep = [n for n in range(N) if n not in (8, 9)]
+    assert torch.equal(dw2[keep], dw[keep])
+
+
+def test_full_scales_and_strided_gradients():
+    from muzero_amd.checkpoints import save_activations, weight_grad
+    from muzero_amd.quantized import quantize_rows
+    R, K, N = 90, 200, 70
+    for dtype in TYPES:
+        x = _x(R, K, dtype)
+        wide = (torch.randn(R, 3 * N) * 0.01).to(dtype).cuda()
+        for dz in (wide[:, :N], wide[:, 1:N + 1], wide[:, ::3], wide[:, :N].contiguous().t().contiguous().t()):
+            assert torch.equal(weight_grad(dz, save_activations(x))[0], weight_grad(dz.contiguous().clone(), save_activations(x))[0])
+        want, tol, _, _ = _grad_reference(wide[:, :N], x, bits=24)
+        dw, _ = weight_grad(wide[:, :N], quantize_rows(x))
+        _within(dw, want, tol + HALF[dtype] * (np.abs(want) + tol) + TINY[dtype])
+    dw, db = weight_grad(torch.zeros(0, N, device="cuda"), save_activations(torch.zeros(0, K, device="cuda")))
+    assert (dw == 0).all() and dw.shape == (N, K) and (db == 0).all()
+
+
+@pytest.mark.parametrize("activation", ["none", "relu", "tanh", "sigmoid"])
+@pytest.mark.parametrize("shape", [(1, 5, 3), (64, 168, 256), (33, 40, 129), (4, 300, 9)])
+def test_checkpointed_layer(shape, activation):
+    """Forward: the layer itself.  Backward: dz = dy act'(y) with what was kept of y, dx = dz W, dW and db from dz and
+    the codes of x."""
+    from muzero_amd.checkpoints import checkpointed_linear, save_activations
+    R, K, N = shape
+    torch.manual_seed(R)
+    lin = torch.nn.Linear(K, N).cuda()
+    x = torch.randn(R, K, device="cuda", requires_grad=True)
+    dy = torch.randn(R, N, device="cuda")
+    y = checkpointed_linear(x, lin.weight, lin.bias, activation)
+    act = {"none": lambda t: t, "relu": torch.relu, "tanh": torch.tanh, "sigmoid": torch.sigmoid}[activation]
+    assert torch.equal(y, act(lin(x)))
+    y.backward(dy)
+    y64, g = y.detach().cpu().double().numpy(), dy.cpu().double().numpy()
+    if activation == "relu":
+        dz = g * (y64 > 0)
+    elif activation == "tanh":
+        dz = g * (1 - (np.rint(y64 * 127) / 127) ** 2)
+    elif activation == "sigmoid":
+        dz = g * (1 - (np.rint(254 * y64 - 127) / 127) ** 2) / 4
+    else:
+        dz = g
+    w64 = lin.weight.detach().cpu().double().numpy()
+    # a code of y next to a border may fall either way in float32 (y is then rounded to a neighbour of the same distance)
+    step = 0.0 if activation in ("none", "relu") else 1e-6
+    _within(x.grad, dz @ w64, (N + 8) * U * (np.abs(dz) @ np.abs(w64)) + step * np.abs(g) @ np.abs(w64) + 1e-37)
+    q, s = _codes64(x, 3)
+    xh = q * s[:, None]
+    _within(lin.weight.grad, dz.T @ xh, (2.0 ** -20 + (R + 8) * U) * (np.abs(dz).T @ np.abs(xh)) + step * np.abs(g).T @ np.abs(xh) + 1e-37)
+    _within(lin.bias.grad, dz.sum(0), (R + 8) * U * np.abs(dz).sum(0) + step * np.abs(g).sum(0) + 1e-37)
+    assert torch.equal(save_activations(x).codes.cpu()[:, :K], torch.from_numpy(q).to(torch.int8))
+
+
+@pytest.mark.parametrize("activation", ["relu", "tanh", "sigmoid"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N", [1, 7, 8, 65, 1000])
+def test_kept_activations(N, dtype, activation):
+    """What is kept of y and the gradient read from it, for every stride; NaN stays NaN."""
+    from muzero_amd.checkpoints import _act_grad, _act_save
+    R = 9
+    y = torch.randn(R, N + 3).cuda()
+    y = {"relu": torch.relu, "tanh": torch.tanh, "sigmoid": torch.sigmoid}[activation](y).to(dtype)[:, 1:N + 1]
+    dy = torch.randn(R, N + 5).to(dtype).cuda()[:, 2:N + 2]
+    saved = _act_save(y, activation)
+    dz = _act_grad(dy, saved, activation)
+    y64, g = y.cpu().double().numpy(), dy.cpu().double().numpy()
+    if activation == "relu":
+        np.testing.assert_array_equal(dz.cpu().double().numpy(), g * (y64 > 0))
+    else:
+        # the product with 127 or 254 is one float32 rounding away from the definition: half-way cases may go either way
+        t = (np.rint(y64 * 127) if activation == "tanh" else np.rint(y64 * 254 - 127)) / 127
+        want = g * (1 - t * t) * (1.0 if activation == "tanh" else 0.25)
+        near = np.abs(np.abs((y64 * 127 if activation == "tanh" else y64 * 254 - 127)) % 1 - 0.5) < 1e-4
+        slack = np.where(near, np.abs(g) * 2 / 127, 0.0)
+        _within(dz, want, slack + 8 * U * np.abs(g) + HALF[dtype] * np.abs(want) + TINY[dtype])
+        y2 = y.clone()
+        y2[1, 0] = torch.nan
+        assert _act_grad(dy, _act_save(y2, activation), activation)[1, 0].isnan()
+
+
+def test_a_layer_keeps_a_quarter_of_the_bytes():
+    from muzero_amd.checkpoints import checkpointed_linear
+    lin = torch.nn.Linear(2048, 1024).cuda()
+    x = torch.randn(4096, 2048, device="cuda", requires_grad=True)
+
+    def kept(fn):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        src = x * 1.0                                   # an input nobody else keeps
+        y = fn(src)
+        del src
+        torch.cuda.synchronize()
+        return torch.cuda.memory_allocated() - before - y.numel() * 4, y
+    full, y0 = kept(lambda t: torch.tanh(lin(t)) + 0.0)
+    small, y1 = kept(lambda t: checkpointed_linear(t, lin.weight, lin.bias, "tanh") + 0.0)
+    assert torch.equal(y0, y1) and small < 0.26 * full + 65536 * 2, (small, full)
+
+
+def _networks(seed=0):
+    from muzero_amd.config import load_config
+    from muzero_amd.neural_networks import DynamicsNetwork, PredictionNetwork, RepresentationNetwork
+    cfg = load_config("config_c4_mlp.yaml")
+    torch.manual_seed(seed)
+    ls = cfg.networks.latent_shape
+    return (RepresentationNetwork((2, 6, 7), ls, cfg.networks.representation).cuda(), DynamicsNetwork(ls, 7, cfg.networks.dynamics).cuda(),
+            PredictionNetwork(ls, 7, cfg.networks.prediction).cuda())
+
+
+def _batch(B, w=5, seed=0):
+    from muzero_amd.learner import WindowBatch
+    g = torch.Generator().manual_seed(seed)
+    return WindowBatch(torch.randn(B, 3, 6, 7, generator=g), torch.randint(0, 7, (B, w + 1), generator=g),
+                       torch.softmax(torch.randn(B, w + 1, 7, generator=g), -1), torch.randn(B, w + 1, generator=g),
+                       torch.randn(B, w + 1, generator=g), torch.rand(B, generator=g) + 0.1).to("cuda")
+
+
+class _PlainCheckpoint(torch.autograd.Function):
+    """A relu or linear layer whose weight gradient reads its input back from codes, in elementary float32 operations."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, relu):
+        y = torch.nn.functional.linear(x, weight, bias)
+        y = torch.relu(y) if relu else y
+        q, s = _codes64(x, 3)
+        ctx.save_for_backward(torch.from_numpy((q * s[:, None]).astype(np.float32)).cuda(), weight, y)
+        ctx.relu = relu
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        xh, weight, y = ctx.saved_tensors
+        dz = dy * (y > 0) if ctx.relu else dy
+        return dz @ weight, dz.t() @ xh, dz.sum(0), None
+
+
+def test_unroll_with_checkpoints(monkeypatch):
+    """Same loss bit for bit, and the gradients of the same unroll with every dense layer replaced by the plain form of a
+    checkpointed one: what differs then is float32 rounding.  A gradient passes at most 6 steps of 4 products of at most
+    512 terms, each off by at most (512 + 8) u of its magnitudes: 24 * 520 * 2^-24 = 7.5e-4."""
+    import muzero_amd.checkpoints as ck
+    from muzero_amd.learner import batched_unroll_loss
+    nets = _networks()
+    batch = _batch(96)
+    params = [p for n in nets for p in n.parameters()]
+    keys = [list(n.state_dict()) for n in nets]
+    loss, per_window, _ = batched_unroll_loss(*nets, batch, 5)
+    loss8, per_window8, _ = batched_unroll_loss(*nets, batch, 5, checkpoints8=True)
+    got = torch.autograd.grad(loss8, params)
+    assert torch.equal(loss, loss8) and torch.equal(per_window, per_window8)
+    assert keys == [list(n.state_dict()) for n in nets] and all("forward" not in m.__dict__ for n in nets for m in n.modules())
+    calls = []
+    monkeypatch.setattr(ck, "checkpointed_linear",
+                        lambda x, w, b, act="none": (calls.append(act), _PlainCheckpoint.apply(x, w, b, act == "relu"))[1])
+    want = torch.autograd.grad(batched_unroll_loss(*nets, batch, 5, checkpoints8=True)[0], params)
+    assert len(calls) == 6 * (3 + 3) + 5 * (1 + 2)     # f six times (two heads of three layers), g five times
+    for p, a, b in zip(params, want, got):
+        assert float((a - b).norm()) <= 7.5e-4 * float(a.norm()), p.shape
+
+
+def test_recorded_learner_step_with_checkpoints():
+    from muzero_amd.learner import DataParallelLearner
+
+    def make():
+        nets = _networks(3)
+        return DataParallelLearner(*nets, torch.optim.Adam([p for n in nets for p in n.parameters()], lr=1e-3, capturable=True), 5,
+                                   checkpoints8=True)
+    eager, recorded = make(), make()
+    for step in range(4):
+        b = _batch(64, seed=step)
+        l0, pw0 = eager.step_local(b)
+        l1, pw1 = recorded.step_local_recorded(b)
+        assert abs(l0 - float(l1)) <= 1e-5 * abs(l0)
+        np.testing.assert_allclose(pw0, pw1.cpu(), rtol=1e-4)
+    for p, q in zip(eager.params, recorded.params):
+        np.testing.assert_allclose(p.detach().cpu(), q.detach().cpu(), atol=2e-5)
+    s = eager.policy_report(_batch(64), top=3)
+    assert s.log_prob.shape == (64,) and s.top_actions.shape == (64, 3) and s.entropy.isfinite().all()
+
+
+def test_heads_in_8_bits_and_their_scores():
+    """The operators in a row, as a server uses them: a policy head in 8-bit integers and the scores of its moves.  The
+    codes of x and W are off by at most half a step of 1/127 of a row's largest value each."""
+    from muzero_amd.policy_scores import policy_scores
+    from muzero_amd.quantized import Int8MLP, quantize_rows
+    _, _, f = _networks(1)
+    head = Int8MLP(f.policy_mlp)
+    lat = torch.randn(200, 4, 6, 7, device="cuda")
+    act = torch.randint(0, 7, (200,), device="cuda")
+    with torch.no_grad():
+        want = f.policy_logits(lat)
+        got = head.logits(lat.reshape(200, -1))
+        assert float((got - want).abs().max()) <= 0.05 * float(want.abs().max())
+        assert torch.equal(head.logits(quantize_rows(lat.reshape(200, -1))), got)
+        s = policy_scores(got, act, top=7)
+        np.testing.assert_allclose(s.log_prob.exp().cpu(), head(lat.reshape(200, -1)).gather(1, act[:, None])[:, 0].cpu(), rtol=1e-5)
+        with torch.no_grad():
+            f.policy_mlp[0].weight.mul_(2.0)
+        head.refresh()
+        assert not torch.equal(head.logits(lat.reshape(200, -1)), got)
+
+
+def test_other_streams_and_replayed_graphs():
+    from muzero_amd.checkpoints import save_activations, weight_grad
+    from muzero_amd.quantized import int8_linear, quantize_rows
+    R, K, N = 100, 400, 300
+    x, dz = torch.randn(R, K, device="cuda"), torch.randn(R, N, device="cuda")
+    qw = quantize_rows(torch.randn(N, K, device="cuda"))
+
+    def step():
+        saved = save_activations(x)
+        return (int8_linear(x, qw, activation="tanh"), int8_linear(x[:2], qw), saved.dequantize()) + weight_grad(dz, saved)
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step())
+    for turn in range(3):
+        x.normal_(), dz.normal_()
+        want = step()
+        for gr, out in zip(graphs, outs):
+            gr.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(want, out)), turn
+
+
+def test_offsets_past_32_bits():
+    from muzero_amd.checkpoints import save_activations
+    R, K = 140000, 16384  # 2.3e9 values
+    x = torch.zeros(R, K, dtype=torch.bfloat16, device="cuda")
+    tail = _x(3, K, torch.bfloat16)
+    x[-3:] = tail
+    c, d = save_activations(x), save_activations(tail)
+    assert torch.equal(c.codes[-3:], d.codes) and torch.equal(c.scales[-3:], d.scales) and (c.scales[:-3] == 0).all()
+    assert torch.equal(c.dequantize()[-3:], d.dequantize())

@@ -1,0 +1,197 @@
+"""Argument checks of the row operators (policy scores, 8-bit codes, products and checkpoints): everything here is
+refused on the host, before anything reaches a GPU."""
+import pytest
+import torch
+
+from muzero_amd import _hip
+
+P = 0x1000   # a pointer no call below gets as far as using
+F32, BF16 = _hip.TYPE_F32, _hip.TYPE_BF16
+
+
+def _refused(rc, *words):
+    assert rc < 0
+    msg = _hip.lib().mz_last_error().decode()
+    assert all(w in msg for w in words), msg
+
+
+def test_policy_scores_refusals():
+    f = _hip.lib().mz_policy_scores
+
+    def call(logits=P, kind=F32, ld=8, actions=P, T=4, V=7, top=2, lp=P, ent=P, stats=P, ids=P, tlp=P):
+        return f(logits, kind, ld, actions, T, V, top, lp, ent, stats, ids, tlp, None, 0, None)
+    _refused(call(kind=9), "type")
+    _refused(call(V=0), "V=0")
+    _refused(call(T=-1), "T=-1")
+    _refused(call(top=33, V=50, ld=50), "top=33")
+    _refused(call(top=8), "top=8", "V=7")
+    _refused(call(top=-1), "top=-1")
+    _refused(call(ld=6), "stride")
+    _refused(call(logits=None), "NULL")
+    _refused(call(logits=P + 2), "misaligned")
+    _refused(call(ent=None), "NULL")
+    _refused(call(stats=None), "NULL")
+    _refused(call(lp=None), "NULL")
+    _refused(call(ids=None), "NULL")
+    _refused(call(tlp=None), "NULL")
+    assert call(T=0, logits=None, ent=None) == 0
+    b = _hip.lib().mz_policy_scores_backward
+
+    def back(logits=P, ld=7, actions=P, T=4, V=7, top=2, stats=P, ent=P, ids=P, g=P, gh=P, gt=P, grad=P, ldg=7):
+        return b(logits, F32, ld, actions, T, V, top, stats, ent, ids, g, gh, gt, grad, ldg, None)
+    _refused(back(grad=None), "NULL")
+    _refused(back(ldg=5), "stride")
+    _refused(back(stats=None), "NULL")
+    _refused(back(ent=None), "NULL")
+    _refused(back(ids=None), "NULL")
+    _refused(back(actions=None), "NULL")
+    assert back(T=0, logits=None, grad=None) == 0
+    large = _hip.lib().mz_policy_scores_workspace(F32, 2, 200000, 32)
+    if large:
+        _refused(f(P, F32, 200000, P, 2, 200000, 32, P, P, P, P, P, None, 0, None), "workspace")
+        _refused(f(P, F32, 200000, P, 2, 200000, 32, P, P, P, P, P, P, large - 1, None), "workspace")
+
+
+def test_row_code_refusals():
+    q, d = _hip.lib().mz_quant8_rows, _hip.lib().mz_dequant8_rows
+
+    def quant(x=P, kind=F32, ldx=100, rows=4, K=100, bits=24, codes=P, ldc=128, scales=P):
+        return q(x, kind, ldx, rows, K, bits, codes, ldc, scales, None)
+    _refused(quant(kind=-1), "type")
+    _refused(quant(K=0), "K=0")
+    _refused(quant(rows=-1), "rows=-1")
+    _refused(quant(ldx=99), "stride")
+    _refused(quant(bits=8), "scale_bits")
+    _refused(quant(x=None), "NULL")
+    _refused(quant(codes=None), "NULL")
+    _refused(quant(scales=None), "NULL")
+    _refused(quant(ldc=96), "stride 96")
+    _refused(quant(ldc=120), "stride 120")
+    _refused(quant(codes=P + 8), "aligned")
+    _refused(quant(x=P + 2), "misaligned")
+    assert quant(rows=0, x=None, codes=None, scales=None) == 0
+    _refused(d(P, 128, P, 4, 100, P, 7, 100, None), "type")
+    _refused(d(P, 128, P, 4, 100, P, F32, 99, None), "stride")
+    _refused(d(P, 128, None, 4, 100, P, F32, 100, None), "NULL")
+    _refused(d(P, 96, P, 4, 100, P, F32, 100, None), "stride 96")
+
+
+def test_int8_refusals():
+    lib = _hip.lib()
+    need = lib.mz_int8_workspace(4, 100, 50)
+    assert need >= 4 * 128 + 16
+
+    def fwd(x=P, kind=F32, ldx=100, rows=4, K=100, w=P, ldw=128, ws=P, N=50, act=0, y=P, ykind=F32, ldy=50, work=P, nwork=need):
+        return lib.mz_int8_forward(x, kind, ldx, rows, K, w, ldw, ws, N, None, act, y, ykind, ldy, work, nwork, None)
+
+    def coded(x=P, ldx=128, xs=P, rows=4, K=100, w=P, ldw=128, ws=P, N=50, act=0, y=P, ykind=F32, ldy=50):
+        return lib.mz_int8_forward_codes(x, ldx, xs, rows, K, w, ldw, ws, N, None, act, y, ykind, ldy, P, 1 << 40, None)
+    for f in (fwd, coded):
+        _refused(f(rows=-1), "rows=-1")
+        _refused(f(K=0), "K=0")
+        _refused(f(N=0), "N=0")
+        _refused(f(w=None), "NULL")
+        _refused(f(ws=None), "NULL")
+        _refused(f(ldw=112), "128 bytes")
+        _refused(f(w=P + 4), "aligned")
+        _refused(f(act=4), "element-wise")
+        _refused(f(ykind=5), "type")
+        _refused(f(x=None), "NULL")
+        _refused(f(y=None), "NULL")
+        _refused(f(ldy=49), "stride 49")
+        assert f(rows=0, x=None, y=None) == 0
+    _refused(fwd(K=131073, ldx=131073, ldw=131200, nwork=1 << 40), "32-bit")
+    _refused(coded(K=131073, ldx=131200, ldw=131200), "32-bit")
+    _refused(fwd(kind=3), "type")
+    _refused(fwd(ldx=99), "stride")
+    _refused(fwd(work=None), "workspace")
+    _refused(fwd(nwork=need - 1), "workspace")
+    _refused(fwd(work=P + 8), "workspace")
+    _refused(coded(xs=None), "NULL")
+    _refused(coded(ldx=64), "128 bytes")
+
+
+def test_checkpoint_refusals():
+    lib = _hip.lib()
+    RELU, TANH = _hip.ACT["relu"], _hip.ACT["tanh"]
+    assert lib.mz_ckpt8_act_bytes(9, RELU) == 2 and lib.mz_ckpt8_act_bytes(9, TANH) == 9 and lib.mz_ckpt8_act_bytes(9, 0) == 0
+    _refused(lib.mz_ckpt8_act_save(P, F32, 9, 4, 9, 0, P, None), "activation")
+    _refused(lib.mz_ckpt8_act_save(P, F32, 9, 4, 9, RELU, None, None), "NULL")
+    _refused(lib.mz_ckpt8_act_save(P, F32, 8, 4, 9, RELU, P, None), "stride")
+    _refused(lib.mz_ckpt8_act_grad(P, F32, 9, None, 4, 9, RELU, P, 9, None), "NULL")
+    _refused(lib.mz_ckpt8_act_grad(P, F32, 9, P, 4, 9, 4, P, 9, None), "activation")
+    _refused(lib.mz_ckpt8_act_grad(P, F32, 9, P, 4, 9, RELU, None, 9, None), "NULL")
+    need = lib.mz_ckpt8_workspace(F32, 3, 4, 50, 100)
+    assert need > 0 and lib.mz_ckpt8_workspace(F32, 3, 0, 50, 100) == 0
+
+    def grad(dz=P, kind=F32, ldz=50, rows=4, N=50, codes=P, ldc=128, scales=P, bits=3, K=100, dw=P, ldw=100, db=P, work=P, nwork=need):
+        return lib.mz_ckpt8_weight_grad(dz, kind, ldz, rows, N, codes, ldc, scales, bits, K, dw, ldw, db, work, nwork, None)
+    _refused(grad(rows=0), "rows=0")
+    _refused(grad(rows=(1 << 28) + 1), "rows")
+    _refused(grad(N=0), "N=0")
+    _refused(grad(K=-1), "K=-1")
+    _refused(grad(kind=3), "type")
+    _refused(grad(bits=7), "scale_bits")
+    for name in ("dz", "codes", "scales", "dw"):
+        _refused(grad(**{name: None}), "NULL")
+    _refused(grad(ldz=49), "stride")
+    _refused(grad(ldw=99), "stride")
+    _refused(grad(ldc=96), "stride")
+    _refused(grad(dw=P + 2), "alignment")
+    _refused(grad(work=None), "workspace")
+    _refused(grad(nwork=need - 1), "workspace")
+
+
+def test_python_refusals():
+    from muzero_amd.checkpoints import checkpointed_linear, save_activations, weight_grad
+    from muzero_amd.policy_scores import policy_scores
+    from muzero_amd.quantized import QuantizedRows, int8_linear, quantize_rows
+    z = torch.zeros(3, 5)
+    for call in (lambda: policy_scores(z), lambda: quantize_rows(z), lambda: save_activations(z), lambda: checkpointed_linear(z, z)):
+        with pytest.raises(_hip.HipError, match="GPU"):   # no CPU fallback
+            call()
+    for call in (lambda: policy_scores(z.double()), lambda: quantize_rows(z.long()), lambda: policy_scores([1.0]),
+                 lambda: checkpointed_linear(z.double(), z)):
+        with pytest.raises(TypeError):
+            call()
+    coded = QuantizedRows(torch.zeros(4, 128, dtype=torch.int8), torch.zeros(4), torch.Size((4, 100)), torch.float32, 24)
+    rows = QuantizedRows(torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2), torch.Size((2, 99)), torch.float32, 24)
+    with pytest.raises(ValueError, match="99"):
+        int8_linear(rows, coded)
+    with pytest.raises(TypeError, match="QuantizedRows"):
+        int8_linear(rows, torch.zeros(4, 99))
+    rows = QuantizedRows(torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2), torch.Size((2, 100)), torch.float32, 24)
+    with pytest.raises(ValueError, match="activation"):
+        int8_linear(rows, coded, activation="softmax")
+    with pytest.raises(TypeError, match="out_dtype"):
+        int8_linear(rows, coded, out_dtype=torch.float64)
+    with pytest.raises(ValueError, match="bias"):
+        int8_linear(rows, coded, bias=torch.zeros(5))
+    with pytest.raises(_hip.HipError, match="GPU"):
+        weight_grad(torch.zeros(2, 3), rows)
+
+
+def test_dense_sequences_are_recognised():
+    from muzero_amd.checkpoints import eight_bit_checkpoints
+    from muzero_amd.config import DenseLayerConfig, load_config
+    from muzero_amd.neural_networks import DynamicsNetwork, PredictionNetwork
+    from muzero_amd.neural_networks.network_builder import build_mlp, dense_pairs, is_dense_sequence
+    seq, _ = build_mlp([DenseLayerConfig(out_features=8), DenseLayerConfig(out_features=3, activation="softmax")], 5)
+    assert [a for _, a in dense_pairs(seq)] == ["relu", "softmax"]
+    for bad in (torch.nn.Sequential(), torch.nn.Sequential(torch.nn.Linear(2, 2)), torch.nn.Sequential(torch.nn.Conv2d(1, 1, 1), torch.nn.ReLU())):
+        assert not is_dense_sequence(bad)
+        with pytest.raises(ValueError):
+            dense_pairs(bad)
+    cfg = load_config("config_c4_mlp.yaml")
+    g = DynamicsNetwork(cfg.networks.latent_shape, 7, cfg.networks.dynamics)
+    f = PredictionNetwork(cfg.networks.latent_shape, 7, cfg.networks.prediction)
+    lat, act = torch.randn(3, *cfg.networks.latent_shape), torch.tensor([0, 3, 6])
+    want = g(lat, act) + f(lat)
+    with eight_bit_checkpoints(g, f) as outer:   # on the CPU the layers run as they are
+        assert len(outer.sequences) == 3 and len(outer.merges) == 1
+        with eight_bit_checkpoints(g, f):
+            got = g(lat, act) + f(lat)
+        assert "merge" in g.__dict__
+    assert "merge" not in g.__dict__ and "forward" not in f.policy_mlp.__dict__
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    torch.testing.assert_close(torch.softmax(f.policy_logits(lat), 1), f(lat)[0])
