@@ -14,106 +14,406 @@ namespace {
 
 using namespace mze;
 
-constexpr int kST = 256;
 constexpr int kMaxTop = 32;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.402823466e38f;
 
-struct Sums {  // running maximum, sum of e^(z - m) and of e^(z - m) (z - m)
+// e^d for d <= 0 (or NaN): the exponent is rounded once, so the result is off by |d| u and one unit.
+__device__ __forceinline__ float exp_le0(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// Running maximum and sums of a set of logits.  m starts at the lowest finite value, not at -inf: z - m is then -inf for
+// a masked logit (e = 0) and never inf - inf.  s == 0 says that nothing but masked logits was met, since the largest
+// live one contributes e^0 = 1.
+struct Sums {
     float m, s, u;
 };
 
-__device__ __forceinline__ Sums none() { return {-INFINITY, 0.0f, 0.0f}; }
+__device__ __forceinline__ Sums none() { return {kLowest, 0.0f, 0.0f}; }
 
-// The sums of two disjoint sets of logits relative to the larger maximum: with d = m_old - m_new <= 0,
-// S' = S e^d and U' = e^d (U + d S).  An empty (or fully masked) side has m = -inf and S = 0.
+// u's share of one logit: e (z - m), with 0 * -inf read as 0 (a NaN is in s already)
+__device__ __forceinline__ float share(float e, float d) { return e * fmaxf(d, -1e30f); }
+
+// The sums of two disjoint sets relative to the larger maximum: with d = m_old - m_new <= 0,
+// S' = S e^d and U' = e^d (U + d S).
 __device__ __forceinline__ Sums join(const Sums &a, const Sums &b) {
-    const float m = fmaxf(a.m, b.m);
-    if (m == -INFINITY) return {m, a.s + b.s, a.u + b.u};  // nothing but masked logits, or NaN sums
-    const float da = a.m == -INFINITY ? -INFINITY : a.m - m, db = b.m == -INFINITY ? -INFINITY : b.m - m;
-    const float ea = expf(da), eb = expf(db);
-    // 0 * -inf would be NaN: an empty side adds nothing
-    const float ua = a.s == 0.0f ? 0.0f : ea * (a.u + fmaxf(da, -1e30f) * a.s);
-    const float ub = b.s == 0.0f ? 0.0f : eb * (b.u + fmaxf(db, -1e30f) * b.s);
-    return {m, (a.s == 0.0f ? 0.0f : a.s * ea) + (b.s == 0.0f ? 0.0f : b.s * eb), ua + ub};
+    const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m;
+    const float ea = exp_le0(da), eb = exp_le0(db);
+    return {m, a.s * ea + b.s * eb, ea * a.u + share(ea, da) * a.s + eb * b.u + share(eb, db) * b.s};
 }
 
-__device__ __forceinline__ Sums one(float z) {
-    if (z != z) return {-INFINITY, z, z};
-    if (z == -INFINITY) return none();
-    if (z == INFINITY) return {z, NAN, NAN};
-    return {z, 1.0f, 0.0f};
+struct Row {  // what follows from the sums of a whole row
+    float m, log_s, h;
+    bool empty, loud;  // nothing but masked logits; a NaN or +inf among them
+};
+
+__device__ __forceinline__ Row row_of(const Sums &a) {
+    Row r;
+    r.empty = a.s == 0.0f;
+    r.loud = a.s != a.s;
+    r.m = r.empty ? -INFINITY : a.m;
+    r.log_s = r.empty ? 0.0f : logf(a.s);
+    r.h = r.empty ? 0.0f : r.log_s - a.u / a.s;
+    return r;
 }
 
-// Order of the alternatives as one unsigned 64-bit key: the larger key comes first.
-__device__ __forceinline__ unsigned long long order_key(float z, unsigned j) {
+__device__ __forceinline__ float log_p(const Row &r, float z) { return r.empty ? -INFINITY : (z - r.m) - r.log_s; }
+
+// Order of the alternatives as one unsigned 64-bit key (value, then lowest index): the larger key comes first, 0 is none.
+__device__ __forceinline__ unsigned order_bits(float z) {
     z = z + 0.0f;  // -0 -> 0
-    unsigned b = z != z ? 0x7FC00000u : __float_as_uint(z);
-    b ^= (b & 0x80000000u) ? 0xFFFFFFFFu : 0x80000000u;
-    return ((unsigned long long)b << 32) | (unsigned)~j;
+    const unsigned b = z != z ? 0x7FC00000u : __float_as_uint(z);
+    return b ^ ((b & 0x80000000u) ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-__device__ __forceinline__ float key_value(unsigned long long k) {
-    unsigned b = (unsigned)(k >> 32);
-    b ^= (b & 0x80000000u) ? 0x80000000u : 0xFFFFFFFFu;
-    return __uint_as_float(b);
+using Key = unsigned long long;
+
+__device__ __forceinline__ Key order_key(float z, int j) { return ((Key)order_bits(z) << 32) | (unsigned)~j; }
+
+__device__ __forceinline__ float bits_value(unsigned b) { return __uint_as_float(b ^ ((b & 0x80000000u) ? 0x80000000u : 0xFFFFFFFFu)); }
+__device__ __forceinline__ float key_value(Key k) { return bits_value((unsigned)(k >> 32)); }
+__device__ __forceinline__ int key_index(Key k) { return (int)~(unsigned)k; }
+
+// Maximum over the 64 lanes (every lane gets it), by lane moves inside the vector unit.
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, true));   // row_shr:1
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, true));   // row_shr:2
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, true));   // row_shr:4
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, true));   // row_shr:8
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false));  // row_bcast:15
+    v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false));  // row_bcast:31
+    return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
 }
 
-// One workgroup per row; the alternatives are found one after the other, each in a pass over the row.
-template <class T>
-__global__ void __launch_bounds__(kST)
-k_scores(const T *__restrict__ logits, int64_t ld, const int64_t *__restrict__ actions, int64_t rows, int V, int top,
-         float *__restrict__ log_prob, float *__restrict__ entropy, float *__restrict__ stats,
-         int64_t *__restrict__ top_actions, float *__restrict__ top_log_probs) {
-    __shared__ Sums part[kST];
-    __shared__ unsigned long long keys[kST];
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        const T *z = logits + row * ld;
+__device__ __forceinline__ Key wave_max(Key k) {
+    const unsigned hi = wave_max((unsigned)(k >> 32));
+    const unsigned lo = wave_max((unsigned)(k >> 32) == hi ? (unsigned)k : 0u);
+    return ((Key)hi << 32) | lo;
+}
+
+struct Out {  // the result arrays of a call
+    const int64_t *actions;
+    float *log_prob, *entropy, *stats;
+    int64_t *top_actions;
+    float *top_log_probs;
+    int V, top;
+
+    template <class T>
+    __device__ void row(int64_t row, const Row &r, const T *z) const {
+        stats[2 * row] = r.m;
+        stats[2 * row + 1] = r.log_s;
+        entropy[row] = r.h;
+        if (!actions) return;
+        const int64_t a = actions[row];
+        log_prob[row] = a < 0 ? 0.0f : a >= V ? NAN : log_p(r, (float)z[a]);
+    }
+    __device__ void alternative(int64_t row, int i, const Row &r, Key k) const {
+        top_actions[row * top + i] = key_index(k);
+        top_log_probs[row * top + i] = log_p(r, key_value(k));
+    }
+};
+
+// ---------------------------------------------------------------- rows of up to 1024 logits: a row stays in registers
+// LANES lanes per row, E logits per lane (logit e * LANES + lane), 256 / LANES rows per workgroup.
+template <class T, int LANES, int E>
+__global__ void __launch_bounds__(256)
+k_scores_small(const T *__restrict__ logits, int64_t ld, int64_t rows, Out out) {
+    const int lane = threadIdx.x % LANES, V = out.V;
+    for (int64_t row0 = (int64_t)blockIdx.x * (256 / LANES); row0 < rows; row0 += (int64_t)gridDim.x * (256 / LANES)) {
+        const int64_t row = row0 + threadIdx.x / LANES;
+        const bool live = row < rows;
+        const T *z = logits + (live ? row : 0) * ld;
+        float v[E];
         Sums acc = none();
-        for (int j = threadIdx.x; j < V; j += kST) acc = join(acc, one((float)z[j]));
-        __syncthreads();
-        part[threadIdx.x] = acc;
-        __syncthreads();
-        for (int k = kST / 2; k > 0; k >>= 1) {
-            if ((int)threadIdx.x < k) part[threadIdx.x] = join(part[threadIdx.x], part[threadIdx.x + k]);
-            __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int j = e * LANES + lane;
+            v[e] = j < V ? (float)z[j] : -INFINITY;
+            acc.m = fmaxf(acc.m, v[e]);
         }
-        acc = part[0];
-        const bool empty = acc.m == -INFINITY && acc.s == 0.0f;
-        const float log_s = logf(acc.s);
-        if (threadIdx.x == 0) {
-            stats[2 * row] = empty ? -INFINITY : acc.m;
-            stats[2 * row + 1] = empty ? 0.0f : log_s;
-            entropy[row] = empty ? 0.0f : log_s - acc.u / acc.s;
-            if (actions) {
-                const int64_t a = actions[row];
-                float lp = 0.0f;
-                if (a >= V) lp = NAN;
-                else if (a >= 0) lp = empty ? -INFINITY : ((float)z[a] - acc.m) - log_s;
-                log_prob[row] = lp;
-            }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) acc.m = fmaxf(acc.m, __shfl_xor(acc.m, o));
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const float d = v[e] - acc.m, x = exp_le0(d);
+            acc.s += x;
+            acc.u += share(x, d);
         }
-        unsigned long long last = ~0ull;
-        for (int i = 0; i < top; ++i) {
-            unsigned long long best = 0;
-            for (int j = threadIdx.x; j < V; j += kST) {
-                const unsigned long long key = order_key((float)z[j], (unsigned)j);
-                if (key < last && key > best) best = key;
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            acc.s += __shfl_xor(acc.s, o);
+            acc.u += __shfl_xor(acc.u, o);
+        }
+        const Row r = row_of(acc);
+        if (live && lane == 0) out.row(row, r, z);
+        Key last = ~0ull;
+        for (int i = 0; i < out.top; ++i) {
+            Key best = 0;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int j = e * LANES + lane;
+                const Key k = j < V ? order_key(v[e], j) : 0;
+                if (k < last && k > best) best = k;
             }
-            keys[threadIdx.x] = best;
-            __syncthreads();
-            for (int k = kST / 2; k > 0; k >>= 1) {
-                if ((int)threadIdx.x < k && keys[threadIdx.x + k] > keys[threadIdx.x]) keys[threadIdx.x] = keys[threadIdx.x + k];
-                __syncthreads();
+#pragma unroll
+            for (int o = LANES / 2; o > 0; o >>= 1) {
+                const Key k = __shfl_xor(best, o);
+                if (k > best) best = k;
             }
-            last = keys[0];
-            if (threadIdx.x == 0) {
-                top_actions[row * top + i] = (int64_t)(unsigned)~(unsigned)last;
-                top_log_probs[row * top + i] = empty ? -INFINITY : (key_value(last) - acc.m) - log_s;
-            }
-            __syncthreads();
+            last = best;
+            if (live && lane == 0) out.alternative(row, i, r, last);
         }
     }
 }
 
+// ---------------------------------------------------------------- long rows: a workgroup streams a row, or a part of it
+constexpr int kLT = 256;          // threads
+constexpr int kCand = 1024;       // candidates for the alternatives that a workgroup can hold
+constexpr int kMaxParts = 64;     // parts of one row (one lane of the joining wave each)
+
+// The logits [lo, hi) of a row as 16-byte packs that lie on 16-byte addresses, whatever the row's own alignment: pack i
+// holds the logits first + i n .. + n - 1, of which the first and last pack may only own some.
+template <class T>
+struct Span {
+    static constexpr int n = Pack<T>::n;
+    const T *z;
+    int lo, hi, first, packs;
+
+    __device__ Span(const T *row, int lo_, int hi_) : z(row), lo(lo_), hi(hi_) {
+        first = lo - (int)(((uintptr_t)(row + lo) & 15) / sizeof(T));
+        packs = (hi - first + n - 1) / n;
+    }
+    __device__ __forceinline__ int at(int i) const { return first + i * n; }
+    __device__ __forceinline__ bool owns(int j) const { return j >= lo && j < hi; }
+    __device__ __forceinline__ void load(int i, float (&v)[n]) const {
+        const int j = at(i);
+        if (j >= lo && j + n <= hi) {
+            const Pack<T> p = *(const Pack<T> *)(z + j);
+#pragma unroll
+            for (int e = 0; e < n; ++e) v[e] = (float)p.v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < n; ++e) v[e] = owns(j + e) ? (float)z[j + e] : -INFINITY;
+        }
+    }
+};
+
+template <int N>
+__device__ __forceinline__ void add(Sums &a, const float (&v)[N]) {
+    float m = v[0];
+#pragma unroll
+    for (int e = 1; e < N; ++e) m = fmaxf(m, v[e]);
+    if (m > a.m) {
+        const float d = a.m - m, x = exp_le0(d);
+        a.u = x * a.u + share(x, d) * a.s;
+        a.s *= x;
+        a.m = m;
+    }
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const float d = v[e] - a.m, x = exp_le0(d);
+        a.s += x;
+        a.u += share(x, d);
+    }
+}
+
+struct Shared {
+    Sums part[kLT / 64];
+    Key cand[kCand];
+    unsigned best[kLT];
+    Key thread_key[kLT];
+    Key found[kMaxTop];
+    Key threshold;
+    int count;
+};
+
+// Largest value t (its low 16 order bits dropped) that at least `top` of the workgroup's threads reach with their own
+// largest logit: at least `top` logits are >= t, so no smaller one is an alternative.  Every wave finds it by itself.
+__device__ __forceinline__ float value_threshold(const Shared &sh, int top) {
+    const int lane = threadIdx.x & 63;
+    unsigned b[kLT / 64], t = 0;
+#pragma unroll
+    for (int w = 0; w < kLT / 64; ++w) b[w] = sh.best[w * 64 + lane];
+    for (int bit = 31; bit >= 16; --bit) {
+        const unsigned probe = t | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int w = 0; w < kLT / 64; ++w) n += __popcll(__ballot(b[w] >= probe));
+        if (n >= top) t = probe;
+    }
+    return t <= order_bits(-INFINITY) ? -INFINITY : bits_value(t);
+}
+
+// The candidates in sh.cand, ranked: the `top` first ones go to sh.found in order.
+__device__ __forceinline__ void rank_candidates(Shared &sh, int count, int top) {
+    for (int c = threadIdx.x; c < count; c += kLT) {
+        const Key k = sh.cand[c];
+        int rank = 0;
+        for (int o = 0; o < count; ++o) rank += sh.cand[o] > k;
+        if (rank < top) sh.found[rank] = k;
+    }
+    __syncthreads();
+}
+
+// sh.found = the `top` first alternatives among the logits of `span` (at least `top` of them), which every thread has
+// streamed in the order of add(): its own largest one is in sh.best.  `loud`: there is a NaN or an infinity.
+//  1. candidates are the logits that reach value_threshold; only the packs of threads that reach it are read again, each
+//     such thread's by its whole wave;
+//  2. rows with too many equal values for that (all masked, all equal): the same with (value, index) keys;
+//  3. whatever overflows that, too: one alternative per pass.
+template <class T>
+__device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool loud) {
+    constexpr int n = Span<T>::n;
+    const int lane = threadIdx.x & 63, wave0 = threadIdx.x & ~63;
+    float v[n];
+    const auto collect = [&](bool mine, auto &&wanted) {
+        for (unsigned long long left = __ballot(mine); left; left &= left - 1) {
+            const int owner = wave0 + __builtin_ctzll(left);
+            for (int i = owner + lane * kLT; i < span.packs; i += 64 * kLT) {
+                span.load(i, v);
+#pragma unroll
+                for (int e = 0; e < n; ++e) {
+                    const int j = span.at(i) + e;
+                    if (span.owns(j) && wanted(v[e], j)) {
+                        const int c = atomicAdd(&sh.count, 1);
+                        if (c < kCand) sh.cand[c] = order_key(v[e], j);
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        return sh.count;
+    };
+    int count = kCand + 1;
+    if (!loud) {
+        const float t = value_threshold(sh, top);
+        if (threadIdx.x == 0) sh.count = 0;
+        __syncthreads();
+        count = collect(sh.best[threadIdx.x] >= order_bits(t), [&](float z, int) { return z >= t; });
+        if (count > kCand) {
+            Key mine = 0;
+            for (int i = threadIdx.x; i < span.packs; i += kLT) {
+                span.load(i, v);
+#pragma unroll
+                for (int e = 0; e < n; ++e) {
+                    const int j = span.at(i) + e;
+                    const Key k = span.owns(j) ? order_key(v[e], j) : 0;
+                    if (k > mine) mine = k;
+                }
+            }
+            __syncthreads();  // everybody has read sh.count
+            sh.thread_key[threadIdx.x] = mine;
+            if (threadIdx.x == 0) sh.count = 0, sh.threshold = 0;  // fewer owning threads than top: everything
+            __syncthreads();
+            int rank = 0;
+            for (int o = 0; o < kLT; ++o) rank += sh.thread_key[o] > mine;
+            if (rank == top - 1 && mine != 0) sh.threshold = mine;
+            __syncthreads();
+            const Key t2 = sh.threshold;
+            count = collect(mine >= t2, [&](float z, int j) { return order_key(z, j) >= t2; });
+        }
+    }
+    if (count <= kCand) {
+        rank_candidates(sh, count, top);
+        return;
+    }
+    Key last = ~0ull;
+    for (int a = 0; a < top; ++a) {
+        Key best = 0;
+        for (int i = threadIdx.x; i < span.packs; i += kLT) {
+            span.load(i, v);
+#pragma unroll
+            for (int e = 0; e < n; ++e) {
+                const int j = span.at(i) + e;
+                const Key k = span.owns(j) ? order_key(v[e], j) : 0;
+                if (k < last && k > best) best = k;
+            }
+        }
+        best = wave_max(best);
+        __syncthreads();
+        if (lane == 0) sh.thread_key[threadIdx.x >> 6] = best;
+        __syncthreads();
+        last = sh.thread_key[0];
+        for (int w = 1; w < kLT / 64; ++w) last = max(last, sh.thread_key[w]);
+        if (threadIdx.x == 0) sh.found[a] = last;
+    }
+    __syncthreads();
+}
+
+// Workgroup (row, part).  One part: the results.  Several: the part's sums and alternatives to the workspace.
+template <class T>
+__global__ void __launch_bounds__(kLT)
+k_scores_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts, Out out, Sums *__restrict__ part_sums,
+              Key *__restrict__ part_keys) {
+    __shared__ Shared sh;
+    constexpr int n = Span<T>::n;
+    const int top = out.top;
+    for (int64_t job = blockIdx.x; job < rows * parts; job += gridDim.x) {
+        const int64_t row = job / parts;
+        const int part = (int)(job - row * parts);
+        const T *z = logits + row * ld;
+        const Span<T> span(z, (int)((int64_t)out.V * part / parts), (int)((int64_t)out.V * (part + 1) / parts));
+        Sums acc = none();
+        int i = threadIdx.x;
+        for (; i + 3 * kLT < span.packs; i += 4 * kLT) {  // four loads in flight
+            float v0[n], v1[n], v2[n], v3[n];
+            span.load(i, v0);
+            span.load(i + kLT, v1);
+            span.load(i + 2 * kLT, v2);
+            span.load(i + 3 * kLT, v3);
+            add(acc, v0);
+            add(acc, v1);
+            add(acc, v2);
+            add(acc, v3);
+        }
+        for (; i < span.packs; i += kLT) {
+            float v0[n];
+            span.load(i, v0);
+            add(acc, v0);
+        }
+        __syncthreads();  // the last job's shared values have been read
+        sh.best[threadIdx.x] = order_bits(acc.s == 0.0f ? -INFINITY : acc.m);
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) acc = join(acc, {__shfl_xor(acc.m, o), __shfl_xor(acc.s, o), __shfl_xor(acc.u, o)});
+        if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = acc;
+        __syncthreads();
+        acc = sh.part[0];
+        for (int w = 1; w < kLT / 64; ++w) acc = join(acc, sh.part[w]);
+        const Row r = row_of(acc);
+        if (top > 0) find_alternatives(span, sh, top, r.loud);
+        if (parts == 1) {
+            if (threadIdx.x == 0) out.row(row, r, z);
+            if ((int)threadIdx.x < top) out.alternative(row, threadIdx.x, r, sh.found[threadIdx.x]);
+        } else {
+            if (threadIdx.x == 0) part_sums[job] = acc;
+            if ((int)threadIdx.x < top) part_keys[job * top + threadIdx.x] = sh.found[threadIdx.x];
+        }
+    }
+}
+
+// One wave per row: joins the sums of its parts in a fixed order and merges their lists, one lane per part.
+template <class T>
+__global__ void __launch_bounds__(64)
+k_scores_join(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts, Out out, const Sums *__restrict__ part_sums,
+              const Key *__restrict__ part_keys) {
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const int lane = threadIdx.x, top = out.top;
+        Sums acc = lane < parts ? part_sums[row * parts + lane] : none();
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) acc = join(acc, {__shfl_xor(acc.m, o), __shfl_xor(acc.s, o), __shfl_xor(acc.u, o)});
+        const Row r = row_of(acc);
+        if (lane == 0) out.row(row, r, logits + row * ld);
+        const Key *list = part_keys + (row * parts + lane) * top;
+        int next = 0;
+        Key head = top > 0 && lane < parts ? list[0] : 0;
+        for (int i = 0; i < top; ++i) {
+            const Key best = wave_max(head);
+            if (lane == 0) out.alternative(row, i, r, best);
+            if (head == best) head = ++next < top ? list[next] : 0;  // keys are unique: one lane moves on
+        }
+    }
+}
+
+// ---------------------------------------------------------------- gradient
 struct RowGrad {
     float m, log_s, h, g_lp, g_ent, g_sum;
     int64_t a;
@@ -121,53 +421,167 @@ struct RowGrad {
 };
 
 // The gradient of one logit without the [j = alternative] terms of the top list.
-__device__ __forceinline__ float grad_one(const RowGrad &r, float z, int64_t j) {
-    if (r.empty) return 0.0f;
-    const float lp = (z - r.m) - r.log_s;
-    const float p = expf(lp);
-    // p (log p + H) is 0 in the limit of p = 0; NaN stays NaN
+__device__ __forceinline__ float grad_one(const RowGrad &r, float z, int j) {
+    const float lp = (z - r.m) - r.log_s, p = exp_le0(lp);
+    // p (log p + H) is 0 in the limit of p = 0
     const float ent = p == 0.0f ? 0.0f : p * (lp + r.h);
-    return (j == r.a ? r.g_lp : 0.0f) - p * r.g_sum - r.g_ent * ent;
+    const float g = (j == r.a ? r.g_lp : 0.0f) - p * r.g_sum - r.g_ent * ent;
+    return r.empty ? 0.0f : g;
 }
 
-__device__ __forceinline__ RowGrad row_grad(const int64_t *actions, int64_t row, int V, int top, const float *stats,
-                                            const float *entropy, const float *g_lp, const float *g_ent, const float *g_top) {
-    RowGrad r;
-    r.m = stats[2 * row], r.log_s = stats[2 * row + 1], r.h = entropy[row];
-    r.empty = r.m == -INFINITY && r.log_s == 0.0f;
-    r.a = actions ? actions[row] : -1;
-    r.g_lp = g_lp && r.a >= 0 ? g_lp[row] : 0.0f;
-    if (r.a >= V) r.g_lp *= NAN;  // an action that does not exist: its score was NaN
-    r.g_ent = g_ent ? g_ent[row] : 0.0f;
-    r.g_sum = r.g_lp;
-    if (g_top)
-        for (int i = 0; i < top; ++i) r.g_sum += g_top[row * top + i];
-    return r;
+struct Grads {
+    const int64_t *actions;
+    const float *stats, *entropy;
+    const int64_t *top_actions;
+    const float *g_lp, *g_ent, *g_top;
+    int V, top;
+
+    __device__ RowGrad row(int64_t row) const {
+        RowGrad r;
+        r.m = stats[2 * row], r.log_s = stats[2 * row + 1], r.h = entropy[row];
+        r.empty = r.m == -INFINITY && r.log_s == 0.0f;
+        r.a = actions ? actions[row] : -1;
+        r.g_lp = g_lp && r.a >= 0 ? g_lp[row] : 0.0f;
+        if (r.a >= V) r.g_lp = NAN;  // an action that does not exist: its score was NaN
+        r.g_ent = g_ent ? g_ent[row] : 0.0f;
+        r.g_sum = r.g_lp;
+        if (g_top)
+            for (int i = 0; i < top; ++i) r.g_sum += g_top[row * top + i];
+        return r;
+    }
+};
+
+// Rows of up to 64 * E logits, LANES lanes per row.
+template <class T, int LANES>
+__global__ void __launch_bounds__(256)
+k_grad_small(const T *__restrict__ logits, int64_t ld, int64_t rows, Grads in, T *__restrict__ grad, int64_t ldg) {
+    const int lane = threadIdx.x % LANES;
+    const int64_t step = (int64_t)gridDim.x * (256 / LANES);
+    for (int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES; row < rows; row += step) {
+        const RowGrad r = in.row(row);
+        for (int j = lane; j < in.V; j += LANES) grad[row * ldg + j] = (T)grad_one(r, (float)logits[row * ld + j], j);
+    }
 }
+
+constexpr int kGradPacks = 4;  // packs per thread of a workgroup's piece of a long row
 
 template <class T>
-__global__ void __launch_bounds__(kST)
-k_scores_grad(const T *__restrict__ logits, int64_t ld, const int64_t *__restrict__ actions, int64_t rows, int V, int top,
-              const float *__restrict__ stats, const float *__restrict__ entropy, const int64_t *__restrict__ top_actions,
-              const float *__restrict__ g_lp, const float *__restrict__ g_ent, const float *__restrict__ g_top,
-              T *__restrict__ grad, int64_t ldg) {
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        const RowGrad r = row_grad(actions, row, V, top, stats, entropy, g_lp, g_ent, g_top);
-        for (int j = threadIdx.x; j < V; j += kST) {
-            float g = grad_one(r, (float)logits[row * ld + j], j);
-            if (g_top && !r.empty)
-                for (int i = 0; i < top; ++i)
-                    if (top_actions[row * top + i] == j) g += g_top[row * top + i];
-            grad[row * ldg + j] = (T)g;
+__global__ void __launch_bounds__(kLT)
+k_grad_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int pieces, Grads in, T *__restrict__ grad, int64_t ldg) {
+    constexpr int n = Span<T>::n;
+    for (int64_t job = blockIdx.x; job < rows * pieces; job += gridDim.x) {
+        const int64_t row = job / pieces;
+        const int piece = (int)(job - row * pieces);
+        const Span<T> span(logits + row * ld, 0, in.V);
+        T *out = grad + row * ldg;
+        // packs of the logits' alignment: stores are whole when the gradient's row has the same one
+        const bool whole = ((uintptr_t)(out + span.first) & 15) == 0;
+        const RowGrad r = in.row(row);
+        float v[kGradPacks][n];
+        const int i0 = piece * kGradPacks * kLT + threadIdx.x;
+#pragma unroll
+        for (int q = 0; q < kGradPacks; ++q)
+            if (i0 + q * kLT < span.packs) span.load(i0 + q * kLT, v[q]);
+#pragma unroll
+        for (int q = 0; q < kGradPacks; ++q) {
+            const int i = i0 + q * kLT, j = span.at(i);
+            if (i >= span.packs) break;
+            Pack<T> p;
+#pragma unroll
+            for (int e = 0; e < n; ++e) p.v[e] = (T)grad_one(r, v[q][e], j + e);
+            if (whole && j >= 0 && j + n <= in.V) {
+                *(Pack<T> *)(out + j) = p;
+            } else {
+#pragma unroll
+                for (int e = 0; e < n; ++e)
+                    if (span.owns(j + e)) out[j + e] = p.v[e];
+            }
         }
     }
 }
 
-dim3 row_grid(int64_t rows) { return dim3((unsigned)(rows < (1 << 20) ? rows : (1 << 20))); }
+// The logits that are alternatives, once more and with all their terms (after the kernels above, which leave those out):
+// one thread per (row, alternative).
+template <class T>
+__global__ void __launch_bounds__(256)
+k_grad_top(const T *__restrict__ logits, int64_t ld, int64_t rows, Grads in, T *__restrict__ grad, int64_t ldg) {
+    const int64_t n = rows * in.top;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
+        const int64_t row = t / in.top;
+        const int j = (int)in.top_actions[t];
+        const RowGrad r = in.row(row);
+        const float g = grad_one(r, (float)logits[row * ld + j], j);
+        grad[row * ldg + j] = (T)(r.empty ? 0.0f : g + in.g_top[t]);
+    }
+}
+
+constexpr int64_t kMaxGrid = 1 << 20;
+
+dim3 grid_of(int64_t n) { return dim3((unsigned)(n < kMaxGrid ? n : kMaxGrid)); }
+
+// Rows of more than kSmall logits are streamed; fewer rows than kFill workgroups are cut into parts of at least
+// kPartBytes, so that a short batch of long rows still reaches all 256 compute units.
+constexpr int kSmall = 1024, kFill = 1024, kPartBytes = 16384;
+
+int parts_of(int32_t type, int64_t T, int32_t V) {
+    if (V <= kSmall || T >= kFill) return 1;
+    const int64_t by_size = (int64_t)V * type_bytes(type) / kPartBytes, by_fill = (kFill + T - 1) / T;
+    const int64_t p = by_size < by_fill ? by_size : by_fill;
+    return (int)(p < 1 ? 1 : p > kMaxParts ? kMaxParts : p);
+}
+
+template <class T>
+void launch_scores(const T *logits, int64_t ld, int64_t rows, int parts, const Out &out, void *workspace, hipStream_t st) {
+    const auto small = [&](auto lanes, auto per_lane) {
+        constexpr int L = decltype(lanes)::value, E = decltype(per_lane)::value;
+        const int64_t per_group = 256 / L;
+        hipLaunchKernelGGL((k_scores_small<T, L, E>), grid_of((rows + per_group - 1) / per_group), dim3(256), 0, st, logits, ld,
+                           rows, out);
+    };
+    using std::integral_constant;
+    const int V = out.V;
+    if (V <= 8) return small(integral_constant<int, 8>{}, integral_constant<int, 1>{});
+    if (V <= 16) return small(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+    if (V <= 32) return small(integral_constant<int, 32>{}, integral_constant<int, 1>{});
+    if (V <= 64) return small(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    if (V <= 256) return small(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    if (V <= kSmall) return small(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    Key *keys = (Key *)workspace;
+    Sums *sums = (Sums *)(keys + (parts > 1 ? rows * parts * out.top : 0));
+    hipLaunchKernelGGL(k_scores_long<T>, grid_of(rows * parts), dim3(kLT), 0, st, logits, ld, rows, parts, out, sums, keys);
+    if (parts > 1)
+        hipLaunchKernelGGL(k_scores_join<T>, grid_of(rows), dim3(64), 0, st, logits, ld, rows, parts, out, (const Sums *)sums,
+                           (const Key *)keys);
+}
+
+template <class T>
+void launch_grad(const T *logits, int64_t ld, int64_t rows, const Grads &in, T *grad, int64_t ldg, hipStream_t st) {
+    const auto small = [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        const int64_t per_group = 256 / L;
+        hipLaunchKernelGGL((k_grad_small<T, L>), grid_of((rows + per_group - 1) / per_group), dim3(256), 0, st, logits, ld, rows,
+                           in, grad, ldg);
+    };
+    if (in.V <= 8) {
+        small(std::integral_constant<int, 8>{});
+    } else if (in.V <= 32) {
+        small(std::integral_constant<int, 32>{});
+    } else if (in.V <= kSmall) {
+        small(std::integral_constant<int, 64>{});
+    } else {
+        const int packs = (in.V + Pack<T>::n - 1) / Pack<T>::n + 1;  // a row that starts off a 16-byte address has one more
+        const int pieces = (packs + kGradPacks * kLT - 1) / (kGradPacks * kLT);
+        hipLaunchKernelGGL(k_grad_long<T>, grid_of(rows * pieces), dim3(kLT), 0, st, logits, ld, rows, pieces, in, grad, ldg);
+    }
+    if (in.g_top) {
+        const int64_t groups = (rows * in.top + 255) / 256;
+        hipLaunchKernelGGL(k_grad_top<T>, grid_of(groups), dim3(256), 0, st, logits, ld, rows, in, grad, ldg);
+    }
+}
 
 int check_logits(const char *what, const void *p, int32_t type, int64_t ld, int64_t T, int32_t V, int32_t top) {
     if (!type_ok(type)) return mz::fail(MZ_ERR_ARG, "%s: unknown element type %d", what, type);
-    if (T < 0 || T > 0x7FFFFFFF || V <= 0) return mz::fail(MZ_ERR_ARG, "%s: bad dimensions T=%lld V=%d", what, (long long)T, V);
+    if (T < 0 || T > 0x7FFFFFFF || V <= 0 || V > (1 << 30)) return mz::fail(MZ_ERR_ARG, "%s: bad dimensions T=%lld V=%d", what, (long long)T, V);
     if (top < 0 || top > kMaxTop || top > V)
         return mz::fail(MZ_ERR_ARG, "%s: top=%d must lie in 0..%d and not exceed V=%d", what, top, kMaxTop, V);
     if (ld < V) return mz::fail(MZ_ERR_ARG, "%s: row stride %lld below V=%d", what, (long long)ld, V);
@@ -181,8 +595,9 @@ int check_logits(const char *what, const void *p, int32_t type, int64_t ld, int6
 extern "C" {
 
 int64_t mz_policy_scores_workspace(int32_t type, int64_t T, int32_t V, int32_t top) {
-    (void)type, (void)T, (void)V, (void)top;
-    return 0;
+    if (!type_ok(type) || T <= 0 || V <= 0 || top < 0 || top > kMaxTop) return 0;
+    const int parts = parts_of(type, T, V);
+    return parts > 1 ? T * parts * ((int64_t)sizeof(Sums) + top * (int64_t)sizeof(Key)) : 0;
 }
 
 int mz_policy_scores(const void *logits, int32_t type, int64_t ld, const int64_t *actions, int64_t T, int32_t V, int32_t top,
@@ -196,10 +611,10 @@ int mz_policy_scores(const void *logits, int32_t type, int64_t ld, const int64_t
     if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
         return mz::fail(MZ_ERR_ARG, "mz_policy_scores: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
                         (long long)workspace_bytes);
+    const Out out{actions, log_prob, entropy, stats, top_actions, top_log_probs, V, top};
     with_type(type, [&](auto t) {
         using E = decltype(t);
-        hipLaunchKernelGGL(k_scores<E>, row_grid(T), dim3(kST), 0, (hipStream_t)stream, (const E *)logits, ld, actions, T, V, top,
-                           log_prob, entropy, stats, top_actions, top_log_probs);
+        launch_scores((const E *)logits, ld, T, parts_of(type, T, V), out, workspace, (hipStream_t)stream);
     });
     return mz::check_launch("k_scores");
 }
@@ -214,10 +629,10 @@ int mz_policy_scores_backward(const void *logits, int32_t type, int64_t ld, cons
     if (!stats || !entropy || (g_top && top > 0 && !top_actions) || (g_log_prob && !actions))
         return mz::fail(MZ_ERR_ARG, "mz_policy_scores_backward: NULL argument");
     if (top == 0) g_top = nullptr;
+    const Grads in{actions, stats, entropy, top_actions, g_log_prob, g_entropy, g_top, V, top};
     with_type(type, [&](auto t) {
         using E = decltype(t);
-        hipLaunchKernelGGL(k_scores_grad<E>, row_grid(T), dim3(kST), 0, (hipStream_t)stream, (const E *)logits, ld, actions, T, V,
-                           top, stats, entropy, top_actions, g_log_prob, g_entropy, g_top, (E *)grad, ld_grad);
+        launch_grad((const E *)logits, ld, T, in, (E *)grad, ld_grad, (hipStream_t)stream);
     });
     return mz::check_launch("k_scores_grad");
 }
