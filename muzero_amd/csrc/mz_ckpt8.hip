@@ -117,27 +117,28 @@ k_codes_t(const int8_t *__restrict__ codes, int64_t ldc, int R, int K, int64_t R
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads)
+template <class T, class Tl>
+__global__ void __launch_bounds__(Tl::threads)
 k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, const float *__restrict__ inverse, int K, int N,
-              int64_t Rp, int n_planes, T *__restrict__ dw, int64_t ldw) {
-    __shared__ __align__(16) uint8_t lds[2 * kTile * kStep];
-    const int tiles_k = (K + kTile - 1) / kTile;
-    const int k0 = (blockIdx.x % tiles_k) * kTile, n0 = (blockIdx.x / tiles_k) * kTile;
+              int64_t Rp, int n_planes, T *__restrict__ dw, int64_t ldw, int tiles_k, int tiles_n) {
+    __shared__ __align__(16) uint8_t lds[Tl::lds_bytes];
+    const TileAt at = tile_at(blockIdx.x, tiles_k, tiles_n, 8);
+    const int k0 = at.inner * Tl::TI, n0 = at.outer * Tl::TO;
     const Operand inner{(const uint8_t *)codes_t, 2 * Rp, K, (int)(2 * Rp)};
     const Operand outer{(const uint8_t *)planes, 2 * Rp * n_planes, N, (int)(2 * Rp * n_planes)};
-    f32x4 acc[4][4];
-    tile_product<OpF16>(inner, k0, outer, n0, (int)(2 * Rp * n_planes), lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave & 1) * 64, wo = (wave >> 1) * 64;
-    for (int b = 0; b < 4; ++b) {
-        const int n = n0 + wo + 16 * b + (lane & 15);
+    typename Tl::Acc acc;
+    Tl::product(inner, k0, outer, n0, 0, outer.wrap / kStep, lds, acc);
+    const int lane = threadIdx.x & 63, k1 = k0 + Tl::wi() + 4 * (lane >> 4);
+#pragma unroll
+    for (int b = 0; b < Tl::NO; ++b) {
+        const int n = n0 + Tl::wo() + 16 * b + (lane & 15);
         if (n >= N) continue;
         const float inv = inverse[n];
-        for (int a = 0; a < 4; ++a)
-            for (int e = 0; e < 4; ++e) {
-                const int k = k0 + wi + 16 * a + 4 * (lane >> 4) + e;
-                if (k < K) dw[n * ldw + k] = (T)(acc[a][b][e] * inv);
-            }
+#pragma unroll
+        for (int a = 0; a < Tl::NI; ++a)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (k1 + 16 * a + e < K) dw[n * ldw + k1 + 16 * a + e] = (T)(acc[a][b][e] * inv);
     }
 }
 
@@ -161,7 +162,7 @@ Layout layout(int32_t type, int32_t scale_bits, int64_t R, int64_t N, int64_t K)
     return l;
 }
 
-constexpr int64_t kMaxRows = 1 << 28;  // two planes of fp16 in 31 bits of bytes
+constexpr int64_t kMaxRows = 1 << 20;  // a row of two fp16 planes is then at most 2^22 bytes (mz_tile.h: Operand)
 
 }  // namespace
 
@@ -189,7 +190,7 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
     if (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 15) != 0)
         return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: needs a 16-byte aligned workspace of %lld bytes (got %lld)",
                         (long long)l.bytes, (long long)workspace_bytes);
-    const int64_t tiles = (round_up(N, kTile) / kTile) * (round_up(K, kTile) / kTile);
+    const int64_t tiles = (round_up(N, 64) / 64) * (round_up(K, 64) / 64);
     if (tiles > (1 << 23) || l.Rp / 64 > 65535)
         return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: rows=%d N=%d K=%d is too large for one call", rows, N, K);
     uint8_t *ws = (uint8_t *)workspace;
@@ -209,8 +210,15 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
             hipLaunchKernelGGL((k_split<T, 2>), split_grid, dim3(kCT), 0, st, (const T *)dz, ldz, scales, rows, N, l.Rp, l.chunks,
                                part_max, part_sum, planes, inverse, (T *)db);
         hipLaunchKernelGGL(k_codes_t, codes_grid, dim3(kCT), 0, st, codes, ldc, rows, K, l.Rp, codes_t);
-        hipLaunchKernelGGL(k_weight_grad<T>, dim3((unsigned)tiles), dim3(kThreads), 0, st, codes_t, planes, inverse, K, N, l.Rp,
-                           l.planes, (T *)dw, ldw);
+        const auto launch = [&](auto tile) {
+            using Tl = decltype(tile);
+            const int tiles_k = (K + Tl::TI - 1) / Tl::TI, tiles_n = (N + Tl::TO - 1) / Tl::TO;
+            hipLaunchKernelGGL((k_weight_grad<T, Tl>), dim3((unsigned)(tiles_k * tiles_n)), dim3(Tl::threads), 0, st, codes_t, planes,
+                               inverse, K, N, l.Rp, l.planes, (T *)dw, ldw, tiles_k, tiles_n);
+        };
+        if ((int64_t)K * N >= 256LL * 256 * 200) launch(Tile<OpF16, 256, 256, 2, 4>{});
+        else if ((int64_t)K * N >= 128LL * 128 * 100) launch(Tile<OpF16, 128, 128, 2, 2>{});
+        else launch(Tile<OpF16, 64, 64, 2, 2>{});
     });
     return mz::check_launch("mz_ckpt8_weight_grad");
 }

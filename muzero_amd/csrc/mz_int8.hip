@@ -22,25 +22,44 @@ __device__ __forceinline__ float activate(float v, int act) {
     }
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads)
+template <class T, class Tl>
+__global__ void __launch_bounds__(Tl::threads)
 k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs, int rows, const int8_t *__restrict__ wc,
        int64_t ldw, const float *__restrict__ ws, int N, int kbytes, const float *__restrict__ bias, int act, T *__restrict__ y,
-       int64_t ldy) {
-    __shared__ __align__(16) uint8_t lds[2 * kTile * kStep];
-    const int tiles_n = (N + kTile - 1) / kTile;
-    const int n0 = (blockIdx.x % tiles_n) * kTile, r0 = (blockIdx.x / tiles_n) * kTile;
+       int64_t ldy, int tiles_n, int tiles_r, int splits, int *__restrict__ partial) {
+    __shared__ __align__(16) uint8_t lds[Tl::lds_bytes];
+    const int split = blockIdx.x % splits;
+    const TileAt at = tile_at(blockIdx.x / splits, tiles_n, tiles_r, 8);
+    const int n0 = at.inner * Tl::TI, r0 = at.outer * Tl::TO;
     const Operand inner{(const uint8_t *)wc, ldw, N, kbytes}, outer{(const uint8_t *)xc, ldxc, rows, kbytes};
-    i32x4 acc[4][4];
-    tile_product<OpI8>(inner, n0, outer, r0, kbytes, lds, acc);
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave & 1) * 64, wo = (wave >> 1) * 64;
-    for (int b = 0; b < 4; ++b) {
-        const int r = r0 + wo + 16 * b + (lane & 15);
+    const int steps = kbytes / kStep;
+    typename Tl::Acc acc;
+    Tl::product(inner, n0, outer, r0, steps * split / splits, steps * (split + 1) / splits, lds, acc);
+    const int lane = threadIdx.x & 63, n1 = n0 + Tl::wi() + 4 * (lane >> 4);
+    if (splits > 1) {
+        int *out = partial + (int64_t)split * rows * N;
+#pragma unroll
+        for (int b = 0; b < Tl::NO; ++b) {
+            const int r = r0 + Tl::wo() + 16 * b + (lane & 15);
+            if (r >= rows) continue;
+#pragma unroll
+            for (int a = 0; a < Tl::NI; ++a)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (n1 + 16 * a + e < N) out[(int64_t)r * N + n1 + 16 * a + e] = acc[a][b][e];
+        }
+        return;
+    }
+#pragma unroll
+    for (int b = 0; b < Tl::NO; ++b) {
+        const int r = r0 + Tl::wo() + 16 * b + (lane & 15);
         if (r >= rows) continue;
         const float s = xs[r];
-        for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int a = 0; a < Tl::NI; ++a)
+#pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int n = n0 + wi + 16 * a + 4 * (lane >> 4) + e;
+                const int n = n1 + 16 * a + e;
                 if (n < N) y[r * ldy + n] = (T)activate((float)acc[a][b][e] * (s * ws[n]) + (bias ? bias[n] : 0.0f), act);
             }
     }
@@ -50,8 +69,8 @@ int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 int check_code_rows(const char *what, const int8_t *codes, int64_t ldc, const float *scales, int32_t K) {
     if (!codes || !scales) return mz::fail(MZ_ERR_ARG, "%s: NULL argument", what);
-    if (ldc < K || ldc % 128 != 0 || ((uintptr_t)codes & 15) != 0)
-        return mz::fail(MZ_ERR_ARG, "%s: codes need 16-byte aligned rows of a multiple of 128 bytes, zero behind K=%d (row stride %lld)",
+    if (ldc < K || ldc % 128 != 0 || ldc > (1 << 22) || ((uintptr_t)codes & 15) != 0)
+        return mz::fail(MZ_ERR_ARG, "%s: codes need 16-byte aligned rows of a multiple of 128 bytes (at most 2^22), zero behind K=%d (row stride %lld)",
                         what, K, (long long)ldc);
     return MZ_OK;
 }
@@ -67,7 +86,7 @@ int check_int8(int32_t rows, int32_t K, const int8_t *w_codes, int64_t ldw, cons
     if (rows > 0 && !y) return mz::fail(MZ_ERR_ARG, "mz_int8_forward: NULL argument");
     if (ldy < N || ((uintptr_t)y & (type_bytes(type) - 1)) != 0)
         return mz::fail(MZ_ERR_ARG, "mz_int8_forward: bad output stride %lld or alignment for N=%d", (long long)ldy, N);
-    if ((round_up(N, kTile) / kTile) * (round_up(rows, kTile) / kTile) > (1 << 23))
+    if ((round_up(N, 64) / 64) * (round_up(rows, 64) / 64) > (1 << 23))
         return mz::fail(MZ_ERR_ARG, "mz_int8_forward: output of %d x %d is too large for one call", rows, N);
     return MZ_OK;
 }
@@ -75,11 +94,18 @@ int check_int8(int32_t rows, int32_t K, const int8_t *w_codes, int64_t ldw, cons
 int launch_codes(const int8_t *x_codes, int64_t ldxc, const float *x_scales, int32_t rows, int32_t K, const int8_t *w_codes,
                  int64_t ldw, const float *w_scales, int32_t N, const float *bias, int32_t activation, void *y, int32_t type,
                  int64_t ldy, hipStream_t stream) {
-    const int64_t tiles = (round_up(N, kTile) / kTile) * (round_up(rows, kTile) / kTile);
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(k_int8<T>, dim3((unsigned)tiles), dim3(kThreads), 0, stream, x_codes, ldxc, x_scales, rows, w_codes, ldw,
-                           w_scales, N, (int)round_up(K, 128), bias, activation, (T *)y, ldy);
+        const auto launch = [&](auto tile) {
+            using Tl = decltype(tile);
+            const int tiles_n = (N + Tl::TI - 1) / Tl::TI, tiles_r = (rows + Tl::TO - 1) / Tl::TO;
+            hipLaunchKernelGGL((k_int8<T, Tl>), dim3((unsigned)(tiles_n * tiles_r)), dim3(Tl::threads), 0, stream, x_codes, ldxc,
+                               x_scales, rows, w_codes, ldw, w_scales, N, (int)round_up(K, 128), bias, activation, (T *)y, ldy, tiles_n,
+                               tiles_r, 1, (int *)nullptr);
+        };
+        if ((int64_t)rows * N >= 256LL * 256 * 200) launch(Tile<OpI8, 256, 256, 2, 4>{});
+        else if ((int64_t)rows * N >= 128LL * 128 * 100) launch(Tile<OpI8, 128, 128, 2, 2>{});
+        else launch(Tile<OpI8, 64, 64, 2, 2>{});
     });
     return mz::check_launch("k_int8");
 }

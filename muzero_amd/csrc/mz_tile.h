@@ -29,8 +29,9 @@ struct OpF16 {
     }
 };
 
-// One operand in memory: `rows` rows of `pitch` bytes (a multiple of 16), the reduction in bytes 0 .. wrap-1 of a row,
-// repeated when the other operand's rows are longer.
+// One operand in memory: `rows` rows of `pitch` bytes (a multiple of 16, below 2^23 so that 256 of them are named by 32
+// bits), the reduction in bytes 0 .. wrap-1 of a row (a multiple of 128), run through again when the other operand's rows
+// are longer.
 struct Operand {
     const uint8_t *p;
     int64_t pitch;
@@ -38,39 +39,124 @@ struct Operand {
     int wrap;
 };
 
-constexpr int kThreads = 256, kTile = 128, kStep = 128;  // 4 waves of 64 x 64; 128 bytes of the reduction per step
+constexpr int kStep = 128;  // bytes of the reduction per step: one cache line of every row
 
-// Byte offset of the 16-byte chunk c (0..7) of tile row r: the chunks of a row are rotated so that the 16 lanes of a
-// fragment read fall into different banks.
+// Byte offset of the 16-byte chunk c (0..7) of tile row r.  A ds_read_b128 is served in groups of 16 lanes that hold
+// rows 0-3 and 12-15 of one chunk and rows 4-11 of its neighbour (and the reverse); rotating the chunks by half the row
+// number gives every group 16 different 16-byte columns of the 256-byte bank row.
 __device__ __forceinline__ int chunk_at(int r, int c) { return r * kStep + ((c ^ ((r >> 1) & 7)) << 4); }
 
-// acc[a][b]: inner rows i0 + wave_i * 64 + 16 a + 4 (lane / 16) + 0..3, outer row o0 + wave_o * 64 + 16 b + lane % 16.
-template <class Op>
-__device__ __forceinline__ void tile_product(const Operand &inner, int i0, const Operand &outer, int o0, int kbytes,
-                                             uint8_t *lds, typename Op::acc (&acc)[4][4]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = (wave & 1) * 64, wo = (wave >> 1) * 64;
-    uint8_t *li = lds, *lo = lds + kTile * kStep;
-    for (int a = 0; a < 4; ++a)
-        for (int b = 0; b < 4; ++b) acc[a][b] = {};
-    for (int k = 0; k < kbytes; k += kStep) {
-        __syncthreads();
-        for (int c = threadIdx.x; c < kTile * 8; c += kThreads) {
-            const int r = c >> 3, ch = c & 7;
-            const int ri = min(i0 + r, inner.rows - 1), ro = min(o0 + r, outer.rows - 1);
-            *(u32x4 *)(li + chunk_at(r, ch)) = *(const u32x4 *)(inner.p + ri * inner.pitch + k % inner.wrap + ch * 16);
-            *(u32x4 *)(lo + chunk_at(r, ch)) = *(const u32x4 *)(outer.p + ro * outer.pitch + k % outer.wrap + ch * 16);
+// One workgroup's tile of TI inner x TO outer rows, WI x WO waves.  Two stages of LDS.  Within a step a wave multiplies
+// the first 64 bytes while it reads the fragments of the second, then -- once the next stage has arrived and everybody is
+// done reading this one: one barrier per step -- starts the loads that refill this stage, and multiplies the second half
+// while it reads the next stage's first.  The loads go from memory to LDS directly and have a whole step to arrive.
+template <class Op_, int TI_, int TO_, int WI_, int WO_>
+struct Tile {
+    using Op = Op_;
+    static constexpr int TI = TI_, TO = TO_, WI = WI_, WO = WO_;
+    static constexpr int threads = 64 * WI * WO;
+    static constexpr int NI = TI / WI / 16, NO = TO / WO / 16;  // fragments of a wave
+    static constexpr int stage = (TI + TO) * kStep;
+    static constexpr int lds_bytes = 2 * stage;
+    static constexpr int loads = (TI + TO) / 8 / (WI * WO);     // 1024-byte pieces (8 rows) per wave and step
+    static_assert((TI + TO) % (8 * WI * WO) == 0 && TI % 8 == 0, "pieces divide among the waves");
+    using Acc = typename Op::acc[NI][NO];
+
+    // acc[a][b], element e: inner row i0 + wi() + 16 a + 4 (lane / 16) + e, outer row o0 + wo() + 16 b + lane % 16.
+    static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+    static __device__ __forceinline__ int wi() { return (wave() % WI) * (TI / WI); }
+    static __device__ __forceinline__ int wo() { return (wave() / WI) * (TO / WO); }
+
+    // Steps step0 .. step1-1 (of 128 bytes) of the product of the rows from i0 and o0; rows behind the last one are
+    // read as the last one (their results are never stored).
+    static __device__ __forceinline__ void product(const Operand &inner, int i0, const Operand &outer, int o0, int step0, int step1,
+                                                   uint8_t *lds, Acc &acc) {
+        const int lane = threadIdx.x & 63, w = wave();
+#pragma unroll
+        for (int a = 0; a < NI; ++a)
+#pragma unroll
+            for (int b = 0; b < NO; ++b) acc[a][b] = typename Op::acc{};
+        if (step0 >= step1) return;
+
+        // where this lane's pieces come from: piece j = w + q * waves holds tile rows 8 j .. 8 j + 7 (inner rows first)
+        const uint8_t *ip = inner.p + (int64_t)i0 * inner.pitch, *op = outer.p + (int64_t)o0 * outer.pitch;
+        unsigned off[loads];
+#pragma unroll
+        for (int q = 0; q < loads; ++q) {
+            const int r = 8 * (w + q * WI * WO) + (lane >> 3), c = ((lane & 7) ^ ((r >> 1) & 7)) << 4;
+            if (8 * (w + q * WI * WO) < TI)
+                off[q] = (unsigned)min(r, inner.rows - 1 - i0) * (unsigned)inner.pitch + c;
+            else
+                off[q] = (unsigned)min(r - TI, outer.rows - 1 - o0) * (unsigned)outer.pitch + c;
         }
-        __syncthreads();
-        for (int s = 0; s < 2; ++s) {
-            u32x4 fi[4], fo[4];
-            for (int a = 0; a < 4; ++a) {
-                fi[a] = *(const u32x4 *)(li + chunk_at(wi + 16 * a + (lane & 15), s * 4 + (lane >> 4)));
-                fo[a] = *(const u32x4 *)(lo + chunk_at(wo + 16 * a + (lane & 15), s * 4 + (lane >> 4)));
+        int ki = step0 * kStep % inner.wrap, ko = step0 * kStep % outer.wrap;
+        const auto fetch = [&](int s) {
+            uint8_t *st = lds + s * stage;
+#pragma unroll
+            for (int q = 0; q < loads; ++q) {
+                const int j = w + q * WI * WO;
+                const uint8_t *src = (8 * j < TI ? ip + ki : op + ko) + off[q];
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                                 (__attribute__((address_space(3))) void *)(st + j * 1024), 16, 0, 0);
             }
-            for (int a = 0; a < 4; ++a)
-                for (int b = 0; b < 4; ++b) acc[a][b] = Op::mfma(fi[a], fo[b], acc[a][b]);
+            ki += kStep, ko += kStep;
+            if (ki == inner.wrap) ki = 0;
+            if (ko == outer.wrap) ko = 0;
+        };
+        const int row_i = wi() + (lane & 15), row_o = TI + wo() + (lane & 15);
+        const int at_i = chunk_at(row_i, lane >> 4), at_o = chunk_at(row_o, lane >> 4);
+        u32x4 fi[2][NI], fo[2][NO];
+        const auto read = [&](int s, int half) {  // the second half's chunks are the first one's with bit 2 flipped
+            const uint8_t *bi = lds + s * stage + (at_i ^ (half * 64)), *bo = lds + s * stage + (at_o ^ (half * 64));
+#pragma unroll
+            for (int b = 0; b < NO; ++b) fo[half][b] = *(const u32x4 *)(bo + b * 16 * kStep);
+#pragma unroll
+            for (int a = 0; a < NI; ++a) fi[half][a] = *(const u32x4 *)(bi + a * 16 * kStep);
+        };
+        const auto multiply = [&](int half) {
+#pragma unroll
+            for (int a = 0; a < NI; ++a)
+#pragma unroll
+                for (int b = 0; b < NO; ++b) acc[a][b] = Op::mfma(fi[half][a], fo[half][b], acc[a][b]);
+        };
+        const int n = step1 - step0;
+        fetch(0);
+        if (n > 1) {
+            fetch(1);
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(loads) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+        read(0, 0);
+        for (int t = 0; t < n; ++t) {
+            const int s = t & 1;
+            read(s, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(0);
+            __builtin_amdgcn_sched_barrier(0);
+            // this wave's reads of the stage have returned, its loads of the next one have arrived
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (t + 2 < n) fetch(s);
+            if (t + 1 < n) read(s ^ 1, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(1);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
+};
+
+// Block b of `tiles` -> tile: consecutive blocks go to the 8 dies in turn, each with an L2 of its own, so die d takes the
+// d-th eighth of the tiles; within that, tiles run through bands of `band` outer tiles so that the blocks at work together
+// share rows of both operands.
+struct TileAt {
+    int inner, outer;
+};
+
+__device__ __forceinline__ TileAt tile_at(int b, int tiles_i, int tiles_o, int band) {
+    const int tiles = tiles_i * tiles_o, per = tiles >> 3, rest = tiles & 7, die = b & 7;
+    const int t = die * per + min(die, rest) + (b >> 3);
+    const int size = band * tiles_i, g = t / size, o0 = g * band, h = min(band, tiles_o - o0), u = t - g * size;
+    return {u / h, o0 + u % h};
 }
 
 }  // namespace mzt8
