@@ -120,7 +120,8 @@ k_codes_t(const int8_t *__restrict__ codes, int64_t ldc, int R, int K, int64_t R
 template <class T, class Tl>
 __global__ void __launch_bounds__(Tl::threads)
 k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, const float *__restrict__ inverse, int K, int N,
-              int64_t Rp, int n_planes, T *__restrict__ dw, int64_t ldw, int tiles_k, int tiles_n) {
+              int64_t Rp, int n_planes, T *__restrict__ dw, int64_t ldw, bool aligned, int tiles_k,
+              int tiles_n) {
     __shared__ __align__(16) uint8_t lds[Tl::lds_bytes];
     const TileAt at = tile_at(blockIdx.x, tiles_k, tiles_n, 8);
     const int k0 = at.inner * Tl::TI, n0 = at.outer * Tl::TO;
@@ -128,18 +129,13 @@ k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, c
     const Operand outer{(const uint8_t *)planes, 2 * Rp * n_planes, N, (int)(2 * Rp * n_planes)};
     typename Tl::Acc acc;
     Tl::product(inner, k0, outer, n0, 0, outer.wrap / kStep, lds, acc);
-    const int lane = threadIdx.x & 63, k1 = k0 + Tl::wi() + 4 * (lane >> 4);
-#pragma unroll
-    for (int b = 0; b < Tl::NO; ++b) {
-        const int n = n0 + Tl::wo() + 16 * b + (lane & 15);
-        if (n >= N) continue;
-        const float inv = inverse[n];
-#pragma unroll
-        for (int a = 0; a < Tl::NI; ++a)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (k1 + 16 * a + e < K) dw[n * ldw + k1 + 16 * a + e] = (T)(acc[a][b][e] * inv);
-    }
+    const int k = k0 + Tl::inner_of();
+    Tl::drain(lds, acc, [&](int n, int, const f32x4 &v) {
+        if (n0 + n >= N) return;
+        const float inv = inverse[n0 + n];
+        const float o[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+        store_quad(dw + (n0 + n) * ldw, k, K, aligned, o);
+    });
 }
 
 struct Layout {
@@ -214,7 +210,8 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
             using Tl = decltype(tile);
             const int tiles_k = (K + Tl::TI - 1) / Tl::TI, tiles_n = (N + Tl::TO - 1) / Tl::TO;
             hipLaunchKernelGGL((k_weight_grad<T, Tl>), dim3((unsigned)(tiles_k * tiles_n)), dim3(Tl::threads), 0, st, codes_t, planes,
-                               inverse, K, N, l.Rp, l.planes, (T *)dw, ldw, tiles_k, tiles_n);
+                               inverse, K, N, l.Rp, l.planes, (T *)dw, ldw, quads_aligned((T *)dw, ldw),
+                               tiles_k, tiles_n);
         };
         if ((int64_t)K * N >= 256LL * 256 * 200) launch(Tile<OpF16, 256, 256, 2, 4>{});
         else if ((int64_t)K * N >= 128LL * 128 * 100) launch(Tile<OpF16, 128, 128, 2, 2>{});

@@ -26,7 +26,7 @@ template <class T, class Tl>
 __global__ void __launch_bounds__(Tl::threads)
 k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs, int rows, const int8_t *__restrict__ wc,
        int64_t ldw, const float *__restrict__ ws, int N, int kbytes, const float *__restrict__ bias, int act, T *__restrict__ y,
-       int64_t ldy, int tiles_n, int tiles_r, int splits, int *__restrict__ partial) {
+       int64_t ldy, bool aligned, int tiles_n, int tiles_r, int splits, int *__restrict__ partial) {
     __shared__ __align__(16) uint8_t lds[Tl::lds_bytes];
     const int split = blockIdx.x % splits;
     const TileAt at = tile_at(blockIdx.x / splits, tiles_n, tiles_r, 8);
@@ -35,34 +35,32 @@ k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs
     const int steps = kbytes / kStep;
     typename Tl::Acc acc;
     Tl::product(inner, n0, outer, r0, steps * split / splits, steps * (split + 1) / splits, lds, acc);
-    const int lane = threadIdx.x & 63, n1 = n0 + Tl::wi() + 4 * (lane >> 4);
+    const int n = n0 + Tl::inner_of();
     if (splits > 1) {
         int *out = partial + (int64_t)split * rows * N;
+        Tl::drain(lds, acc, [&](int r, int, const i32x4 &v) {
+            if (r0 + r >= rows) return;
+            int *row = out + (int64_t)(r0 + r) * N;
 #pragma unroll
-        for (int b = 0; b < Tl::NO; ++b) {
-            const int r = r0 + Tl::wo() + 16 * b + (lane & 15);
-            if (r >= rows) continue;
-#pragma unroll
-            for (int a = 0; a < Tl::NI; ++a)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (n1 + 16 * a + e < N) out[(int64_t)r * N + n1 + 16 * a + e] = acc[a][b][e];
-        }
+            for (int e = 0; e < 4; ++e)
+                if (n + e < N) row[n + e] = v[e];
+        });
         return;
     }
+    float t[4], c[4];
 #pragma unroll
-    for (int b = 0; b < Tl::NO; ++b) {
-        const int r = r0 + Tl::wo() + 16 * b + (lane & 15);
-        if (r >= rows) continue;
-        const float s = xs[r];
-#pragma unroll
-        for (int a = 0; a < Tl::NI; ++a)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = n1 + 16 * a + e;
-                if (n < N) y[r * ldy + n] = (T)activate((float)acc[a][b][e] * (s * ws[n]) + (bias ? bias[n] : 0.0f), act);
-            }
+    for (int e = 0; e < 4; ++e) {
+        t[e] = n + e < N ? ws[n + e] : 0.0f;
+        c[e] = bias && n + e < N ? bias[n + e] : 0.0f;
     }
+    Tl::drain(lds, acc, [&](int r, int, const i32x4 &v) {
+        if (r0 + r >= rows) return;
+        const float s = xs[r0 + r];
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = activate((float)v[e] * (s * t[e]) + c[e], act);
+        store_quad(y + (r0 + r) * ldy, n, N, aligned, o);
+    });
 }
 
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
@@ -100,8 +98,8 @@ int launch_codes(const int8_t *x_codes, int64_t ldxc, const float *x_scales, int
             using Tl = decltype(tile);
             const int tiles_n = (N + Tl::TI - 1) / Tl::TI, tiles_r = (rows + Tl::TO - 1) / Tl::TO;
             hipLaunchKernelGGL((k_int8<T, Tl>), dim3((unsigned)(tiles_n * tiles_r)), dim3(Tl::threads), 0, stream, x_codes, ldxc,
-                               x_scales, rows, w_codes, ldw, w_scales, N, (int)round_up(K, 128), bias, activation, (T *)y, ldy, tiles_n,
-                               tiles_r, 1, (int *)nullptr);
+                               x_scales, rows, w_codes, ldw, w_scales, N, (int)round_up(K, 128), bias, activation, (T *)y, ldy,
+                               quads_aligned((T *)y, ldy), tiles_n, tiles_r, 1, (int *)nullptr);
         };
         if ((int64_t)rows * N >= 256LL * 256 * 200) launch(Tile<OpI8, 256, 256, 2, 4>{});
         else if ((int64_t)rows * N >= 128LL * 128 * 100) launch(Tile<OpI8, 128, 128, 2, 2>{});

@@ -17,6 +17,7 @@ using h16x8 = __attribute__((ext_vector_type(8))) _Float16;
 
 struct OpI8 {  // exact: |sum| <= 127 * 127 * K < 2^31 for K <= 131072
     using acc = i32x4;
+    using elem = int;
     static __device__ __forceinline__ acc mfma(const u32x4 &a, const u32x4 &b, const acc &c) {
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
     }
@@ -24,6 +25,7 @@ struct OpI8 {  // exact: |sum| <= 127 * 127 * K < 2^31 for K <= 131072
 
 struct OpF16 {
     using acc = f32x4;
+    using elem = float;
     static __device__ __forceinline__ acc mfma(const u32x4 &a, const u32x4 &b, const acc &c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
     }
@@ -143,7 +145,52 @@ struct Tile {
             __builtin_amdgcn_sched_barrier(0);
         }
     }
+
+    // The tile on its way out: f(outer row, inner row, v) for every four consecutive inner values, both counted within the
+    // tile, in an order that lets a wave store whole cache lines of an output row: the accumulator's layout (one outer row
+    // per lane) would store 16 to 64 bytes of 16 rows at a time.  Sixteen outer rows of a wave at a time go through its
+    // own part of LDS, which is free after product().  A lane's inner row is the same in every call (inner_of()).
+    static constexpr int WC = TI / WI, lanes_per_row = WC / 4, out_ld = WC + 4;
+    static_assert(WI * WO * 16 * out_ld * 4 <= lds_bytes, "the outgoing rows fit the stages");
+    static __device__ __forceinline__ int inner_of() { return wi() + 4 * (threadIdx.x % lanes_per_row); }
+
+    template <class F>
+    static __device__ __forceinline__ void drain(uint8_t *lds, const Acc &acc, F &&f) {
+        using V = typename Op::acc;
+        const int lane = threadIdx.x & 63;
+        typename Op::elem *mine = (typename Op::elem *)lds + wave() * 16 * out_ld;
+#pragma unroll
+        for (int b = 0; b < NO; ++b) {
+#pragma unroll
+            for (int a = 0; a < NI; ++a) *(V *)(mine + (lane & 15) * out_ld + 16 * a + 4 * (lane >> 4)) = acc[a][b];
+            for (int r = lane / lanes_per_row; r < 16; r += 64 / lanes_per_row)
+                f(wo() + 16 * b + r, inner_of(), *(const V *)(mine + r * out_ld + 4 * (lane % lanes_per_row)));
+        }
+    }
 };
+
+// Stores four consecutive values of an output row: at once where the row's address allows it.
+template <class T>
+struct alignas(4 * sizeof(T)) Quad {
+    T v[4];
+};
+
+template <class T>
+__device__ __forceinline__ void store_quad(T *row, int at, int n, bool aligned, const float (&v)[4]) {
+    if (aligned && at + 4 <= n) {
+        *(Quad<T> *)(row + at) = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (at + e < n) row[at + e] = (T)v[e];
+    }
+}
+
+// Every row starts on a multiple of four elements.
+template <class T>
+inline bool quads_aligned(const T *p, int64_t ld) {
+    return (uintptr_t)p % (4 * sizeof(T)) == 0 && ld % 4 == 0;
+}
 
 // Block b of `tiles` -> tile: consecutive blocks go to the 8 dies in turn, each with an L2 of its own, so die d takes the
 // d-th eighth of the tiles; within that, tiles run through bands of `band` outer tiles so that the blocks at work together
