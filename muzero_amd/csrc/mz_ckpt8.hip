@@ -130,10 +130,12 @@ k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, c
     typename Tl::Acc acc;
     Tl::product(inner, k0, outer, n0, 0, outer.wrap / kStep, lds, acc);
     const int k = k0 + Tl::inner_of();
-    Tl::drain(lds, acc, [&](int n, int, const f32x4 &v) {
+    float inv[Tl::NO];
+#pragma unroll
+    for (int b = 0; b < Tl::NO; ++b) inv[b] = inverse[min(n0 + Tl::outer_of(b), N - 1)];
+    Tl::template drain<true>(lds, acc, [&](int b, const f32x4 &v) { return v * inv[b]; }, [&](int n, const f32x4 &v) {
         if (n0 + n >= N) return;
-        const float inv = inverse[n0 + n];
-        const float o[4] = {v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv};
+        const float o[4] = {v[0], v[1], v[2], v[3]};
         store_quad(dw + (n0 + n) * ldw, k, K, aligned, o);
     });
 }
@@ -213,7 +215,7 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
                                inverse, K, N, l.Rp, l.planes, (T *)dw, ldw, quads_aligned((T *)dw, ldw),
                                tiles_k, tiles_n);
         };
-        if ((int64_t)K * N >= 256LL * 256 * 200) launch(Tile<OpF16, 256, 256, 2, 4>{});
+        if ((int64_t)K * N >= 256LL * 256 * 200) launch(Tile<OpF16, 256, 256, 4, 2>{});
         else if ((int64_t)K * N >= 128LL * 128 * 100) launch(Tile<OpF16, 128, 128, 2, 2>{});
         else launch(Tile<OpF16, 64, 64, 2, 2>{});
     });

@@ -1,6 +1,6 @@
 // Dense layers in 8-bit integers (gfx950): y = act(x W^T + b) with a scale for each row of x and each row of W
 // (mz_quant8_rows with full scales),
-//     y_rn = act(fl(sum_k q_rk w_nk) (s_r t_n) + b_n),
+//     y_rn = act((fl(sum_k q_rk w_nk) s_r) t_n + b_n),
 // the sum in 32-bit integers, which K <= 131072 keeps exact.
 #include <cmath>
 
@@ -38,7 +38,7 @@ k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs
     const int n = n0 + Tl::inner_of();
     if (splits > 1) {
         int *out = partial + (int64_t)split * rows * N;
-        Tl::drain(lds, acc, [&](int r, int, const i32x4 &v) {
+        Tl::template drain<true>(lds, acc, [](int, const i32x4 &v) { return v; }, [&](int r, const i32x4 &v) {
             if (r0 + r >= rows) return;
             int *row = out + (int64_t)(r0 + r) * N;
 #pragma unroll
@@ -47,20 +47,26 @@ k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs
         });
         return;
     }
-    float t[4], c[4];
+    float t[4], c[4], s[Tl::NO];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         t[e] = n + e < N ? ws[n + e] : 0.0f;
         c[e] = bias && n + e < N ? bias[n + e] : 0.0f;
     }
-    Tl::drain(lds, acc, [&](int r, int, const i32x4 &v) {
-        if (r0 + r >= rows) return;
-        const float s = xs[r0 + r];
-        float o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = activate((float)v[e] * (s * t[e]) + c[e], act);
+    for (int b = 0; b < Tl::NO; ++b) s[b] = xs[min(r0 + Tl::outer_of(b), rows - 1)];
+    const auto scaled = [&](int b, const i32x4 &v) { return f32x4{(float)v[0] * s[b], (float)v[1] * s[b], (float)v[2] * s[b], (float)v[3] * s[b]}; };
+    const auto put = [&](int r, const f32x4 &v, auto &&f) {
+        if (r0 + r >= rows) return;
+        const float o[4] = {f(v[0] * t[0] + c[0]), f(v[1] * t[1] + c[1]), f(v[2] * t[2] + c[2]), f(v[3] * t[3] + c[3])};
         store_quad(y + (r0 + r) * ldy, n, N, aligned, o);
-    });
+    };
+    if (act == MZ_ACT_NONE || act == MZ_ACT_RELU) {
+        const float least = act == MZ_ACT_RELU ? 0.0f : -INFINITY;  // a NaN is not less: it passes
+        Tl::template drain<true>(lds, acc, scaled, [&](int r, const f32x4 &v) { put(r, v, [&](float x) { return x < least ? least : x; }); });
+    } else {
+        Tl::template drain<false>(lds, acc, scaled, [&](int r, const f32x4 &v) { put(r, v, [&](float x) { return activate(x, act); }); });
+    }
 }
 
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
@@ -101,7 +107,7 @@ int launch_codes(const int8_t *x_codes, int64_t ldxc, const float *x_scales, int
                                x_scales, rows, w_codes, ldw, w_scales, N, (int)round_up(K, 128), bias, activation, (T *)y, ldy,
                                quads_aligned((T *)y, ldy), tiles_n, tiles_r, 1, (int *)nullptr);
         };
-        if ((int64_t)rows * N >= 256LL * 256 * 200) launch(Tile<OpI8, 256, 256, 2, 4>{});
+        if ((int64_t)rows * N >= 256LL * 256 * 200) launch(Tile<OpI8, 256, 256, 4, 2>{});
         else if ((int64_t)rows * N >= 128LL * 128 * 100) launch(Tile<OpI8, 128, 128, 2, 2>{});
         else launch(Tile<OpI8, 64, 64, 2, 2>{});
     });

@@ -17,7 +17,6 @@ using h16x8 = __attribute__((ext_vector_type(8))) _Float16;
 
 struct OpI8 {  // exact: |sum| <= 127 * 127 * K < 2^31 for K <= 131072
     using acc = i32x4;
-    using elem = int;
     static __device__ __forceinline__ acc mfma(const u32x4 &a, const u32x4 &b, const acc &c) {
         return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
     }
@@ -25,7 +24,6 @@ struct OpI8 {  // exact: |sum| <= 127 * 127 * K < 2^31 for K <= 131072
 
 struct OpF16 {
     using acc = f32x4;
-    using elem = float;
     static __device__ __forceinline__ acc mfma(const u32x4 &a, const u32x4 &b, const acc &c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
     }
@@ -48,10 +46,15 @@ constexpr int kStep = 128;  // bytes of the reduction per step: one cache line o
 // number gives every group 16 different 16-byte columns of the 256-byte bank row.
 __device__ __forceinline__ int chunk_at(int r, int c) { return r * kStep + ((c ^ ((r >> 1) & 7)) << 4); }
 
-// One workgroup's tile of TI inner x TO outer rows, WI x WO waves.  Two stages of LDS.  Within a step a wave multiplies
-// the first 64 bytes while it reads the fragments of the second, then -- once the next stage has arrived and everybody is
-// done reading this one: one barrier per step -- starts the loads that refill this stage, and multiplies the second half
-// while it reads the next stage's first.  The loads go from memory to LDS directly and have a whole step to arrive.
+// One workgroup's tile of TI inner x TO outer rows, WI x WO waves.  Two stages of LDS, filled from memory directly; a step
+// is two halves of 64 bytes, and each half a read of its fragments and their products.
+//   8 waves  two waves on every SIMD, half of them (`late`) one phase behind: while one reads LDS and starts the loads, the
+//            other one multiplies, and a barrier ends every phase, so that the matrix pipe always has a wave to serve.
+//            8192^2 x 16384 bytes, 256 x 256 tiles: 2880 TOP/s int8, 1440 TFLOP/s fp16; with all waves in the same phase
+//            (the 4-wave form) 2700 and 1330.
+//   4 waves  several workgroups share a compute unit and fill each other's gaps.  Fragments are double-buffered in
+//            registers: the second half is read while the first is multiplied, and one barrier per step -- the next stage
+//            has arrived, everybody is done reading this one -- comes before the loads that refill this stage.
 template <class Op_, int TI_, int TO_, int WI_, int WO_>
 struct Tile {
     using Op = Op_;
@@ -107,64 +110,111 @@ struct Tile {
         };
         const int row_i = wi() + (lane & 15), row_o = TI + wo() + (lane & 15);
         const int at_i = chunk_at(row_i, lane >> 4), at_o = chunk_at(row_o, lane >> 4);
-        u32x4 fi[2][NI], fo[2][NO];
-        const auto read = [&](int s, int half) {  // the second half's chunks are the first one's with bit 2 flipped
-            const uint8_t *bi = lds + s * stage + (at_i ^ (half * 64)), *bo = lds + s * stage + (at_o ^ (half * 64));
-#pragma unroll
-            for (int b = 0; b < NO; ++b) fo[half][b] = *(const u32x4 *)(bo + b * 16 * kStep);
-#pragma unroll
-            for (int a = 0; a < NI; ++a) fi[half][a] = *(const u32x4 *)(bi + a * 16 * kStep);
-        };
-        const auto multiply = [&](int half) {
-#pragma unroll
-            for (int a = 0; a < NI; ++a)
-#pragma unroll
-                for (int b = 0; b < NO; ++b) acc[a][b] = Op::mfma(fi[half][a], fo[half][b], acc[a][b]);
-        };
         const int n = step1 - step0;
         fetch(0);
         if (n > 1) {
             fetch(1);
-            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(loads) : "memory");
+            asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(loads) : "memory");  // the first stage has arrived
         } else {
             asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         }
-        read(0, 0);
-        for (int t = 0; t < n; ++t) {
-            const int s = t & 1;
-            read(s, 1);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(0);
-            __builtin_amdgcn_sched_barrier(0);
-            // this wave's reads of the stage have returned, its loads of the next one have arrived
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (t + 2 < n) fetch(s);
-            if (t + 1 < n) read(s ^ 1, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(1);
-            __builtin_amdgcn_sched_barrier(0);
+        // the second half's chunks are the first one's with bit 2 flipped
+        const auto read = [&](int s, int half, u32x4(&fi)[NI], u32x4(&fo)[NO]) {
+            const uint8_t *bi = lds + s * stage + (at_i ^ (half * 64)), *bo = lds + s * stage + (at_o ^ (half * 64));
+#pragma unroll
+            for (int b = 0; b < NO; ++b) fo[b] = *(const u32x4 *)(bo + b * 16 * kStep);
+#pragma unroll
+            for (int a = 0; a < NI; ++a) fi[a] = *(const u32x4 *)(bi + a * 16 * kStep);
+        };
+        const auto multiply = [&](const u32x4(&fi)[NI], const u32x4(&fo)[NO]) {
+#pragma unroll
+            for (int a = 0; a < NI; ++a)
+#pragma unroll
+                for (int b = 0; b < NO; ++b) acc[a][b] = Op::mfma(fi[a], fo[b], acc[a][b]);
+        };
+        if constexpr (WI * WO == 8) {
+            // Barriers of step t: early waves pass 4t+1 .. 4t+4, late ones 4t+2 .. 4t+5.  Step t's stage is complete at
+            // barrier 4t, where every wave has waited for its own loads; the last reads of step t-1 are done before
+            // barrier 4t, and the loads that overwrite its stage start behind it.
+            const bool late = w >= 4;
+            u32x4 fi[NI], fo[NO];
+            const auto products = [&] {
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+                multiply(fi, fo);
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            if (late) asm volatile("s_barrier" ::: "memory");
+            for (int t = 0; t < n; ++t) {
+                read(t & 1, 0, fi, fo);
+                if (t >= 1 && t + 1 < n) fetch((t & 1) ^ 1);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                products();
+                asm volatile("s_barrier" ::: "memory");
+                read(t & 1, 1, fi, fo);
+                if (late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                products();
+                if (!late) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                asm volatile("s_barrier" ::: "memory");
+            }
+            if (!late) asm volatile("s_barrier" ::: "memory");
+        } else {
+            u32x4 fi[2][NI], fo[2][NO];
+            const auto spread = [] {  // the reads between the products
+#pragma unroll
+                for (int z = 0; z < NI + NO; ++z) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x008, NI * NO / (NI + NO), 0);
+                }
+                __builtin_amdgcn_sched_group_barrier(0x008, NI * NO, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            read(0, 0, fi[0], fo[0]);
+            for (int t = 0; t < n; ++t) {
+                const int s = t & 1;
+                read(s, 1, fi[1], fo[1]);
+                multiply(fi[0], fo[0]);
+                spread();
+                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (t + 2 < n) fetch(s);
+                if (t + 1 < n) read(s ^ 1, 0, fi[0], fo[0]);
+                multiply(fi[1], fo[1]);
+                spread();
+            }
         }
     }
 
-    // The tile on its way out: f(outer row, inner row, v) for every four consecutive inner values, both counted within the
-    // tile, in an order that lets a wave store whole cache lines of an output row: the accumulator's layout (one outer row
-    // per lane) would store 16 to 64 bytes of 16 rows at a time.  Sixteen outer rows of a wave at a time go through its
-    // own part of LDS, which is free after product().  A lane's inner row is the same in every call (inner_of()).
+    // The tile on its way out: f(outer row, v) for every four consecutive inner values, in an order that lets a wave store
+    // whole cache lines of an output row; the accumulator's layout (one outer row per lane) would store 16 to 64 bytes of
+    // 16 rows at a time.  Sixteen outer rows of a wave at a time go through its own part of LDS, which is free after
+    // product().  The rows are counted within the tile; a lane's inner row is the same in every call (inner_of()).
+    // pre(b, v) maps an accumulator on the way in, where the lane's outer row is outer_of(b).
     static constexpr int WC = TI / WI, lanes_per_row = WC / 4, out_ld = WC + 4;
     static_assert(WI * WO * 16 * out_ld * 4 <= lds_bytes, "the outgoing rows fit the stages");
     static __device__ __forceinline__ int inner_of() { return wi() + 4 * (threadIdx.x % lanes_per_row); }
+    static __device__ __forceinline__ int outer_of(int b) { return wo() + 16 * b + (threadIdx.x & 15); }
 
-    template <class F>
-    static __device__ __forceinline__ void drain(uint8_t *lds, const Acc &acc, F &&f) {
-        using V = typename Op::acc;
+    template <bool UNROLL, class P, class F>
+    static __device__ __forceinline__ void drain(uint8_t *lds, const Acc &acc, P &&pre, F &&f) {
+        using V = decltype(pre(0, acc[0][0]));
         const int lane = threadIdx.x & 63;
-        typename Op::elem *mine = (typename Op::elem *)lds + wave() * 16 * out_ld;
+        uint8_t *mine = lds + wave() * 16 * out_ld * 4;
+        const auto pass = [&](int b, int r) {
+            f(wo() + 16 * b + r, *(const V *)(mine + (r * out_ld + 4 * (lane % lanes_per_row)) * 4));
+        };
 #pragma unroll
         for (int b = 0; b < NO; ++b) {
 #pragma unroll
-            for (int a = 0; a < NI; ++a) *(V *)(mine + (lane & 15) * out_ld + 16 * a + 4 * (lane >> 4)) = acc[a][b];
-            for (int r = lane / lanes_per_row; r < 16; r += 64 / lanes_per_row)
-                f(wo() + 16 * b + r, inner_of(), *(const V *)(mine + r * out_ld + 4 * (lane % lanes_per_row)));
+            for (int a = 0; a < NI; ++a) *(V *)(mine + ((lane & 15) * out_ld + 16 * a + 4 * (lane >> 4)) * 4) = pre(b, acc[a][b]);
+            if constexpr (UNROLL) {
+#pragma unroll
+                for (int q = 0; q < lanes_per_row / 4; ++q) pass(b, q * (64 / lanes_per_row) + lane / lanes_per_row);
+            } else {
+#pragma nounroll
+                for (int q = 0; q < lanes_per_row / 4; ++q) pass(b, q * (64 / lanes_per_row) + lane / lanes_per_row);
+            }
         }
     }
 };
