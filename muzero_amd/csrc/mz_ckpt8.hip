@@ -15,7 +15,7 @@
 //   k_col_stats   per column of dz: largest |v| and sum of dz, for chunks of rows
 //   k_split       dz -> planes, transposed to [n][plane][r]; db and 1 / c_n from the chunks
 //   k_codes_t     codes -> fp16, transposed to [k][r]
-//   k_weight_grad the product
+//   k_weight_grad the product; k_weight_join the sum of its parts where the reduction is split
 #include "mz_tile.h"
 
 namespace {
@@ -120,16 +120,26 @@ k_codes_t(const int8_t *__restrict__ codes, int64_t ldc, int R, int K, int64_t R
 template <class T, class Tl>
 __global__ void __launch_bounds__(Tl::threads)
 k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, const float *__restrict__ inverse, int K, int N,
-              int64_t Rp, int n_planes, T *__restrict__ dw, int64_t ldw, bool aligned, int tiles_k,
-              int tiles_n) {
+              int64_t Rp, int n_planes, T *__restrict__ dw, int64_t ldw, bool aligned, int tiles_k, int tiles_n, int splits,
+              float *__restrict__ partial) {
     __shared__ __align__(16) uint8_t lds[Tl::lds_bytes];
-    const TileAt at = tile_at(blockIdx.x, tiles_k, tiles_n, 8);
+    const int split = blockIdx.x % splits;
+    const TileAt at = tile_at(blockIdx.x / splits, tiles_k, tiles_n, 8);
     const int k0 = at.inner * Tl::TI, n0 = at.outer * Tl::TO;
     const Operand inner{(const uint8_t *)codes_t, 2 * Rp, K, (int)(2 * Rp)};
     const Operand outer{(const uint8_t *)planes, 2 * Rp * n_planes, N, (int)(2 * Rp * n_planes)};
+    const int steps = outer.wrap / kStep;
     typename Tl::Acc acc;
-    Tl::product(inner, k0, outer, n0, 0, outer.wrap / kStep, lds, acc);
+    Tl::product(inner, k0, outer, n0, (int)((int64_t)steps * split / splits), (int)((int64_t)steps * (split + 1) / splits), lds, acc);
     const int k = k0 + Tl::inner_of();
+    if (splits > 1) {
+        const int Kq = (K + 3) / 4 * 4;
+        float *out = partial + (int64_t)split * N * Kq;
+        Tl::template drain<true>(lds, acc, [](int, const f32x4 &v) { return v; }, [&](int n, const f32x4 &v) {
+            if (n0 + n < N && k < K) *(f32x4 *)(out + (int64_t)(n0 + n) * Kq + k) = v;
+        });
+        return;
+    }
     float inv[Tl::NO];
 #pragma unroll
     for (int b = 0; b < Tl::NO; ++b) inv[b] = inverse[min(n0 + Tl::outer_of(b), N - 1)];
@@ -140,9 +150,27 @@ k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, c
     });
 }
 
+// Sums of the parts of a split reduction, in a fixed order: one thread per four values of a row of dW.
+template <class T>
+__global__ void __launch_bounds__(256)
+k_weight_join(const float *__restrict__ partial, int splits, const float *__restrict__ inverse, int K, int N, T *__restrict__ dw,
+              int64_t ldw, bool aligned) {
+    const int quads = (K + 3) / 4;
+    const int64_t jobs = (int64_t)N * quads;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < jobs; q += (int64_t)gridDim.x * 256) {
+        const int n = (int)(q / quads), k = 4 * (int)(q - (int64_t)n * quads);
+        f32x4 sum = *(const f32x4 *)(partial + q * 4);
+        for (int p = 1; p < splits; ++p) sum += *(const f32x4 *)(partial + (p * jobs + q) * 4);
+        sum *= inverse[n];
+        const float o[4] = {sum[0], sum[1], sum[2], sum[3]};
+        store_quad(dw + n * ldw, k, K, aligned, o);
+    }
+}
+
 struct Layout {
     int planes, chunks, chunk_rows;
-    int64_t Rp, off_sum, off_inverse, off_planes, off_codes, bytes;
+    Shape shape;
+    int64_t Rp, off_sum, off_inverse, off_planes, off_codes, off_partial, bytes;
 };
 
 Layout layout(int32_t type, int32_t scale_bits, int64_t R, int64_t N, int64_t K) {
@@ -156,7 +184,9 @@ Layout layout(int32_t type, int32_t scale_bits, int64_t R, int64_t N, int64_t K)
     l.off_inverse = 2 * stat;
     l.off_planes = l.off_inverse + round_up(N * 4, 128);
     l.off_codes = l.off_planes + N * l.planes * l.Rp * 2;
-    l.bytes = l.off_codes + K * l.Rp * 2;
+    l.off_partial = l.off_codes + round_up(K * l.Rp * 2, 128);
+    l.shape = shape_of(N, K, l.Rp * 2 * l.planes / kStep);
+    l.bytes = l.off_partial + (l.shape.splits > 1 ? l.shape.splits * N * round_up(K, 4) * 4 : 0);
     return l;
 }
 
@@ -195,6 +225,7 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
     unsigned *part_max = (unsigned *)ws;
     float *part_sum = (float *)(ws + l.off_sum), *inverse = (float *)(ws + l.off_inverse);
     f16 *planes = (f16 *)(ws + l.off_planes), *codes_t = (f16 *)(ws + l.off_codes);
+    float *partial = (float *)(ws + l.off_partial);
     hipStream_t st = (hipStream_t)stream;
     const dim3 split_grid((unsigned)((N + 63) / 64), (unsigned)(l.Rp / 64)), codes_grid((unsigned)((K + 63) / 64), (unsigned)(l.Rp / 64));
     with_type(type, [&](auto t) {
@@ -211,12 +242,18 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
         const auto launch = [&](auto tile) {
             using Tl = decltype(tile);
             const int tiles_k = (K + Tl::TI - 1) / Tl::TI, tiles_n = (N + Tl::TO - 1) / Tl::TO;
-            hipLaunchKernelGGL((k_weight_grad<T, Tl>), dim3((unsigned)(tiles_k * tiles_n)), dim3(Tl::threads), 0, st, codes_t, planes,
-                               inverse, K, N, l.Rp, l.planes, (T *)dw, ldw, quads_aligned((T *)dw, ldw),
-                               tiles_k, tiles_n);
+            const bool aligned = quads_aligned((T *)dw, ldw);
+            hipLaunchKernelGGL((k_weight_grad<T, Tl>), dim3((unsigned)(tiles_k * tiles_n * l.shape.splits)), dim3(Tl::threads), 0, st,
+                               codes_t, planes, inverse, K, N, l.Rp, l.planes, (T *)dw, ldw, aligned, tiles_k, tiles_n, l.shape.splits,
+                               partial);
+            if (l.shape.splits > 1) {
+                const int64_t groups = ((int64_t)N * ((K + 3) / 4) + 255) / 256;
+                hipLaunchKernelGGL(k_weight_join<T>, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, st, partial,
+                                   l.shape.splits, inverse, K, N, (T *)dw, ldw, aligned);
+            }
         };
-        if ((int64_t)K * N >= 256LL * 256 * 200) launch(Tile<OpF16, 256, 256, 4, 2>{});
-        else if ((int64_t)K * N >= 128LL * 128 * 100) launch(Tile<OpF16, 128, 128, 2, 2>{});
+        if (l.shape.tile == 256) launch(Tile<OpF16, 256, 256, 4, 2>{});
+        else if (l.shape.tile == 128) launch(Tile<OpF16, 128, 256, 2, 4>{});
         else launch(Tile<OpF16, 64, 64, 2, 2>{});
     });
     return mz::check_launch("mz_ckpt8_weight_grad");

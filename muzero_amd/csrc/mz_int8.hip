@@ -37,13 +37,10 @@ k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs
     Tl::product(inner, n0, outer, r0, steps * split / splits, steps * (split + 1) / splits, lds, acc);
     const int n = n0 + Tl::inner_of();
     if (splits > 1) {
-        int *out = partial + (int64_t)split * rows * N;
+        const int Nq = (N + 3) / 4 * 4;
+        int *out = partial + (int64_t)split * rows * Nq;
         Tl::template drain<true>(lds, acc, [](int, const i32x4 &v) { return v; }, [&](int r, const i32x4 &v) {
-            if (r0 + r >= rows) return;
-            int *row = out + (int64_t)(r0 + r) * N;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < N) row[n + e] = v[e];
+            if (r0 + r < rows && n < N) *(i32x4 *)(out + (int64_t)(r0 + r) * Nq + n) = v;
         });
         return;
     }
@@ -66,6 +63,26 @@ k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs
         Tl::template drain<true>(lds, acc, scaled, [&](int r, const f32x4 &v) { put(r, v, [&](float x) { return x < least ? least : x; }); });
     } else {
         Tl::template drain<false>(lds, acc, scaled, [&](int r, const f32x4 &v) { put(r, v, [&](float x) { return activate(x, act); }); });
+    }
+}
+
+// Sums of the parts of a split reduction, scales, bias, activation: one thread per four values of an output row.
+template <class T>
+__global__ void __launch_bounds__(256)
+k_int8_join(const int *__restrict__ partial, int splits, const float *__restrict__ xs, int rows, const float *__restrict__ ws, int N,
+            const float *__restrict__ bias, int act, T *__restrict__ y, int64_t ldy, bool aligned) {
+    const int quads = (N + 3) / 4;
+    const int64_t jobs = (int64_t)rows * quads;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < jobs; q += (int64_t)gridDim.x * 256) {
+        const int r = (int)(q / quads), n = 4 * (int)(q - (int64_t)r * quads);
+        i32x4 sum = *(const i32x4 *)(partial + q * 4);
+        for (int p = 1; p < splits; ++p) sum += *(const i32x4 *)(partial + (p * jobs + q) * 4);
+        const float s = xs[r];
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            o[e] = n + e < N ? activate((float)sum[e] * s * ws[n + e] + (bias ? bias[n + e] : 0.0f), act) : 0.0f;
+        store_quad(y + r * ldy, n, N, aligned, o);
     }
 }
 
@@ -95,23 +112,56 @@ int check_int8(int32_t rows, int32_t K, const int8_t *w_codes, int64_t ldw, cons
     return MZ_OK;
 }
 
-int launch_codes(const int8_t *x_codes, int64_t ldxc, const float *x_scales, int32_t rows, int32_t K, const int8_t *w_codes,
-                 int64_t ldw, const float *w_scales, int32_t N, const float *bias, int32_t activation, void *y, int32_t type,
-                 int64_t ldy, hipStream_t stream) {
-    with_type(type, [&](auto t) {
-        using T = decltype(t);
-        const auto launch = [&](auto tile) {
-            using Tl = decltype(tile);
-            const int tiles_n = (N + Tl::TI - 1) / Tl::TI, tiles_r = (rows + Tl::TO - 1) / Tl::TO;
-            hipLaunchKernelGGL((k_int8<T, Tl>), dim3((unsigned)(tiles_n * tiles_r)), dim3(Tl::threads), 0, stream, x_codes, ldxc,
-                               x_scales, rows, w_codes, ldw, w_scales, N, (int)round_up(K, 128), bias, activation, (T *)y, ldy,
-                               quads_aligned((T *)y, ldy), tiles_n, tiles_r, 1, (int *)nullptr);
-        };
-        if ((int64_t)rows * N >= 256LL * 256 * 200) launch(Tile<OpI8, 256, 256, 4, 2>{});
-        else if ((int64_t)rows * N >= 128LL * 128 * 100) launch(Tile<OpI8, 128, 128, 2, 2>{});
-        else launch(Tile<OpI8, 64, 64, 2, 2>{});
-    });
-    return mz::check_launch("k_int8");
+int check_workspace(const void *workspace, int64_t bytes, int64_t need) {
+    if (need > 0 && (!workspace || bytes < need || ((uintptr_t)workspace & 15) != 0))
+        return mz::fail(MZ_ERR_ARG, "mz_int8_forward: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
+                        (long long)bytes);
+    return MZ_OK;
+}
+
+struct Int8Args {
+    const int8_t *xc;
+    int64_t ldxc;
+    const float *xs;
+    int rows;
+    const int8_t *wc;
+    int64_t ldw;
+    const float *ws;
+    int N, K;
+    const float *bias;
+    int act;
+    void *y;
+    int64_t ldy;
+    int *partial;
+};
+
+template <class T, class Tl>
+void launch_tiles(const Int8Args &a, int splits, hipStream_t st) {
+    const int tiles_n = (a.N + Tl::TI - 1) / Tl::TI, tiles_r = (a.rows + Tl::TO - 1) / Tl::TO;
+    const bool aligned = quads_aligned((T *)a.y, a.ldy);
+    hipLaunchKernelGGL((k_int8<T, Tl>), dim3((unsigned)(tiles_n * tiles_r * splits)), dim3(Tl::threads), 0, st, a.xc, a.ldxc, a.xs, a.rows,
+                       a.wc, a.ldw, a.ws, a.N, (int)round_up(a.K, kStep), a.bias, a.act, (T *)a.y, a.ldy, aligned, tiles_n, tiles_r, splits,
+                       a.partial);
+    if (splits > 1) {
+        const int64_t groups = ((int64_t)a.rows * ((a.N + 3) / 4) + 255) / 256;
+        hipLaunchKernelGGL(k_int8_join<T>, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, st, a.partial, splits, a.xs, a.rows,
+                           a.ws, a.N, a.bias, a.act, (T *)a.y, a.ldy, aligned);
+    }
+}
+
+Shape shape_of_int8(int64_t rows, int64_t N, int64_t K) { return shape_of(rows, N, round_up(K, kStep) / kStep); }
+
+template <class T>
+void launch_shape(const Int8Args &a, hipStream_t st) {
+    const Shape s = shape_of_int8(a.rows, a.N, a.K);
+    if (s.tile == 256) launch_tiles<T, Tile<OpI8, 256, 256, 4, 2>>(a, s.splits, st);
+    else if (s.tile == 128) launch_tiles<T, Tile<OpI8, 128, 256, 2, 4>>(a, s.splits, st);
+    else launch_tiles<T, Tile<OpI8, 64, 64, 2, 2>>(a, s.splits, st);
+}
+
+int64_t partial_bytes(int64_t rows, int64_t N, int64_t K) {
+    const Shape s = shape_of_int8(rows, N, K);
+    return s.splits > 1 ? s.splits * rows * round_up(N, 4) * 4 : 0;
 }
 
 }  // namespace
@@ -119,8 +169,7 @@ int launch_codes(const int8_t *x_codes, int64_t ldxc, const float *x_scales, int
 extern "C" {
 
 int64_t mz_int8_codes_workspace(int32_t rows, int32_t K, int32_t N) {
-    (void)rows, (void)K, (void)N;
-    return 0;
+    return rows <= 0 || K <= 0 || N <= 0 ? 0 : partial_bytes(rows, N, K);
 }
 
 int mz_int8_forward_codes(const int8_t *x_codes, int64_t ldxc, const float *x_scales, int32_t rows, int32_t K,
@@ -130,30 +179,30 @@ int mz_int8_forward_codes(const int8_t *x_codes, int64_t ldxc, const float *x_sc
     MZ_TRY(check_int8(rows, K, w_codes, ldw, w_scales, N, activation, y, type, ldy));
     if (rows == 0) return MZ_OK;
     MZ_TRY(check_code_rows("mz_int8_forward", x_codes, ldxc, x_scales, K));
-    (void)workspace, (void)workspace_bytes;
-    return launch_codes(x_codes, ldxc, x_scales, rows, K, w_codes, ldw, w_scales, N, bias, activation, y, type, ldy,
-                        (hipStream_t)stream);
+    MZ_TRY(check_workspace(workspace, workspace_bytes, mz_int8_codes_workspace(rows, K, N)));
+    const Int8Args a{x_codes, ldxc, x_scales, rows, w_codes, ldw, w_scales, N, K, bias, activation, y, ldy, (int *)workspace};
+    with_type(type, [&](auto t) { launch_shape<decltype(t)>(a, (hipStream_t)stream); });
+    return mz::check_launch("k_int8");
 }
 
 int64_t mz_int8_workspace(int32_t rows, int32_t K, int32_t N) {
     if (rows <= 0 || K <= 0 || N <= 0) return 0;
-    return round_up((int64_t)rows * 4, 128) + (int64_t)rows * round_up(K, 128);
+    return round_up(partial_bytes(rows, N, K), 128) + round_up((int64_t)rows * 4, 128) + (int64_t)rows * round_up(K, kStep);
 }
 
 int mz_int8_forward(const void *x, int32_t x_type, int64_t ldx, int32_t rows, int32_t K, const int8_t *w_codes, int64_t ldw,
                     const float *w_scales, int32_t N, const float *bias, int32_t activation, void *y, int32_t type, int64_t ldy,
                     void *workspace, int64_t workspace_bytes, void *stream) {
     MZ_TRY(check_int8(rows, K, w_codes, ldw, w_scales, N, activation, y, type, ldy));
-    const int64_t need = mz_int8_workspace(rows, K, N);
-    if (rows > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
-        return mz::fail(MZ_ERR_ARG, "mz_int8_forward: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
-                        (long long)workspace_bytes);
-    float *scales = (float *)workspace;
-    int8_t *codes = (int8_t *)workspace + round_up((int64_t)rows * 4, 128);
-    const int64_t ldc = round_up(K, 128);
+    MZ_TRY(check_workspace(workspace, workspace_bytes, mz_int8_workspace(rows, K, N)));
+    const int64_t partial = round_up(partial_bytes(rows, N, K), 128), ldc = round_up(K, kStep);
+    float *scales = (float *)((uint8_t *)workspace + partial);
+    int8_t *codes = (int8_t *)workspace + partial + round_up((int64_t)rows * 4, 128);
     MZ_TRY(mz_quant8_rows(x, x_type, ldx, rows, K, 24, codes, ldc, scales, stream));
     if (rows == 0) return MZ_OK;
-    return launch_codes(codes, ldc, scales, rows, K, w_codes, ldw, w_scales, N, bias, activation, y, type, ldy, (hipStream_t)stream);
+    const Int8Args a{codes, ldc, scales, rows, w_codes, ldw, w_scales, N, K, bias, activation, y, ldy, (int *)workspace};
+    with_type(type, [&](auto t) { launch_shape<decltype(t)>(a, (hipStream_t)stream); });
+    return mz::check_launch("k_int8");
 }
 
 }  // extern "C"

@@ -6,6 +6,8 @@
 // The inner operand is the instruction's first one: its 16 rows are the accumulator's rows, four consecutive ones per
 // lane, so that a lane holds four consecutive values of an output row and stores them together.
 #pragma once
+#include <algorithm>
+
 #include "mz_elem.h"
 
 namespace mzt8 {
@@ -254,6 +256,31 @@ __device__ __forceinline__ TileAt tile_at(int b, int tiles_i, int tiles_o, int b
     const int t = die * per + min(die, rest) + (b >> 3);
     const int size = band * tiles_i, g = t / size, o0 = g * band, h = min(band, tiles_o - o0), u = t - g * size;
     return {u / h, o0 + u % h};
+}
+
+// Tile size and parts of the reduction for an output of `outer` x `inner` values and `steps` steps.
+struct Shape {
+    int tile;    // 64 x 64, 128 (inner) x 256 (outer) or 256 x 256, named by the inner size
+    int splits;  // parts of the reduction, joined by a second kernel
+};
+
+inline int64_t tiles_of(int64_t n, int64_t t) { return (n + t - 1) / t; }
+
+// Large tiles read each operand less often, small ones fill the 256 compute units with less work.  Measured (int8, us;
+// 64 / 128 x 256 / 256 tiles, best number of parts in brackets):
+//     8192 x 8192, 32 steps       - / 267 / 240              2048 x 4096, 32 steps      55 / 39 / 49
+//     4096 x 4096,  4 steps      26 / 26 / 19                1024 x 4096, 32 steps      29 / 35 / 43 (3)
+//      256 x 9216, 144 steps     80 / 66 (3) / 62 (6)         256 x 9216, 72 steps      41 / 43 (3) / 47 (4)
+//       64 x 9216, 144 steps     34 (3) / 52 (3) / 45 (6)     128 x 4096, 32 steps      13 / 19 (4) / 23 (6)
+//      100 x  500, 128 steps     13 (8), undivided 39         1024 x 1024, 8 steps     6.4 / 13 / 19
+inline Shape shape_of(int64_t outer, int64_t inner, int64_t steps) {
+    const int64_t large = tiles_of(outer, 256) * tiles_of(inner, 256), medium = tiles_of(outer, 256) * tiles_of(inner, 128);
+    if (large >= 200) return {256, 1};
+    if (medium >= 200) return {128, 1};
+    if (outer * inner * steps >= 240LL * 1000 * 1000 && steps >= 64)  // a long reduction: the operands are what is read
+        return {256, (int)std::max<int64_t>(1, std::min(256 / large, steps / 16))};
+    const int64_t small = tiles_of(outer, 64) * tiles_of(inner, 64);
+    return {64, (int)std::max<int64_t>(1, std::min({(int64_t)8, 400 / small, steps / 16}))};
 }
 
 }  // namespace mzt8
