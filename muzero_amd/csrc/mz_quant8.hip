@@ -19,20 +19,8 @@ constexpr float kTiny = 0x1p-119f;
 
 __device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
-// Maximum over the workgroup of unsigned values (NaN bit patterns order above infinity, so they win).
-__device__ __forceinline__ unsigned block_max(unsigned v) {
-    __shared__ unsigned part[kQT / 64];
-    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o));
-    __syncthreads();  // the last row's values have been read
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = part[0];
-    for (int w = 1; w < kQT / 64; ++w) v = max(v, part[w]);
-    return v;
-}
-
 struct RowScale {
-    float scale, inverse;
+    float scale, inverse;  // inverse 0: the row is held as zeros
 };
 
 __device__ __forceinline__ RowScale row_scale(unsigned amax_bits, int scale_bits) {
@@ -45,76 +33,206 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits, int scale_bits
     return {s, 1.0f / s};
 }
 
-// One workgroup per row: the row is read twice (the second time from cache).
-template <class T>
-__global__ void __launch_bounds__(kQT)
-k_quant8(const T *__restrict__ x, int64_t ldx, int64_t rows, int K, int scale_bits, int8_t *__restrict__ codes, int64_t ldc,
-         float *__restrict__ scales) {
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-    const T *xr = x + row * ldx;
-    unsigned m = 0;
-    for (int k = threadIdx.x; k < K; k += kQT) m = max(m, abs_bits((float)xr[k]));
-    m = block_max(m);
-    const RowScale rs = row_scale(m, scale_bits);
-    if (threadIdx.x == 0) scales[row] = rs.scale;
-    const bool live = rs.inverse != 0.0f;
-    for (int k = threadIdx.x; k < ldc; k += kQT)
-        codes[row * ldc + k] = (k < K && live) ? (int8_t)(int)rintf((float)xr[k] * rs.inverse) : (int8_t)0;
+// Elements j .. j + n - 1 of a row of K, zeros behind its end; WHOLE: rows start on 16-byte addresses.
+template <class T, bool WHOLE>
+__device__ __forceinline__ Pack<T> load_pack(const T *__restrict__ row, int j, int K) {
+    constexpr int n = Pack<T>::n;
+    if (WHOLE && j + n <= K) return *(const Pack<T> *)(row + j);
+    Pack<T> p;
+#pragma unroll
+    for (int e = 0; e < n; ++e) p.v[e] = j + e < K ? row[j + e] : (T)0.0f;
+    return p;
+}
+
+template <class T, bool WHOLE>
+__device__ __forceinline__ void store_pack(T *__restrict__ row, int j, int K, const Pack<T> &p) {
+    constexpr int n = Pack<T>::n;
+    if (WHOLE && j + n <= K) {
+        *(Pack<T> *)(row + j) = p;
+    } else {
+#pragma unroll
+        for (int e = 0; e < n; ++e)
+            if (j + e < K) row[j + e] = p.v[e];
     }
 }
 
+// One pack's codes.  Adding 1.5 * 2^23 rounds to a whole number, half to even, and leaves it in the low bits; the product
+// is rounded before (no fused multiply-add), as the definition says.
 template <class T>
+__device__ __forceinline__ void store_codes(int8_t *out, const Pack<T> &p, float inverse) {
+#pragma clang fp contract(off)
+    constexpr int n = Pack<T>::n;
+    unsigned w[n / 4];
+#pragma unroll
+    for (int q = 0; q < n / 4; ++q) {
+        unsigned b[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float v = (float)p.v[4 * q + e] * inverse;
+            b[e] = __float_as_uint(v + 12582912.0f) & 0xFFu;
+        }
+        w[q] = inverse == 0.0f ? 0u : b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
+    }
+    if constexpr (n == 4) *(unsigned *)out = w[0];
+    else *(uint2 *)out = make_uint2(w[0], w[1]);
+}
+
+// THREADS threads per row (64: four rows per workgroup, 256: one).  The first HELD packs of a thread stay in registers
+// between the maximum and the codes; the rest of a longer row is read again, from cache.  Bound by the memory: 113 MB of
+// float32 in (1536 x 18432) in 34 us, 4.1 TB/s with the codes.
+template <class T, int THREADS, int HELD, bool WHOLE>
+__global__ void __launch_bounds__(kQT)
+k_quant8(const T *__restrict__ x, int64_t ldx, int64_t rows, int K, int scale_bits, int8_t *__restrict__ codes, int64_t ldc,
+         float *__restrict__ scales) {
+    constexpr int n = Pack<T>::n, per = kQT / THREADS;
+    __shared__ unsigned part[kQT / 64];
+    const int t = threadIdx.x % THREADS, packs = (int)(ldc / n);
+    for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < rows; row0 += (int64_t)gridDim.x * per) {
+        const int64_t row = row0 + threadIdx.x / THREADS;
+        if (THREADS == 64 && row >= rows) break;
+        const T *xr = x + row * ldx;
+        Pack<T> held[HELD];
+        unsigned m = 0;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h)
+            if ((t + h * THREADS) * n < K) held[h] = load_pack<T, WHOLE>(xr, (t + h * THREADS) * n, K);
+            else held[h] = Pack<T>{};
+#pragma unroll
+        for (int h = 0; h < HELD; ++h)
+#pragma unroll
+            for (int e = 0; e < n; ++e) m = max(m, abs_bits((float)held[h].v[e]));
+        for (int i = t + HELD * THREADS; i < packs; i += THREADS) {
+            const Pack<T> p = load_pack<T, WHOLE>(xr, i * n, K);
+#pragma unroll
+            for (int e = 0; e < n; ++e) m = max(m, abs_bits((float)p.v[e]));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o));
+        if (THREADS > 64) {
+            __syncthreads();  // the last row's maxima have been read
+            if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kQT / 64; ++w) m = max(m, part[w]);
+        }
+        const RowScale rs = row_scale(m, scale_bits);
+        if (t == 0) scales[row] = rs.scale;
+        int8_t *cr = codes + row * ldc;
+#pragma unroll
+        for (int h = 0; h < HELD; ++h)
+            if (t + h * THREADS < packs) store_codes(cr + (t + h * THREADS) * n, held[h], rs.inverse);
+        for (int i = t + HELD * THREADS; i < packs; i += THREADS) store_codes(cr + i * n, load_pack<T, WHOLE>(xr, i * n, K), rs.inverse);
+    }
+}
+
+template <class T, int THREADS, bool WHOLE>
 __global__ void __launch_bounds__(kQT)
 k_dequant8(const int8_t *__restrict__ codes, int64_t ldc, const float *__restrict__ scales, int64_t rows, int K,
            T *__restrict__ x, int64_t ldx) {
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    constexpr int n = Pack<T>::n, per = kQT / THREADS;
+    const int t = threadIdx.x % THREADS;
+    for (int64_t row = (int64_t)blockIdx.x * per + threadIdx.x / THREADS; row < rows; row += (int64_t)gridDim.x * per) {
         const float s = scales[row];
-        for (int k = threadIdx.x; k < K; k += kQT) x[row * ldx + k] = (T)((float)codes[row * ldc + k] * s);
+        const int8_t *cr = codes + row * ldc;
+#pragma unroll 4
+        for (int j = t * n; j < K; j += THREADS * n) {
+            alignas(8) int8_t q[n];  // the padding of a row covers a pack
+            if constexpr (n == 4) *(unsigned *)q = *(const unsigned *)(cr + j);
+            else *(uint2 *)q = *(const uint2 *)(cr + j);
+            Pack<T> p;
+#pragma unroll
+            for (int e = 0; e < n; ++e) p.v[e] = (T)((float)q[e] * s);
+            store_pack<T, WHOLE>(x + row * ldx, j, K, p);
+        }
+    }
+}
+
+// Eight consecutive values of a row, zeros behind its end.
+template <class T, bool WHOLE>
+__device__ __forceinline__ void load8(const T *row, int j, int N, float (&v)[8]) {
+    constexpr int n = Pack<T>::n;
+#pragma unroll
+    for (int h = 0; h < 8 / n; ++h) {
+        const Pack<T> p = load_pack<T, WHOLE>(row, j + h * n, N);
+#pragma unroll
+        for (int e = 0; e < n; ++e) v[h * n + e] = (float)p.v[e];
     }
 }
 
 // What the backward pass needs of y = act(z): relu one bit, [not y <= 0]; tanh and sigmoid a code of 8 bits on a fixed
-// scale, -128 for a NaN.
-template <class T>
+// scale, -128 for a NaN.  A thread takes 8 values: a byte of bits, or 8 codes.
+template <class T, bool WHOLE>
 __global__ void __launch_bounds__(kQT)
 k_act_save(const T *__restrict__ y, int64_t ldy, int64_t rows, int N, int act, uint8_t *__restrict__ saved, int64_t lds) {
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
-        for (int j = threadIdx.x; j < lds; j += kQT) {
-            unsigned out = 0;
+    const int t = threadIdx.x % 64;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; row < rows; row += (int64_t)gridDim.x * 4)
+#pragma unroll 2
+        for (int j = t * 8; j < N; j += 64 * 8) {
+            float v[8];
+            load8<T, WHOLE>(y + row * ldy, j, N, v);
             if (act == MZ_ACT_RELU) {
-                for (int b = 0; b < 8; ++b)
-                    if (8 * j + b < N && !((float)y[row * ldy + 8 * j + b] <= 0.0f)) out |= 1u << b;
+                unsigned bits = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) bits |= (unsigned)(j + e < N && !(v[e] <= 0.0f)) << e;
+                saved[row * lds + (j >> 3)] = (uint8_t)bits;
             } else {
-                const float v = (float)y[row * ldy + j];
-                const float c = rintf(act == MZ_ACT_TANH ? v * 127.0f : v * 254.0f - 127.0f);
-                out = v == v ? (unsigned)(int)fminf(fmaxf(c, -127.0f), 127.0f) : 0x80u;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float c = rintf(act == MZ_ACT_TANH ? v[e] * 127.0f : v[e] * 254.0f - 127.0f);
+                    const unsigned code = v[e] == v[e] ? (unsigned)(int)fminf(fmaxf(c, -127.0f), 127.0f) : 0x80u;
+                    if (j + e < N) saved[row * lds + j + e] = (uint8_t)code;
+                }
             }
-            saved[row * lds + j] = (uint8_t)out;
         }
 }
 
 // dz = dy act'(y): relu [y > 0]; tanh 1 - t^2 with t = q / 127; sigmoid s (1 - s) = (1 - t^2) / 4 with t = 2 s - 1.
-template <class T>
+template <class T, bool WHOLE>
 __global__ void __launch_bounds__(kQT)
 k_act_grad(const T *dy, int64_t ldy, const uint8_t *__restrict__ saved, int64_t lds, int64_t rows, int N, int act, T *dz,
            int64_t ldz) {
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
-    for (int j = threadIdx.x; j < N; j += kQT) {
-        const float g = (float)dy[row * ldy + j];
-        float d;
-        if (act == MZ_ACT_RELU) {
-            d = (saved[row * lds + (j >> 3)] >> (j & 7)) & 1 ? g : 0.0f;
-        } else {
-            const int q = (int8_t)saved[row * lds + j];
-            const float t = q == -128 ? __uint_as_float(0x7FC00000u) : (float)q / 127.0f;
-            d = g * ((1.0f - t * t) * (act == MZ_ACT_TANH ? 1.0f : 0.25f));
+    constexpr int n = Pack<T>::n;
+    const int t = threadIdx.x % 64;
+    for (int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; row < rows; row += (int64_t)gridDim.x * 4)
+#pragma unroll 2
+        for (int j = t * 8; j < N; j += 64 * 8) {
+            float v[8];
+            load8<T, WHOLE>(dy + row * ldy, j, N, v);
+            if (act == MZ_ACT_RELU) {
+                const unsigned bits = saved[row * lds + (j >> 3)];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = bits >> e & 1 ? v[e] : 0.0f;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int q = j + e < N ? (int8_t)saved[row * lds + j + e] : 0;
+                    const float u = q == -128 ? __uint_as_float(0x7FC00000u) : (float)q / 127.0f;
+                    v[e] *= (1.0f - u * u) * (act == MZ_ACT_TANH ? 1.0f : 0.25f);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 8 / n; ++h) {
+                Pack<T> p;
+#pragma unroll
+                for (int e = 0; e < n; ++e) p.v[e] = (T)v[h * n + e];
+                store_pack<T, WHOLE>(dz + row * ldz, j + h * n, N, p);
+            }
         }
-        dz[row * ldz + j] = (T)d;
-    }
 }
 
-// One workgroup per row up to this many (a grid holds fewer than 2^32 threads); more rows are taken in turns.
-dim3 row_grid(int64_t rows) { return dim3((unsigned)(rows < (1 << 20) ? rows : (1 << 20))); }
+// Workgroups for `rows` rows, `per` of them each, up to this many (a grid holds fewer than 2^32 threads); more rows are
+// taken in turns.
+dim3 row_grid(int64_t rows, int per) {
+    const int64_t groups = (rows + per - 1) / per;
+    return dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20)));
+}
+
+// f(true / false as a type) with whether rows can be read in 16-byte packs.
+template <class F>
+void with_flag(bool flag, F &&f) {
+    if (flag) f(std::true_type{});
+    else f(std::false_type{});
+}
 
 int check_rows(const char *what, const void *x, int type, int64_t ld, int64_t rows, int64_t K) {
     if (!type_ok(type)) return mz::fail(MZ_ERR_ARG, "%s: unknown element type %d", what, type);
@@ -148,8 +266,18 @@ int mz_quant8_rows(const void *x, int32_t type, int64_t ldx, int64_t rows, int32
     if (rows == 0) return MZ_OK;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(k_quant8<T>, row_grid(rows), dim3(kQT), 0, (hipStream_t)stream, (const T *)x, ldx, rows, K, scale_bits,
-                           codes, ldc, scales);
+        with_flag(rows_aligned<T>(x, ldx), [&](auto whole) {
+            constexpr bool W = decltype(whole)::value;
+            const auto launch = [&](auto kernel, int per) {
+                hipLaunchKernelGGL(kernel, row_grid(rows, per), dim3(kQT), 0, (hipStream_t)stream, (const T *)x, ldx, rows, K, scale_bits,
+                                   codes, ldc, scales);
+            };
+            // a wave per row up to 4 packs a lane, else a workgroup per row with as many packs as it takes, up to 20
+            const int64_t packs = ldc / Pack<T>::n;
+            if (packs <= 4 * 64) launch(k_quant8<T, 64, 4, W>, 4);
+            else if (packs <= 4 * 256) launch(k_quant8<T, 256, 4, W>, 1);
+            else launch(k_quant8<T, 256, 20, W>, 1);
+        });
     });
     return mz::check_launch("k_quant8");
 }
@@ -161,8 +289,15 @@ int mz_dequant8_rows(const int8_t *codes, int64_t ldc, const float *scales, int6
     if (rows == 0) return MZ_OK;
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(k_dequant8<T>, row_grid(rows), dim3(kQT), 0, (hipStream_t)stream, codes, ldc, scales, rows, K,
-                           (T *)x, ldx);
+        with_flag(rows_aligned<T>(x, ldx), [&](auto whole) {
+            constexpr bool W = decltype(whole)::value;
+            if (K <= 4 * 64 * Pack<T>::n)
+                hipLaunchKernelGGL((k_dequant8<T, 64, W>), row_grid(rows, 4), dim3(kQT), 0, (hipStream_t)stream, codes, ldc, scales, rows,
+                                   K, (T *)x, ldx);
+            else
+                hipLaunchKernelGGL((k_dequant8<T, 256, W>), row_grid(rows, 1), dim3(kQT), 0, (hipStream_t)stream, codes, ldc, scales, rows,
+                                   K, (T *)x, ldx);
+        });
     });
     return mz::check_launch("k_dequant8");
 }
@@ -180,8 +315,10 @@ int mz_ckpt8_act_save(const void *y, int32_t type, int64_t ldy, int64_t rows, in
     if (!saved) return mz::fail(MZ_ERR_ARG, "mz_ckpt8_act_save: NULL argument");
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(k_act_save<T>, row_grid(rows), dim3(kQT), 0, (hipStream_t)stream, (const T *)y, ldy, rows, N,
-                           activation, saved, mz_ckpt8_act_bytes(N, activation));
+        with_flag(rows_aligned<T>(y, ldy), [&](auto whole) {
+            hipLaunchKernelGGL((k_act_save<T, decltype(whole)::value>), row_grid(rows, 4), dim3(kQT), 0, (hipStream_t)stream, (const T *)y,
+                               ldy, rows, N, activation, saved, mz_ckpt8_act_bytes(N, activation));
+        });
     });
     return mz::check_launch("k_act_save");
 }
@@ -195,8 +332,10 @@ int mz_ckpt8_act_grad(const void *dy, int32_t type, int64_t ldy, const uint8_t *
     if (!saved) return mz::fail(MZ_ERR_ARG, "mz_ckpt8_act_grad: NULL argument");
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(k_act_grad<T>, row_grid(rows), dim3(kQT), 0, (hipStream_t)stream, (const T *)dy, ldy, saved,
-                           mz_ckpt8_act_bytes(N, activation), rows, N, activation, (T *)dz, ldz);
+        with_flag(rows_aligned<T>(dy, ldy) && rows_aligned<T>(dz, ldz), [&](auto whole) {
+            hipLaunchKernelGGL((k_act_grad<T, decltype(whole)::value>), row_grid(rows, 4), dim3(kQT), 0, (hipStream_t)stream, (const T *)dy,
+                               ldy, saved, mz_ckpt8_act_bytes(N, activation), rows, N, activation, (T *)dz, ldz);
+        });
     });
     return mz::check_launch("k_act_grad");
 }
