@@ -12,10 +12,10 @@
 // (values below 2^-16 of their row's largest lose bits of the second plane, values below 2^-28 of the first one: an
 // absolute error of at most 2^-25 c_n^-1 then, 2^-39 of the largest).  The two planes' products go to one float32
 // accumulator, and 1 / c_n is applied at the end, exact.
-//   k_col_stats   per column of dz: largest |v| and sum of dz, for chunks of rows
-//   k_split       dz -> planes, transposed to [n][plane][r]; db and 1 / c_n from the chunks
-//   k_codes_t     codes -> fp16, transposed to [k][r]
-//   k_weight_grad the product; k_weight_join the sum of its parts where the reduction is split
+// Both operands of the product run along the rows, so both are transposed on the way:
+//   k_col_stats, k_col_factors   per column of dz: the largest |v|, hence c_n, and the sum of dz (db); few rows: k_prepare
+//   k_prepare                    dz -> planes [n][plane][r] and codes -> fp16 [k][r], 64 rows per workgroup
+//   k_weight_grad                the product; k_weight_join the sum of its parts where the reduction is split
 #include "mz_tile.h"
 
 namespace {
@@ -24,26 +24,11 @@ using namespace mze;
 using namespace mzt8;
 
 constexpr int kCT = 256;
-constexpr int kMaxChunks = 64;
+constexpr int kMaxChunks = 64, kFewRows = 256;
 
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-template <class T>
-__global__ void __launch_bounds__(kCT)
-k_col_stats(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int chunk_rows,
-            unsigned *__restrict__ part_max, float *__restrict__ part_sum) {
-    const int n = blockIdx.x * kCT + threadIdx.x, chunk = blockIdx.y;
-    if (n >= N) return;
-    unsigned m = 0;
-    float s = 0.0f;
-    for (int r = chunk * chunk_rows; r < min(R, (chunk + 1) * chunk_rows); ++r) {
-        const float g = (float)dz[r * ldz + n];
-        m = max(m, __float_as_uint(g * scales[r]) & 0x7FFFFFFFu);
-        s += g;
-    }
-    part_max[(int64_t)chunk * N + n] = m;
-    part_sum[(int64_t)chunk * N + n] = s;
-}
+__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // The power of two that brings a column with largest magnitude `bits` to 2^14 .. 2^15, and its inverse; NaN for a column
 // with an infinity or a NaN.
@@ -58,63 +43,186 @@ __device__ __forceinline__ float column_factor(unsigned bits, float *inverse) {
     return __uint_as_float((unsigned)(127 + e) << 23);
 }
 
-// 64 x 64 values per workgroup, transposed through LDS; rows behind the last one become zeros.
-template <class T, int PLANES>
+// A workgroup takes 64 packs of columns and a chunk of rows, its four waves every fourth row.
+template <class T, bool WHOLE>
 __global__ void __launch_bounds__(kCT)
-k_split(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int64_t Rp, int chunks,
-        const unsigned *__restrict__ part_max, const float *__restrict__ part_sum, f16 *__restrict__ planes,
-        float *__restrict__ inverse, T *__restrict__ db) {
-    __shared__ float tile[64][65];
-    __shared__ float factor[64];
-    const int n0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-    if (threadIdx.x < 64) {
-        const int n = n0 + threadIdx.x;
-        unsigned m = 0;
-        float s = 0.0f;
-        if (n < N)
-            for (int c = 0; c < chunks; ++c) {
-                m = max(m, part_max[(int64_t)c * N + n]);
-                s += part_sum[(int64_t)c * N + n];
+k_col_stats(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int chunk_rows,
+            unsigned *__restrict__ part_max, float *__restrict__ part_sum) {
+    constexpr int n = Pack<T>::n;
+    __shared__ unsigned wave_max[4][64 * n];
+    __shared__ float wave_sum[4][64 * n];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunk = blockIdx.y, c0 = blockIdx.x * 64 * n, c = c0 + lane * n;
+    unsigned m[n] = {};
+    float s[n] = {};
+    const int end = min(R, (chunk + 1) * chunk_rows);
+    if (c < N)
+#pragma unroll 4
+        for (int r = chunk * chunk_rows + wave; r < end; r += 4) {
+            const Pack<T> p = load_pack<T, WHOLE>(dz + r * ldz, c, N);
+            const float scale = scales[r];
+#pragma unroll
+            for (int e = 0; e < n; ++e) {
+                const float g = (float)p.v[e];
+                m[e] = max(m[e], abs_bits(g * scale));
+                s[e] += g;
             }
-        float inv;
-        factor[threadIdx.x] = column_factor(m, &inv);
-        if (n < N && blockIdx.y == 0) {
-            inverse[n] = inv;
-            if (db) db[n] = (T)s;
+        }
+#pragma unroll
+    for (int e = 0; e < n; ++e) wave_max[wave][lane * n + e] = m[e], wave_sum[wave][lane * n + e] = s[e];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 64 * n; i += kCT)
+        if (c0 + i < N) {
+            unsigned top = 0;
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) top = max(top, wave_max[w][i]), sum += wave_sum[w][i];
+            part_max[(int64_t)chunk * N + c0 + i] = top;
+            part_sum[(int64_t)chunk * N + c0 + i] = sum;
+        }
+}
+
+template <class T>
+__global__ void __launch_bounds__(64)
+k_col_factors(const unsigned *__restrict__ part_max, const float *__restrict__ part_sum, int chunks, int N, float *__restrict__ factor,
+              float *__restrict__ inverse, T *__restrict__ db) {
+    const int n = blockIdx.x * 64 + threadIdx.x;
+    if (n >= N) return;
+    unsigned m = 0;
+    float s = 0.0f;
+#pragma unroll 8
+    for (int c = 0; c < chunks; ++c) {
+        m = max(m, part_max[(int64_t)c * N + n]);
+        s += part_sum[(int64_t)c * N + n];
+    }
+    factor[n] = column_factor(m, inverse + n);
+    if (db) db[n] = (T)s;
+}
+
+struct Prepared {  // what k_prepare leaves
+    float *factor, *inverse;
+    f16 *planes, *codes_t;
+};
+
+constexpr int kSplitCols = 64, kCodeCols = 128;
+
+// dz -> planes for 64 columns and 64 rows (STATS: the columns' factors first, from all rows).  v = dz s c is formed in
+// float32 and split before it goes to LDS; a lane then collects 8 rows of one column, 16 bytes of each plane.
+template <class T, int PLANES, bool WHOLE, bool STATS>
+__device__ void split_block(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int64_t Rp, int n0,
+                            int r0, const Prepared &out, T *__restrict__ db, uint8_t *lds) {
+    constexpr int n = Pack<T>::n, packs = kSplitCols / n, ld = kSplitCols + 1;
+    unsigned(*tile)[ld] = (unsigned(*)[ld])lds;              // [64 rows]: hi | lo << 16
+    float *factor = (float *)(lds + 64 * ld * 4);
+    const int t = threadIdx.x;
+    if constexpr (STATS) {
+        unsigned *top = (unsigned *)lds;                     // [16 row groups][64 columns]
+        float *sum = (float *)lds + 16 * kSplitCols;
+        static_assert(2 * 16 * kSplitCols <= 64 * ld, "the statistics fit the tile");
+        const int g = t >> 4, c = (t & 15) * 4;              // 4 columns, every 16th row
+        unsigned m[4] = {};
+        float s[4] = {};
+        for (int r = g; r < R; r += 16) {
+            const float scale = scales[r];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float x = n0 + c + e < N ? (float)dz[r * ldz + n0 + c + e] : 0.0f;
+                m[e] = max(m[e], abs_bits(x * scale));
+                s[e] += x;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[g * kSplitCols + c + e] = m[e], sum[g * kSplitCols + c + e] = s[e];
+        __syncthreads();
+        if (t < kSplitCols) {
+            unsigned mm = 0;
+            float ss = 0.0f;
+            for (int q = 0; q < 16; ++q) mm = max(mm, top[q * kSplitCols + t]), ss += sum[q * kSplitCols + t];
+            float inv;
+            factor[t] = column_factor(mm, &inv);
+            if (r0 == 0 && n0 + t < N) {
+                out.inverse[n0 + t] = inv;
+                if (db) db[n0 + t] = (T)ss;
+            }
+        }
+    } else if (t < kSplitCols) {
+        factor[t] = n0 + t < N ? out.factor[n0 + t] : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = t; i < 64 * packs; i += kCT) {
+        const int r = i / packs, c = i % packs * n;
+        Pack<T> p{};
+        float scale = 0.0f;
+        if (r0 + r < R && n0 + c < N) {
+            p = load_pack<T, WHOLE>(dz + (r0 + r) * ldz, n0 + c, N);
+            scale = scales[r0 + r];
+        }
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+            const float v = r0 + r < R ? ((float)p.v[e] * scale) * factor[c + e] : 0.0f;
+            const f16 hi = (f16)v, lo = (f16)(v - (float)hi);
+            tile[r][c + e] = (unsigned)__builtin_bit_cast(unsigned short, hi) | (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
         }
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 64; i += kCT) {
-        const int r = i >> 6, n = i & 63;
-        float v = 0.0f;
-        if (r0 + r < R && n0 + n < N) v = ((float)dz[(r0 + r) * ldz + n0 + n] * scales[r0 + r]) * factor[n];
-        tile[r][n] = v;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 64; i += kCT) {
-        const int n = i >> 6, r = i & 63;
-        if (n0 + n >= N) continue;
-        const float v = tile[r][n];
-        const f16 hi = (f16)v;
-        f16 *row = planes + (int64_t)(n0 + n) * PLANES * Rp;
-        row[r0 + r] = hi;
-        if (PLANES == 2) row[Rp + r0 + r] = (f16)(v - (float)hi);
+#pragma unroll
+    for (int i = t; i < kSplitCols * 8; i += kCT) {
+        const int c = i >> 3, r = (i & 7) * 8;
+        if (n0 + c >= N) continue;
+        u32x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const unsigned x = tile[r + 2 * e][c], y = tile[r + 2 * e + 1][c];
+            hi[e] = (x & 0xFFFFu) | y << 16;
+            lo[e] = x >> 16 | (y & 0xFFFF0000u);
+        }
+        f16 *row = out.planes + (int64_t)(n0 + c) * PLANES * Rp + r0 + r;
+        *(u32x4 *)row = hi;
+        if (PLANES == 2) *(u32x4 *)(row + Rp) = lo;
     }
 }
 
-__global__ void __launch_bounds__(kCT)
-k_codes_t(const int8_t *__restrict__ codes, int64_t ldc, int R, int K, int64_t Rp, f16 *__restrict__ out) {
-    __shared__ int8_t tile[64][68];
-    const int k0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-    for (int i = threadIdx.x; i < 64 * 64; i += kCT) {
-        const int r = i >> 6, k = i & 63;
-        tile[r][k] = r0 + r < R && k0 + k < K ? codes[(r0 + r) * ldc + k0 + k] : (int8_t)0;
+// codes -> fp16 for 128 columns and 64 rows: a lane collects 8 rows of 4 columns from 8 words.
+__device__ void codes_block(const int8_t *__restrict__ codes, int64_t ldc, int R, int K, int64_t Rp, int k0, int r0,
+                            f16 *__restrict__ codes_t, uint8_t *lds) {
+    constexpr int ld = kCodeCols + 4;
+    const int t = threadIdx.x;
+#pragma unroll
+    for (int i = t; i < 64 * kCodeCols / 16; i += kCT) {
+        const int r = i / (kCodeCols / 16), c = i % (kCodeCols / 16) * 16;
+        u32x4 v = {};
+        if (r0 + r < R && k0 + c < ldc) v = *(const u32x4 *)(codes + (r0 + r) * ldc + k0 + c);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *(unsigned *)(lds + r * ld + c + 4 * e) = v[e];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * 64; i += kCT) {
-        const int k = i >> 6, r = i & 63;
-        if (k0 + k < K) out[(k0 + k) * Rp + r0 + r] = (f16)(float)tile[r][k];
+#pragma unroll
+    for (int i = t; i < kCodeCols / 4 * 8; i += kCT) {
+        const int c = (i >> 3) * 4, r = (i & 7) * 8;
+        unsigned w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = *(const unsigned *)(lds + (r + e) * ld + c);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            h16x8 h;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] = (f16)(float)(int8_t)(w[e] >> 8 * q);
+            if (k0 + c + q < K) *(h16x8 *)(codes_t + (int64_t)(k0 + c + q) * Rp + r0 + r) = h;
+        }
     }
+}
+
+// Workgroups 0 .. split_blocks - 1: 64 columns of dz each; the others 128 columns of codes; all of them 64 rows.
+template <class T, int PLANES, bool WHOLE, bool STATS>
+__global__ void __launch_bounds__(kCT)
+k_prepare(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, const int8_t *__restrict__ codes,
+          int64_t ldc, int K, int64_t Rp, int split_blocks, Prepared out, T *__restrict__ db) {
+    __shared__ __align__(16) uint8_t lds[64 * (kSplitCols + 1) * 4 + kSplitCols * 4];
+    const int r0 = blockIdx.y * 64;
+    if ((int)blockIdx.x < split_blocks)
+        split_block<T, PLANES, WHOLE, STATS>(dz, ldz, scales, R, N, Rp, blockIdx.x * kSplitCols, r0, out, db, lds);
+    else
+        codes_block(codes, ldc, R, K, Rp, (blockIdx.x - split_blocks) * kCodeCols, r0, out.codes_t, lds);
 }
 
 template <class T, class Tl>
@@ -170,18 +278,20 @@ k_weight_join(const float *__restrict__ partial, int splits, const float *__rest
 struct Layout {
     int planes, chunks, chunk_rows;
     Shape shape;
-    int64_t Rp, off_sum, off_inverse, off_planes, off_codes, off_partial, bytes;
+    int64_t Rp, off_sum, off_factor, off_inverse, off_planes, off_codes, off_partial, bytes;
 };
 
 Layout layout(int32_t type, int32_t scale_bits, int64_t R, int64_t N, int64_t K) {
     Layout l;
     l.planes = type == MZ_TYPE_BF16 && scale_bits == 3 ? 1 : 2;
     l.Rp = round_up(R, 64);
-    l.chunks = (int)(R < 32 * kMaxChunks ? (R + 31) / 32 : kMaxChunks);
-    l.chunk_rows = (int)((R + l.chunks - 1) / l.chunks);
+    // few rows: every workgroup of k_prepare forms its columns' statistics itself, no launches of their own
+    l.chunks = R <= kFewRows ? 0 : (int)(R < 64 * kMaxChunks ? (R + 63) / 64 : kMaxChunks);
+    l.chunk_rows = l.chunks ? (int)((R + l.chunks - 1) / l.chunks) : 0;
     const int64_t stat = round_up((int64_t)l.chunks * N * 4, 128);
     l.off_sum = stat;
-    l.off_inverse = 2 * stat;
+    l.off_factor = 2 * stat;
+    l.off_inverse = l.off_factor + round_up(N * 4, 128);
     l.off_planes = l.off_inverse + round_up(N * 4, 128);
     l.off_codes = l.off_planes + N * l.planes * l.Rp * 2;
     l.off_partial = l.off_codes + round_up(K * l.Rp * 2, 128);
@@ -227,18 +337,31 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
     f16 *planes = (f16 *)(ws + l.off_planes), *codes_t = (f16 *)(ws + l.off_codes);
     float *partial = (float *)(ws + l.off_partial);
     hipStream_t st = (hipStream_t)stream;
-    const dim3 split_grid((unsigned)((N + 63) / 64), (unsigned)(l.Rp / 64)), codes_grid((unsigned)((K + 63) / 64), (unsigned)(l.Rp / 64));
+    const Prepared prepared{(float *)(ws + l.off_factor), inverse, planes, codes_t};
+    const int split_blocks = (N + kSplitCols - 1) / kSplitCols;
+    const dim3 grid((unsigned)(split_blocks + (K + kCodeCols - 1) / kCodeCols), (unsigned)(l.Rp / 64));
     with_type(type, [&](auto t) {
         using T = decltype(t);
-        hipLaunchKernelGGL(k_col_stats<T>, dim3((unsigned)((N + kCT - 1) / kCT), (unsigned)l.chunks), dim3(kCT), 0, st, (const T *)dz,
-                           ldz, scales, rows, N, l.chunk_rows, part_max, part_sum);
-        if (l.planes == 1)
-            hipLaunchKernelGGL((k_split<T, 1>), split_grid, dim3(kCT), 0, st, (const T *)dz, ldz, scales, rows, N, l.Rp, l.chunks,
-                               part_max, part_sum, planes, inverse, (T *)db);
-        else
-            hipLaunchKernelGGL((k_split<T, 2>), split_grid, dim3(kCT), 0, st, (const T *)dz, ldz, scales, rows, N, l.Rp, l.chunks,
-                               part_max, part_sum, planes, inverse, (T *)db);
-        hipLaunchKernelGGL(k_codes_t, codes_grid, dim3(kCT), 0, st, codes, ldc, rows, K, l.Rp, codes_t);
+        with_flag(rows_aligned<T>(dz, ldz), [&](auto whole) {
+            constexpr bool W = decltype(whole)::value;
+            if (l.chunks > 0) {
+                hipLaunchKernelGGL((k_col_stats<T, W>), dim3((unsigned)tiles_of(N, 64 * Pack<T>::n), (unsigned)l.chunks), dim3(kCT), 0, st,
+                                   (const T *)dz, ldz, scales, rows, N, l.chunk_rows, part_max, part_sum);
+                hipLaunchKernelGGL(k_col_factors<T>, dim3((unsigned)tiles_of(N, 64)), dim3(64), 0, st, part_max, part_sum, l.chunks, N,
+                                   prepared.factor, inverse, (T *)db);
+            }
+            const auto prepare = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, grid, dim3(kCT), 0, st, (const T *)dz, ldz, scales, rows, N, codes, ldc, K, l.Rp, split_blocks,
+                                   prepared, (T *)db);
+            };
+            if (l.planes == 1) {
+                if (l.chunks) prepare(k_prepare<T, 1, W, false>);
+                else prepare(k_prepare<T, 1, W, true>);
+            } else {
+                if (l.chunks) prepare(k_prepare<T, 2, W, false>);
+                else prepare(k_prepare<T, 2, W, true>);
+            }
+        });
         const auto launch = [&](auto tile) {
             using Tl = decltype(tile);
             const int tiles_k = (K + Tl::TI - 1) / Tl::TI, tiles_n = (N + Tl::TO - 1) / Tl::TO;

@@ -39,4 +39,34 @@ inline bool rows_aligned(const void *p, int64_t ld) {
     return ((uintptr_t)p & 15) == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0;
 }
 
+// Elements j .. j + n - 1 of a row of K, zeros behind its end; WHOLE: rows start on 16-byte addresses.
+template <class T, bool WHOLE>
+__device__ __forceinline__ Pack<T> load_pack(const T *__restrict__ row, int j, int K) {
+    constexpr int n = Pack<T>::n;
+    if (WHOLE && j + n <= K) return *(const Pack<T> *)(row + j);
+    Pack<T> p;
+#pragma unroll
+    for (int e = 0; e < n; ++e) p.v[e] = j + e < K ? row[j + e] : (T)0.0f;
+    return p;
+}
+
+template <class T, bool WHOLE>
+__device__ __forceinline__ void store_pack(T *__restrict__ row, int j, int K, const Pack<T> &p) {
+    constexpr int n = Pack<T>::n;
+    if (WHOLE && j + n <= K) {
+        *(Pack<T> *)(row + j) = p;
+    } else {
+#pragma unroll
+        for (int e = 0; e < n; ++e)
+            if (j + e < K) row[j + e] = p.v[e];
+    }
+}
+
+// f(true / false as a type) with whether rows can be read in 16-byte packs.
+template <class F>
+inline void with_flag(bool flag, F &&f) {
+    if (flag) f(std::true_type{});
+    else f(std::false_type{});
+}
+
 }  // namespace mze

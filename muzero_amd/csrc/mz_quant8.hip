@@ -33,29 +33,6 @@ __device__ __forceinline__ RowScale row_scale(unsigned amax_bits, int scale_bits
     return {s, 1.0f / s};
 }
 
-// Elements j .. j + n - 1 of a row of K, zeros behind its end; WHOLE: rows start on 16-byte addresses.
-template <class T, bool WHOLE>
-__device__ __forceinline__ Pack<T> load_pack(const T *__restrict__ row, int j, int K) {
-    constexpr int n = Pack<T>::n;
-    if (WHOLE && j + n <= K) return *(const Pack<T> *)(row + j);
-    Pack<T> p;
-#pragma unroll
-    for (int e = 0; e < n; ++e) p.v[e] = j + e < K ? row[j + e] : (T)0.0f;
-    return p;
-}
-
-template <class T, bool WHOLE>
-__device__ __forceinline__ void store_pack(T *__restrict__ row, int j, int K, const Pack<T> &p) {
-    constexpr int n = Pack<T>::n;
-    if (WHOLE && j + n <= K) {
-        *(Pack<T> *)(row + j) = p;
-    } else {
-#pragma unroll
-        for (int e = 0; e < n; ++e)
-            if (j + e < K) row[j + e] = p.v[e];
-    }
-}
-
 // One pack's codes.  Adding 1.5 * 2^23 rounds to a whole number, half to even, and leaves it in the low bits; the product
 // is rounded before (no fused multiply-add), as the definition says.
 template <class T>
@@ -225,13 +202,6 @@ k_act_grad(const T *dy, int64_t ldy, const uint8_t *__restrict__ saved, int64_t 
 dim3 row_grid(int64_t rows, int per) {
     const int64_t groups = (rows + per - 1) / per;
     return dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20)));
-}
-
-// f(true / false as a type) with whether rows can be read in 16-byte packs.
-template <class F>
-void with_flag(bool flag, F &&f) {
-    if (flag) f(std::true_type{});
-    else f(std::false_type{});
 }
 
 int check_rows(const char *what, const void *x, int type, int64_t ld, int64_t rows, int64_t K) {
