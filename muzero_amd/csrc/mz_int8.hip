@@ -86,6 +86,61 @@ k_int8_join(const int *__restrict__ partial, int splits, const float *__restrict
     }
 }
 
+// A few rows (at most 16 NB): bound by reading the weights once.  A workgroup takes 16 output channels and all rows, its
+// eight waves every eighth 128 bytes of the reduction; a lane reads 32 consecutive bytes of one channel and of NB rows of x
+// and feeds them to the instructions straight from registers: weights are used once, so LDS would only add a barrier.
+// The waves' sums meet in LDS.  1 x 9216 x 9216: 18 us, 4.7 TB/s (64 x 64 tiles, the reduction in four: 18 + the quantiser;
+// 1 x 4096 x 4096: 4.5 against 8.6).  32 channels per workgroup: 23 us.
+constexpr int kFewWaves = 8;
+
+template <class T, int NB>
+__global__ void __launch_bounds__(64 * kFewWaves)
+k_int8_few(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs, int rows, const int8_t *__restrict__ wc,
+           int64_t ldw, const float *__restrict__ ws, int N, int kbytes, const float *__restrict__ bias, int act, T *__restrict__ y,
+           int64_t ldy) {
+    __shared__ __align__(16) int sums[kFewWaves][256 * NB];  // [row][channel]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, n0 = blockIdx.x * 16;
+    const int8_t *w = wc + (int64_t)min(n0 + c, N - 1) * ldw + (lane >> 4) * 32, *x[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) x[b] = xc + (int64_t)min(16 * b + c, rows - 1) * ldxc + (lane >> 4) * 32;
+    i32x4 acc[NB] = {};
+    int k = wave * kStep;
+    const auto steps = [&](auto count) {  // the loads of `count` steps in flight
+        constexpr int C = decltype(count)::value;
+        u32x4 p[C][2], q[C][NB][2];
+#pragma unroll
+        for (int u = 0; u < C; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) p[u][h] = *(const u32x4 *)(w + k + u * kFewWaves * kStep + h * 16);
+#pragma unroll
+        for (int u = 0; u < C; ++u)
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) q[u][b][h] = *(const u32x4 *)(x[b] + k + u * kFewWaves * kStep + h * 16);
+#pragma unroll
+        for (int u = 0; u < C; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) acc[b] = OpI8::mfma(p[u][h], q[u][b][h], acc[b]);
+        k += C * kFewWaves * kStep;
+    };
+    while (k + 3 * kFewWaves * kStep < kbytes) steps(std::integral_constant<int, 4>{});
+    while (k < kbytes) steps(std::integral_constant<int, 1>{});
+#pragma unroll
+    for (int b = 0; b < NB; ++b) *(i32x4 *)&sums[wave][(16 * b + c) * 16 + 4 * (lane >> 4)] = acc[b];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 256 * NB; i += 64 * kFewWaves) {
+        const int r = i >> 4, n = n0 + (i & 15);
+        if (r >= rows || n >= N) continue;
+        int sum = 0;
+#pragma unroll
+        for (int q = 0; q < kFewWaves; ++q) sum += sums[q][i];
+        y[r * ldy + n] = (T)activate((float)sum * xs[r] * ws[n] + (bias ? bias[n] : 0.0f), act);
+    }
+}
+
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 int check_code_rows(const char *what, const int8_t *codes, int64_t ldc, const float *scales, int32_t K) {
@@ -151,8 +206,24 @@ void launch_tiles(const Int8Args &a, int splits, hipStream_t st) {
 
 Shape shape_of_int8(int64_t rows, int64_t N, int64_t K) { return shape_of(rows, N, round_up(K, kStep) / kStep); }
 
+template <class T, int NB>
+void launch_few(const Int8Args &a, hipStream_t st) {
+    hipLaunchKernelGGL((k_int8_few<T, NB>), dim3((unsigned)tiles_of(a.N, 16)), dim3(64 * kFewWaves), 0, st, a.xc, a.ldxc, a.xs, a.rows, a.wc,
+                       a.ldw, a.ws, a.N, (int)round_up(a.K, kStep), a.bias, a.act, (T *)a.y, a.ldy);
+}
+
+// Few rows go by k_int8_few: up to 4 always, up to 32 where the weights are small (us, k_int8_few / tiles: 16 x 4096 x 4096
+// 5.8 / 9.1, 32 x 4096 x 4096 7.8 / 10; but 16 x 9216 x 9216 26 / 19, 32 x 9216 x 18432 73 / 31, as every workgroup reads
+// all rows of x again).
+bool few_rows(int64_t rows, int64_t N, int64_t K) { return rows <= 4 || (rows <= 32 && N * K <= 24LL * 1000 * 1000); }
+
 template <class T>
 void launch_shape(const Int8Args &a, hipStream_t st) {
+    if (few_rows(a.rows, a.N, a.K)) {
+        if (a.rows <= 16) launch_few<T, 1>(a, st);
+        else launch_few<T, 2>(a, st);
+        return;
+    }
     const Shape s = shape_of_int8(a.rows, a.N, a.K);
     if (s.tile == 256) launch_tiles<T, Tile<OpI8, 256, 256, 4, 2>>(a, s.splits, st);
     else if (s.tile == 128) launch_tiles<T, Tile<OpI8, 128, 256, 2, 4>>(a, s.splits, st);
@@ -161,7 +232,7 @@ void launch_shape(const Int8Args &a, hipStream_t st) {
 
 int64_t partial_bytes(int64_t rows, int64_t N, int64_t K) {
     const Shape s = shape_of_int8(rows, N, K);
-    return s.splits > 1 ? s.splits * rows * round_up(N, 4) * 4 : 0;
+    return !few_rows(rows, N, K) && s.splits > 1 ? s.splits * rows * round_up(N, 4) * 4 : 0;
 }
 
 }  // namespace

@@ -280,7 +280,7 @@ inline Shape shape_of(int64_t outer, int64_t inner, int64_t steps) {
     if (outer * inner * steps >= 240LL * 1000 * 1000 && steps >= 64)  // a long reduction: the operands are what is read
         return {256, (int)std::max<int64_t>(1, std::min(256 / large, steps / 16))};
     const int64_t small = tiles_of(outer, 64) * tiles_of(inner, 64);
-    return {64, (int)std::max<int64_t>(1, std::min({(int64_t)8, 400 / small, steps / 16}))};
+    return {64, (int)std::max<int64_t>(1, std::min({(int64_t)8, 600 / small, steps / 16}))};
 }
 
 }  // namespace mzt8
