@@ -777,7 +777,8 @@ int mz_policy_post(const float *policy_in, int32_t B, int32_t A, int32_t softmax
  *   log_prob f32[T]   log softmax(row)[action]; actions i64[T] or NULL.  A negative action scores 0 (no action), one of
  *                     V or more NaN;
  *   entropy f32[T]    -sum p log p;
- *   stats f32[T][2]   row maximum and log of the sum of exponentials relative to it (what the backward call needs);
+ *   stats f32[T][3]   what the backward call needs of a row: its maximum, the log of the sum of exponentials relative to
+ *                     it, the entropy; NULL if no gradient will be asked for;
  *   top_actions i64[T][top], top_log_probs f32[T][top]   the `top` (0..32, at most V) largest logits, the lowest index
  *                     first among equals, NaN before everything; their log probabilities.
  * A logit of -inf is an illegal action (probability 0).  A row of nothing else has log probabilities -inf, entropy 0
@@ -790,9 +791,9 @@ int mz_policy_scores(const void *logits, int32_t type, int64_t ld, const int64_t
 /* grad[T][V] (type and shape of the logits, row stride ld_grad; it must not overlap them) =
  * d(sum g_log_prob log_prob + g_entropy entropy + g_top top_log_probs) / d logits; each g f32 and may be NULL. */
 int mz_policy_scores_backward(const void *logits, int32_t type, int64_t ld, const int64_t *actions, int64_t T,
-                              int32_t V, int32_t top, const float *stats, const float *entropy,
-                              const int64_t *top_actions, const float *g_log_prob, const float *g_entropy,
-                              const float *g_top, void *grad, int64_t ld_grad, void *stream);
+                              int32_t V, int32_t top, const float *stats, const int64_t *top_actions,
+                              const float *g_log_prob, const float *g_entropy, const float *g_top, void *grad,
+                              int64_t ld_grad, void *stream);
 
 /* Row codes: q i8[rows][ldc] and scales f32[rows] with x_rk about scales[r] * q_rk, q in -127..127 (round half to even).
  * scale_bits 24: scale = fl(max |row| / 127), q = rne(x * fl(127 / max)); scale_bits 3: that scale rounded up to three

@@ -200,7 +200,7 @@ _SIGS = {
     "mz_policy_scores": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P, C.c_int64,
                                    _P]),
     "mz_policy_scores_backward": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P,
-                                            _P, C.c_int64, _P]),
+                                            C.c_int64, _P]),
     "mz_quant8_rows": (C.c_int, [_P, C.c_int32, C.c_int64, C.c_int64, C.c_int32, C.c_int32, _P, C.c_int64, _P, _P]),
     "mz_dequant8_rows": (C.c_int, [_P, C.c_int64, _P, C.c_int64, C.c_int32, _P, C.c_int32, C.c_int64, _P]),
     "mz_int8_workspace": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32]),

@@ -265,12 +265,12 @@ int mz_int8_forward(const void *x, int32_t x_type, int64_t ldx, int32_t rows, in
                     const float *w_scales, int32_t N, const float *bias, int32_t activation, void *y, int32_t type, int64_t ldy,
                     void *workspace, int64_t workspace_bytes, void *stream) {
     MZ_TRY(check_int8(rows, K, w_codes, ldw, w_scales, N, activation, y, type, ldy));
+    if (rows == 0) return MZ_OK;
     MZ_TRY(check_workspace(workspace, workspace_bytes, mz_int8_workspace(rows, K, N)));
     const int64_t partial = round_up(partial_bytes(rows, N, K), 128), ldc = round_up(K, kStep);
     float *scales = (float *)((uint8_t *)workspace + partial);
     int8_t *codes = (int8_t *)workspace + partial + round_up((int64_t)rows * 4, 128);
     MZ_TRY(mz_quant8_rows(x, x_type, ldx, rows, K, 24, codes, ldc, scales, stream));
-    if (rows == 0) return MZ_OK;
     const Int8Args a{codes, ldc, scales, rows, w_codes, ldw, w_scales, N, K, bias, activation, y, ldy, (int *)workspace};
     with_type(type, [&](auto t) { launch_shape<decltype(t)>(a, (hipStream_t)stream); });
     return mz::check_launch("k_int8");

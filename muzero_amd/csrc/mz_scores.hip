@@ -99,9 +99,8 @@ struct Out {  // the result arrays of a call
 
     template <class T>
     __device__ void row(int64_t row, const Row &r, const T *z) const {
-        stats[2 * row] = r.m;
-        stats[2 * row + 1] = r.log_s;
         entropy[row] = r.h;
+        if (stats) stats[3 * row] = r.m, stats[3 * row + 1] = r.log_s, stats[3 * row + 2] = r.h;
         if (!actions) return;
         const int64_t a = actions[row];
         log_prob[row] = a < 0 ? 0.0f : a >= V ? NAN : log_p(r, (float)z[a]);
@@ -431,14 +430,14 @@ __device__ __forceinline__ float grad_one(const RowGrad &r, float z, int j) {
 
 struct Grads {
     const int64_t *actions;
-    const float *stats, *entropy;
+    const float *stats;
     const int64_t *top_actions;
     const float *g_lp, *g_ent, *g_top;
     int V, top;
 
     __device__ RowGrad row(int64_t row) const {
         RowGrad r;
-        r.m = stats[2 * row], r.log_s = stats[2 * row + 1], r.h = entropy[row];
+        r.m = stats[3 * row], r.log_s = stats[3 * row + 1], r.h = stats[3 * row + 2];
         r.empty = r.m == -INFINITY && r.log_s == 0.0f;
         r.a = actions ? actions[row] : -1;
         r.g_lp = g_lp && r.a >= 0 ? g_lp[row] : 0.0f;
@@ -605,7 +604,7 @@ int mz_policy_scores(const void *logits, int32_t type, int64_t ld, const int64_t
                      void *workspace, int64_t workspace_bytes, void *stream) {
     MZ_TRY(check_logits("mz_policy_scores", logits, type, ld, T, V, top));
     if (T == 0) return MZ_OK;
-    if (!entropy || !stats || (actions && !log_prob) || (top > 0 && (!top_actions || !top_log_probs)))
+    if (!entropy || (actions && !log_prob) || (top > 0 && (!top_actions || !top_log_probs)))
         return mz::fail(MZ_ERR_ARG, "mz_policy_scores: NULL argument");
     const int64_t need = mz_policy_scores_workspace(type, T, V, top);
     if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
@@ -620,16 +619,16 @@ int mz_policy_scores(const void *logits, int32_t type, int64_t ld, const int64_t
 }
 
 int mz_policy_scores_backward(const void *logits, int32_t type, int64_t ld, const int64_t *actions, int64_t T, int32_t V,
-                              int32_t top, const float *stats, const float *entropy, const int64_t *top_actions,
+                              int32_t top, const float *stats, const int64_t *top_actions,
                               const float *g_log_prob, const float *g_entropy, const float *g_top, void *grad, int64_t ld_grad,
                               void *stream) {
     MZ_TRY(check_logits("mz_policy_scores_backward", logits, type, ld, T, V, top));
     MZ_TRY(check_logits("mz_policy_scores_backward", grad, type, ld_grad, T, V, top));
     if (T == 0) return MZ_OK;
-    if (!stats || !entropy || (g_top && top > 0 && !top_actions) || (g_log_prob && !actions))
+    if (!stats || (g_top && top > 0 && !top_actions) || (g_log_prob && !actions))
         return mz::fail(MZ_ERR_ARG, "mz_policy_scores_backward: NULL argument");
     if (top == 0) g_top = nullptr;
-    const Grads in{actions, stats, entropy, top_actions, g_log_prob, g_entropy, g_top, V, top};
+    const Grads in{actions, stats, top_actions, g_log_prob, g_entropy, g_top, V, top};
     with_type(type, [&](auto t) {
         using E = decltype(t);
         launch_grad((const E *)logits, ld, T, in, (E *)grad, ld_grad, (hipStream_t)stream);

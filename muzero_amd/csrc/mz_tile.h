@@ -264,7 +264,7 @@ struct Shape {
     int splits;  // parts of the reduction, joined by a second kernel
 };
 
-inline int64_t tiles_of(int64_t n, int64_t t) { return (n + t - 1) / t; }
+inline int64_t tiles_of(int64_t n, int64_t t) { return n > 0 ? (n + t - 1) / t : 1; }
 
 // Large tiles read each operand less often, small ones fill the 256 compute units with less work.  Measured (int8, us;
 // 64 / 128 x 256 / 256 tiles, best number of parts in brackets):

@@ -28,17 +28,17 @@ MAX_TOP = 32
 class PolicyScores(NamedTuple):
     log_prob: Optional[torch.Tensor]       # f32[...]       log p(action), None without actions
     entropy: torch.Tensor                  # f32[...]       -sum p log p
-    top_actions: torch.Tensor              # i64[..., top]  largest logits first, the lowest index among equals
-    top_log_probs: torch.Tensor            # f32[..., top]
+    top_actions: Optional[torch.Tensor]    # i64[..., top]  largest logits first, the lowest index among equals; None: top=0
+    top_log_probs: Optional[torch.Tensor]  # f32[..., top]
 
 
-def _forward(logits: torch.Tensor, actions: Optional[torch.Tensor], top: int):
+def _forward(logits: torch.Tensor, actions: Optional[torch.Tensor], top: int, want_stats: bool):
     T, V = logits.shape
-    f32 = dict(dtype=torch.float32, device=logits.device)
-    log_prob = torch.empty(T, **f32) if actions is not None else None
-    entropy, stats = torch.empty(T, **f32), torch.empty((T, 2), **f32)
-    top_actions = torch.empty((T, top), dtype=torch.int64, device=logits.device)
-    top_log_probs = torch.empty((T, top), **f32)
+    log_prob = None if actions is None else logits.new_empty(T, dtype=torch.float32)
+    entropy = logits.new_empty(T, dtype=torch.float32)
+    stats = logits.new_empty((T, 3), dtype=torch.float32) if want_stats else None
+    top_actions = logits.new_empty((T, top), dtype=torch.int64) if top else None
+    top_log_probs = logits.new_empty((T, top), dtype=torch.float32) if top else None
     if T > 0:
         lib, kind = _hip.lib(), TYPE[logits.dtype]
         with on_device(logits):
@@ -50,29 +50,37 @@ def _forward(logits: torch.Tensor, actions: Optional[torch.Tensor], top: int):
     return log_prob, entropy, stats, top_actions, top_log_probs
 
 
+def _gradient(ctx, g_log_prob, g_entropy, _g_actions, g_top):
+    logits, actions, stats, top_actions = ctx.saved_tensors
+    T, V = logits.shape
+    grad = logits.new_empty((T, V))
+    if T > 0:
+        g_log_prob, g_entropy, g_top = (g if g is None else g.contiguous() for g in (g_log_prob, g_entropy, g_top))
+        with on_device(logits):
+            _hip.check(_hip.lib().mz_policy_scores_backward(
+                ptr(logits), TYPE[logits.dtype], row_stride(logits), ptr(actions), T, V, 0 if g_top is None else g_top.shape[1],
+                ptr(stats), ptr(top_actions), ptr(g_log_prob), ptr(g_entropy), ptr(g_top), ptr(grad), V,
+                stream_of(logits)), "mz_policy_scores_backward")
+    return grad, None, None
+
+
 class _PolicyScores(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, actions, top):
-        log_prob, entropy, stats, top_actions, top_log_probs = _forward(logits, actions, top)
-        ctx.save_for_backward(logits, actions, stats, entropy, top_actions)
+        log_prob, entropy, stats, top_actions, top_log_probs = _forward(logits, actions, top, True)
+        ctx.save_for_backward(logits, actions, stats, top_actions)
         ctx.set_materialize_grads(False)
-        ctx.mark_non_differentiable(top_actions)
+        if top:
+            ctx.mark_non_differentiable(top_actions)
         return log_prob, entropy, top_actions, top_log_probs
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g_log_prob, g_entropy, _g_actions, g_top):
-        logits, actions, stats, entropy, top_actions = ctx.saved_tensors
-        T, V = logits.shape
-        grad = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
-        if T > 0:
-            g_log_prob, g_entropy, g_top = (g if g is None else g.contiguous() for g in (g_log_prob, g_entropy, g_top))
-            with on_device(logits):
-                _hip.check(_hip.lib().mz_policy_scores_backward(
-                    ptr(logits), TYPE[logits.dtype], row_stride(logits), ptr(actions), T, V, top_actions.shape[1], ptr(stats),
-                    ptr(entropy), ptr(top_actions), ptr(g_log_prob), ptr(g_entropy), ptr(g_top), ptr(grad), V,
-                    stream_of(logits)), "mz_policy_scores_backward")
-        return grad, None, None
+    def backward(ctx, *grads):
+        # the guard against a second derivative is needed (and paid for) only where a graph of the gradient is built
+        return _guarded_gradient(ctx, *grads) if torch.is_grad_enabled() else _gradient(ctx, *grads)
+
+
+_guarded_gradient = once_differentiable(_gradient)
 
 
 def policy_scores(logits: torch.Tensor, actions: Optional[torch.Tensor] = None, top: int = 0) -> PolicyScores:
@@ -101,10 +109,13 @@ def policy_scores(logits: torch.Tensor, actions: Optional[torch.Tensor] = None, 
     if torch.is_grad_enabled() and rows.requires_grad:
         log_prob, entropy, top_actions, top_log_probs = _PolicyScores.apply(rows, actions, top)
     else:
-        log_prob, entropy, _, top_actions, top_log_probs = _forward(rows, actions, top)
+        log_prob, entropy, _, top_actions, top_log_probs = _forward(rows, actions, top, False)
     if len(lead) != 1:
-        log_prob = log_prob if log_prob is None else log_prob.reshape(lead)
-        entropy, top_actions, top_log_probs = entropy.reshape(lead), top_actions.reshape(*lead, top), top_log_probs.reshape(*lead, top)
+        entropy = entropy.reshape(lead)
+        if log_prob is not None:
+            log_prob = log_prob.reshape(lead)
+        if top:
+            top_actions, top_log_probs = top_actions.reshape(*lead, top), top_log_probs.reshape(*lead, top)
     return PolicyScores(log_prob, entropy, top_actions, top_log_probs)
 
 

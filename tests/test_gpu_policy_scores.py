@@ -190,10 +190,11 @@ def test_gradient_matches_the_formula(T, V, top, dtype):
     got, = torch.autograd.grad(outs, z, gs)
     assert got.dtype == dtype and got.shape == z.shape
     d = lambda t: t.detach().cpu().double()  # noqa: E731
-    want, tol = _grad_reference(d(z), a.cpu(), s.top_actions.cpu(), d(g_lp), d(g_ent), d(g_top) if top else None)
+    want, tol = _grad_reference(d(z), a.cpu(), s.top_actions.cpu() if top else None, d(g_lp), d(g_ent),
+                                d(g_top) if top else None)
     _close(got, want, tol + HALF[dtype] * (want.abs() + tol) + TINY[dtype])
     only_h, = torch.autograd.grad(_scores(z).entropy, z, g_ent)
-    want, tol = _grad_reference(d(z), a.cpu(), s.top_actions.cpu(), None, d(g_ent), None)
+    want, tol = _grad_reference(d(z), a.cpu(), None, None, d(g_ent), None)
     _close(only_h, want, tol + HALF[dtype] * (want.abs() + tol) + TINY[dtype])
 
 
@@ -315,3 +316,19 @@ def test_network_scores_and_learner_report():
     assert torch.equal(s.top_actions[:, 0], policy.argmax(1))
     (-s.log_prob.mean() - 0.01 * s.entropy.mean()).backward()
     assert all(p.grad is not None and p.grad.isfinite().all() for n, p in f.named_parameters() if n.startswith("policy"))
+
+
+def test_results_may_be_changed_in_place_and_have_no_second_derivative():
+    z, a = _make(5, 9, torch.float32)
+    z.requires_grad_(True)
+    s = _scores(z, a)
+    assert s.top_actions is None and s.top_log_probs is None and _scores(z).log_prob is None
+    want, = torch.autograd.grad(s.log_prob.clamp(min=-2.0).sum(), z)
+    s = _scores(z, a)
+    loss = s.log_prob.clamp_(min=-2.0).sum()
+    s.entropy.detach().zero_()
+    got, = torch.autograd.grad(loss, z)
+    assert torch.equal(want, got)
+    g, = torch.autograd.grad(_scores(z, a).entropy.sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()

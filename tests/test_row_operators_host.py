@@ -30,19 +30,17 @@ def test_policy_scores_refusals():
     _refused(call(logits=None), "NULL")
     _refused(call(logits=P + 2), "misaligned")
     _refused(call(ent=None), "NULL")
-    _refused(call(stats=None), "NULL")
     _refused(call(lp=None), "NULL")
     _refused(call(ids=None), "NULL")
     _refused(call(tlp=None), "NULL")
     assert call(T=0, logits=None, ent=None) == 0
     b = _hip.lib().mz_policy_scores_backward
 
-    def back(logits=P, ld=7, actions=P, T=4, V=7, top=2, stats=P, ent=P, ids=P, g=P, gh=P, gt=P, grad=P, ldg=7):
-        return b(logits, F32, ld, actions, T, V, top, stats, ent, ids, g, gh, gt, grad, ldg, None)
+    def back(logits=P, ld=7, actions=P, T=4, V=7, top=2, stats=P, ids=P, g=P, gh=P, gt=P, grad=P, ldg=7):
+        return b(logits, F32, ld, actions, T, V, top, stats, ids, g, gh, gt, grad, ldg, None)
     _refused(back(grad=None), "NULL")
     _refused(back(ldg=5), "stride")
     _refused(back(stats=None), "NULL")
-    _refused(back(ent=None), "NULL")
     _refused(back(ids=None), "NULL")
     _refused(back(actions=None), "NULL")
     assert back(T=0, logits=None, grad=None) == 0
