@@ -16,6 +16,7 @@
 //   k_col_stats, k_col_factors   per column of dz: the largest |v|, hence c_n, and the sum of dz (db); few rows: k_prepare
 //   k_prepare                    dz -> planes [n][plane][r] and codes -> fp16 [k][r], 64 rows per workgroup
 //   k_weight_grad                the product; k_weight_join the sum of its parts where the reduction is split
+#include "mz_codes.h"
 #include "mz_tile.h"
 
 namespace {
@@ -27,8 +28,6 @@ constexpr int kCT = 256;
 constexpr int kMaxChunks = 64, kFewRows = 256;
 
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
-
-__device__ __forceinline__ unsigned abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
 
 // The power of two that brings a column with largest magnitude `bits` to 2^14 .. 2^15, and its inverse; NaN for a column
 // with an infinity or a NaN.
@@ -263,13 +262,9 @@ template <class T>
 __global__ void __launch_bounds__(256)
 k_weight_join(const float *__restrict__ partial, int splits, const float *__restrict__ inverse, int K, int N, T *__restrict__ dw,
               int64_t ldw, bool aligned) {
-    const int quads = (K + 3) / 4;
-    const int64_t jobs = (int64_t)N * quads;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < jobs; q += (int64_t)gridDim.x * 256) {
-        const int n = (int)(q / quads), k = 4 * (int)(q - (int64_t)n * quads);
-        f32x4 sum = *(const f32x4 *)(partial + q * 4);
-        for (int p = 1; p < splits; ++p) sum += *(const f32x4 *)(partial + (p * jobs + q) * 4);
-        sum *= inverse[n];
+    const int quads = (K + 3) / 4, n = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x, k = 4 * c;
+    if (c < quads) {
+        const f32x4 sum = sum_parts<f32x4>(partial, splits, (int64_t)N * quads, (int64_t)n * quads + c) * inverse[n];
         const float o[4] = {sum[0], sum[1], sum[2], sum[3]};
         store_quad(dw + n * ldw, k, K, aligned, o);
     }
@@ -370,8 +365,7 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
                                codes_t, planes, inverse, K, N, l.Rp, l.planes, (T *)dw, ldw, aligned, tiles_k, tiles_n, l.shape.splits,
                                partial);
             if (l.shape.splits > 1) {
-                const int64_t groups = ((int64_t)N * ((K + 3) / 4) + 255) / 256;
-                hipLaunchKernelGGL(k_weight_join<T>, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, st, partial,
+                hipLaunchKernelGGL(k_weight_join<T>, dim3((unsigned)tiles_of(K, 1024), (unsigned)N), dim3(256), 0, st, partial,
                                    l.shape.splits, inverse, K, N, (T *)dw, ldw, aligned);
             }
         };

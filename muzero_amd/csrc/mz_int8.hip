@@ -4,6 +4,7 @@
 // the sum in 32-bit integers, which K <= 131072 keeps exact.
 #include <cmath>
 
+#include "mz_codes.h"
 #include "mz_tile.h"
 
 namespace {
@@ -71,19 +72,14 @@ template <class T>
 __global__ void __launch_bounds__(256)
 k_int8_join(const int *__restrict__ partial, int splits, const float *__restrict__ xs, int rows, const float *__restrict__ ws, int N,
             const float *__restrict__ bias, int act, T *__restrict__ y, int64_t ldy, bool aligned) {
-    const int quads = (N + 3) / 4;
-    const int64_t jobs = (int64_t)rows * quads;
-    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < jobs; q += (int64_t)gridDim.x * 256) {
-        const int r = (int)(q / quads), n = 4 * (int)(q - (int64_t)r * quads);
-        i32x4 sum = *(const i32x4 *)(partial + q * 4);
-        for (int p = 1; p < splits; ++p) sum += *(const i32x4 *)(partial + (p * jobs + q) * 4);
-        const float s = xs[r];
-        float o[4];
+    const int quads = (N + 3) / 4, r = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x, n = 4 * c;
+    if (c >= quads) return;
+    const i32x4 sum = sum_parts<i32x4>(partial, splits, (int64_t)rows * quads, (int64_t)r * quads + c);
+    const float s = xs[r];
+    float o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            o[e] = n + e < N ? activate((float)sum[e] * s * ws[n + e] + (bias ? bias[n + e] : 0.0f), act) : 0.0f;
-        store_quad(y + r * ldy, n, N, aligned, o);
-    }
+    for (int e = 0; e < 4; ++e) o[e] = n + e < N ? activate((float)sum[e] * s * ws[n + e] + (bias ? bias[n + e] : 0.0f), act) : 0.0f;
+    store_quad(y + r * ldy, n, N, aligned, o);
 }
 
 // A few rows (at most 16 NB): bound by reading the weights once.  A workgroup takes 16 output channels and all rows, its
@@ -138,6 +134,93 @@ k_int8_few(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict_
 #pragma unroll
         for (int q = 0; q < kFewWaves; ++q) sum += sums[q][i];
         y[r * ldy + n] = (T)activate((float)sum * xs[r] * ws[n] + (bias ? bias[n] : 0.0f), act);
+    }
+}
+
+// The same for up to kFusedRows rows that are not coded yet, in one launch: every workgroup codes them for itself, into
+// LDS, while its first weights are on their way (a row of 9216 float32 comes from L2; a launch of the quantiser of its own
+// costs more than that).
+constexpr int kFusedRows = 4, kFusedBytes = 40960;
+
+int64_t fused_stride(int64_t K) { return (K + 127) / 128 * 128 + 16; }  // rows of codes in different banks
+
+template <class T, bool WHOLE>
+__global__ void __launch_bounds__(64 * kFewWaves)
+k_int8_fused(const T *__restrict__ xp, int64_t ldx, int rows, int K, const int8_t *__restrict__ wc, int64_t ldw,
+             const float *__restrict__ ws, int N, const float *__restrict__ bias, int act, T *__restrict__ y, int64_t ldy) {
+    extern __shared__ __align__(16) uint8_t codes[];
+    __shared__ __align__(16) int sums[kFewWaves][16 * 16];
+    __shared__ unsigned top[kFusedRows][kFewWaves];
+    constexpr int n = Pack<T>::n, threads = 64 * kFewWaves, U = 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, n0 = blockIdx.x * 16, kbytes = (K + 127) / 128 * 128,
+              stride = kbytes + 16;
+    const int8_t *w = wc + (int64_t)min(n0 + c, N - 1) * ldw + (lane >> 4) * 32;
+    u32x4 first[U][2];  // the first weights, before anything is waited for
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int k = (wave + u * kFewWaves) * kStep;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) first[u][h] = k < kbytes ? *(const u32x4 *)(w + k + h * 16) : u32x4{};
+    }
+    for (int r = 0; r < rows; ++r) {
+        unsigned m = 0;
+#pragma unroll 4
+        for (int j = threadIdx.x * n; j < K; j += threads * n) {
+            const Pack<T> p = load_pack<T, WHOLE>(xp + r * ldx, j, K);
+#pragma unroll
+            for (int e = 0; e < n; ++e) m = max(m, abs_bits((float)p.v[e]));
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o));
+        if (lane == 0) top[r][wave] = m;
+    }
+    __syncthreads();
+    for (int r = 0; r < rows; ++r) {
+        unsigned m = 0;
+#pragma unroll
+        for (int q = 0; q < kFewWaves; ++q) m = max(m, top[r][q]);
+        const RowScale rs = row_scale(m, 24);
+#pragma unroll 4
+        for (int j = threadIdx.x * n; j < kbytes; j += threads * n)
+            store_codes((int8_t *)codes + r * stride + j, load_pack<T, WHOLE>(xp + r * ldx, j, K), rs.inverse);
+    }
+    __syncthreads();
+    const uint8_t *x = codes + min(c, rows - 1) * stride + (lane >> 4) * 32;
+    i32x4 acc = {};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int k = (wave + u * kFewWaves) * kStep;
+        if (k < kbytes)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc = OpI8::mfma(first[u][h], *(const u32x4 *)(x + k + h * 16), acc);
+    }
+    int k = (wave + U * kFewWaves) * kStep;
+    const auto steps = [&](auto count) {
+        constexpr int C = decltype(count)::value;
+        u32x4 p[C][2];
+#pragma unroll
+        for (int u = 0; u < C; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) p[u][h] = *(const u32x4 *)(w + k + u * kFewWaves * kStep + h * 16);
+#pragma unroll
+        for (int u = 0; u < C; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) acc = OpI8::mfma(p[u][h], *(const u32x4 *)(x + k + u * kFewWaves * kStep + h * 16), acc);
+        k += C * kFewWaves * kStep;
+    };
+    while (k + (U - 1) * kFewWaves * kStep < kbytes) steps(std::integral_constant<int, U>{});
+    while (k < kbytes) steps(std::integral_constant<int, 1>{});
+    *(i32x4 *)&sums[wave][c * 16 + 4 * (lane >> 4)] = acc;
+    __syncthreads();
+    if (threadIdx.x < 256) {
+        const int r = threadIdx.x >> 4, o = n0 + (threadIdx.x & 15);
+        if (r < rows && o < N) {
+            unsigned m = 0;
+            int sum = 0;
+#pragma unroll
+            for (int q = 0; q < kFewWaves; ++q) m = max(m, top[r][q]), sum += sums[q][threadIdx.x];
+            y[r * ldy + o] = (T)activate((float)sum * row_scale(m, 24).scale * ws[o] + (bias ? bias[o] : 0.0f), act);
+        }
     }
 }
 
@@ -198,9 +281,8 @@ void launch_tiles(const Int8Args &a, int splits, hipStream_t st) {
                        a.wc, a.ldw, a.ws, a.N, (int)round_up(a.K, kStep), a.bias, a.act, (T *)a.y, a.ldy, aligned, tiles_n, tiles_r, splits,
                        a.partial);
     if (splits > 1) {
-        const int64_t groups = ((int64_t)a.rows * ((a.N + 3) / 4) + 255) / 256;
-        hipLaunchKernelGGL(k_int8_join<T>, dim3((unsigned)(groups < 4096 ? groups : 4096)), dim3(256), 0, st, a.partial, splits, a.xs, a.rows,
-                           a.ws, a.N, a.bias, a.act, (T *)a.y, a.ldy, aligned);
+        hipLaunchKernelGGL(k_int8_join<T>, dim3((unsigned)tiles_of(a.N, 1024), (unsigned)a.rows), dim3(256), 0, st, a.partial, splits, a.xs,
+                           a.rows, a.ws, a.N, a.bias, a.act, (T *)a.y, a.ldy, aligned);
     }
 }
 
@@ -216,6 +298,11 @@ void launch_few(const Int8Args &a, hipStream_t st) {
 // 5.8 / 9.1, 32 x 4096 x 4096 7.8 / 10; but 16 x 9216 x 9216 26 / 19, 32 x 9216 x 18432 73 / 31, as every workgroup reads
 // all rows of x again).
 bool few_rows(int64_t rows, int64_t N, int64_t K) { return rows <= 4 || (rows <= 32 && N * K <= 24LL * 1000 * 1000); }
+
+// One launch where x has the result's type and its codes fit a workgroup's share of LDS.
+bool fused(int32_t x_type, int32_t type, int64_t rows, int64_t K) {
+    return x_type == type && rows <= kFusedRows && rows * fused_stride(K) <= kFusedBytes;
+}
 
 template <class T>
 void launch_shape(const Int8Args &a, hipStream_t st) {
@@ -267,6 +354,18 @@ int mz_int8_forward(const void *x, int32_t x_type, int64_t ldx, int32_t rows, in
     MZ_TRY(check_int8(rows, K, w_codes, ldw, w_scales, N, activation, y, type, ldy));
     if (rows == 0) return MZ_OK;
     MZ_TRY(check_workspace(workspace, workspace_bytes, mz_int8_workspace(rows, K, N)));
+    if (fused(x_type, type, rows, K)) {
+        MZ_TRY(check_rows("mz_int8_forward", x, x_type, ldx, rows, K));
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            with_flag(rows_aligned<T>(x, ldx), [&](auto whole) {
+                hipLaunchKernelGGL((k_int8_fused<T, decltype(whole)::value>), dim3((unsigned)tiles_of(N, 16)), dim3(64 * kFewWaves),
+                                   (size_t)(rows * fused_stride(K)), (hipStream_t)stream, (const T *)x, ldx, rows, K, w_codes, ldw, w_scales, N,
+                                   bias, activation, (T *)y, ldy);
+            });
+        });
+        return mz::check_launch("k_int8_fused");
+    }
     const int64_t partial = round_up(partial_bytes(rows, N, K), 128), ldc = round_up(K, kStep);
     float *scales = (float *)((uint8_t *)workspace + partial);
     int8_t *codes = (int8_t *)workspace + partial + round_up((int64_t)rows * 4, 128);

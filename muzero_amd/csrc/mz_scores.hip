@@ -220,9 +220,10 @@ struct Shared {
     Key cand[kCand];
     unsigned best[kLT];
     Key thread_key[kLT];
+    int owner[kLT];
     Key found[kMaxTop];
     Key threshold;
-    int count;
+    int count, owners;
 };
 
 // Largest value t (its low 16 order bits dropped) that at least `top` of the workgroup's threads reach with their own
@@ -242,40 +243,56 @@ __device__ __forceinline__ float value_threshold(const Shared &sh, int top) {
     return t <= order_bits(-INFINITY) ? -INFINITY : bits_value(t);
 }
 
-// The candidates in sh.cand, ranked: the `top` first ones go to sh.found in order.
+// The candidates in sh.cand, ranked by counting the larger ones: the `top` first go to sh.found in order.
 __device__ __forceinline__ void rank_candidates(Shared &sh, int count, int top) {
-    for (int c = threadIdx.x; c < count; c += kLT) {
-        const Key k = sh.cand[c];
-        int rank = 0;
-        for (int o = 0; o < count; ++o) rank += sh.cand[o] > k;
-        if (rank < top) sh.found[rank] = k;
+    if (count <= 64) {  // in the registers of one wave
+        if (threadIdx.x < 64) {
+            const Key k = (int)threadIdx.x < count ? sh.cand[threadIdx.x] : 0;
+            int rank = 0;
+            for (int o = 0; o < count; ++o) {
+                const Key other = ((Key)(unsigned)__builtin_amdgcn_readlane((int)(k >> 32), o) << 32) |
+                                  (unsigned)__builtin_amdgcn_readlane((int)k, o);
+                rank += other > k;
+            }
+            if (rank < top && k != 0) sh.found[rank] = k;
+        }
+    } else {
+        for (int c = threadIdx.x; c < count; c += kLT) {
+            const Key k = sh.cand[c];
+            int rank = 0;
+            for (int o = 0; o < count; ++o) rank += sh.cand[o] > k;
+            if (rank < top) sh.found[rank] = k;
+        }
     }
     __syncthreads();
 }
 
 // sh.found = the `top` first alternatives among the logits of `span` (at least `top` of them), which every thread has
 // streamed in the order of add(): its own largest one is in sh.best.  `loud`: there is a NaN or an infinity.
-//  1. candidates are the logits that reach value_threshold; only the packs of threads that reach it are read again, each
-//     such thread's by its whole wave;
+//  1. candidates are the logits that reach value_threshold; only the packs of threads that reach it are read again, by
+//     all threads together;
 //  2. rows with too many equal values for that (all masked, all equal): the same with (value, index) keys;
 //  3. whatever overflows that, too: one alternative per pass.
 template <class T>
 __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool loud) {
     constexpr int n = Span<T>::n;
-    const int lane = threadIdx.x & 63, wave0 = threadIdx.x & ~63;
+    const int per_thread = (span.packs + kLT - 1) / kLT;
     float v[n];
+    // the logits of the threads with `mine` that are `wanted`; sh.count and sh.owners are 0 before
     const auto collect = [&](bool mine, auto &&wanted) {
-        for (unsigned long long left = __ballot(mine); left; left &= left - 1) {
-            const int owner = wave0 + __builtin_ctzll(left);
-            for (int i = owner + lane * kLT; i < span.packs; i += 64 * kLT) {
-                span.load(i, v);
+        if (mine) sh.owner[atomicAdd(&sh.owners, 1)] = threadIdx.x;
+        __syncthreads();
+        const int items = sh.owners * per_thread;
+        for (int q = threadIdx.x; q < items; q += kLT) {
+            const int o = q / per_thread, i = sh.owner[o] + (q - o * per_thread) * kLT;
+            if (i >= span.packs) continue;
+            span.load(i, v);
 #pragma unroll
-                for (int e = 0; e < n; ++e) {
-                    const int j = span.at(i) + e;
-                    if (span.owns(j) && wanted(v[e], j)) {
-                        const int c = atomicAdd(&sh.count, 1);
-                        if (c < kCand) sh.cand[c] = order_key(v[e], j);
-                    }
+            for (int e = 0; e < n; ++e) {
+                const int j = span.at(i) + e;
+                if (span.owns(j) && wanted(v[e], j)) {
+                    const int c = atomicAdd(&sh.count, 1);
+                    if (c < kCand) sh.cand[c] = order_key(v[e], j);
                 }
             }
         }
@@ -285,7 +302,7 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
     int count = kCand + 1;
     if (!loud) {
         const float t = value_threshold(sh, top);
-        if (threadIdx.x == 0) sh.count = 0;
+        if (threadIdx.x == 0) sh.count = 0, sh.owners = 0;
         __syncthreads();
         count = collect(sh.best[threadIdx.x] >= order_bits(t), [&](float z, int) { return z >= t; });
         if (count > kCand) {
@@ -301,14 +318,14 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
             }
             __syncthreads();  // everybody has read sh.count
             sh.thread_key[threadIdx.x] = mine;
-            if (threadIdx.x == 0) sh.count = 0, sh.threshold = 0;  // fewer owning threads than top: everything
+            if (threadIdx.x == 0) sh.count = 0, sh.owners = 0, sh.threshold = 0;  // fewer owning threads than top: everything
             __syncthreads();
             int rank = 0;
             for (int o = 0; o < kLT; ++o) rank += sh.thread_key[o] > mine;
             if (rank == top - 1 && mine != 0) sh.threshold = mine;
             __syncthreads();
             const Key t2 = sh.threshold;
-            count = collect(mine >= t2, [&](float z, int j) { return order_key(z, j) >= t2; });
+            count = collect(mine >= t2 && mine != 0, [&](float z, int j) { return order_key(z, j) >= t2; });
         }
     }
     if (count <= kCand) {
@@ -329,7 +346,7 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
         }
         best = wave_max(best);
         __syncthreads();
-        if (lane == 0) sh.thread_key[threadIdx.x >> 6] = best;
+        if ((threadIdx.x & 63) == 0) sh.thread_key[threadIdx.x >> 6] = best;
         __syncthreads();
         last = sh.thread_key[0];
         for (int w = 1; w < kLT / 64; ++w) last = max(last, sh.thread_key[w]);
@@ -394,21 +411,28 @@ template <class T>
 __global__ void __launch_bounds__(64)
 k_scores_join(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts, Out out, const Sums *__restrict__ part_sums,
               const Key *__restrict__ part_keys) {
+    __shared__ Key lists[kMaxParts * kMaxTop], found[kMaxTop];
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const int lane = threadIdx.x, top = out.top;
+#pragma unroll 8
+        for (int i = lane; i < parts * top; i += 64) lists[i] = part_keys[row * parts * top + i];
         Sums acc = lane < parts ? part_sums[row * parts + lane] : none();
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1) acc = join(acc, {__shfl_xor(acc.m, o), __shfl_xor(acc.s, o), __shfl_xor(acc.u, o)});
         const Row r = row_of(acc);
         if (lane == 0) out.row(row, r, logits + row * ld);
-        const Key *list = part_keys + (row * parts + lane) * top;
-        int next = 0;
-        Key head = top > 0 && lane < parts ? list[0] : 0;
+        __syncthreads();
+        int next = lane * top;
+        const int end = lane < parts ? next + top : next;
+        Key head = next < end ? lists[next] : 0;
         for (int i = 0; i < top; ++i) {
             const Key best = wave_max(head);
-            if (lane == 0) out.alternative(row, i, r, best);
-            if (head == best) head = ++next < top ? list[next] : 0;  // keys are unique: one lane moves on
+            if (lane == 0) found[i] = best;
+            if (head == best) head = ++next < end ? lists[next] : 0;  // keys are unique: one lane moves on
         }
+        __syncthreads();
+        if (lane < top) out.alternative(row, lane, r, found[lane]);
+        __syncthreads();
     }
 }
 
@@ -519,8 +543,11 @@ constexpr int64_t kMaxGrid = 1 << 20;
 dim3 grid_of(int64_t n) { return dim3((unsigned)(n < kMaxGrid ? n : kMaxGrid)); }
 
 // Rows of more than kSmall logits are streamed; fewer rows than kFill workgroups are cut into parts of at least
-// kPartBytes, so that a short batch of long rows still reaches all 256 compute units.
-constexpr int kSmall = 1024, kFill = 1024, kPartBytes = 16384;
+// kPartBytes, so that a short batch of long rows still reaches all 256 compute units.  us for kFill 256 / 512 / 1024:
+// 64 x 131072 (fp16, 20 alternatives) 20.8 / 17.2 / 18.6, 256 x 131072 40.8 / 33.7 / 31.0, 300 x 32768 (float32, 5)
+// 14.1 / 16.4 / 17.3, 1000 x 8192 10.5 / 10.3 / 18.0; kPartBytes 8192 / 16384 / 32768: 1 x 131072 (bf16, 5) 10.2 / 10.5 /
+// 11.4, 8 x 4096 (float32) 9.3 / 5.8 / 5.8.
+constexpr int kSmall = 1024, kFill = 512, kPartBytes = 16384;
 
 int parts_of(int32_t type, int64_t T, int32_t V) {
     if (V <= kSmall || T >= kFill) return 1;

@@ -258,6 +258,23 @@ __device__ __forceinline__ TileAt tile_at(int b, int tiles_i, int tiles_o, int b
     return {u / h, o0 + u % h};
 }
 
+// Four consecutive values summed over the parts of a split reduction, in the order of the parts, eight loads in flight:
+// part p's quad q lies at partial + (p quads + q) * 4.
+template <class V, class E>
+__device__ __forceinline__ V sum_parts(const E *__restrict__ partial, int splits, int64_t quads, int64_t q) {
+    V sum = *(const V *)(partial + q * 4);
+    for (int p0 = 1; p0 < splits; p0 += 8) {
+        V v[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+            if (p0 + p < splits) v[p] = *(const V *)(partial + ((p0 + p) * quads + q) * 4);
+#pragma unroll
+        for (int p = 0; p < 8; ++p)
+            if (p0 + p < splits) sum += v[p];
+    }
+    return sum;
+}
+
 // Tile size and parts of the reduction for an output of `outer` x `inner` values and `steps` steps.
 struct Shape {
     int tile;    // 64 x 64, 128 (inner) x 256 (outer) or 256 x 256, named by the inner size
@@ -280,7 +297,7 @@ inline Shape shape_of(int64_t outer, int64_t inner, int64_t steps) {
     if (outer * inner * steps >= 240LL * 1000 * 1000 && steps >= 64)  // a long reduction: the operands are what is read
         return {256, (int)std::max<int64_t>(1, std::min(256 / large, steps / 16))};
     const int64_t small = tiles_of(outer, 64) * tiles_of(inner, 64);
-    return {64, (int)std::max<int64_t>(1, std::min({(int64_t)8, 600 / small, steps / 16}))};
+    return {64, (int)std::max<int64_t>(1, std::min({(int64_t)32, 600 / small, steps / 16}))};
 }
 
 }  // namespace mzt8
