@@ -120,6 +120,7 @@ __device__ void split_block(const T *__restrict__ dz, int64_t ldz, const float *
         const int g = t >> 4, c = (t & 15) * 4;              // 4 columns, every 16th row
         unsigned m[4] = {};
         float s[4] = {};
+#pragma unroll 4
         for (int r = g; r < R; r += 16) {
             const float scale = scales[r];
 #pragma unroll

@@ -15,15 +15,15 @@ namespace {
 using namespace mze;
 
 constexpr int kQT = 256;
-// THREADS threads per row (64: four rows per workgroup, 256: one).  The first HELD packs of a thread stay in registers
-// between the maximum and the codes; the rest of a longer row is read again, from cache.  Bound by the memory: 113 MB of
-// float32 in (1536 x 18432) in 34 us, 4.1 TB/s with the codes.
+// THREADS threads per row (64: four rows per workgroup).  The first HELD packs of a thread stay in registers between the
+// maximum and the codes; the rest of a longer row is read again, from cache.  Bound by the memory: 1536 x 18432 float32,
+// 142 MB with the codes, 26 us, 5.3 TB/s.
 template <class T, int THREADS, int HELD, bool WHOLE>
-__global__ void __launch_bounds__(kQT)
+__global__ void __launch_bounds__(THREADS < kQT ? kQT : THREADS)
 k_quant8(const T *__restrict__ x, int64_t ldx, int64_t rows, int K, int scale_bits, int8_t *__restrict__ codes, int64_t ldc,
          float *__restrict__ scales) {
-    constexpr int n = Pack<T>::n, per = kQT / THREADS;
-    __shared__ unsigned part[kQT / 64];
+    constexpr int n = Pack<T>::n, per = THREADS < kQT ? kQT / THREADS : 1;
+    __shared__ unsigned part[THREADS / 64];
     const int t = threadIdx.x % THREADS, packs = (int)(ldc / n);
     for (int64_t row0 = (int64_t)blockIdx.x * per; row0 < rows; row0 += (int64_t)gridDim.x * per) {
         const int64_t row = row0 + threadIdx.x / THREADS;
@@ -51,7 +51,7 @@ k_quant8(const T *__restrict__ x, int64_t ldx, int64_t rows, int K, int scale_bi
             if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < kQT / 64; ++w) m = max(m, part[w]);
+            for (int w = 0; w < THREADS / 64; ++w) m = max(m, part[w]);
         }
         const RowScale rs = row_scale(m, scale_bits);
         if (t == 0) scales[row] = rs.scale;
@@ -189,15 +189,19 @@ int mz_quant8_rows(const void *x, int32_t type, int64_t ldx, int64_t rows, int32
         using T = decltype(t);
         with_flag(rows_aligned<T>(x, ldx), [&](auto whole) {
             constexpr bool W = decltype(whole)::value;
-            const auto launch = [&](auto kernel, int per) {
-                hipLaunchKernelGGL(kernel, row_grid(rows, per), dim3(kQT), 0, (hipStream_t)stream, (const T *)x, ldx, rows, K, scale_bits,
+            const auto launch = [&](auto kernel, int per, int threads = kQT) {
+                hipLaunchKernelGGL(kernel, row_grid(rows, per), dim3(threads), 0, (hipStream_t)stream, (const T *)x, ldx, rows, K, scale_bits,
                                    codes, ldc, scales);
             };
-            // a wave per row up to 4 packs a lane, else a workgroup per row with as many packs as it takes, up to 20
+            // A wave per row up to 4 packs a lane, else a workgroup of 256 or 1024 threads, with as few registers for packs
+            // as hold the row (1536 x 18432 float32: 1024 threads 26 us, 512 29 us, 256 37 us).
             const int64_t packs = ldc / Pack<T>::n;
-            if (packs <= 4 * 64) launch(k_quant8<T, 64, 4, W>, 4);
+            if (packs <= 2 * 64) launch(k_quant8<T, 64, 2, W>, 4);
+            else if (packs <= 4 * 64) launch(k_quant8<T, 64, 4, W>, 4);
+            else if (packs <= 2 * 256) launch(k_quant8<T, 256, 2, W>, 1);
             else if (packs <= 4 * 256) launch(k_quant8<T, 256, 4, W>, 1);
-            else launch(k_quant8<T, 256, 20, W>, 1);
+            else if (packs <= 2 * 1024) launch(k_quant8<T, 1024, 2, W>, 1, 1024);
+            else launch(k_quant8<T, 1024, 5, W>, 1, 1024);
         });
     });
     return mz::check_launch("k_quant8");
