@@ -9,6 +9,7 @@ import torch
 from muzero_amd import _hip
 
 TYPE = {torch.float32: _hip.TYPE_F32, torch.bfloat16: _hip.TYPE_BF16, torch.float16: _hip.TYPE_F16}
+MAX_ROWS, MAX_COLUMNS = (1 << 31) - 1, 1 << 30
 _NULL = contextlib.nullcontext()
 
 
@@ -18,6 +19,10 @@ def check_tensor(t: torch.Tensor, what: str) -> None:
         raise TypeError(f"{what} must be a tensor, not {type(t).__name__}")
     if t.dtype not in TYPE:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+    check_on_gpu(t, what)
+
+
+def check_on_gpu(t: torch.Tensor, what: str) -> None:
     if not t.is_cuda:
         raise _hip.HipError(f"{what} must be on the GPU (there is no CPU fallback for the kernels)")
 
@@ -30,6 +35,8 @@ def rows_of(t: torch.Tensor) -> torch.Tensor:
         t = t.reshape(-1, cols) if cols else t.reshape(t.shape[:-1].numel(), 0)
     if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
         t = t.contiguous()
+    if t.shape[0] > MAX_ROWS or t.shape[1] > MAX_COLUMNS:
+        raise ValueError(f"{t.shape[0]} rows of {t.shape[1]} values are more than a call takes ({MAX_ROWS} of {MAX_COLUMNS})")
     return t
 
 

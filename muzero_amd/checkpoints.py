@@ -52,7 +52,7 @@ def weight_grad(dz: torch.Tensor, saved: QuantizedRows, want_bias: bool = True):
         with on_device(dz):
             need = lib.mz_ckpt8_workspace(kind, saved.scale_bits, R, N, K)
             ws = workspace(need, dz)
-            _hip.check(lib.mz_ckpt8_weight_grad(ptr(dz), kind, row_stride(dz), R, N, ptr(saved.codes), saved.codes.stride(0),
+            _hip.check(lib.mz_ckpt8_weight_grad(ptr(dz), kind, row_stride(dz), R, N, ptr(saved.codes), saved.ld,
                                                 ptr(saved.scales), saved.scale_bits, K, ptr(dw), K, ptr(db), ptr(ws), need,
                                                 stream_of(dz)), "mz_ckpt8_weight_grad")
     return dw, db
@@ -79,16 +79,20 @@ def _act_grad(dy: torch.Tensor, saved: torch.Tensor, activation: str) -> torch.T
     return dz
 
 
+def _activate_(y: torch.Tensor, activation: str) -> torch.Tensor:
+    if activation == "relu":
+        return y.relu_()
+    if activation == "tanh":
+        return y.tanh_()
+    if activation == "sigmoid":
+        return y.sigmoid_()
+    return y
+
+
 class _CheckpointedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, activation):
-        y = F.linear(x, weight, bias)
-        if activation == "relu":
-            y = y.relu_()
-        elif activation == "tanh":
-            y = y.tanh_()
-        elif activation == "sigmoid":
-            y = y.sigmoid_()
+        y = _activate_(F.linear(x, weight, bias), activation)
         codes = scales = act = None
         if y.numel() > 0:
             if ctx.needs_input_grad[1]:
@@ -111,7 +115,7 @@ class _CheckpointedLinear(torch.autograd.Function):
         if want_x:
             dx = (dz @ weight.to(dz.dtype)).reshape(ctx.x_shape).to(ctx.x_dtype)
         if codes is not None:
-            saved = QuantizedRows(codes, scales, torch.Size((codes.shape[0], K)), ctx.x_dtype, 3)
+            saved = QuantizedRows._of(codes, scales, torch.Size((codes.shape[0], K)), ctx.x_dtype, 3)
             dw, db = weight_grad(dz, saved, want_bias=want_b)
             dw, db = dw.to(ctx.w_dtype), None if db is None else db.to(ctx.w_dtype)
         else:
@@ -132,6 +136,8 @@ def checkpointed_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[to
         raise ValueError(f"x of shape {tuple(x.shape)} does not match a weight of shape {tuple(weight.shape)}")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be one of {ACTIVATIONS}, not {activation!r}")
+    if not torch.is_grad_enabled():
+        return _activate_(F.linear(x, weight, bias), activation)
     return _CheckpointedLinear.apply(x, weight, bias, activation)
 
 

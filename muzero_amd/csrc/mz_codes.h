@@ -46,7 +46,7 @@ __device__ __forceinline__ void store_codes(int8_t *out, const Pack<T> &p, float
 
 inline int check_rows(const char *what, const void *x, int type, int64_t ld, int64_t rows, int64_t K) {
     if (!type_ok(type)) return mz::fail(MZ_ERR_ARG, "%s: unknown element type %d", what, type);
-    if (rows < 0 || rows > 0x7FFFFFFF || K <= 0 || K > 0x7FFFFF00)
+    if (rows < 0 || rows > 0x7FFFFFFF || K <= 0 || K > (1 << 30))
         return mz::fail(MZ_ERR_ARG, "%s: bad dimensions rows=%lld K=%lld", what, (long long)rows, (long long)K);
     if (rows > 0 && !x) return mz::fail(MZ_ERR_ARG, "%s: NULL argument", what);
     if (ld < K) return mz::fail(MZ_ERR_ARG, "%s: row stride %lld below the %lld values of a row", what, (long long)ld, (long long)K);

@@ -236,7 +236,7 @@ int check_code_rows(const char *what, const int8_t *codes, int64_t ldc, const fl
 
 int check_int8(int32_t rows, int32_t K, const int8_t *w_codes, int64_t ldw, const float *w_scales, int32_t N, int32_t activation,
                const void *y, int32_t type, int64_t ldy) {
-    if (rows < 0 || K <= 0 || N <= 0) return mz::fail(MZ_ERR_ARG, "mz_int8_forward: bad dimensions rows=%d K=%d N=%d", rows, K, N);
+    if (rows < 0 || K <= 0 || N <= 0 || N > (1 << 26)) return mz::fail(MZ_ERR_ARG, "mz_int8_forward: bad dimensions rows=%d K=%d N=%d", rows, K, N);
     if (K > kMaxK) return mz::fail(MZ_ERR_ARG, "mz_int8_forward: K=%d above %d would overflow the 32-bit sums", K, kMaxK);
     if (!type_ok(type)) return mz::fail(MZ_ERR_ARG, "mz_int8_forward: unknown element type %d", type);
     if (activation < MZ_ACT_NONE || activation > MZ_ACT_SIGMOID)

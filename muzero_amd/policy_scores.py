@@ -92,8 +92,6 @@ def policy_scores(logits: torch.Tensor, actions: Optional[torch.Tensor] = None, 
     if logits.dim() < 1 or logits.shape[-1] < 1:
         raise ValueError(f"logits need at least one action in their last dimension, not shape {tuple(logits.shape)}")
     lead, V = logits.shape[:-1], logits.shape[-1]
-    if V > 1 << 30:
-        raise ValueError(f"{V} actions are more than a call takes")
     if not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"top={top} must lie in 0..{MAX_TOP} and not exceed the {V} actions")
     if actions is not None:

@@ -11,28 +11,53 @@ networks (muzero_amd.engine): choose it where that is enough.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
 from typing import Optional
 
 import torch
 
 from muzero_amd import _hip
 from muzero_amd._hip import ptr
-from muzero_amd._rows import TYPE, check_tensor, on_device, row_stride, rows_of, stream_of, workspace
+from muzero_amd._rows import TYPE, check_on_gpu, check_tensor, on_device, row_stride, rows_of, stream_of, workspace
 
 MAX_K = 131072  # sums of K products of codes stay exact in 32 bits
 ACTIVATIONS = ("none", "linear", "relu", "tanh", "sigmoid")
 
 
-@dataclass(frozen=True)
 class QuantizedRows:
-    """Rows in 8 bits: x[r, k] is about scales[r] * codes[r, k].  `codes` is padded with zeros to a row stride of a
-    multiple of 128 bytes."""
-    codes: torch.Tensor        # i8[rows, ldc]
-    scales: torch.Tensor       # f32[rows]
-    shape: torch.Size          # of the tensor that was coded
-    dtype: torch.dtype         # of the tensor that was coded
-    scale_bits: int            # significant bits of the scales: 24 or 3
+    """Rows in 8 bits: x[r, k] is about scales[r] * codes[r, k].
+
+    codes       i8[rows, ldc], ldc a multiple of 128, rows on 16-byte addresses; zero behind the last column
+    scales      f32[rows]
+    shape       of the tensor that was coded
+    dtype       of the tensor that was coded, float32, bfloat16 or float16
+    scale_bits  significant bits of the scales: 24, or 3 if every one is 1, 1.25, 1.5 or 1.75 times a power of two"""
+
+    __slots__ = ("codes", "scales", "shape", "dtype", "scale_bits")
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape, dtype: torch.dtype, scale_bits: int):
+        shape = torch.Size(shape)
+        if codes.dtype != torch.int8 or codes.dim() != 2 or scales.dtype != torch.float32 or scales.dim() != 1:
+            raise TypeError("codes must be an int8 matrix and scales a float32 vector")
+        if codes.device != scales.device:
+            raise ValueError(f"codes are on {codes.device}, scales on {scales.device}")
+        if dtype not in TYPE:
+            raise TypeError(f"rows are of float32, bfloat16 or float16, not {dtype}")
+        if scale_bits not in (24, 3):
+            raise ValueError(f"scale_bits must be 24 or 3, not {scale_bits}")
+        rows, ldc = codes.shape
+        if len(shape) < 1 or not 1 <= shape[-1] <= ldc or rows != shape[:-1].numel() or scales.shape[0] != rows:
+            raise ValueError(f"codes of shape {tuple(codes.shape)} and {scales.shape[0]} scales do not hold a tensor of shape {tuple(shape)}")
+        if ldc % 128 or codes.data_ptr() % 16 or not scales.is_contiguous() or codes.stride(1) != 1 or (
+                rows > 1 and (codes.stride(0) % 128 or codes.stride(0) < ldc)):
+            raise ValueError("codes need rows of a multiple of 128 adjacent bytes on 16-byte addresses, scales adjacent values")
+        self.codes, self.scales, self.shape, self.dtype, self.scale_bits = codes, scales, shape, dtype, scale_bits
+
+    @classmethod
+    def _of(cls, codes, scales, shape, dtype, scale_bits) -> "QuantizedRows":
+        """Without the checks, for codes this package has laid out itself."""
+        q = object.__new__(cls)
+        q.codes, q.scales, q.shape, q.dtype, q.scale_bits = codes, scales, shape, dtype, scale_bits
+        return q
 
     @property
     def rows(self) -> int:
@@ -42,16 +67,22 @@ class QuantizedRows:
     def columns(self) -> int:
         return self.shape[-1]
 
+    @property
+    def ld(self) -> int:
+        """Bytes from one row of codes to the next."""
+        return self.codes.stride(0) if self.codes.shape[0] > 1 else self.codes.shape[1]
+
     def dequantize(self, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
         """scales * codes in the shape and (by default) the type of the tensor that was coded."""
         dtype = self.dtype if dtype is None else dtype
         if dtype not in TYPE:
             raise TypeError(f"rows can be read back as float32, bfloat16 or float16, not {dtype}")
+        check_on_gpu(self.codes, "codes")
         out = torch.empty(self.shape, dtype=dtype, device=self.codes.device)
         if self.rows > 0:
             with on_device(out):
-                _hip.check(_hip.lib().mz_dequant8_rows(ptr(self.codes), self.codes.stride(0), ptr(self.scales), self.rows, self.columns,
-                                                       ptr(out), TYPE[dtype], self.columns, stream_of(out)), "mz_dequant8_rows")
+                _hip.check(_hip.lib().mz_dequant8_rows(ptr(self.codes), self.ld, ptr(self.scales), self.rows, self.columns, ptr(out),
+                                                       TYPE[dtype], self.columns, stream_of(out)), "mz_dequant8_rows")
         return out
 
 
@@ -65,13 +96,13 @@ def quantize_rows(x: torch.Tensor, scale_bits: int = 24) -> QuantizedRows:
         raise ValueError(f"x needs at least one value in a row, not shape {tuple(x.shape)}")
     rows = rows_of(x.detach())
     R, K = rows.shape
-    codes = torch.empty((R, (K + 127) // 128 * 128), dtype=torch.int8, device=x.device)
-    scales = torch.empty(R, dtype=torch.float32, device=x.device)
+    codes = rows.new_empty((R, (K + 127) // 128 * 128), dtype=torch.int8)
+    scales = rows.new_empty(R, dtype=torch.float32)
     if R > 0:
         with on_device(rows):
             _hip.check(_hip.lib().mz_quant8_rows(ptr(rows), TYPE[rows.dtype], row_stride(rows), R, K, scale_bits, ptr(codes),
-                                                 codes.stride(0), ptr(scales), stream_of(rows)), "mz_quant8_rows")
-    return QuantizedRows(codes, scales, x.shape, x.dtype, scale_bits)
+                                                 codes.shape[1], ptr(scales), stream_of(rows)), "mz_quant8_rows")
+    return QuantizedRows._of(codes, scales, x.shape, x.dtype, scale_bits)
 
 
 def _check_weight(weight: QuantizedRows, K: int) -> int:
@@ -111,6 +142,7 @@ def int8_linear(x, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, a
         if bias.shape != (N,) or bias.device != dev:
             raise ValueError(f"bias must be {N} values on {dev}")
         bias = bias.detach().to(torch.float32).contiguous()
+    check_on_gpu(weight.codes, "weight")
     K = weight.columns
     y = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype, device=dev)
     if y.numel() == 0:
@@ -120,15 +152,15 @@ def int8_linear(x, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, a
         if coded:
             need = lib.mz_int8_codes_workspace(x.rows, K, N)
             ws = workspace(need, y)
-            _hip.check(lib.mz_int8_forward_codes(ptr(x.codes), x.codes.stride(0), ptr(x.scales), x.rows, K, ptr(weight.codes),
-                                                 weight.codes.stride(0), ptr(weight.scales), N, ptr(bias), act, ptr(y), TYPE[out_dtype],
+            _hip.check(lib.mz_int8_forward_codes(ptr(x.codes), x.ld, ptr(x.scales), x.rows, K, ptr(weight.codes),
+                                                 weight.ld, ptr(weight.scales), N, ptr(bias), act, ptr(y), TYPE[out_dtype],
                                                  N, ptr(ws), need, stream_of(y)), "mz_int8_forward_codes")
         else:
             rows = rows_of(x.detach())
             need = lib.mz_int8_workspace(rows.shape[0], K, N)
             ws = workspace(need, y)
             _hip.check(lib.mz_int8_forward(ptr(rows), TYPE[rows.dtype], row_stride(rows), rows.shape[0], K, ptr(weight.codes),
-                                           weight.codes.stride(0), ptr(weight.scales), N, ptr(bias), act, ptr(y), TYPE[out_dtype], N,
+                                           weight.ld, ptr(weight.scales), N, ptr(bias), act, ptr(y), TYPE[out_dtype], N,
                                            ptr(ws), need, stream_of(y)), "mz_int8_forward")
     return y
 

@@ -311,6 +311,48 @@ def test_kept_activations(N, dtype, activation):
         assert _act_grad(dy, _act_save(y2, activation), activation)[1, 0].isnan()
 
 
+def test_a_row_with_an_infinity_is_loud_in_the_gradient():
+    from muzero_amd.checkpoints import save_activations, weight_grad
+    for R in (20, 700):
+        x, dz = torch.randn(R, 50, device="cuda"), torch.randn(R, 30, device="cuda")
+        x[3, 7] = torch.inf
+        for t in TYPES:
+            dw, db = weight_grad(dz.to(t), save_activations(x.to(t)))
+            assert dw.isnan().all() and db.isfinite().all()
+
+
+def test_layers_of_unusual_use():
+    """No gradient wanted of some inputs, several leading dimensions, no rows at all, a strided gradient, no_grad."""
+    from muzero_amd.checkpoints import checkpointed_linear
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(40, 24).cuda()
+    x = torch.randn(3, 5, 40, device="cuda")
+    want = torch.relu(lin(x))
+    dy = torch.randn(3, 24, 5, device="cuda").transpose(1, 2)
+    full = checkpointed_linear(x.clone().requires_grad_(True), lin.weight, lin.bias, "relu")
+    assert torch.equal(full, want)
+    xr = x.clone().requires_grad_(True)
+    ref = torch.autograd.grad(checkpointed_linear(xr, lin.weight, lin.bias, "relu"), (xr, lin.weight, lin.bias), dy)
+    w, b = lin.weight.detach(), lin.bias.detach()
+    got, = torch.autograd.grad(checkpointed_linear(xr, w, b, "relu"), xr, dy)
+    assert torch.equal(got, ref[0]) and got.shape == x.shape
+    got, = torch.autograd.grad(checkpointed_linear(x, lin.weight, b, "relu"), lin.weight, dy)
+    assert torch.equal(got, ref[1])
+    got, = torch.autograd.grad(checkpointed_linear(x, w, lin.bias, "relu"), lin.bias, dy)
+    np.testing.assert_allclose(got.detach().cpu(), ref[2].detach().cpu(), rtol=0, atol=15 * U * float(dy.abs().max()) * 15)
+    got = torch.autograd.grad(checkpointed_linear(xr, lin.weight, None, "tanh"), (xr, lin.weight), dy)
+    assert all(g.isfinite().all() for g in got)
+    none = torch.zeros(0, 40, device="cuda", requires_grad=True)
+    got = torch.autograd.grad(checkpointed_linear(none, lin.weight, lin.bias, "relu").sum(), (none, lin.weight, lin.bias))
+    assert got[0].shape == (0, 40) and all((g == 0).all() for g in got)
+    with torch.no_grad():
+        y = checkpointed_linear(xr, lin.weight, lin.bias, "sigmoid")
+    assert not y.requires_grad and torch.equal(y, torch.sigmoid(lin(x)))
+    g, = torch.autograd.grad(checkpointed_linear(xr, lin.weight, lin.bias).sum(), xr, create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
+
+
 def test_a_layer_keeps_a_quarter_of_the_bytes():
     from muzero_amd.checkpoints import checkpointed_linear
     lin = torch.nn.Linear(2048, 1024).cuda()

@@ -57,6 +57,7 @@ def test_row_code_refusals():
         return q(x, kind, ldx, rows, K, bits, codes, ldc, scales, None)
     _refused(quant(kind=-1), "type")
     _refused(quant(K=0), "K=0")
+    _refused(quant(K=(1 << 30) + 16, ldx=1 << 31, ldc=1 << 31), "K=")
     _refused(quant(rows=-1), "rows=-1")
     _refused(quant(ldx=99), "stride")
     _refused(quant(bits=8), "scale_bits")
@@ -88,6 +89,7 @@ def test_int8_refusals():
         _refused(f(rows=-1), "rows=-1")
         _refused(f(K=0), "K=0")
         _refused(f(N=0), "N=0")
+        _refused(f(N=(1 << 26) + 1, ldy=1 << 27), "N=")
         _refused(f(w=None), "NULL")
         _refused(f(ws=None), "NULL")
         _refused(f(ldw=112), "128 bytes")
@@ -167,6 +169,28 @@ def test_python_refusals():
         int8_linear(rows, coded, bias=torch.zeros(5))
     with pytest.raises(_hip.HipError, match="GPU"):
         weight_grad(torch.zeros(2, 3), rows)
+    with pytest.raises(_hip.HipError, match="GPU"):   # codes on the CPU do not reach a kernel
+        int8_linear(rows, coded)
+    with pytest.raises(_hip.HipError, match="GPU"):
+        rows.dequantize()
+
+
+def test_rows_that_do_not_hold_their_shape_are_refused():
+    """A kernel trusts the shape of QuantizedRows; whoever builds them by hand is checked."""
+    from muzero_amd.quantized import QuantizedRows
+    c, s = torch.zeros(4, 256, dtype=torch.int8), torch.zeros(4)
+    make = lambda codes=c, scales=s, shape=(4, 200), dtype=torch.float32, bits=24: QuantizedRows(codes, scales, shape, dtype, bits)  # noqa: E731
+    q = make()
+    assert (q.rows, q.columns, q.ld, q.shape) == (4, 200, 256, torch.Size((4, 200))) and make(shape=(2, 2, 256)).rows == 4
+    assert make(codes=torch.zeros(8, 256, dtype=torch.int8)[::2]).ld == 512
+    for bad in (dict(codes=c.float()), dict(codes=c[0]), dict(scales=s.double()), dict(scales=torch.zeros(4, 1)), dict(dtype=torch.float64)):
+        with pytest.raises(TypeError):
+            make(**bad)
+    for bad in (dict(shape=(4, 257)), dict(shape=(5, 200)), dict(shape=(4, 0)), dict(shape=()), dict(scales=torch.zeros(3)), dict(bits=8),
+                dict(codes=c[:, :200]), dict(codes=c[:, ::2]), dict(codes=c[:, 8:136]), dict(codes=torch.zeros(4, 264, dtype=torch.int8)[:, :256]),
+                dict(codes=c[:1].expand(4, 256)), dict(scales=torch.zeros(8)[::2])):
+        with pytest.raises(ValueError):
+            make(**bad)
 
 
 def test_dense_sequences_are_recognised():
