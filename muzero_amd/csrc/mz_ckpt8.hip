@@ -13,7 +13,9 @@
 // absolute error of at most 2^-25 c_n^-1 then, 2^-39 of the largest).  The two planes' products go to one float32
 // accumulator, and 1 / c_n is applied at the end, exact.
 // Both operands of the product run along the rows, so both are transposed on the way:
-//   k_col_stats, k_col_factors   per column of dz: the largest |v|, hence c_n, and the sum of dz (db); few rows: k_prepare
+//   k_col_stats, k_col_factors   per column of dz: the largest |v|, hence c_n, and the sum of dz (db), from chunks of rows;
+//                                up to 1024 rows k_prepare joins the chunks itself, up to 256 it reads the columns itself:
+//                                a launch costs more than that
 //   k_prepare                    dz -> planes [n][plane][r] and codes -> fp16 [k][r], 64 rows per workgroup
 //   k_weight_grad                the product; k_weight_join the sum of its parts where the reduction is split
 #include "mz_codes.h"
@@ -25,7 +27,9 @@ using namespace mze;
 using namespace mzt8;
 
 constexpr int kCT = 256;
-constexpr int kMaxChunks = 64, kFewRows = 256;
+constexpr int kMaxChunks = 64, kFewRows = 256, kFewChunks = 16;
+
+enum Stats { kOwn, kChunks, kReady };  // where k_prepare's column factors come from
 
 int64_t round_up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
@@ -97,23 +101,25 @@ k_col_factors(const unsigned *__restrict__ part_max, const float *__restrict__ p
     if (db) db[n] = (T)s;
 }
 
-struct Prepared {  // what k_prepare leaves
+struct Prepared {  // what k_prepare reads of the statistics, and what it leaves
+    const unsigned *part_max;
+    const float *part_sum;
+    int chunks;
     float *factor, *inverse;
     f16 *planes, *codes_t;
 };
 
 constexpr int kSplitCols = 64, kCodeCols = 128;
 
-// dz -> planes for 64 columns and 64 rows (STATS: the columns' factors first, from all rows).  v = dz s c is formed in
-// float32 and split before it goes to LDS; a lane then collects 8 rows of one column, 16 bytes of each plane.
-template <class T, int PLANES, bool WHOLE, bool STATS>
+// dz -> planes for 64 columns and 64 rows, the columns' factors first.  v = dz s c is formed in float32 and split before it goes to LDS; a lane then collects 8 rows of one column, 16 bytes of each plane.
+template <class T, int PLANES, bool WHOLE, Stats STATS>
 __device__ void split_block(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int64_t Rp, int n0,
                             int r0, const Prepared &out, T *__restrict__ db, uint8_t *lds) {
     constexpr int n = Pack<T>::n, packs = kSplitCols / n, ld = kSplitCols + 1;
     unsigned(*tile)[ld] = (unsigned(*)[ld])lds;              // [64 rows]: hi | lo << 16
     float *factor = (float *)(lds + 64 * ld * 4);
     const int t = threadIdx.x;
-    if constexpr (STATS) {
+    if constexpr (STATS == kOwn) {
         unsigned *top = (unsigned *)lds;                     // [16 row groups][64 columns]
         float *sum = (float *)lds + 16 * kSplitCols;
         static_assert(2 * 16 * kSplitCols <= 64 * ld, "the statistics fit the tile");
@@ -143,6 +149,18 @@ __device__ void split_block(const T *__restrict__ dz, int64_t ldz, const float *
                 out.inverse[n0 + t] = inv;
                 if (db) db[n0 + t] = (T)ss;
             }
+        }
+    } else if (STATS == kChunks && t < kSplitCols) {
+        unsigned m = 0;
+        float s = 0.0f, inv;
+        if (n0 + t < N)
+#pragma unroll
+            for (int c = 0; c < kFewChunks; ++c)
+                if (c < out.chunks) m = max(m, out.part_max[(int64_t)c * N + n0 + t]), s += out.part_sum[(int64_t)c * N + n0 + t];
+        factor[t] = column_factor(m, &inv);
+        if (r0 == 0 && n0 + t < N) {
+            out.inverse[n0 + t] = inv;
+            if (db) db[n0 + t] = (T)s;
         }
     } else if (t < kSplitCols) {
         factor[t] = n0 + t < N ? out.factor[n0 + t] : 0.0f;
@@ -213,7 +231,7 @@ __device__ void codes_block(const int8_t *__restrict__ codes, int64_t ldc, int R
 }
 
 // Workgroups 0 .. split_blocks - 1: 64 columns of dz each; the others 128 columns of codes; all of them 64 rows.
-template <class T, int PLANES, bool WHOLE, bool STATS>
+template <class T, int PLANES, bool WHOLE, Stats STATS>
 __global__ void __launch_bounds__(kCT)
 k_prepare(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, const int8_t *__restrict__ codes,
           int64_t ldc, int K, int64_t Rp, int split_blocks, Prepared out, T *__restrict__ db) {
@@ -333,7 +351,7 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
     f16 *planes = (f16 *)(ws + l.off_planes), *codes_t = (f16 *)(ws + l.off_codes);
     float *partial = (float *)(ws + l.off_partial);
     hipStream_t st = (hipStream_t)stream;
-    const Prepared prepared{(float *)(ws + l.off_factor), inverse, planes, codes_t};
+    const Prepared prepared{part_max, part_sum, l.chunks, (float *)(ws + l.off_factor), inverse, planes, codes_t};
     const int split_blocks = (N + kSplitCols - 1) / kSplitCols;
     const dim3 grid((unsigned)(split_blocks + (K + kCodeCols - 1) / kCodeCols), (unsigned)(l.Rp / 64));
     with_type(type, [&](auto t) {
@@ -343,20 +361,22 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
             if (l.chunks > 0) {
                 hipLaunchKernelGGL((k_col_stats<T, W>), dim3((unsigned)tiles_of(N, 64 * Pack<T>::n), (unsigned)l.chunks), dim3(kCT), 0, st,
                                    (const T *)dz, ldz, scales, rows, N, l.chunk_rows, part_max, part_sum);
+            }
+            if (l.chunks > kFewChunks)
                 hipLaunchKernelGGL(k_col_factors<T>, dim3((unsigned)tiles_of(N, 64)), dim3(64), 0, st, part_max, part_sum, l.chunks, N,
                                    prepared.factor, inverse, (T *)db);
-            }
-            const auto prepare = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, grid, dim3(kCT), 0, st, (const T *)dz, ldz, scales, rows, N, codes, ldc, K, l.Rp, split_blocks,
-                                   prepared, (T *)db);
+            const auto prepare = [&](auto planes_tag) {
+                constexpr int P = decltype(planes_tag)::value;
+                const auto go = [&](auto kernel) {
+                    hipLaunchKernelGGL(kernel, grid, dim3(kCT), 0, st, (const T *)dz, ldz, scales, rows, N, codes, ldc, K, l.Rp, split_blocks,
+                                       prepared, (T *)db);
+                };
+                if (l.chunks == 0) go(k_prepare<T, P, W, kOwn>);
+                else if (l.chunks <= kFewChunks) go(k_prepare<T, P, W, kChunks>);
+                else go(k_prepare<T, P, W, kReady>);
             };
-            if (l.planes == 1) {
-                if (l.chunks) prepare(k_prepare<T, 1, W, false>);
-                else prepare(k_prepare<T, 1, W, true>);
-            } else {
-                if (l.chunks) prepare(k_prepare<T, 2, W, false>);
-                else prepare(k_prepare<T, 2, W, true>);
-            }
+            if (l.planes == 1) prepare(std::integral_constant<int, 1>{});
+            else prepare(std::integral_constant<int, 2>{});
         });
         const auto launch = [&](auto tile) {
             using Tl = decltype(tile);

@@ -51,16 +51,23 @@ def _forward(logits: torch.Tensor, actions: Optional[torch.Tensor], top: int, wa
 
 
 def _gradient(ctx, g_log_prob, g_entropy, _g_actions, g_top):
+    # Runs on autograd's thread for the device, where every Python object it touches comes from another core's cache: few
+    # calls, no helpers on the way of the common case.
     logits, actions, stats, top_actions = ctx.saved_tensors
     T, V = logits.shape
-    grad = logits.new_empty((T, V))
+    grad = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
     if T > 0:
-        g_log_prob, g_entropy, g_top = (g if g is None else g.contiguous() for g in (g_log_prob, g_entropy, g_top))
-        with on_device(logits):
-            _hip.check(_hip.lib().mz_policy_scores_backward(
-                ptr(logits), TYPE[logits.dtype], row_stride(logits), ptr(actions), T, V, 0 if g_top is None else g_top.shape[1],
-                ptr(stats), ptr(top_actions), ptr(g_log_prob), ptr(g_entropy), ptr(g_top), ptr(grad), V,
-                stream_of(logits)), "mz_policy_scores_backward")
+        g_log_prob = None if g_log_prob is None else g_log_prob.contiguous()
+        g_entropy = None if g_entropy is None else g_entropy.contiguous()
+        g_top = None if g_top is None else g_top.contiguous()
+        args = (logits.data_ptr(), ctx.kind, logits.stride(0) if T > 1 else V, None if actions is None else actions.data_ptr(), T, V,
+                0 if g_top is None else g_top.shape[1], stats.data_ptr(), None if top_actions is None else top_actions.data_ptr(),
+                None if g_log_prob is None else g_log_prob.data_ptr(), None if g_entropy is None else g_entropy.data_ptr(),
+                None if g_top is None else g_top.data_ptr(), grad.data_ptr(), V, stream_of(logits))
+        # autograd has made the logits' device the current one
+        rc = _hip.lib().mz_policy_scores_backward(*args)
+        if rc:
+            _hip.check(rc, "mz_policy_scores_backward")
     return grad, None, None
 
 
@@ -70,6 +77,7 @@ class _PolicyScores(torch.autograd.Function):
         log_prob, entropy, stats, top_actions, top_log_probs = _forward(logits, actions, top, True)
         ctx.save_for_backward(logits, actions, stats, top_actions)
         ctx.set_materialize_grads(False)
+        ctx.kind = TYPE[logits.dtype]
         if top:
             ctx.mark_non_differentiable(top_actions)
         return log_prob, entropy, top_actions, top_log_probs

@@ -193,7 +193,7 @@ def _grad_reference(dz, x, bits=3):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("R,K,N", [(1, 1, 1), (1, 168, 7), (2, 16, 300), (31, 129, 5), (64, 64, 64), (65, 168, 256), (256, 336, 168), (300, 100, 130),
-                                   (1000, 257, 33), (2049, 40, 50), (5000, 128, 128), (256, 1152, 640), (130, 2000, 700), (40, 3601, 3700), (200, 3700, 3601),
+                                   (1000, 257, 33), (257, 60, 200), (1024, 100, 65), (1025, 30, 129), (2049, 40, 50), (5000, 128, 128), (256, 1152, 640), (130, 2000, 700), (40, 3601, 3700), (200, 3700, 3601),
                                    (330, 3300, 2049), (9000, 130, 70), (9000, 1400, 900)])
 def test_weight_gradient(R, K, N, dtype):
     from muzero_amd.checkpoints import save_activations, weight_grad
