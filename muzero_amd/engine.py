@@ -232,11 +232,15 @@ class PackedNetworks:
 
 
 def make_networks(dynamics: torch.nn.Module, prediction: torch.nn.Module, device="cuda", track_running_stats: bool = False,
-                  root_final: torch.nn.Module | None = None):
+                  root_final: torch.nn.Module | None = None, int8: bool = False):
     """Device evaluator for a (g, f) pair: `PackedNetworks` (fused kernels, single-launch search)
     for `res_net: []` configurations, `muzero_amd.towers.TowerNetworks` when either network has
     residual blocks or a res_final convolution (`track_running_stats`: its BatchNorm layers' running
-    statistics advance with every call as in the reference; the MLP networks have none)."""
+    statistics advance with every call as in the reference; the MLP networks have none).
+    `int8`: `res_net: []` networks with their dense layers in 8-bit integers (`muzero_amd.quantized.Int8Networks`)."""
+    if int8:
+        from muzero_amd.quantized import Int8Networks
+        return Int8Networks(dynamics, prediction, device=device)
     plain = (len(dynamics.res_blocks) == 0 and len(prediction.res_blocks) == 0 and
              isinstance(dynamics.res_final, torch.nn.Identity) and isinstance(prediction.res_final, torch.nn.Identity))
     if plain:

@@ -192,3 +192,86 @@ class Int8MLP:
     def __call__(self, x) -> torch.Tensor:
         y = self.logits(x)
         return torch.softmax(y, dim=-1) if self.softmax else y
+
+
+class Int8Networks:
+    """Device evaluator of a (g, f) pair without residual blocks whose dense layers are in 8-bit integers: what
+    `muzero_amd.engine.make_networks(g, f, int8=True)` returns, for `BatchedMCTS` in lock step (the single-launch search is
+    written for the float32-accurate networks).  Meant for wide layers, where a search is bound by the weights it reads.
+
+    g merges per latent, not per child: fc_merge of [latent ; embedding] is its latent half in 8 bits, once for the A
+    children of a node, plus the float32 row of the action (mz_action_table; src/neural_networks/neural_network.py:168-172).
+    Call `refresh()` after the weights change."""
+
+    fusable = False
+    strided_outputs = True    # results may go to strided columns; the A children of a node share one row index
+
+    def __init__(self, dynamics: torch.nn.Module, prediction: torch.nn.Module, device="cuda"):
+        if len(dynamics.res_blocks) or len(prediction.res_blocks) or not isinstance(dynamics.res_final, torch.nn.Identity) \
+                or not isinstance(prediction.res_final, torch.nn.Identity):
+            raise NotImplementedError("8-bit networks cover res_net: [] configurations")
+        self.device = torch.device(device)
+        self.dynamics_net, self.prediction_net = dynamics, prediction
+        c, h, w = dynamics.latent_shape
+        self.D, self.A = c * h * w, dynamics.num_actions
+        self.heads = [Int8MLP(m, device) for m in (dynamics.reward_mlp, prediction.value_mlp, prediction.policy_mlp)]
+        self._merge()
+
+    def refresh(self) -> None:
+        for head in self.heads:
+            head.refresh()
+        self._merge()
+
+    def _merge(self) -> None:
+        g, D, A = self.dynamics_net, self.D, self.A
+        emb, w, b = (t.detach().to(self.device, torch.float32).contiguous()
+                     for t in (g.action_embedding.weight, g.fc_merge.weight, g.fc_merge.bias))
+        self.merge = quantize_rows(w[:, :D])
+        self.table = torch.empty((A, D), dtype=torch.float32, device=self.device)
+        with on_device(self.table):
+            _hip.check(_hip.lib().mz_action_table(ptr(emb), ptr(w), ptr(b), D, A, ptr(self.table), stream_of(self.table)),
+                       "mz_action_table")
+
+    def _rows(self, latent: torch.Tensor, B: int, rows: Optional[torch.Tensor]) -> torch.Tensor:
+        """Latent rows [B, D]; a negative index names a row of zeros."""
+        flat = latent.reshape(-1, self.D)
+        if rows is None:
+            return flat[:B]
+        picked = flat[rows.clamp(min=0).long()]
+        return torch.where((rows >= 0)[:, None], picked, torch.zeros((), device=picked.device))
+
+    @torch.no_grad()
+    def dynamics(self, latent, B, *, ld=None, rows=None, action=None, next_latent=None, ld_next=None, next_rows=None, reward=None) -> None:
+        A = self.A
+        U = B if action is not None else B // A
+        base = int8_linear(self._rows(latent, U, rows), self.merge)
+        if action is not None:
+            nxt = (base + self.table[action.long()]).relu_()
+        else:
+            nxt = (base[:, None, :] + self.table).relu_().reshape(B, self.D)
+        if reward is not None:
+            (reward.view(B) if reward.is_contiguous() else reward).copy_(self.heads[0](nxt)[:, 0])
+        if next_latent is not None:
+            out = next_latent.view(-1, self.D)
+            if next_rows is None:
+                out[:B] = nxt
+            else:  # rows below 0 are skipped: they put back what row 0, a root's and no child's, holds
+                at = next_rows.clamp(min=0).long()
+                out[at] = torch.where((next_rows >= 0)[:, None], nxt, out[at])
+
+    @torch.no_grad()
+    def prediction(self, latent, B, *, ld=None, rows=None, softmax_times=0, policy=None, value=None, argmax=None) -> None:
+        x = quantize_rows(self._rows(latent, B, rows))     # both heads read the same rows
+        if value is not None:
+            value.copy_(self.heads[1](x)[:, 0])
+        if policy is None and argmax is None:
+            return
+        probs = self.heads[2].logits(x)
+        lib, A = _hip.lib(), self.A
+        with on_device(probs):
+            st = stream_of(probs)
+            _hip.check(lib.mz_policy_post(ptr(probs), B, A, 1, ptr(probs), None, st), "mz_policy_post")
+            out = probs if softmax_times == 0 else torch.empty_like(probs)
+            _hip.check(lib.mz_policy_post(ptr(probs), B, A, softmax_times, ptr(out), ptr(argmax), st), "mz_policy_post")
+        if policy is not None:
+            policy.copy_(out)

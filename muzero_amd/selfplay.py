@@ -195,7 +195,7 @@ def episodes_from_records(rec, G: int):
 class SelfPlayEngine:
     def __init__(self, repr_net, dyn_net, pred_net, G: int, config, device="cuda", seed: int = 0,
                  device_rng: bool = False, env=None, track_running_stats: bool = False, root_form: bool = True,
-                 share: "SelfPlayEngine | None" = None, graph_moves: bool = False):
+                 share: "SelfPlayEngine | None" = None, graph_moves: bool = False, int8: bool = False):
         """`config`: TrainingDataGeneratorConfig (mcts settings, epsilon schedule, max steps).
         `env`: a batched environment (`observe`, `step`, `reset(mask)`, `num_actions`,
         `observation_space`); default: G Connect-Four games on the GPU.  Host-side simulators go
@@ -222,6 +222,9 @@ class SelfPlayEngine:
         launches of which all but the search take a few microseconds -- is recorded as one HIP graph and replayed;
         `move` then returns the graph's own output tensors, valid until the next move (`generate` copies them).
 
+        `int8`: g and f (`res_net: []`) run with their dense layers in 8-bit integers, in lock step
+        (muzero_amd.quantized.Int8Networks): for wide layers, at the accuracy of 127 steps per row.
+
         `share`: another engine over the same three modules whose device copies of the weights (h runner,
         packed g / f) this one uses instead of packing its own; the two must issue their device work on the
         same stream."""
@@ -239,7 +242,7 @@ class SelfPlayEngine:
             self.h = RepresentationRunner(repr_net, device=device, track_running_stats=track_running_stats)
             self._root_final = self.h.root_final() if root_form else None
             self.nets = make_networks(dyn_net, pred_net, device=device, track_running_stats=track_running_stats,
-                                      root_final=self._root_final)
+                                      root_final=self._root_final, int8=int8)
         self.mcts = BatchedMCTS(self.nets, G, m.max_iterations, m.model_look_ahead, m.discount_factor, m.noise_frac,
                                 device=device, keep_latents=False)  # nothing here reads the children's latents
         self.history = DeviceHistory(G, repr_net.history_length, self.env.observation_space, device=device)

@@ -474,6 +474,86 @@ def test_heads_in_8_bits_and_their_scores():
         assert not torch.equal(head.logits(lat.reshape(200, -1)), got)
 
 
+def test_networks_in_8_bits_are_their_layers():
+    """Int8Networks against the same layers written out: rows gathered and scattered, per-node and per-row actions."""
+    from muzero_amd.engine import make_networks
+    from muzero_amd.quantized import int8_linear, quantize_rows
+    _, g, f = _networks(2)
+    nets = make_networks(g, f, int8=True)
+    A, D, U = 7, 168, 5
+    lat = torch.randn(40, D, device="cuda")
+    rows = torch.tensor([3, 39, -1, 0, 7], dtype=torch.int32, device="cuda")
+    x = torch.where((rows >= 0)[:, None], lat[rows.clamp(min=0).long()], torch.zeros((), device="cuda"))
+    W, b, emb = g.fc_merge.weight.detach(), g.fc_merge.bias.detach(), g.action_embedding.weight.detach()
+    base = int8_linear(x, quantize_rows(W[:, :D]))
+    table = (emb.double() @ W[:, D:].double().t() + b.double()).float()
+
+    def reward_of(nxt):
+        (w0, b0, a0), (w1, b1, a1) = nets.heads[0].layers
+        assert (a0, a1) == ("relu", "linear") or (a0, a1) == ("relu", "none")
+        return int8_linear(int8_linear(nxt, w0, b0, "relu"), w1, b1)[:, 0]
+    out, rew = torch.full((60, D), 9.0, device="cuda"), torch.empty(U, A, device="cuda")
+    next_rows = (20 + torch.arange(U * A, device="cuda", dtype=torch.int32))
+    next_rows[4] = -1
+    nets.dynamics(lat, U * A, rows=rows, next_latent=out, next_rows=next_rows, reward=rew)
+    kids = torch.relu(base[:, None] + table[None]).reshape(U * A, D)
+    got = torch.where((next_rows >= 0)[:, None], out[next_rows.clamp(min=0).long()], kids)
+    torch.testing.assert_close(got, kids, rtol=0, atol=1e-5)                 # the table's float32 sums of 168 terms
+    assert (out[0:20] == 9.0).all() and (out[24] == 9.0).all()
+    act = torch.tensor([0, 6, 2, 2, 5], dtype=torch.int32, device="cuda")
+    one, col = torch.empty(U, D, device="cuda"), torch.zeros(U, 3, device="cuda")
+    nets.dynamics(lat, U, rows=rows, action=act, next_latent=one, reward=col[:, 1])
+    torch.testing.assert_close(one, kids.view(U, A, D)[torch.arange(U), act.long()], rtol=0, atol=1e-5)
+    assert torch.equal(col[:, 1], reward_of(one)) and (col[:, 0] == 0).all()
+    pol, val, arg = torch.empty(U, A, device="cuda"), torch.empty(U, device="cuda"), torch.empty(U, dtype=torch.int32, device="cuda")
+    nets.prediction(lat, U, rows=rows, softmax_times=1, policy=pol, value=val, argmax=arg)
+    p = torch.softmax(nets.heads[2].logits(x), 1)
+    torch.testing.assert_close(pol, torch.softmax(p, 1), rtol=1e-6, atol=1e-7)
+    assert torch.equal(val, nets.heads[1](x)[:, 0]) and torch.equal(arg.long(), p.argmax(1))
+    before = val.clone()
+    with torch.no_grad():
+        f.value_mlp[0].weight.mul_(1.5)
+    nets.refresh()
+    nets.prediction(lat, U, rows=rows, value=val)
+    assert not torch.equal(val, before)
+
+
+def test_search_with_networks_in_8_bits():
+    """A lock-step search on Int8Networks: its trees are the CPU oracle's on the network outputs it produced, and a whole
+    self-play move runs."""
+    from muzero_amd.config import load_config
+    from muzero_amd.engine import BatchedMCTS, make_networks
+    from muzero_amd.selfplay import SelfPlayEngine
+    from oracle import tree as otree
+    h, g, f = _networks(4)
+    nets = make_networks(g, f, int8=True)
+    G, A, S, D = 24, 7, 12, 168
+    mcts = BatchedMCTS(nets, G, S, 1, discount=0.998, noise_frac=0.25)
+    rng = np.random.default_rng(0)
+    lat = torch.from_numpy(rng.standard_normal((G, D)).astype(np.float32)).cuda()
+    eta = rng.dirichlet(np.full(A, 0.3), size=G).astype(np.float32)
+    rand = rng.integers(0, A, size=(G, S + 1)).astype(np.int32)
+    tp = np.ones(G, np.int8)
+    trace = {}
+    res = mcts.run(lat, torch.from_numpy(tp).cuda(), torch.from_numpy(eta).cuda(), torch.from_numpy(rand).cuda(), trace)
+    torch.cuda.synchronize()
+    pool = mcts.pool
+    root_prior = torch.empty(G, A, device="cuda")
+    nets.prediction(lat, G, softmax_times=1, policy=root_prior)
+    prior = np.concatenate([root_prior.cpu().numpy()[:, None]] + [p.cpu().numpy()[:, None] for p in trace["prior"]], 1)
+    nodes = pool.reward.cpu().numpy()
+    reward = np.stack([nodes[:, 1 + e * A:1 + (e + 1) * A] for e in range(S + 1)], 1)
+    rollout = np.stack([r.cpu().numpy() for r in trace["rollout"]], 1)
+    ref = otree.run_batch(A, S, 1, tp, prior, reward, rand, rollout, eta, 0.25, 0.998)
+    assert np.array_equal(pool.visit.cpu().numpy(), ref["visit"]) and np.array_equal(pool.value_sum.cpu().numpy(), ref["value_sum"])
+    np.testing.assert_allclose(res.policy.cpu().numpy(), ref["policy"], rtol=1e-12)
+    cfg = load_config("config_c4_mlp.yaml").training_data_generator
+    cfg.mcts.max_iterations = 6
+    eng = SelfPlayEngine(h, g, f, G=16, config=cfg, int8=True)
+    obs, policy, value, action, _, _ = eng.move()
+    assert policy.shape == (16, 7) and bool(policy.isfinite().all()) and bool(value.isfinite().all()) and bool((action >= 0).all())
+
+
 def test_other_streams_and_replayed_graphs():
     from muzero_amd.checkpoints import save_activations, weight_grad
     from muzero_amd.quantized import int8_linear, quantize_rows
