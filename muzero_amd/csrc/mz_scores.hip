@@ -170,37 +170,59 @@ constexpr int kCand = 1024;       // candidates for the alternatives that a work
 constexpr int kMaxParts = 64;     // parts of one row (one lane of the joining wave each)
 
 // The logits [lo, hi) of a row as 16-byte packs that lie on 16-byte addresses, whatever the row's own alignment: pack i
-// holds the logits first + i n .. + n - 1, of which the first and last pack may only own some.
+// holds the logits first + i n .. + n - 1.  Packs whole_lo .. whole_hi - 1 are owned whole; the first and the last pack may
+// only be owned in part.
 template <class T>
 struct Span {
     static constexpr int n = Pack<T>::n;
     const T *z;
-    int lo, hi, first, packs;
+    int lo, hi, first, packs, whole_lo, whole_hi;
 
     __device__ Span(const T *row, int lo_, int hi_) : z(row), lo(lo_), hi(hi_) {
         first = lo - (int)(((uintptr_t)(row + lo) & 15) / sizeof(T));
         packs = (hi - first + n - 1) / n;
+        whole_lo = first < lo ? 1 : 0;
+        whole_hi = first + packs * n > hi ? packs - 1 : packs;
     }
     __device__ __forceinline__ int at(int i) const { return first + i * n; }
     __device__ __forceinline__ bool owns(int j) const { return j >= lo && j < hi; }
-    __device__ __forceinline__ void load(int i, float (&v)[n]) const {
-        const int j = at(i);
-        if (j >= lo && j + n <= hi) {
-            const Pack<T> p = *(const Pack<T> *)(z + j);
+    __device__ __forceinline__ Pack<T> whole(int i) const { return *(const Pack<T> *)(z + at(i)); }
+    __device__ __forceinline__ Pack<T> part(int i) const {  // -inf where the pack is not owned
+        Pack<T> p;
 #pragma unroll
-            for (int e = 0; e < n; ++e) v[e] = (float)p.v[e];
-        } else {
-#pragma unroll
-            for (int e = 0; e < n; ++e) v[e] = owns(j + e) ? (float)z[j + e] : -INFINITY;
+        for (int e = 0; e < n; ++e) p.v[e] = owns(at(i) + e) ? z[at(i) + e] : (T)-INFINITY;
+        return p;
+    }
+    __device__ __forceinline__ Pack<T> load(int i) const { return i >= whole_lo && i < whole_hi ? whole(i) : part(i); }
+    // f(pack) for packs t, t + THREADS, ...: four whole ones in flight, without a branch between the loads
+    template <int THREADS, class F>
+    __device__ __forceinline__ void each(int t, F &&f) const {
+        int i = t;
+        if (i < whole_lo && i < packs) {
+            f(part(i), i);
+            i += THREADS;
         }
+        for (; i + 3 * THREADS < whole_hi; i += 4 * THREADS) {
+            Pack<T> p[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) p[q] = whole(i + q * THREADS);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) f(p[q], i + q * THREADS);
+        }
+        for (; i < whole_hi; i += THREADS) f(whole(i), i);
+        if (i < packs) f(part(i), i);
     }
 };
 
-template <int N>
-__device__ __forceinline__ void add(Sums &a, const float (&v)[N]) {
+template <class T>
+__device__ __forceinline__ void add(Sums &a, const Pack<T> &p) {
+    constexpr int n = Pack<T>::n;
+    float v[n];
+#pragma unroll
+    for (int e = 0; e < n; ++e) v[e] = (float)p.v[e];
     float m = v[0];
 #pragma unroll
-    for (int e = 1; e < N; ++e) m = fmaxf(m, v[e]);
+    for (int e = 1; e < n; ++e) m = fmaxf(m, v[e]);
     if (m > a.m) {
         const float d = a.m - m, x = exp_le0(d);
         a.u = x * a.u + share(x, d) * a.s;
@@ -208,7 +230,7 @@ __device__ __forceinline__ void add(Sums &a, const float (&v)[N]) {
         a.m = m;
     }
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
+    for (int e = 0; e < n; ++e) {
         const float d = v[e] - a.m, x = exp_le0(d);
         a.s += x;
         a.u += share(x, d);
@@ -277,7 +299,6 @@ template <class T>
 __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool loud) {
     constexpr int n = Span<T>::n;
     const int per_thread = (span.packs + kLT - 1) / kLT;
-    float v[n];
     // the logits of the threads with `mine` that are `wanted`; sh.count and sh.owners are 0 before
     const auto collect = [&](bool mine, auto &&wanted) {
         if (mine) sh.owner[atomicAdd(&sh.owners, 1)] = threadIdx.x;
@@ -286,13 +307,14 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
         for (int q = threadIdx.x; q < items; q += kLT) {
             const int o = q / per_thread, i = sh.owner[o] + (q - o * per_thread) * kLT;
             if (i >= span.packs) continue;
-            span.load(i, v);
+            const Pack<T> p = span.load(i);
 #pragma unroll
             for (int e = 0; e < n; ++e) {
                 const int j = span.at(i) + e;
-                if (span.owns(j) && wanted(v[e], j)) {
+                const float z = (float)p.v[e];
+                if (span.owns(j) && wanted(z, j)) {
                     const int c = atomicAdd(&sh.count, 1);
-                    if (c < kCand) sh.cand[c] = order_key(v[e], j);
+                    if (c < kCand) sh.cand[c] = order_key(z, j);
                 }
             }
         }
@@ -307,15 +329,14 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
         count = collect(sh.best[threadIdx.x] >= order_bits(t), [&](float z, int) { return z >= t; });
         if (count > kCand) {
             Key mine = 0;
-            for (int i = threadIdx.x; i < span.packs; i += kLT) {
-                span.load(i, v);
+            span.template each<kLT>(threadIdx.x, [&](const Pack<T> &p, int i) {
 #pragma unroll
                 for (int e = 0; e < n; ++e) {
                     const int j = span.at(i) + e;
-                    const Key k = span.owns(j) ? order_key(v[e], j) : 0;
+                    const Key k = span.owns(j) ? order_key((float)p.v[e], j) : 0;
                     if (k > mine) mine = k;
                 }
-            }
+            });
             __syncthreads();  // everybody has read sh.count
             sh.thread_key[threadIdx.x] = mine;
             if (threadIdx.x == 0) sh.count = 0, sh.owners = 0, sh.threshold = 0;  // fewer owning threads than top: everything
@@ -335,15 +356,14 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
     Key last = ~0ull;
     for (int a = 0; a < top; ++a) {
         Key best = 0;
-        for (int i = threadIdx.x; i < span.packs; i += kLT) {
-            span.load(i, v);
+        span.template each<kLT>(threadIdx.x, [&](const Pack<T> &p, int i) {
 #pragma unroll
             for (int e = 0; e < n; ++e) {
                 const int j = span.at(i) + e;
-                const Key k = span.owns(j) ? order_key(v[e], j) : 0;
+                const Key k = span.owns(j) ? order_key((float)p.v[e], j) : 0;
                 if (k < last && k > best) best = k;
             }
-        }
+        });
         best = wave_max(best);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) sh.thread_key[threadIdx.x >> 6] = best;
@@ -361,7 +381,6 @@ __global__ void __launch_bounds__(kLT)
 k_scores_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts, Out out, Sums *__restrict__ part_sums,
               Key *__restrict__ part_keys) {
     __shared__ Shared sh;
-    constexpr int n = Span<T>::n;
     const int top = out.top;
     for (int64_t job = blockIdx.x; job < rows * parts; job += gridDim.x) {
         const int64_t row = job / parts;
@@ -369,23 +388,7 @@ k_scores_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts,
         const T *z = logits + row * ld;
         const Span<T> span(z, (int)((int64_t)out.V * part / parts), (int)((int64_t)out.V * (part + 1) / parts));
         Sums acc = none();
-        int i = threadIdx.x;
-        for (; i + 3 * kLT < span.packs; i += 4 * kLT) {  // four loads in flight
-            float v0[n], v1[n], v2[n], v3[n];
-            span.load(i, v0);
-            span.load(i + kLT, v1);
-            span.load(i + 2 * kLT, v2);
-            span.load(i + 3 * kLT, v3);
-            add(acc, v0);
-            add(acc, v1);
-            add(acc, v2);
-            add(acc, v3);
-        }
-        for (; i < span.packs; i += kLT) {
-            float v0[n];
-            span.load(i, v0);
-            add(acc, v0);
-        }
+        span.template each<kLT>(threadIdx.x, [&](const Pack<T> &p, int) { add(acc, p); });
         __syncthreads();  // the last job's shared values have been read
         sh.best[threadIdx.x] = order_bits(acc.s == 0.0f ? -INFINITY : acc.m);
 #pragma unroll
@@ -500,25 +503,28 @@ k_grad_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int pieces, 
         // packs of the logits' alignment: stores are whole when the gradient's row has the same one
         const bool whole = ((uintptr_t)(out + span.first) & 15) == 0;
         const RowGrad r = in.row(row);
-        float v[kGradPacks][n];
         const int i0 = piece * kGradPacks * kLT + threadIdx.x;
-#pragma unroll
-        for (int q = 0; q < kGradPacks; ++q)
-            if (i0 + q * kLT < span.packs) span.load(i0 + q * kLT, v[q]);
-#pragma unroll
-        for (int q = 0; q < kGradPacks; ++q) {
-            const int i = i0 + q * kLT, j = span.at(i);
-            if (i >= span.packs) break;
+        const auto put = [&](const Pack<T> &z, int i) {
+            const int j = span.at(i);
             Pack<T> p;
 #pragma unroll
-            for (int e = 0; e < n; ++e) p.v[e] = (T)grad_one(r, v[q][e], j + e);
-            if (whole && j >= 0 && j + n <= in.V) {
+            for (int e = 0; e < n; ++e) p.v[e] = (T)grad_one(r, (float)z.v[e], j + e);
+            if (whole && i >= span.whole_lo && i < span.whole_hi) {
                 *(Pack<T> *)(out + j) = p;
             } else {
 #pragma unroll
                 for (int e = 0; e < n; ++e)
                     if (span.owns(j + e)) out[j + e] = p.v[e];
             }
+        };
+        if (i0 >= span.whole_lo && i0 + (kGradPacks - 1) * kLT < span.whole_hi) {  // all loads in flight
+            Pack<T> z[kGradPacks];
+#pragma unroll
+            for (int q = 0; q < kGradPacks; ++q) z[q] = span.whole(i0 + q * kLT);
+#pragma unroll
+            for (int q = 0; q < kGradPacks; ++q) put(z[q], i0 + q * kLT);
+        } else {
+            for (int q = 0; q < kGradPacks && i0 + q * kLT < span.packs; ++q) put(span.load(i0 + q * kLT), i0 + q * kLT);
         }
     }
 }
