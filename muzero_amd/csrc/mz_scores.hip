@@ -90,6 +90,10 @@ __device__ __forceinline__ Key wave_max(Key k) {
     return ((Key)hi << 32) | lo;
 }
 
+__device__ __forceinline__ Key lane_key(Key k, int lane) {
+    return ((Key)(unsigned)__builtin_amdgcn_readlane((int)(k >> 32), lane) << 32) | (unsigned)__builtin_amdgcn_readlane((int)k, lane);
+}
+
 struct Out {  // the result arrays of a call
     const int64_t *actions;
     float *log_prob, *entropy, *stats;
@@ -111,9 +115,10 @@ struct Out {  // the result arrays of a call
     }
 };
 
-// ---------------------------------------------------------------- rows of up to 1024 logits: a row stays in registers
-// LANES lanes per row, E logits per lane (logit e * LANES + lane), 256 / LANES rows per workgroup.
-template <class T, int LANES, int E>
+// ---------------------------------------------------------------- rows of up to 64 logits
+// LANES lanes per row, one logit each, 256 / LANES rows per workgroup.  An alternative costs log2(LANES) exchanges, against
+// a list built in shared memory for longer rows.  Bound by the launch: 1536 x 7 (bf16, 3 alternatives) is one wave's chain.
+template <class T, int LANES>
 __global__ void __launch_bounds__(256)
 k_scores_small(const T *__restrict__ logits, int64_t ld, int64_t rows, Out out) {
     const int lane = threadIdx.x % LANES, V = out.V;
@@ -121,22 +126,13 @@ k_scores_small(const T *__restrict__ logits, int64_t ld, int64_t rows, Out out) 
         const int64_t row = row0 + threadIdx.x / LANES;
         const bool live = row < rows;
         const T *z = logits + (live ? row : 0) * ld;
-        float v[E];
-        Sums acc = none();
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int j = e * LANES + lane;
-            v[e] = j < V ? (float)z[j] : -INFINITY;
-            acc.m = fmaxf(acc.m, v[e]);
-        }
+        const float v = lane < V ? (float)z[lane] : -INFINITY;
+        Sums acc = {fmaxf(v, kLowest), 0.0f, 0.0f};
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) acc.m = fmaxf(acc.m, __shfl_xor(acc.m, o));
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const float d = v[e] - acc.m, x = exp_le0(d);
-            acc.s += x;
-            acc.u += share(x, d);
-        }
+        const float d = v - acc.m;
+        acc.s = exp_le0(d);
+        acc.u = share(acc.s, d);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) {
             acc.s += __shfl_xor(acc.s, o);
@@ -144,30 +140,19 @@ k_scores_small(const T *__restrict__ logits, int64_t ld, int64_t rows, Out out) 
         }
         const Row r = row_of(acc);
         if (live && lane == 0) out.row(row, r, z);
-        Key last = ~0ull;
+        Key mine = lane < V ? order_key(v, lane) : 0;
         for (int i = 0; i < out.top; ++i) {
-            Key best = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int j = e * LANES + lane;
-                const Key k = j < V ? order_key(v[e], j) : 0;
-                if (k < last && k > best) best = k;
-            }
+            Key best = mine;
 #pragma unroll
             for (int o = LANES / 2; o > 0; o >>= 1) {
                 const Key k = __shfl_xor(best, o);
                 if (k > best) best = k;
             }
-            last = best;
-            if (live && lane == 0) out.alternative(row, i, r, last);
+            if (mine == best) mine = 0;  // keys are unique
+            if (live && lane == 0) out.alternative(row, i, r, best);
         }
     }
 }
-
-// ---------------------------------------------------------------- long rows: a workgroup streams a row, or a part of it
-constexpr int kLT = 256;          // threads
-constexpr int kCand = 1024;       // candidates for the alternatives that a workgroup can hold
-constexpr int kMaxParts = 64;     // parts of one row (one lane of the joining wave each)
 
 // The logits [lo, hi) of a row as 16-byte packs that lie on 16-byte addresses, whatever the row's own alignment: pack i
 // holds the logits first + i n .. + n - 1.  Packs whole_lo .. whole_hi - 1 are owned whole; the first and the last pack may
@@ -213,6 +198,113 @@ struct Span {
         if (i < packs) f(part(i), i);
     }
 };
+
+// ---------------------------------------------------------------- rows of up to about 4096 logits: one wave per row
+// The row stays in registers (P packs a lane).  The alternatives: every lane's largest logit gives a lower bound of the
+// `top`-th largest one (as many lanes reach it); the few logits that reach the bound are collected and ranked by counting.
+// Rows with more than 64 of those (equal values, everything masked, a NaN) find one alternative per pass.
+// No barrier and no second read; bound by the bytes with many rows and by the load's latency with few.  us for 20000 rows
+// (fp16, without / with 5 alternatives), and in brackets for a workgroup per row: 1000 logits 12.7 / 18.9, 2048 21.6 / 32.6
+// (58.9 / 109), 3000 34 / 53 (68 / 119), 4000 68 / 113 (72 / 122); 256 rows of 2048 3.9 / 5.6 (4.3 / 6.8), of 4000 4.7 / 6.9
+// (4.6 / 7.2).  2048 half-precision logits without alternatives are 3.8 TB/s, the rate of reading.
+template <class T, int P>
+__global__ void __launch_bounds__(256)
+k_scores_wave(const T *__restrict__ logits, int64_t ld, int64_t rows, Out out) {
+    constexpr int n = Span<T>::n;
+    __shared__ Key cand[4][64];
+    const int lane = threadIdx.x & 63, top = out.top;
+    Key *list = cand[threadIdx.x >> 6];
+    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
+        const T *z = logits + row * ld;
+        const Span<T> span(z, 0, out.V);
+        Pack<T> p[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q)  // no branch between the loads: other lanes read a pack that exists, and correct it
+            p[q] = span.whole(min(max(lane + 64 * q, span.whole_lo), span.whole_hi - 1));
+        float m = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+            const int i = lane + 64 * q;
+            if (i >= span.packs) {
+#pragma unroll
+                for (int e = 0; e < n; ++e) p[q].v[e] = (T)-INFINITY;
+            } else if (i < span.whole_lo || i >= span.whole_hi) {
+                p[q] = span.part(i);
+            }
+#pragma unroll
+            for (int e = 0; e < n; ++e) m = fmaxf(m, (float)p[q].v[e]);
+        }
+        const unsigned mine = order_bits(m);
+        Sums acc = {fmaxf(bits_value(wave_max(mine)), kLowest), 0.0f, 0.0f};
+#pragma unroll
+        for (int q = 0; q < P; ++q)
+#pragma unroll
+            for (int e = 0; e < n; ++e) {
+                const float d = (float)p[q].v[e] - acc.m, x = exp_le0(d);
+                acc.s += x;
+                acc.u += share(x, d);
+            }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            acc.s += __shfl_xor(acc.s, o);
+            acc.u += __shfl_xor(acc.u, o);
+        }
+        const Row r = row_of(acc);
+        if (lane == 0) out.row(row, r, z);
+        if (top == 0) continue;
+        unsigned bound = 0;
+        for (int bit = 31; bit >= 16; --bit) {
+            const unsigned probe = bound | (1u << bit);
+            if (__popcll(__ballot(mine >= probe)) >= top) bound = probe;
+        }
+        int count = 65;
+        if (!r.loud && bound > order_bits(-INFINITY)) {
+            const float t = bits_value(bound);
+            count = 0;
+            __builtin_amdgcn_wave_barrier();  // the list is the wave's own: LDS keeps a wave's order, the compiler has to as well
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+#pragma unroll
+                for (int e = 0; e < n; ++e) {
+                    const float x = (float)p[q].v[e];
+                    const unsigned long long hits = __ballot(x >= t);
+                    if (hits) {
+                        const int at = count + __builtin_amdgcn_mbcnt_hi((unsigned)(hits >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)hits, 0));
+                        if (x >= t && at < 64) list[at] = order_key(x, span.at(lane + 64 * q) + e);
+                        count += __popcll(hits);
+                    }
+                }
+        }
+        if (count <= 64) {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const Key k = lane < count ? list[lane] : 0;
+            int rank = 0;
+            for (int o = 0; o < count; ++o) rank += lane_key(k, o) > k;
+            if (rank < top && k != 0) out.alternative(row, rank, r, k);
+            continue;
+        }
+        Key last = ~0ull;
+        for (int a = 0; a < top; ++a) {
+            Key best = 0;
+#pragma unroll
+            for (int q = 0; q < P; ++q)
+#pragma unroll
+                for (int e = 0; e < n; ++e) {
+                    const int j = span.at(lane + 64 * q) + e;
+                    const Key k = span.owns(j) ? order_key((float)p[q].v[e], j) : 0;
+                    if (k < last && k > best) best = k;
+                }
+            last = wave_max(best);
+            if (lane == 0) out.alternative(row, a, r, last);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- long rows: a workgroup streams a row, or a part of it
+constexpr int kLT = 256;          // threads
+constexpr int kCand = 1024;       // candidates for the alternatives that a workgroup can hold
+constexpr int kMaxParts = 64;     // parts of one row (one lane of the joining wave each)
 
 template <class T>
 __device__ __forceinline__ void add(Sums &a, const Pack<T> &p) {
@@ -271,11 +363,7 @@ __device__ __forceinline__ void rank_candidates(Shared &sh, int count, int top) 
         if (threadIdx.x < 64) {
             const Key k = (int)threadIdx.x < count ? sh.cand[threadIdx.x] : 0;
             int rank = 0;
-            for (int o = 0; o < count; ++o) {
-                const Key other = ((Key)(unsigned)__builtin_amdgcn_readlane((int)(k >> 32), o) << 32) |
-                                  (unsigned)__builtin_amdgcn_readlane((int)k, o);
-                rank += other > k;
-            }
+            for (int o = 0; o < count; ++o) rank += lane_key(k, o) > k;
             if (rank < top && k != 0) sh.found[rank] = k;
         }
     } else {
@@ -376,12 +464,12 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
 }
 
 // Workgroup (row, part).  One part: the results.  Several: the part's sums and alternatives to the workspace.
-template <class T>
+template <class T, bool TOP>
 __global__ void __launch_bounds__(kLT)
 k_scores_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts, Out out, Sums *__restrict__ part_sums,
               Key *__restrict__ part_keys) {
     __shared__ Shared sh;
-    const int top = out.top;
+    const int top = TOP ? out.top : 0;
     for (int64_t job = blockIdx.x; job < rows * parts; job += gridDim.x) {
         const int64_t row = job / parts;
         const int part = (int)(job - row * parts);
@@ -398,7 +486,7 @@ k_scores_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts,
         acc = sh.part[0];
         for (int w = 1; w < kLT / 64; ++w) acc = join(acc, sh.part[w]);
         const Row r = row_of(acc);
-        if (top > 0) find_alternatives(span, sh, top, r.loud);
+        if constexpr (TOP) find_alternatives(span, sh, top, r.loud);
         if (parts == 1) {
             if (threadIdx.x == 0) out.row(row, r, z);
             if ((int)threadIdx.x < top) out.alternative(row, threadIdx.x, r, sh.found[threadIdx.x]);
@@ -548,15 +636,16 @@ constexpr int64_t kMaxGrid = 1 << 20;
 
 dim3 grid_of(int64_t n) { return dim3((unsigned)(n < kMaxGrid ? n : kMaxGrid)); }
 
-// Rows of more than kSmall logits are streamed; fewer rows than kFill workgroups are cut into parts of at least
-// kPartBytes, so that a short batch of long rows still reaches all 256 compute units.  us for kFill 256 / 512 / 1024:
+// Rows of up to kSmall logits take part of a wave, up to kWave a whole one (16 packs of 4 float32 a lane, wherever the row
+// starts), longer ones are streamed by a workgroup; fewer of those than kFill are cut into parts of at least kPartBytes, so
+// that a short batch of long rows still reaches all 256 compute units.  us for kFill 256 / 512 / 1024:
 // 64 x 131072 (fp16, 20 alternatives) 20.8 / 17.2 / 18.6, 256 x 131072 40.8 / 33.7 / 31.0, 300 x 32768 (float32, 5)
 // 14.1 / 16.4 / 17.3, 1000 x 8192 10.5 / 10.3 / 18.0; kPartBytes 8192 / 16384 / 32768: 1 x 131072 (bf16, 5) 10.2 / 10.5 /
 // 11.4, 8 x 4096 (float32) 9.3 / 5.8 / 5.8.
-constexpr int kSmall = 1024, kFill = 512, kPartBytes = 16384;
+constexpr int kSmall = 64, kWave = 4088, kFill = 512, kPartBytes = 16384;
 
 int parts_of(int32_t type, int64_t T, int32_t V) {
-    if (V <= kSmall || T >= kFill) return 1;
+    if (V <= kWave || T >= kFill) return 1;
     const int64_t by_size = (int64_t)V * type_bytes(type) / kPartBytes, by_fill = (kFill + T - 1) / T;
     const int64_t p = by_size < by_fill ? by_size : by_fill;
     return (int)(p < 1 ? 1 : p > kMaxParts ? kMaxParts : p);
@@ -564,23 +653,39 @@ int parts_of(int32_t type, int64_t T, int32_t V) {
 
 template <class T>
 void launch_scores(const T *logits, int64_t ld, int64_t rows, int parts, const Out &out, void *workspace, hipStream_t st) {
-    const auto small = [&](auto lanes, auto per_lane) {
-        constexpr int L = decltype(lanes)::value, E = decltype(per_lane)::value;
-        const int64_t per_group = 256 / L;
-        hipLaunchKernelGGL((k_scores_small<T, L, E>), grid_of((rows + per_group - 1) / per_group), dim3(256), 0, st, logits, ld,
-                           rows, out);
-    };
     using std::integral_constant;
     const int V = out.V;
-    if (V <= 8) return small(integral_constant<int, 8>{}, integral_constant<int, 1>{});
-    if (V <= 16) return small(integral_constant<int, 16>{}, integral_constant<int, 1>{});
-    if (V <= 32) return small(integral_constant<int, 32>{}, integral_constant<int, 1>{});
-    if (V <= 64) return small(integral_constant<int, 64>{}, integral_constant<int, 1>{});
-    if (V <= 256) return small(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-    if (V <= kSmall) return small(integral_constant<int, 64>{}, integral_constant<int, 16>{});
+    const auto small = [&](auto lanes) {
+        constexpr int L = decltype(lanes)::value;
+        hipLaunchKernelGGL((k_scores_small<T, L>), grid_of((rows + 256 / L - 1) / (256 / L)), dim3(256), 0, st, logits, ld, rows, out);
+    };
+    if (V <= 8) return small(integral_constant<int, 8>{});
+    if (V <= 16) return small(integral_constant<int, 16>{});
+    if (V <= 32) return small(integral_constant<int, 32>{});
+    if (V <= kSmall) return small(integral_constant<int, 64>{});
+    if (V <= kWave) {
+        const auto wave = [&](auto packs) {
+            hipLaunchKernelGGL((k_scores_wave<T, decltype(packs)::value>), grid_of((rows + 3) / 4), dim3(256), 0, st, logits, ld, rows, out);
+        };
+        constexpr int n = Pack<T>::n;
+        const bool aligned = (uintptr_t)logits % 16 == 0 && (ld % n == 0 || rows == 1);
+        const int packs = (V + (aligned ? n - 1 : 2 * (n - 1))) / n;  // of a row that starts anywhere: up to one more
+        if (packs <= 64) wave(integral_constant<int, 1>{});
+        else if (packs <= 128) wave(integral_constant<int, 2>{});
+        else if (packs <= 192) wave(integral_constant<int, 3>{});
+        else if (packs <= 256) wave(integral_constant<int, 4>{});
+        else if (packs <= 384) wave(integral_constant<int, 6>{});
+        else if (packs <= 512) wave(integral_constant<int, 8>{});
+        else if (packs <= 768) wave(integral_constant<int, 12>{});
+        else wave(integral_constant<int, 16>{});
+        return;
+    }
     Key *keys = (Key *)workspace;
     Sums *sums = (Sums *)(keys + (parts > 1 ? rows * parts * out.top : 0));
-    hipLaunchKernelGGL(k_scores_long<T>, grid_of(rows * parts), dim3(kLT), 0, st, logits, ld, rows, parts, out, sums, keys);
+    if (out.top > 0)
+        hipLaunchKernelGGL((k_scores_long<T, true>), grid_of(rows * parts), dim3(kLT), 0, st, logits, ld, rows, parts, out, sums, keys);
+    else
+        hipLaunchKernelGGL((k_scores_long<T, false>), grid_of(rows * parts), dim3(kLT), 0, st, logits, ld, rows, parts, out, sums, keys);
     if (parts > 1)
         hipLaunchKernelGGL(k_scores_join<T>, grid_of(rows), dim3(64), 0, st, logits, ld, rows, parts, out, (const Sums *)sums,
                            (const Key *)keys);
@@ -598,7 +703,7 @@ void launch_grad(const T *logits, int64_t ld, int64_t rows, const Grads &in, T *
         small(std::integral_constant<int, 8>{});
     } else if (in.V <= 32) {
         small(std::integral_constant<int, 32>{});
-    } else if (in.V <= kSmall) {
+    } else if (in.V <= 1024) {
         small(std::integral_constant<int, 64>{});
     } else {
         const int packs = (in.V + Pack<T>::n - 1) / Pack<T>::n + 1;  // a row that starts off a 16-byte address has one more

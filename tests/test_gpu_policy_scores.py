@@ -332,3 +332,21 @@ def test_results_may_be_changed_in_place_and_have_no_second_derivative():
     g, = torch.autograd.grad(_scores(z, a).entropy.sum(), z, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [65, 256, 257, 505, 513, 777, 1500, 1537, 2042, 2048, 2049, 3000, 3075, 4080, 4088, 4089, 4096])
+@pytest.mark.parametrize("offset", [0, 3])
+def test_row_lengths_between_the_variants(V, offset, dtype):
+    """Every count of packs that a wave keeps, for rows on 16-byte addresses and off them, with more rows than one
+    workgroup takes; the logits around a row hold larger values that no result may see."""
+    g = torch.Generator().manual_seed(V)
+    big = torch.full((13, V + 16 - V % 8), 500.0).to(dtype).cuda()
+    z = big[:, offset : offset + V]
+    z.copy_(torch.randn(13, V, generator=g).to(dtype))
+    z[4] = -torch.inf
+    z[5, 3:] = -torch.inf
+    z[6, V - 1], z[7, 0] = 9.0, 9.0
+    a = torch.randint(0, V, (13,), generator=g).cuda()
+    _check(z, a, 8)
+    _check(z, a, 0)
