@@ -565,7 +565,7 @@ struct Grads {
     }
 };
 
-// Rows of up to 64 * E logits, LANES lanes per row.
+// Rows of up to 64 logits, LANES lanes per row.
 template <class T, int LANES>
 __global__ void __launch_bounds__(256)
 k_grad_small(const T *__restrict__ logits, int64_t ld, int64_t rows, Grads in, T *__restrict__ grad, int64_t ldg) {
@@ -577,13 +577,16 @@ k_grad_small(const T *__restrict__ logits, int64_t ld, int64_t rows, Grads in, T
     }
 }
 
-constexpr int kGradPacks = 4;  // packs per thread of a workgroup's piece of a long row
+// Longer rows in pieces of LANES lanes with kGradPacks packs each: a wave per piece while that covers a row, else a workgroup.
+// Bound by the bytes: 20000 x 32768 (bf16 or fp16) runs at 5.5 TB/s.
+constexpr int kGradPacks = 4;
 
-template <class T>
+template <class T, int LANES>
 __global__ void __launch_bounds__(kLT)
 k_grad_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int pieces, Grads in, T *__restrict__ grad, int64_t ldg) {
     constexpr int n = Span<T>::n;
-    for (int64_t job = blockIdx.x; job < rows * pieces; job += gridDim.x) {
+    constexpr int64_t kTeams = kLT / LANES;
+    for (int64_t job = blockIdx.x * kTeams + threadIdx.x / LANES; job < rows * pieces; job += gridDim.x * kTeams) {
         const int64_t row = job / pieces;
         const int piece = (int)(job - row * pieces);
         const Span<T> span(logits + row * ld, 0, in.V);
@@ -591,7 +594,7 @@ k_grad_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int pieces, 
         // packs of the logits' alignment: stores are whole when the gradient's row has the same one
         const bool whole = ((uintptr_t)(out + span.first) & 15) == 0;
         const RowGrad r = in.row(row);
-        const int i0 = piece * kGradPacks * kLT + threadIdx.x;
+        const int i0 = piece * kGradPacks * LANES + threadIdx.x % LANES;
         const auto put = [&](const Pack<T> &z, int i) {
             const int j = span.at(i);
             Pack<T> p;
@@ -605,14 +608,14 @@ k_grad_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int pieces, 
                     if (span.owns(j + e)) out[j + e] = p.v[e];
             }
         };
-        if (i0 >= span.whole_lo && i0 + (kGradPacks - 1) * kLT < span.whole_hi) {  // all loads in flight
+        if (i0 >= span.whole_lo && i0 + (kGradPacks - 1) * LANES < span.whole_hi) {  // all loads in flight
             Pack<T> z[kGradPacks];
 #pragma unroll
-            for (int q = 0; q < kGradPacks; ++q) z[q] = span.whole(i0 + q * kLT);
+            for (int q = 0; q < kGradPacks; ++q) z[q] = span.whole(i0 + q * LANES);
 #pragma unroll
-            for (int q = 0; q < kGradPacks; ++q) put(z[q], i0 + q * kLT);
+            for (int q = 0; q < kGradPacks; ++q) put(z[q], i0 + q * LANES);
         } else {
-            for (int q = 0; q < kGradPacks && i0 + q * kLT < span.packs; ++q) put(span.load(i0 + q * kLT), i0 + q * kLT);
+            for (int q = 0; q < kGradPacks && i0 + q * LANES < span.packs; ++q) put(span.load(i0 + q * LANES), i0 + q * LANES);
         }
     }
 }
@@ -703,12 +706,20 @@ void launch_grad(const T *logits, int64_t ld, int64_t rows, const Grads &in, T *
         small(std::integral_constant<int, 8>{});
     } else if (in.V <= 32) {
         small(std::integral_constant<int, 32>{});
-    } else if (in.V <= 1024) {
+    } else if (in.V <= 64) {
         small(std::integral_constant<int, 64>{});
     } else {
         const int packs = (in.V + Pack<T>::n - 1) / Pack<T>::n + 1;  // a row that starts off a 16-byte address has one more
-        const int pieces = (packs + kGradPacks * kLT - 1) / (kGradPacks * kLT);
-        hipLaunchKernelGGL(k_grad_long<T>, grid_of(rows * pieces), dim3(kLT), 0, st, logits, ld, rows, pieces, in, grad, ldg);
+        const auto large = [&](auto lanes) {
+            constexpr int L = decltype(lanes)::value, teams = kLT / L;
+            const int pieces = (packs + kGradPacks * L - 1) / (kGradPacks * L);
+            hipLaunchKernelGGL((k_grad_long<T, L>), grid_of((rows * pieces + teams - 1) / teams), dim3(kLT), 0, st, logits, ld, rows,
+                               pieces, in, grad, ldg);
+        };
+        if (packs <= kGradPacks * 64)
+            large(std::integral_constant<int, 64>{});
+        else
+            large(std::integral_constant<int, 256>{});
     }
     if (in.g_top) {
         const int64_t groups = (rows * in.top + 255) / 256;

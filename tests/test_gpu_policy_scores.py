@@ -350,3 +350,9 @@ def test_row_lengths_between_the_variants(V, offset, dtype):
     a = torch.randint(0, V, (13,), generator=g).cuda()
     _check(z, a, 8)
     _check(z, a, 0)
+    base = z.detach().requires_grad_(True)  # keeps the strides and the offset
+    g_lp, g_ent = (torch.randn(13, generator=g).cuda() for _ in range(2))
+    s = _scores(base, a)
+    got, = torch.autograd.grad([s.log_prob, s.entropy], base, [g_lp, g_ent])
+    want, tol = _grad_reference(z.cpu().double(), a.cpu(), None, g_lp.cpu().double(), g_ent.cpu().double(), None)
+    _close(got, want, tol + HALF[dtype] * (want.abs() + tol) + TINY[dtype])
