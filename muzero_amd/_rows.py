@@ -31,6 +31,8 @@ def rows_of(t: torch.Tensor) -> torch.Tensor:
     """t as [rows, columns] with adjacent columns and rows that do not overlap: a view where its strides allow one, else
     a copy."""
     cols = t.shape[-1]
+    if t.is_neg():  # a view whose minus sign is not in memory yet
+        t = t.resolve_neg()
     if t.dim() != 2:
         t = t.reshape(-1, cols) if cols else t.reshape(t.shape[:-1].numel(), 0)
     if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):

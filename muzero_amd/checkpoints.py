@@ -15,6 +15,8 @@ derivatives of tanh and sigmoid that of a byte.
 """
 from __future__ import annotations
 
+import threading
+import types
 from typing import Optional
 
 import torch
@@ -25,6 +27,9 @@ from muzero_amd import _hip
 from muzero_amd._hip import ptr
 from muzero_amd._rows import TYPE, check_tensor, on_device, row_stride, rows_of, stream_of, workspace
 from muzero_amd.quantized import ACTIVATIONS, QuantizedRows, quantize_rows
+
+
+MAX_CHECKPOINT_ROWS = 1 << 20  # that one weight gradient takes
 
 
 def save_activations(x: torch.Tensor) -> QuantizedRows:
@@ -96,6 +101,8 @@ class _CheckpointedLinear(torch.autograd.Function):
         codes = scales = act = None
         if y.numel() > 0:
             if ctx.needs_input_grad[1]:
+                if x.shape[:-1].numel() > MAX_CHECKPOINT_ROWS:
+                    raise ValueError(f"{x.shape[:-1].numel()} rows are more than the {MAX_CHECKPOINT_ROWS} of one weight gradient")
                 saved = save_activations(x)
                 codes, scales = saved.codes, saved.scales
             if activation not in ("none", "linear"):
@@ -141,45 +148,82 @@ def checkpointed_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[to
     return _CheckpointedLinear.apply(x, weight, bias, activation)
 
 
+def _bound(fn, module):
+    return types.MethodType(fn, module)
+
+
+class _Taken:
+    """Stands in for a module's method (`forward`, `merge`) while contexts are open.  Copies and pickles of the module get
+    the method itself: they belong to no context."""
+
+    def __init__(self, module: torch.nn.Module, name: str, fn):
+        self.module, self.name, self.fn, self.depth, self.before = module, name, fn, 0, module.__dict__.get(name)
+
+    def __call__(self, x):
+        return self.fn(self.module, x)
+
+    def __reduce__(self):
+        return _bound, (getattr(type(self.module), self.name), self.module)
+
+
+_LOCK = threading.Lock()  # of every module's open contexts
+
+
 class eight_bit_checkpoints:
     """Context manager: inside it the dense layers of the given networks -- every build_mlp sequence and the merge layer
-    of a DynamicsNetwork -- keep 8-bit checkpoints on the GPU.  Convolutions and BatchNorm layers are left as they are,
-    and so is everything on the CPU.  Parameters, state_dict keys and results of the forward pass do not change."""
+    of a DynamicsNetwork -- keep 8-bit checkpoints on the GPU.  Convolutions and BatchNorm layers are left as they are, and
+    so are layers with hooks or a forward of their own and everything on the CPU or in float64.  Parameters, state_dict
+    keys and results of the forward pass do not change.  Contexts may be nested and overlap: a layer is as it was when the
+    last one that names it has ended."""
 
     def __init__(self, *modules: torch.nn.Module):
-        from muzero_amd.neural_networks.network_builder import is_dense_sequence
+        from muzero_amd.neural_networks.network_builder import is_dense_sequence, is_plain
+        from muzero_amd.neural_networks.neural_network import DynamicsNetwork
         self.sequences = [m for net in modules for m in net.modules() if is_dense_sequence(m)]
-        self.merges = [m for net in modules for m in net.modules() if hasattr(m, "fc_merge") and hasattr(m, "merge")]
-        self._patched: list[tuple[torch.nn.Module, str]] = []
+        self.merges = [m for net in modules for m in net.modules() if isinstance(m, DynamicsNetwork) and
+                       type(m).merge is DynamicsNetwork.merge and is_plain(m.fc_merge, torch.nn.Linear)]
+        self._open: list[list[_Taken]] = []
 
     @staticmethod
     def _sequence_forward(seq, x):
         from muzero_amd.neural_networks.network_builder import dense_pairs
-        if not x.is_cuda:
-            return torch.nn.Sequential.forward(seq, x)
-        for lin, act in dense_pairs(seq):
+        if not x.is_cuda or x.dtype not in TYPE:
+            return type(seq).forward(seq, x)
+        for i, (lin, act) in enumerate(dense_pairs(seq)):
             if act == "softmax":
-                x = torch.softmax(checkpointed_linear(x, lin.weight, lin.bias), dim=1)
+                x = seq[2 * i + 1](checkpointed_linear(x, lin.weight, lin.bias))
             else:
                 x = checkpointed_linear(x, lin.weight, lin.bias, act)
         return x
 
     @staticmethod
     def _merge(net, merged):
-        if not merged.is_cuda:
+        if not merged.is_cuda or merged.dtype not in TYPE:
             return type(net).merge(net, merged)
         return checkpointed_linear(merged, net.fc_merge.weight, net.fc_merge.bias, "relu")
 
     def __enter__(self):
-        for mods, name, fn in ((self.sequences, "forward", self._sequence_forward), (self.merges, "merge", self._merge)):
-            for m in mods:
-                if name not in m.__dict__:  # an outer context of the same kind has done it already
-                    m.__dict__[name] = (lambda x, _m=m, _f=fn: _f(_m, x))
-                    self._patched.append((m, name))
+        taken = []
+        with _LOCK:
+            kinds = ((self.sequences, "forward", self._sequence_forward), (self.merges, "merge", self._merge))
+            for m, name, fn in ((m, name, fn) for mods, name, fn in kinds for m in mods):
+                own = m.__dict__.get(name)
+                if isinstance(own, types.MethodType) and own.__func__ is getattr(type(m), name):
+                    own = None
+                if own is None:
+                    m.__dict__[name] = own = _Taken(m, name, fn)
+                if isinstance(own, _Taken):  # anything else is somebody's own method: left alone
+                    own.depth += 1
+                    taken.append(own)
+            self._open.append(taken)
         return self
 
     def __exit__(self, *exc):
-        while self._patched:
-            m, name = self._patched.pop()
-            del m.__dict__[name]
+        with _LOCK:
+            for t in self._open.pop():
+                t.depth -= 1
+                if t.depth == 0 and t.before is None:
+                    del t.module.__dict__[t.name]
+                elif t.depth == 0:
+                    t.module.__dict__[t.name] = t.before
         return False

@@ -556,7 +556,7 @@ struct Grads {
         r.empty = r.m == -INFINITY && r.log_s == 0.0f;
         r.a = actions ? actions[row] : -1;
         r.g_lp = g_lp && r.a >= 0 ? g_lp[row] : 0.0f;
-        if (r.a >= V) r.g_lp = NAN;  // an action that does not exist: its score was NaN
+        if (g_lp && r.a >= V) r.g_lp = NAN;  // an action that does not exist: its score was NaN
         r.g_ent = g_ent ? g_ent[row] : 0.0f;
         r.g_sum = r.g_lp;
         if (g_top)
@@ -628,7 +628,9 @@ k_grad_top(const T *__restrict__ logits, int64_t ld, int64_t rows, Grads in, T *
     const int64_t n = rows * in.top;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n; t += (int64_t)gridDim.x * 256) {
         const int64_t row = t / in.top;
-        const int j = (int)in.top_actions[t];
+        const int64_t at = in.top_actions[t];
+        if (at < 0 || at >= in.V) continue;
+        const int j = (int)at;
         const RowGrad r = in.row(row);
         const float g = grad_one(r, (float)logits[row * ld + j], j);
         grad[row * ldg + j] = (T)(r.empty ? 0.0f : g + in.g_top[t]);

@@ -115,11 +115,17 @@ def build_mlp(layers_config: list[DenseLayerConfig], input_dim: int) -> tuple[nn
 _DENSE_ACTIVATIONS = {nn.Identity: "none", nn.ReLU: "relu", nn.Tanh: "tanh", nn.Sigmoid: "sigmoid", nn.Softmax: "softmax"}
 
 
+def is_plain(module: nn.Module, kind: type) -> bool:
+    """A `kind` that does what a `kind` does: no forward of its own, no hooks."""
+    return (isinstance(module, kind) and type(module).forward is kind.forward and
+            not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
+
+
 def is_dense_sequence(module: nn.Module) -> bool:
-    """True for what build_mlp makes: Linear and activation in turn."""
-    mods = list(module) if isinstance(module, nn.Sequential) else []
+    """True for what build_mlp makes: plain Linear and activation modules in turn."""
+    mods = list(module) if isinstance(module, nn.Sequential) and type(module).forward is nn.Sequential.forward else []
     return len(mods) > 0 and len(mods) % 2 == 0 and all(
-        isinstance(m, nn.Linear) if i % 2 == 0 else type(m) in _DENSE_ACTIVATIONS for i, m in enumerate(mods))
+        is_plain(m, nn.Linear) if i % 2 == 0 else type(m) in _DENSE_ACTIVATIONS and is_plain(m, type(m)) for i, m in enumerate(mods))
 
 
 def dense_pairs(seq: nn.Sequential) -> list[tuple[nn.Linear, str]]:

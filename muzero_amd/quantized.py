@@ -26,7 +26,7 @@ ACTIVATIONS = ("none", "linear", "relu", "tanh", "sigmoid")
 class QuantizedRows:
     """Rows in 8 bits: x[r, k] is about scales[r] * codes[r, k].
 
-    codes       i8[rows, ldc], ldc a multiple of 128, rows on 16-byte addresses; zero behind the last column
+    codes       i8[rows, ldc] in -127..127, ldc a multiple of 128, rows on 16-byte addresses; zero behind the last column
     scales      f32[rows]
     shape       of the tensor that was coded
     dtype       of the tensor that was coded, float32, bfloat16 or float16
@@ -165,24 +165,37 @@ def int8_linear(x, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, a
     return y
 
 
+def _renew(old, new):
+    """`new` in the memory of `old`, where that fits."""
+    if old is None or new is None or old.shape != new.shape:
+        return new
+    if isinstance(new, QuantizedRows):
+        old.codes.copy_(new.codes), old.scales.copy_(new.scales)
+    else:
+        old.copy_(new)
+    return old
+
+
 class Int8MLP:
     """A build_mlp sequence (Linear + activation pairs) with its weights in 8 bits.  Call `refresh()` after the weights
-    change.  `logits(x)` stops in front of a final softmax."""
+    change: it writes the new codes where the old ones are, so recorded graphs go on with them.  `logits(x)` stops in
+    front of a final softmax."""
 
     def __init__(self, seq: torch.nn.Sequential, device="cuda"):
         self.seq, self.device = seq, torch.device(device)
+        self.layers, self.softmax = [], False
         self.refresh()
 
     def refresh(self) -> None:
         from muzero_amd.neural_networks.network_builder import dense_pairs
-        self.layers, self.softmax = [], False
-        for lin, act in dense_pairs(self.seq):
-            if self.softmax:
-                raise ValueError("softmax is supported as the last activation only")
-            self.softmax = act == "softmax"
-            w = quantize_rows(lin.weight.detach().to(self.device))
-            b = None if lin.bias is None else lin.bias.detach().to(self.device, torch.float32).clone()
-            self.layers.append((w, b, "none" if self.softmax else act))
+        pairs = dense_pairs(self.seq)
+        if any(act == "softmax" for _, act in pairs[:-1]):
+            raise ValueError("softmax is supported as the last activation only")
+        self.softmax = pairs[-1][1] == "softmax"
+        old = self.layers if len(self.layers) == len(pairs) else [(None, None, None)] * len(pairs)
+        self.layers = [(_renew(w, quantize_rows(lin.weight.detach().to(self.device))),
+                        None if lin.bias is None else _renew(b, lin.bias.detach().to(self.device, torch.float32, copy=True)),
+                        "none" if act == "softmax" else act) for (w, b, _), (lin, act) in zip(old, pairs)]
 
     def logits(self, x) -> torch.Tensor:
         for w, b, act in self.layers:
@@ -191,7 +204,7 @@ class Int8MLP:
 
     def __call__(self, x) -> torch.Tensor:
         y = self.logits(x)
-        return torch.softmax(y, dim=-1) if self.softmax else y
+        return self.seq[-1](y) if self.softmax else y
 
 
 class Int8Networks:
@@ -215,6 +228,8 @@ class Int8Networks:
         c, h, w = dynamics.latent_shape
         self.D, self.A = c * h * w, dynamics.num_actions
         self.heads = [Int8MLP(m, device) for m in (dynamics.reward_mlp, prediction.value_mlp, prediction.policy_mlp)]
+        self.merge = None
+        self.table = torch.empty((self.A, self.D), dtype=torch.float32, device=self.device)
         self._merge()
 
     def refresh(self) -> None:
@@ -226,8 +241,7 @@ class Int8Networks:
         g, D, A = self.dynamics_net, self.D, self.A
         emb, w, b = (t.detach().to(self.device, torch.float32).contiguous()
                      for t in (g.action_embedding.weight, g.fc_merge.weight, g.fc_merge.bias))
-        self.merge = quantize_rows(w[:, :D])
-        self.table = torch.empty((A, D), dtype=torch.float32, device=self.device)
+        self.merge = _renew(self.merge, quantize_rows(w[:, :D]))
         with on_device(self.table):
             _hip.check(_hip.lib().mz_action_table(ptr(emb), ptr(w), ptr(b), D, A, ptr(self.table), stream_of(self.table)),
                        "mz_action_table")

@@ -356,3 +356,35 @@ def test_row_lengths_between_the_variants(V, offset, dtype):
     got, = torch.autograd.grad([s.log_prob, s.entropy], base, [g_lp, g_ent])
     want, tol = _grad_reference(z.cpu().double(), a.cpu(), None, g_lp.cpu().double(), g_ent.cpu().double(), None)
     _close(got, want, tol + HALF[dtype] * (want.abs() + tol) + TINY[dtype])
+
+
+def test_an_action_that_does_not_exist_spoils_only_its_own_score():
+    z, a = _make(4, 30, torch.float32)
+    a[1] = 30
+    z.requires_grad_(True)
+    s = _scores(z, a, top=2)
+    got, = torch.autograd.grad(s.entropy.sum() + s.top_log_probs.sum(), z)
+    t = _scores(z, None, top=2)
+    want, = torch.autograd.grad(t.entropy.sum() + t.top_log_probs.sum(), z)
+    assert s.log_prob[1].isnan() and got.isfinite().all() and torch.equal(got, want)
+
+
+def test_views_with_a_pending_minus_sign():
+    z, a = _make(5, 90, torch.float32)
+    view = torch.conj(torch.complex(torch.zeros_like(z), z)).imag  # -z, not in memory yet
+    assert view.is_neg()
+    _check(view, a, 3, _scores(view, a, top=3))
+
+
+def test_alternatives_out_of_range_are_not_written():
+    """The C entry takes the list of alternatives from memory: an index outside the row changes nothing."""
+    from muzero_amd import _hip
+    z, a = _make(3, 40, torch.float32)
+    stats = torch.tensor([[3.0, 2.0, 1.0]] * 3, device="cuda")
+    ids = torch.tensor([[0, 40], [-1, 39], [1 << 40, 5]], device="cuda")
+    g_top = torch.ones(3, 2, device="cuda")
+    room = torch.full((5, 40), 7.0, device="cuda")
+    p = _hip.ptr
+    _hip.check(_hip.lib().mz_policy_scores_backward(p(z), _hip.TYPE_F32, 40, None, 3, 40, 2, p(stats), p(ids), None, None, p(g_top),
+                                                    room[1:4].data_ptr(), 40, torch.cuda.current_stream().cuda_stream), "backward")
+    assert (room[0] == 7).all() and (room[4] == 7).all() and room[1:4].isfinite().all()

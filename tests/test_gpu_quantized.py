@@ -594,3 +594,56 @@ def test_offsets_past_32_bits():
     c, d = save_activations(x), save_activations(tail)
     assert torch.equal(c.codes[-3:], d.codes) and torch.equal(c.scales[-3:], d.scales) and (c.scales[:-3] == 0).all()
     assert torch.equal(c.dequantize()[-3:], d.dequantize())
+
+
+def test_a_recorded_graph_follows_refreshed_weights():
+    from muzero_amd.engine import make_networks
+    from muzero_amd.quantized import Int8MLP
+    _, g, f = _networks(6)
+    head, nets = Int8MLP(f.policy_mlp), make_networks(g, f, int8=True)
+    x = torch.randn(9, 168, device="cuda")
+    out = torch.empty(9 * 7, 168, device="cuda")
+
+    def step():
+        nets.dynamics(x, 9 * 7, next_latent=out)
+        return head(x), out.clone()
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        rec = step()
+    for turn in range(3):
+        with torch.no_grad():
+            for p in list(g.parameters()) + list(f.parameters()):
+                p.normal_(0, 0.1)
+        head.refresh(), nets.refresh()
+        graph.replay()
+        torch.cuda.synchronize()
+        with torch.no_grad():
+            assert all(torch.equal(a, b) for a, b in zip(rec, step())), turn
+            fresh = Int8MLP(f.policy_mlp)(x)
+        assert torch.equal(rec[0], fresh)
+
+
+def test_more_rows_than_a_weight_gradient_takes_are_refused_in_front():
+    from muzero_amd.checkpoints import MAX_CHECKPOINT_ROWS, checkpointed_linear
+    w = torch.randn(1, 16, device="cuda", requires_grad=True)
+    x = torch.randn(MAX_CHECKPOINT_ROWS + 1, 16, device="cuda")
+    with pytest.raises(ValueError, match="rows"):
+        checkpointed_linear(x, w)
+    y = checkpointed_linear(x[1:], w)  # the largest number
+    y.sum().backward()
+    want = x[1:].double().sum(0)
+    # codes are off by half a step of at most 1.25 / 127 of a row's largest value; the sum of 2^20 terms of one sign each
+    bound = float(x[1:].abs().amax(1).double().sum()) * 1.25 / 254 + 2.0 ** -24 * 2 ** 20 * float(x.abs().max())
+    assert float((w.grad[0].double() - want).abs().max()) <= bound
+
+
+def test_contexts_leave_float64_layers_alone():
+    from muzero_amd.checkpoints import eight_bit_checkpoints
+    _, g, f = _networks(7)
+    g, f = g.double(), f.double()
+    lat, act = torch.randn(3, 4, 6, 7, device="cuda", dtype=torch.float64), torch.tensor([0, 3, 6], device="cuda")
+    want = g(lat, act) + f(lat)
+    with eight_bit_checkpoints(g, f):
+        got = g(lat, act) + f(lat)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))

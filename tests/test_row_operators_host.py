@@ -217,3 +217,78 @@ def test_dense_sequences_are_recognised():
     assert "merge" not in g.__dict__ and "forward" not in f.policy_mlp.__dict__
     assert all(torch.equal(x, y) for x, y in zip(want, got))
     torch.testing.assert_close(torch.softmax(f.policy_logits(lat), 1), f(lat)[0])
+
+
+def _small_networks():
+    from muzero_amd.config import load_config
+    from muzero_amd.neural_networks import DynamicsNetwork, PredictionNetwork
+    cfg = load_config("config_c4_mlp.yaml")
+    return (DynamicsNetwork(cfg.networks.latent_shape, 7, cfg.networks.dynamics),
+            PredictionNetwork(cfg.networks.latent_shape, 7, cfg.networks.prediction), torch.randn(3, *cfg.networks.latent_shape))
+
+
+def test_checkpoint_contexts_may_overlap_and_be_entered_again():
+    from muzero_amd.checkpoints import eight_bit_checkpoints
+    g, f, _ = _small_networks()
+    a, b = eight_bit_checkpoints(g, f), eight_bit_checkpoints(g)
+    a.__enter__(), b.__enter__()
+    a.__exit__(None, None, None)                  # the first ends before the second
+    assert "merge" in g.__dict__ and "forward" in g.reward_mlp.__dict__ and "forward" not in f.value_mlp.__dict__
+    b.__exit__(None, None, None)
+    assert "merge" not in g.__dict__ and "forward" not in g.reward_mlp.__dict__
+    with a:
+        with a:
+            pass
+        assert "merge" in g.__dict__
+    assert "merge" not in g.__dict__
+    with eight_bit_checkpoints(g, g):
+        pass
+    assert "merge" not in g.__dict__ and "forward" not in g.reward_mlp.__dict__
+
+
+def test_copies_made_inside_a_context_are_themselves():
+    import copy
+    import io
+
+    from muzero_amd.checkpoints import eight_bit_checkpoints
+    g, f, lat = _small_networks()
+    act = torch.tensor([0, 3, 6])
+    with eight_bit_checkpoints(g, f):
+        g2, f2 = copy.deepcopy(g), copy.deepcopy(f)
+        data = io.BytesIO()
+        torch.save((g, f), data)
+    data.seek(0)
+    g3, f3 = torch.load(data, weights_only=False)
+    want = f(lat) + g(lat, act)
+    with torch.no_grad():
+        for p in list(g.parameters()) + list(f.parameters()):
+            p.zero_()
+    for gg, ff in ((g2, f2), (g3, f3)):
+        assert all(torch.equal(x, y) for x, y in zip(want, ff(lat) + gg(lat, act)))
+        with eight_bit_checkpoints(gg, ff) as ctx:
+            assert len(ctx.sequences) == 3 and type(gg.__dict__["merge"]).__name__ == "_Taken"
+        assert all(torch.equal(x, y) for x, y in zip(want, ff(lat) + gg(lat, act)))
+
+
+def test_layers_that_do_more_than_a_layer_are_left_alone():
+    from muzero_amd.checkpoints import eight_bit_checkpoints
+    from muzero_amd.neural_networks.network_builder import is_dense_sequence
+
+    class Twice(torch.nn.Linear):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Sum(torch.nn.Sequential):
+        def forward(self, x):
+            return super().forward(x) + x
+    assert is_dense_sequence(torch.nn.Sequential(torch.nn.Linear(3, 3), torch.nn.ReLU()))
+    assert not is_dense_sequence(torch.nn.Sequential(Twice(3, 3), torch.nn.ReLU()))
+    assert not is_dense_sequence(Sum(torch.nn.Linear(3, 3), torch.nn.ReLU()))
+    hooked = torch.nn.Sequential(torch.nn.Linear(3, 3), torch.nn.ReLU())
+    hooked[0].register_forward_hook(lambda m, x, y: y + 1)
+    assert not is_dense_sequence(hooked)
+    own = torch.nn.Sequential(torch.nn.Linear(3, 3), torch.nn.ReLU())
+    own.forward = lambda x: x
+    with eight_bit_checkpoints(own):
+        assert own(5) == 5
+    assert own(5) == 5
