@@ -111,7 +111,8 @@ struct Prepared {  // what k_prepare reads of the statistics, and what it leaves
 
 constexpr int kSplitCols = 64, kCodeCols = 128;
 
-// dz -> planes for 64 columns and 64 rows, the columns' factors first.  v = dz s c is formed in float32 and split before it goes to LDS; a lane then collects 8 rows of one column, 16 bytes of each plane.
+// dz -> planes for 64 columns and 64 rows, the columns' factors first.  v = dz s c is formed in float32 and split before it
+// goes to LDS; a lane then collects 8 rows of one column, 16 bytes of each plane.
 template <class T, int PLANES, bool WHOLE, Stats STATS>
 __device__ void split_block(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int64_t Rp, int n0,
                             int r0, const Prepared &out, T *__restrict__ db, uint8_t *lds) {
@@ -172,7 +173,7 @@ __device__ void split_block(const T *__restrict__ dz, int64_t ldz, const float *
         Pack<T> p{};
         float scale = 0.0f;
         if (r0 + r < R && n0 + c < N) {
-            p = load_pack<T, WHOLE>(dz + (r0 + r) * ldz, n0 + c, N);
+            p = load_pack<T, WHOLE, STATS != kOwn>(dz + (r0 + r) * ldz, n0 + c, N);
             scale = scales[r0 + r];
         }
 #pragma unroll
@@ -272,7 +273,7 @@ k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, c
     Tl::template drain<true>(lds, acc, [&](int b, const f32x4 &v) { return v * inv[b]; }, [&](int n, const f32x4 &v) {
         if (n0 + n >= N) return;
         const float o[4] = {v[0], v[1], v[2], v[3]};
-        store_quad(dw + (n0 + n) * ldw, k, K, aligned, o);
+        store_quad<false>(dw + (n0 + n) * ldw, k, K, aligned, o);
     });
 }
 
@@ -285,7 +286,7 @@ k_weight_join(const float *__restrict__ partial, int splits, const float *__rest
     if (c < quads) {
         const f32x4 sum = sum_parts<f32x4>(partial, splits, (int64_t)N * quads, (int64_t)n * quads + c) * inverse[n];
         const float o[4] = {sum[0], sum[1], sum[2], sum[3]};
-        store_quad(dw + n * ldw, k, K, aligned, o);
+        store_quad<false>(dw + n * ldw, k, K, aligned, o);
     }
 }
 

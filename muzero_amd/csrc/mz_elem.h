@@ -39,22 +39,42 @@ inline bool rows_aligned(const void *p, int64_t ld) {
     return ((uintptr_t)p & 15) == 0 && (ld * (int64_t)sizeof(T)) % 16 == 0;
 }
 
-// Elements j .. j + n - 1 of a row of K, zeros behind its end; WHOLE: rows start on 16-byte addresses.
-template <class T, bool WHOLE>
+// Elements j .. j + n - 1 of a row of K, zeros behind its end; WHOLE: rows start on 16-byte addresses; PAST: this is the
+// last time the call reads them, their lines need not stay in cache.
+template <class T, bool WHOLE, bool PAST = false>
 __device__ __forceinline__ Pack<T> load_pack(const T *__restrict__ row, int j, int K) {
     constexpr int n = Pack<T>::n;
-    if (WHOLE && j + n <= K) return *(const Pack<T> *)(row + j);
+    if (WHOLE && j + n <= K) {
+        using words = __attribute__((ext_vector_type(4))) unsigned;
+        if (PAST) return __builtin_bit_cast(Pack<T>, __builtin_nontemporal_load((const words *)(row + j)));
+        return *(const Pack<T> *)(row + j);
+    }
     Pack<T> p;
 #pragma unroll
     for (int e = 0; e < n; ++e) p.v[e] = j + e < K ? row[j + e] : (T)0.0f;
     return p;
 }
 
-template <class T, bool WHOLE>
+// A store whose line need not stay in cache.
+template <class T>
+__device__ __forceinline__ void store_past(T *to, const T &v) {
+    using words = __attribute__((ext_vector_type(sizeof(T) / 4))) unsigned;
+    __builtin_nontemporal_store(__builtin_bit_cast(words, v), (words *)to);
+}
+
+// Results of this size go past the caches: written through them they push out the operands, of which other workgroups
+// (or the next call) still need parts, and whoever reads them finds little of them in the 256 MB of the last level anyway.
+// us with / without: int8 product of 8192 x 4096 x 8192 to bf16 (134 MB) 236 / 262, 113 MB of codes read back 53.5 / 55.5
+// with their coding; but four layers in a row, each reading what the last one wrote, 256 x 4096 x 4096 22.4 / 22.0,
+// 4096 x 4096 x 4096 to float32 (67 MB) 78 / 74, 8192 x 8192 x 8192 to bf16 465 / 471.
+inline bool past_caches(int64_t bytes) { return bytes >= 100LL << 20; }
+
+template <class T, bool WHOLE, bool PAST = false>
 __device__ __forceinline__ void store_pack(T *__restrict__ row, int j, int K, const Pack<T> &p) {
     constexpr int n = Pack<T>::n;
     if (WHOLE && j + n <= K) {
-        *(Pack<T> *)(row + j) = p;
+        if constexpr (PAST) store_past((Pack<T> *)(row + j), p);
+        else *(Pack<T> *)(row + j) = p;
     } else {
 #pragma unroll
         for (int e = 0; e < n; ++e)

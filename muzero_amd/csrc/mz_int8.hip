@@ -23,7 +23,7 @@ __device__ __forceinline__ float activate(float v, int act) {
     }
 }
 
-template <class T, class Tl>
+template <class T, class Tl, bool PAST>
 __global__ void __launch_bounds__(Tl::threads)
 k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs, int rows, const int8_t *__restrict__ wc,
        int64_t ldw, const float *__restrict__ ws, int N, int kbytes, const float *__restrict__ bias, int act, T *__restrict__ y,
@@ -57,7 +57,7 @@ k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs
     const auto put = [&](int r, const f32x4 &v, auto &&f) {
         if (r0 + r >= rows) return;
         const float o[4] = {f(v[0] * t[0] + c[0]), f(v[1] * t[1] + c[1]), f(v[2] * t[2] + c[2]), f(v[3] * t[3] + c[3])};
-        store_quad(y + (r0 + r) * ldy, n, N, aligned, o);
+        store_quad<PAST>(y + (r0 + r) * ldy, n, N, aligned, o);
     };
     if (act == MZ_ACT_NONE || act == MZ_ACT_RELU) {
         const float least = act == MZ_ACT_RELU ? 0.0f : -INFINITY;  // a NaN is not less: it passes
@@ -79,7 +79,7 @@ k_int8_join(const int *__restrict__ partial, int splits, const float *__restrict
     float o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = n + e < N ? activate((float)sum[e] * s * ws[n + e] + (bias ? bias[n + e] : 0.0f), act) : 0.0f;
-    store_quad(y + r * ldy, n, N, aligned, o);
+    store_quad<false>(y + r * ldy, n, N, aligned, o);
 }
 
 // A few rows (at most 16 NB): bound by reading the weights once.  A workgroup takes 16 output channels and all rows, its
@@ -273,11 +273,11 @@ struct Int8Args {
     int *partial;
 };
 
-template <class T, class Tl>
+template <class T, class Tl, bool PAST = false>
 void launch_tiles(const Int8Args &a, int splits, hipStream_t st) {
     const int tiles_n = (a.N + Tl::TI - 1) / Tl::TI, tiles_r = (a.rows + Tl::TO - 1) / Tl::TO;
     const bool aligned = quads_aligned((T *)a.y, a.ldy);
-    hipLaunchKernelGGL((k_int8<T, Tl>), dim3((unsigned)(tiles_n * tiles_r * splits)), dim3(Tl::threads), 0, st, a.xc, a.ldxc, a.xs, a.rows,
+    hipLaunchKernelGGL((k_int8<T, Tl, PAST>), dim3((unsigned)(tiles_n * tiles_r * splits)), dim3(Tl::threads), 0, st, a.xc, a.ldxc, a.xs, a.rows,
                        a.wc, a.ldw, a.ws, a.N, (int)round_up(a.K, kStep), a.bias, a.act, (T *)a.y, a.ldy, aligned, tiles_n, tiles_r, splits,
                        a.partial);
     if (splits > 1) {
@@ -312,7 +312,9 @@ void launch_shape(const Int8Args &a, hipStream_t st) {
         return;
     }
     const Shape s = shape_of_int8(a.rows, a.N, a.K);
-    if (s.tile == 256) launch_tiles<T, Tile<OpI8, 256, 256, 4, 2>>(a, s.splits, st);
+    const bool past = past_caches((int64_t)a.rows * a.N * (int64_t)sizeof(T));  // such outputs have 256 x 256 tiles
+    if (s.tile == 256 && past) launch_tiles<T, Tile<OpI8, 256, 256, 4, 2>, true>(a, s.splits, st);
+    else if (s.tile == 256) launch_tiles<T, Tile<OpI8, 256, 256, 4, 2>>(a, s.splits, st);
     else if (s.tile == 128) launch_tiles<T, Tile<OpI8, 128, 256, 2, 4>>(a, s.splits, st);
     else launch_tiles<T, Tile<OpI8, 64, 64, 2, 2>>(a, s.splits, st);
 }

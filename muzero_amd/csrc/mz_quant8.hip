@@ -33,7 +33,7 @@ k_quant8(const T *__restrict__ x, int64_t ldx, int64_t rows, int K, int scale_bi
         unsigned m = 0;
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
-            if ((t + h * THREADS) * n < K) held[h] = load_pack<T, WHOLE>(xr, (t + h * THREADS) * n, K);
+            if ((t + h * THREADS) * n < K) held[h] = load_pack<T, WHOLE, true>(xr, (t + h * THREADS) * n, K);
             else held[h] = Pack<T>{};
 #pragma unroll
         for (int h = 0; h < HELD; ++h)
@@ -63,7 +63,7 @@ k_quant8(const T *__restrict__ x, int64_t ldx, int64_t rows, int K, int scale_bi
     }
 }
 
-template <class T, int THREADS, bool WHOLE>
+template <class T, int THREADS, bool WHOLE, bool PAST>
 __global__ void __launch_bounds__(kQT)
 k_dequant8(const int8_t *__restrict__ codes, int64_t ldc, const float *__restrict__ scales, int64_t rows, int K,
            T *__restrict__ x, int64_t ldx) {
@@ -80,7 +80,7 @@ k_dequant8(const int8_t *__restrict__ codes, int64_t ldc, const float *__restric
             Pack<T> p;
 #pragma unroll
             for (int e = 0; e < n; ++e) p.v[e] = (T)((float)q[e] * s);
-            store_pack<T, WHOLE>(x + row * ldx, j, K, p);
+            store_pack<T, WHOLE, PAST>(x + row * ldx, j, K, p);
         }
     }
 }
@@ -216,12 +216,14 @@ int mz_dequant8_rows(const int8_t *codes, int64_t ldc, const float *scales, int6
         using T = decltype(t);
         with_flag(rows_aligned<T>(x, ldx), [&](auto whole) {
             constexpr bool W = decltype(whole)::value;
-            if (K <= 4 * 64 * Pack<T>::n)
-                hipLaunchKernelGGL((k_dequant8<T, 64, W>), row_grid(rows, 4), dim3(kQT), 0, (hipStream_t)stream, codes, ldc, scales, rows,
-                                   K, (T *)x, ldx);
-            else
-                hipLaunchKernelGGL((k_dequant8<T, 256, W>), row_grid(rows, 1), dim3(kQT), 0, (hipStream_t)stream, codes, ldc, scales, rows,
-                                   K, (T *)x, ldx);
+            const auto launch = [&](auto kernel, int per) {
+                hipLaunchKernelGGL(kernel, row_grid(rows, per), dim3(kQT), 0, (hipStream_t)stream, codes, ldc, scales, rows, K, (T *)x, ldx);
+            };
+            with_flag(past_caches(rows * K * (int64_t)sizeof(T)), [&](auto past) {
+                constexpr bool P = decltype(past)::value;
+                if (K <= 4 * 64 * Pack<T>::n) launch(k_dequant8<T, 64, W, P>, 4);
+                else launch(k_dequant8<T, 256, W, P>, 1);
+            });
         });
     });
     return mz::check_launch("k_dequant8");

@@ -578,7 +578,8 @@ k_grad_small(const T *__restrict__ logits, int64_t ld, int64_t rows, Grads in, T
 }
 
 // Longer rows in pieces of LANES lanes with kGradPacks packs each: a wave per piece while that covers a row, else a workgroup.
-// Bound by the bytes: 20000 x 32768 (bf16 or fp16) runs at 5.5 TB/s.
+// From the last row to the first, as the forward pass left the last ones in cache (4096 x 32768 bf16, both passes: 170
+// against 176 us), and past the caches on the way out (140).  Bound by the bytes: 20000 x 32768 fp16 5.5 TB/s.
 constexpr int kGradPacks = 4;
 
 template <class T, int LANES>
@@ -587,8 +588,8 @@ k_grad_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int pieces, 
     constexpr int n = Span<T>::n;
     constexpr int64_t kTeams = kLT / LANES;
     for (int64_t job = blockIdx.x * kTeams + threadIdx.x / LANES; job < rows * pieces; job += gridDim.x * kTeams) {
-        const int64_t row = job / pieces;
-        const int piece = (int)(job - row * pieces);
+        const int64_t at = rows * pieces - 1 - job, row = at / pieces;
+        const int piece = (int)(at - row * pieces);
         const Span<T> span(logits + row * ld, 0, in.V);
         T *out = grad + row * ldg;
         // packs of the logits' alignment: stores are whole when the gradient's row has the same one
@@ -601,7 +602,7 @@ k_grad_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int pieces, 
 #pragma unroll
             for (int e = 0; e < n; ++e) p.v[e] = (T)grad_one(r, (float)z.v[e], j + e);
             if (whole && i >= span.whole_lo && i < span.whole_hi) {
-                *(Pack<T> *)(out + j) = p;
+                store_past((Pack<T> *)(out + j), p);  // of any size: 67 MB 55 against 58 us, and not slower with a reader
             } else {
 #pragma unroll
                 for (int e = 0; e < n; ++e)

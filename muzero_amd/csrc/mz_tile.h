@@ -227,10 +227,12 @@ struct alignas(4 * sizeof(T)) Quad {
     T v[4];
 };
 
-template <class T>
+template <bool PAST, class T>
 __device__ __forceinline__ void store_quad(T *row, int at, int n, bool aligned, const float (&v)[4]) {
     if (aligned && at + 4 <= n) {
-        *(Quad<T> *)(row + at) = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+        const Quad<T> q = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+        if constexpr (PAST) mze::store_past((Quad<T> *)(row + at), q);
+        else *(Quad<T> *)(row + at) = q;
     } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
