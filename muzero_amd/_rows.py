@@ -30,15 +30,16 @@ def check_on_gpu(t: torch.Tensor, what: str) -> None:
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """t as [rows, columns] with adjacent columns and rows that do not overlap: a view where its strides allow one, else
     a copy."""
-    cols = t.shape[-1]
     if t.is_neg():  # a view whose minus sign is not in memory yet
         t = t.resolve_neg()
     if t.dim() != 2:
+        cols = t.shape[-1]
         t = t.reshape(-1, cols) if cols else t.reshape(t.shape[:-1].numel(), 0)
-    if (cols > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < cols):
+    (rows, cols), (step, one) = t.shape, t.stride()
+    if (cols > 1 and one != 1) or (rows > 1 and step < cols):
         t = t.contiguous()
-    if t.shape[0] > MAX_ROWS or t.shape[1] > MAX_COLUMNS:
-        raise ValueError(f"{t.shape[0]} rows of {t.shape[1]} values are more than a call takes ({MAX_ROWS} of {MAX_COLUMNS})")
+    if rows > MAX_ROWS or cols > MAX_COLUMNS:
+        raise ValueError(f"{rows} rows of {cols} values are more than a call takes ({MAX_ROWS} of {MAX_COLUMNS})")
     return t
 
 

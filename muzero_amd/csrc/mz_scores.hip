@@ -8,6 +8,8 @@
 // float32 values), as their sum would round the log probabilities of large logits.  A row without any finite or infinite
 // value left (every logit -inf) has log p = -inf, H = 0 and no gradient.  NaN and +inf make the row's results NaN.
 // Alternatives are ordered by (logit, lowest index first); NaN counts as the largest value, -0 equals 0.
+#include <algorithm>
+
 #include "mz_elem.h"
 
 namespace {
@@ -302,7 +304,6 @@ k_scores_wave(const T *__restrict__ logits, int64_t ld, int64_t rows, Out out) {
 }
 
 // ---------------------------------------------------------------- long rows: a workgroup streams a row, or a part of it
-constexpr int kLT = 256;          // threads
 constexpr int kCand = 1024;       // candidates for the alternatives that a workgroup can hold
 constexpr int kMaxParts = 64;     // parts of one row (one lane of the joining wave each)
 
@@ -329,36 +330,36 @@ __device__ __forceinline__ void add(Sums &a, const Pack<T> &p) {
     }
 }
 
+template <int LT>
 struct Shared {
-    Sums part[kLT / 64];
+    Sums part[LT / 64];
     Key cand[kCand];
-    unsigned best[kLT];
-    Key thread_key[kLT];
-    int owner[kLT];
+    unsigned best[LT];
+    Key thread_key[LT];
+    int owner[LT];
     Key found[kMaxTop];
     Key threshold;
     int count, owners;
 };
 
-// Largest value t (its low 16 order bits dropped) that at least `top` of the workgroup's threads reach with their own
-// largest logit: at least `top` logits are >= t, so no smaller one is an alternative.  Every wave finds it by itself.
-__device__ __forceinline__ float value_threshold(const Shared &sh, int top) {
+// Largest value t (its low 16 order bits dropped) that at least `top` of 64 groups of threads reach with their largest
+// logit: at least `top` logits are >= t, so no smaller one is an alternative.  Every wave finds it by itself.
+template <int LT>
+__device__ __forceinline__ float value_threshold(const Shared<LT> &sh, int top) {
     const int lane = threadIdx.x & 63;
-    unsigned b[kLT / 64], t = 0;
+    unsigned b = 0, t = 0;
 #pragma unroll
-    for (int w = 0; w < kLT / 64; ++w) b[w] = sh.best[w * 64 + lane];
+    for (int w = 0; w < LT / 64; ++w) b = max(b, sh.best[w * 64 + lane]);
     for (int bit = 31; bit >= 16; --bit) {
         const unsigned probe = t | (1u << bit);
-        int n = 0;
-#pragma unroll
-        for (int w = 0; w < kLT / 64; ++w) n += __popcll(__ballot(b[w] >= probe));
-        if (n >= top) t = probe;
+        if (__popcll(__ballot(b >= probe)) >= top) t = probe;
     }
     return t <= order_bits(-INFINITY) ? -INFINITY : bits_value(t);
 }
 
 // The candidates in sh.cand, ranked by counting the larger ones: the `top` first go to sh.found in order.
-__device__ __forceinline__ void rank_candidates(Shared &sh, int count, int top) {
+template <int LT>
+__device__ __forceinline__ void rank_candidates(Shared<LT> &sh, int count, int top) {
     if (count <= 64) {  // in the registers of one wave
         if (threadIdx.x < 64) {
             const Key k = (int)threadIdx.x < count ? sh.cand[threadIdx.x] : 0;
@@ -367,7 +368,7 @@ __device__ __forceinline__ void rank_candidates(Shared &sh, int count, int top) 
             if (rank < top && k != 0) sh.found[rank] = k;
         }
     } else {
-        for (int c = threadIdx.x; c < count; c += kLT) {
+        for (int c = threadIdx.x; c < count; c += LT) {
             const Key k = sh.cand[c];
             int rank = 0;
             for (int o = 0; o < count; ++o) rank += sh.cand[o] > k;
@@ -383,17 +384,17 @@ __device__ __forceinline__ void rank_candidates(Shared &sh, int count, int top) 
 //     all threads together;
 //  2. rows with too many equal values for that (all masked, all equal): the same with (value, index) keys;
 //  3. whatever overflows that, too: one alternative per pass.
-template <class T>
-__device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool loud) {
+template <class T, int LT>
+__device__ void find_alternatives(const Span<T> &span, Shared<LT> &sh, int top, bool loud) {
     constexpr int n = Span<T>::n;
-    const int per_thread = (span.packs + kLT - 1) / kLT;
+    const int per_thread = (span.packs + LT - 1) / LT;
     // the logits of the threads with `mine` that are `wanted`; sh.count and sh.owners are 0 before
     const auto collect = [&](bool mine, auto &&wanted) {
         if (mine) sh.owner[atomicAdd(&sh.owners, 1)] = threadIdx.x;
         __syncthreads();
         const int items = sh.owners * per_thread;
-        for (int q = threadIdx.x; q < items; q += kLT) {
-            const int o = q / per_thread, i = sh.owner[o] + (q - o * per_thread) * kLT;
+        for (int q = threadIdx.x; q < items; q += LT) {
+            const int o = q / per_thread, i = sh.owner[o] + (q - o * per_thread) * LT;
             if (i >= span.packs) continue;
             const Pack<T> p = span.load(i);
 #pragma unroll
@@ -417,7 +418,7 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
         count = collect(sh.best[threadIdx.x] >= order_bits(t), [&](float z, int) { return z >= t; });
         if (count > kCand) {
             Key mine = 0;
-            span.template each<kLT>(threadIdx.x, [&](const Pack<T> &p, int i) {
+            span.template each<LT>(threadIdx.x, [&](const Pack<T> &p, int i) {
 #pragma unroll
                 for (int e = 0; e < n; ++e) {
                     const int j = span.at(i) + e;
@@ -430,7 +431,7 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
             if (threadIdx.x == 0) sh.count = 0, sh.owners = 0, sh.threshold = 0;  // fewer owning threads than top: everything
             __syncthreads();
             int rank = 0;
-            for (int o = 0; o < kLT; ++o) rank += sh.thread_key[o] > mine;
+            for (int o = 0; o < LT; ++o) rank += sh.thread_key[o] > mine;
             if (rank == top - 1 && mine != 0) sh.threshold = mine;
             __syncthreads();
             const Key t2 = sh.threshold;
@@ -444,7 +445,7 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
     Key last = ~0ull;
     for (int a = 0; a < top; ++a) {
         Key best = 0;
-        span.template each<kLT>(threadIdx.x, [&](const Pack<T> &p, int i) {
+        span.template each<LT>(threadIdx.x, [&](const Pack<T> &p, int i) {
 #pragma unroll
             for (int e = 0; e < n; ++e) {
                 const int j = span.at(i) + e;
@@ -457,18 +458,18 @@ __device__ void find_alternatives(const Span<T> &span, Shared &sh, int top, bool
         if ((threadIdx.x & 63) == 0) sh.thread_key[threadIdx.x >> 6] = best;
         __syncthreads();
         last = sh.thread_key[0];
-        for (int w = 1; w < kLT / 64; ++w) last = max(last, sh.thread_key[w]);
+        for (int w = 1; w < LT / 64; ++w) last = max(last, sh.thread_key[w]);
         if (threadIdx.x == 0) sh.found[a] = last;
     }
     __syncthreads();
 }
 
 // Workgroup (row, part).  One part: the results.  Several: the part's sums and alternatives to the workspace.
-template <class T, bool TOP>
-__global__ void __launch_bounds__(kLT)
+template <class T, int LT, bool TOP>
+__global__ void __launch_bounds__(LT)
 k_scores_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts, Out out, Sums *__restrict__ part_sums,
               Key *__restrict__ part_keys) {
-    __shared__ Shared sh;
+    __shared__ Shared<LT> sh;
     const int top = TOP ? out.top : 0;
     for (int64_t job = blockIdx.x; job < rows * parts; job += gridDim.x) {
         const int64_t row = job / parts;
@@ -476,7 +477,7 @@ k_scores_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts,
         const T *z = logits + row * ld;
         const Span<T> span(z, (int)((int64_t)out.V * part / parts), (int)((int64_t)out.V * (part + 1) / parts));
         Sums acc = none();
-        span.template each<kLT>(threadIdx.x, [&](const Pack<T> &p, int) { add(acc, p); });
+        span.template each<LT>(threadIdx.x, [&](const Pack<T> &p, int) { add(acc, p); });
         __syncthreads();  // the last job's shared values have been read
         sh.best[threadIdx.x] = order_bits(acc.s == 0.0f ? -INFINITY : acc.m);
 #pragma unroll
@@ -484,7 +485,7 @@ k_scores_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts,
         if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = acc;
         __syncthreads();
         acc = sh.part[0];
-        for (int w = 1; w < kLT / 64; ++w) acc = join(acc, sh.part[w]);
+        for (int w = 1; w < LT / 64; ++w) acc = join(acc, sh.part[w]);
         const Row r = row_of(acc);
         if constexpr (TOP) find_alternatives(span, sh, top, r.loud);
         if (parts == 1) {
@@ -583,10 +584,10 @@ k_grad_small(const T *__restrict__ logits, int64_t ld, int64_t rows, Grads in, T
 constexpr int kGradPacks = 4;
 
 template <class T, int LANES>
-__global__ void __launch_bounds__(kLT)
+__global__ void __launch_bounds__(256)
 k_grad_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int pieces, Grads in, T *__restrict__ grad, int64_t ldg) {
     constexpr int n = Span<T>::n;
-    constexpr int64_t kTeams = kLT / LANES;
+    constexpr int64_t kTeams = 256 / LANES;
     for (int64_t job = blockIdx.x * kTeams + threadIdx.x / LANES; job < rows * pieces; job += gridDim.x * kTeams) {
         const int64_t at = rows * pieces - 1 - job, row = at / pieces;
         const int piece = (int)(at - row * pieces);
@@ -643,22 +644,35 @@ constexpr int64_t kMaxGrid = 1 << 20;
 dim3 grid_of(int64_t n) { return dim3((unsigned)(n < kMaxGrid ? n : kMaxGrid)); }
 
 // Rows of up to kSmall logits take part of a wave, up to kWave a whole one (16 packs of 4 float32 a lane, wherever the row
-// starts), longer ones are streamed by a workgroup; fewer of those than kFill are cut into parts of at least kPartBytes, so
-// that a short batch of long rows still reaches all 256 compute units.  us for kFill 256 / 512 / 1024:
-// 64 x 131072 (fp16, 20 alternatives) 20.8 / 17.2 / 18.6, 256 x 131072 40.8 / 33.7 / 31.0, 300 x 32768 (float32, 5)
-// 14.1 / 16.4 / 17.3, 1000 x 8192 10.5 / 10.3 / 18.0; kPartBytes 8192 / 16384 / 32768: 1 x 131072 (bf16, 5) 10.2 / 10.5 /
-// 11.4, 8 x 4096 (float32) 9.3 / 5.8 / 5.8.
-constexpr int kSmall = 64, kWave = 4088, kFill = 512, kPartBytes = 16384;
+// starts).  Longer ones are streamed by workgroups; a short batch of them has to reach all 256 compute units and still be
+// few launches, as the one that joins the parts of rows costs 3 us and as much again on the host:
+//   more than kRows rows      256 threads per row, below kFill workgroups in parts of at least kPartBytes
+//   rows up to kShort bytes   256 threads
+//   up to kWhole bytes, or    1024 threads
+//     from kManyRows rows on
+//   else                      256 threads, in parts as above
+// GPU us (bf16; with 5 or 20 alternatives) for 256 threads / 1024 threads / parts: 1 x 5000 6.2 / 8.3 / -, 1 x 20000 7.7 /
+// 9.5 / 10.3, 1 x 32768 - / 10.1 / 9.5 (16 against 20 for a call with its host's work), 1 x 65536 - / 12.4 / 9.7,
+// 1 x 131072 - / 16.7 / 10.2, 64 x 131072 - / 18.4 / 16.8, 100 x 131072 - / 18.5 / 21.8, 200 x 131072 - / 20 / 27.8,
+// 300 x 131072 - / 47 / 27; kFill 256 / 512 / 1024: 300 x 32768 (float32) 14.1 / 16.4 / 17.3, 64 x 131072 20.8 / 17.2 / 18.6;
+// kPartBytes 8192 / 16384 / 32768: 1 x 131072 10.2 / 10.5 / 11.4.
+constexpr int kSmall = 64, kWave = 4088, kRows = 256, kManyRows = 96, kShort = 48 << 10, kWhole = 96 << 10, kFill = 512,
+              kPartBytes = 16 << 10;
 
-int parts_of(int32_t type, int64_t T, int32_t V) {
-    if (V <= kWave || T >= kFill) return 1;
-    const int64_t by_size = (int64_t)V * type_bytes(type) / kPartBytes, by_fill = (kFill + T - 1) / T;
-    const int64_t p = by_size < by_fill ? by_size : by_fill;
-    return (int)(p < 1 ? 1 : p > kMaxParts ? kMaxParts : p);
+struct Split {
+    int threads, parts;
+};
+
+Split split_of(int32_t type, int64_t T, int32_t V) {
+    const int64_t bytes = (int64_t)V * type_bytes(type);
+    if (V <= kWave || (T <= kRows && bytes <= kShort)) return {256, 1};
+    if (T <= kRows && (bytes <= kWhole || T >= kManyRows)) return {1024, 1};
+    const int64_t parts = std::min(bytes / kPartBytes, (kFill + T - 1) / T);
+    return {256, (int)std::max<int64_t>(1, std::min<int64_t>(parts, kMaxParts))};
 }
 
 template <class T>
-void launch_scores(const T *logits, int64_t ld, int64_t rows, int parts, const Out &out, void *workspace, hipStream_t st) {
+void launch_scores(const T *logits, int64_t ld, int64_t rows, Split split, const Out &out, void *workspace, hipStream_t st) {
     using std::integral_constant;
     const int V = out.V;
     const auto small = [&](auto lanes) {
@@ -686,12 +700,14 @@ void launch_scores(const T *logits, int64_t ld, int64_t rows, int parts, const O
         else wave(integral_constant<int, 16>{});
         return;
     }
+    const int parts = split.parts;
     Key *keys = (Key *)workspace;
     Sums *sums = (Sums *)(keys + (parts > 1 ? rows * parts * out.top : 0));
-    if (out.top > 0)
-        hipLaunchKernelGGL((k_scores_long<T, true>), grid_of(rows * parts), dim3(kLT), 0, st, logits, ld, rows, parts, out, sums, keys);
-    else
-        hipLaunchKernelGGL((k_scores_long<T, false>), grid_of(rows * parts), dim3(kLT), 0, st, logits, ld, rows, parts, out, sums, keys);
+    const auto stream = [&](auto kernel, int threads) {
+        hipLaunchKernelGGL(kernel, grid_of(rows * parts), dim3(threads), 0, st, logits, ld, rows, parts, out, sums, keys);
+    };
+    if (split.threads == 1024) out.top > 0 ? stream(k_scores_long<T, 1024, true>, 1024) : stream(k_scores_long<T, 1024, false>, 1024);
+    else out.top > 0 ? stream(k_scores_long<T, 256, true>, 256) : stream(k_scores_long<T, 256, false>, 256);
     if (parts > 1)
         hipLaunchKernelGGL(k_scores_join<T>, grid_of(rows), dim3(64), 0, st, logits, ld, rows, parts, out, (const Sums *)sums,
                            (const Key *)keys);
@@ -714,9 +730,9 @@ void launch_grad(const T *logits, int64_t ld, int64_t rows, const Grads &in, T *
     } else {
         const int packs = (in.V + Pack<T>::n - 1) / Pack<T>::n + 1;  // a row that starts off a 16-byte address has one more
         const auto large = [&](auto lanes) {
-            constexpr int L = decltype(lanes)::value, teams = kLT / L;
+            constexpr int L = decltype(lanes)::value, teams = 256 / L;
             const int pieces = (packs + kGradPacks * L - 1) / (kGradPacks * L);
-            hipLaunchKernelGGL((k_grad_long<T, L>), grid_of((rows * pieces + teams - 1) / teams), dim3(kLT), 0, st, logits, ld, rows,
+            hipLaunchKernelGGL((k_grad_long<T, L>), grid_of((rows * pieces + teams - 1) / teams), dim3(256), 0, st, logits, ld, rows,
                                pieces, in, grad, ldg);
         };
         if (packs <= kGradPacks * 64)
@@ -747,7 +763,7 @@ extern "C" {
 
 int64_t mz_policy_scores_workspace(int32_t type, int64_t T, int32_t V, int32_t top) {
     if (!type_ok(type) || T <= 0 || V <= 0 || top < 0 || top > kMaxTop) return 0;
-    const int parts = parts_of(type, T, V);
+    const int parts = split_of(type, T, V).parts;
     return parts > 1 ? T * parts * ((int64_t)sizeof(Sums) + top * (int64_t)sizeof(Key)) : 0;
 }
 
@@ -765,7 +781,7 @@ int mz_policy_scores(const void *logits, int32_t type, int64_t ld, const int64_t
     const Out out{actions, log_prob, entropy, stats, top_actions, top_log_probs, V, top};
     with_type(type, [&](auto t) {
         using E = decltype(t);
-        launch_scores((const E *)logits, ld, T, parts_of(type, T, V), out, workspace, (hipStream_t)stream);
+        launch_scores((const E *)logits, ld, T, split_of(type, T, V), out, workspace, (hipStream_t)stream);
     });
     return mz::check_launch("k_scores");
 }

@@ -20,9 +20,10 @@ from torch.autograd.function import once_differentiable
 
 from muzero_amd import _hip
 from muzero_amd._hip import ptr
-from muzero_amd._rows import TYPE, check_tensor, on_device, row_stride, rows_of, stream_of, workspace
+from muzero_amd._rows import TYPE, check_tensor, on_device, rows_of, stream_of, workspace
 
 MAX_TOP = 32
+_WHOLE = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
 
 class PolicyScores(NamedTuple):
@@ -33,20 +34,27 @@ class PolicyScores(NamedTuple):
 
 
 def _forward(logits: torch.Tensor, actions: Optional[torch.Tensor], top: int, want_stats: bool):
+    # A small batch is bound by this function: few calls, no helpers.
     T, V = logits.shape
-    log_prob = None if actions is None else logits.new_empty(T, dtype=torch.float32)
-    entropy = logits.new_empty(T, dtype=torch.float32)
-    stats = logits.new_empty((T, 3), dtype=torch.float32) if want_stats else None
-    top_actions = logits.new_empty((T, top), dtype=torch.int64) if top else None
-    top_log_probs = logits.new_empty((T, top), dtype=torch.float32) if top else None
+    empty, dev = torch.empty, logits.device
+    log_prob = None if actions is None else empty(T, dtype=torch.float32, device=dev)
+    entropy = empty(T, dtype=torch.float32, device=dev)
+    stats = empty((T, 3), dtype=torch.float32, device=dev) if want_stats else None
+    top_actions = top_log_probs = None
+    if top:
+        top_actions, top_log_probs = empty((T, top), dtype=torch.int64, device=dev), empty((T, top), dtype=torch.float32, device=dev)
     if T > 0:
         lib, kind = _hip.lib(), TYPE[logits.dtype]
         with on_device(logits):
             need = lib.mz_policy_scores_workspace(kind, T, V, top)
-            ws = workspace(need, logits)
-            _hip.check(lib.mz_policy_scores(ptr(logits), kind, row_stride(logits), ptr(actions), T, V, top, ptr(log_prob),
-                                            ptr(entropy), ptr(stats), ptr(top_actions), ptr(top_log_probs), ptr(ws), need,
-                                            stream_of(logits)), "mz_policy_scores")
+            ws = workspace(need, logits) if need else None
+            rc = lib.mz_policy_scores(logits.data_ptr(), kind, logits.stride(0) if T > 1 else V,
+                                      None if actions is None else actions.data_ptr(), T, V, top,
+                                      None if actions is None else log_prob.data_ptr(), entropy.data_ptr(), ptr(stats),
+                                      top_actions.data_ptr() if top else None, top_log_probs.data_ptr() if top else None,
+                                      ptr(ws), need, stream_of(logits))
+            if rc:
+                _hip.check(rc, "mz_policy_scores")
     return log_prob, entropy, stats, top_actions, top_log_probs
 
 
@@ -103,14 +111,14 @@ def policy_scores(logits: torch.Tensor, actions: Optional[torch.Tensor] = None, 
     if not 0 <= top <= min(MAX_TOP, V):
         raise ValueError(f"top={top} must lie in 0..{MAX_TOP} and not exceed the {V} actions")
     if actions is not None:
-        if not isinstance(actions, torch.Tensor) or actions.dtype not in (torch.int64, torch.int32, torch.int16, torch.int8,
-                                                                          torch.uint8):
+        if not isinstance(actions, torch.Tensor) or actions.dtype not in _WHOLE:
             raise TypeError("actions must be a tensor of whole numbers")
         if actions.shape != lead:
             raise ValueError(f"actions of shape {tuple(actions.shape)} do not match logits of shape {tuple(logits.shape)}")
         if actions.device != logits.device:
             raise ValueError(f"actions are on {actions.device}, logits on {logits.device}")
-        actions = actions.reshape(-1).to(torch.int64).contiguous()
+        if actions.dtype is not torch.int64 or actions.dim() != 1 or not actions.is_contiguous():
+            actions = actions.reshape(-1).to(torch.int64).contiguous()
     rows = rows_of(logits)
     if torch.is_grad_enabled() and rows.requires_grad:
         log_prob, entropy, top_actions, top_log_probs = _PolicyScores.apply(rows, actions, top)

@@ -388,3 +388,14 @@ def test_alternatives_out_of_range_are_not_written():
     _hip.check(_hip.lib().mz_policy_scores_backward(p(z), _hip.TYPE_F32, 40, None, 3, 40, 2, p(stats), p(ids), None, None, p(g_top),
                                                     room[1:4].data_ptr(), 40, torch.cuda.current_stream().cuda_stream), "backward")
     assert (room[0] == 7).all() and (room[4] == 7).all() and room[1:4].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("T,V,top", [(1, 24577, 5), (3, 40000, 0), (2, 49153, 32), (96, 30011, 3), (95, 30011, 3), (256, 13001, 4),
+                                     (257, 13001, 4), (300, 24000, 0), (97, 60000, 0)])
+def test_long_rows_between_the_variants(T, V, top, dtype):
+    z, a = _make(T, V, dtype, seed=T + V)
+    z[0, :: 2] = -torch.inf
+    z[T // 2] = 0.25                             # all equal
+    z[T - 1, 1:] = torch.finfo(dtype).min
+    _check(z, a, top)
