@@ -3,7 +3,8 @@
 //     dW_nk = sum_r dz_rn s_r q_rk,     db_n = sum_r dz_rn
 // without writing x out again.
 //
-// The product runs on the fp16 matrix instruction.  Codes are whole numbers up to 127: exact in fp16.  The row scale lies
+// Few rows and a small dW take one launch of their own (k_weight_grad_few).  For the rest the product runs on the fp16
+// matrix instruction.  Codes are whole numbers up to 127: exact in fp16.  The row scale lies
 // along the reduction, so it goes to the other side: v_rn = dz_rn s_r, which fp16 cannot hold as it is.  Each output row n
 // is first brought into range by a power of two c_n (the largest |v_rn c_n| lies in 2^14 .. 2^15) and then held as
 //     one plane   hi = fp16(v c)                       bfloat16 dz with scales of 3 significant bits: 8 + 3 = 11 bits,
@@ -290,6 +291,123 @@ k_weight_join(const float *__restrict__ partial, int splits, const float *__rest
     }
 }
 
+// ---------------------------------------------------------------- few rows: one launch
+// A workgroup forms 32 x 64 values of dW, its eight waves every eighth 32 rows; a lane reads 2 columns of dz and 4 of the
+// codes from 8 rows, which is a fragment of the instruction already, so nothing is transposed and nothing waits for the
+// columns' factors: v = dz s is held in bfloat16 planes, which have float32's range,
+//     two    hi = bf16(v), mid = bf16(v - hi)         16 bits: 16-bit dz with scales of 3 significant bits, exact
+//     three  and lo = bf16(v - hi - mid)              24 bits, as v itself
+// (below 2^-110 the last one loses bits to its smallest value, 2^-133).
+constexpr int kFewN = 32, kFewK = 64, kFewWaves = 8;
+
+using b16x8 = __attribute__((ext_vector_type(8))) __bf16;
+
+template <class T, int PLANES, bool PAIRS>
+__global__ void __launch_bounds__(64 * kFewWaves, 4)
+k_weight_grad_few(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N,
+                  const int8_t *__restrict__ codes, int64_t ldc, int K, T *__restrict__ dw, int64_t ldw, bool aligned,
+                  T *__restrict__ db, int tiles_k) {
+    constexpr int ld = kFewK + 4;
+    __shared__ __align__(16) float sums[kFewWaves][kFewN * ld];
+    __shared__ float db_sums[kFewWaves][kFewN];
+    struct alignas(2 * sizeof(T)) Pair {
+        T v[2];
+    };
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int k0 = (int)(blockIdx.x % tiles_k) * kFewK, n0 = (int)(blockIdx.x / tiles_k) * kFewN;
+    // rows and columns behind the last one are read as the last one: the rows count as zero, the columns are not stored
+    const int8_t *q0 = codes + min((int64_t)(k0 + 4 * c), ldc - 4);
+    const T *d0 = dz + min(n0 + 2 * c, PAIRS ? N - 2 : N - 1), *d1 = dz + min(n0 + 2 * c + 1, N - 1);
+    struct Rows {
+        unsigned q[8];
+        Pair d[8];
+        float s[8];
+    };
+    const auto load = [&](int r0) {
+        Rows x;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t r = min(r0 + 8 * g + j, R - 1);
+            x.s[j] = scales[r];
+            x.q[j] = *(const unsigned *)(q0 + r * ldc);
+            if (PAIRS) x.d[j] = *(const Pair *)(d0 + r * ldz);
+            else x.d[j] = {d0[r * ldz], d1[r * ldz]};
+        }
+        return x;
+    };
+    f32x4 acc[2][4] = {};
+    float col[2] = {};
+    const int waves = min(kFewWaves, (R + 31) / 32);  // with rows to take
+    if (wave < waves) {
+        Rows next = load(wave * 32);
+        for (int r0 = wave * 32; r0 < R; r0 += kFewWaves * 32) {
+            const Rows x = next;
+            next = load(r0 + kFewWaves * 32);
+            b16x8 plane[2][PLANES], code[4];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool live = r0 + 8 * g + j < R;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float d = live ? (float)x.d[j].v[e] : 0.0f;
+                    float v = live ? d * x.s[j] : 0.0f;
+                    col[e] += d;
+#pragma unroll
+                    for (int p = 0; p < PLANES; ++p) {
+                        plane[e][p][j] = (__bf16)v;
+                        v -= (float)plane[e][p][j];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) code[e][j] = (__bf16)(float)(int8_t)(x.q[j] >> 8 * e);
+            }
+#pragma unroll
+            for (int p = PLANES - 1; p >= 0; --p)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+                        acc[e][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(code[h], plane[e][p], acc[e][h], 0, 0, 0);
+        }
+    }
+    // acc[e][h][i] of a lane: dW of column n0 + 2 c + e, input k0 + 4 (4 g + i) + h
+    if (wave < waves) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(f32x4 *)&sums[wave][(2 * c + e) * ld + 4 * (4 * g + i)] = f32x4{acc[e][0][i], acc[e][1][i], acc[e][2][i], acc[e][3][i]};
+            col[e] += __shfl_xor(col[e], 16);
+            col[e] += __shfl_xor(col[e], 32);
+            if (g == 0) db_sums[wave][2 * c + e] = col[e];
+        }
+    }
+    __syncthreads();
+    const int row = threadIdx.x >> 4, kq = (threadIdx.x & 15) * 4;
+    f32x4 sum = {};
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w)
+        if (w < waves) sum += *(const f32x4 *)&sums[w][row * ld + kq];
+    if (n0 + row < N) {
+        const float o[4] = {sum[0], sum[1], sum[2], sum[3]};
+        store_quad<false>(dw + (n0 + row) * ldw, k0 + kq, K, aligned, o);
+    }
+    if (db && k0 == 0 && threadIdx.x < kFewN && n0 + (int)threadIdx.x < N) {
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; ++w)
+            if (w < waves) total += db_sums[w][threadIdx.x];
+        db[n0 + threadIdx.x] = (T)total;
+    }
+}
+
+// Up to here the one launch wins (us, this / the kernels below; float32): 256 x 168 x 256 (rows, K, N) 5.1 / 15.0,
+// 1024 x 512 x 512 10 / 29, 2048 x 1024 x 1024 33 / 41, 4096 x 64 x 64 27 / 24 (but one launch for five, each 3 us of the
+// host), 512 x 2048 x 2048 35 / 35; behind it not: 256 x 4096 x 4096 83 / 43, 64 x 4096 x 4096 46 / 24, 16384 x 168 x 256
+// 112 / 44.  Its time is the latency of the rows' loads, 1.5 us for every 256 rows, or with many tiles the conversions,
+// which every workgroup does for itself.
+bool few_rows(int64_t R, int64_t N, int64_t K) { return R <= 4096 && N * K <= 1LL << 22 && R * N * K <= 1LL << 31; }
+
 struct Layout {
     int planes, chunks, chunk_rows;
     Shape shape;
@@ -322,7 +440,7 @@ constexpr int64_t kMaxRows = 1 << 20;  // a row of two fp16 planes is then at mo
 extern "C" {
 
 int64_t mz_ckpt8_workspace(int32_t type, int32_t scale_bits, int32_t rows, int32_t N, int32_t K) {
-    if (rows <= 0 || N <= 0 || K <= 0 || rows > kMaxRows) return 0;
+    if (rows <= 0 || N <= 0 || K <= 0 || rows > kMaxRows || few_rows(rows, N, K)) return 0;
     return layout(type, scale_bits, rows, N, K).bytes;
 }
 
@@ -339,6 +457,20 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
         (((uintptr_t)dz | (uintptr_t)dw | (uintptr_t)db) & (type_bytes(type) - 1)) != 0)
         return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: bad stride or alignment (ldz=%lld ldw=%lld ldc=%lld)", (long long)ldz,
                         (long long)ldw, (long long)ldc);
+    if (few_rows(rows, N, K)) {
+        const int tiles_k = (K + kFewK - 1) / kFewK, tiles_n = (N + kFewN - 1) / kFewN;
+        with_type(type, [&](auto t) {
+            using T = decltype(t);
+            const bool pairs = (uintptr_t)dz % (2 * sizeof(T)) == 0 && ldz % 2 == 0 && N % 2 == 0;
+            const auto go = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_k * tiles_n)), dim3(64 * kFewWaves), 0, (hipStream_t)stream, (const T *)dz, ldz,
+                                   scales, rows, N, codes, ldc, K, (T *)dw, ldw, quads_aligned((T *)dw, ldw), (T *)db, tiles_k);
+            };
+            if (type != MZ_TYPE_F32 && scale_bits == 3) pairs ? go(k_weight_grad_few<T, 2, true>) : go(k_weight_grad_few<T, 2, false>);
+            else pairs ? go(k_weight_grad_few<T, 3, true>) : go(k_weight_grad_few<T, 3, false>);
+        });
+        return mz::check_launch("mz_ckpt8_weight_grad");
+    }
     const Layout l = layout(type, scale_bits, rows, N, K);
     if (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 15) != 0)
         return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: needs a 16-byte aligned workspace of %lld bytes (got %lld)",

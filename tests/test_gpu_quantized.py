@@ -647,3 +647,28 @@ def test_contexts_leave_float64_layers_alone():
     with eight_bit_checkpoints(g, f):
         got = g(lat, act) + f(lat)
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("bits", [3, 24])
+@pytest.mark.parametrize("R,K,N", [(1, 5, 2), (7, 65, 33), (33, 64, 31), (255, 200, 97), (257, 130, 34), (4096, 100, 70), (4097, 100, 70),
+                                   (500, 2048, 2047), (530, 2048, 2048), (90, 3000, 1500)])
+def test_weight_gradient_on_both_sides_of_its_variants(R, K, N, bits, dtype):
+    """Rows on pairs of elements and off them, the last row at the end of its memory, garbage around the rest."""
+    from muzero_amd.checkpoints import weight_grad
+    from muzero_amd.quantized import quantize_rows
+    x = _x(R, K, dtype, seed=N)
+    saved = quantize_rows(x, scale_bits=bits)
+    g = torch.Generator().manual_seed(R)
+    dz = (torch.randn(R, N, generator=g) * 0.1).to(dtype)
+    want, tol, want_b, tol_b = _grad_reference(dz, x, bits)
+    first = None
+    for width, at in ((N, 0), (N + 1, 0), (N + 2 + N % 2, 1), (N + 6, 6)):
+        big = torch.full((R * width + at,), torch.nan, dtype=dtype, device="cuda")[: (R - 1) * width + at + N]
+        view = big.as_strided((R, N), (width, 1), at)
+        view.copy_(dz)
+        dw, db = weight_grad(view, saved)
+        _within(dw, want, tol + HALF[dtype] * (np.abs(want) + tol) + TINY[dtype])
+        _within(db, want_b, tol_b + HALF[dtype] * (np.abs(want_b) + tol_b) + TINY[dtype])
+        first = dw if first is None else first
+        assert torch.equal(dw, first)

@@ -121,10 +121,10 @@ def test_checkpoint_refusals():
     _refused(lib.mz_ckpt8_act_grad(P, F32, 9, None, 4, 9, RELU, P, 9, None), "NULL")
     _refused(lib.mz_ckpt8_act_grad(P, F32, 9, P, 4, 9, 4, P, 9, None), "activation")
     _refused(lib.mz_ckpt8_act_grad(P, F32, 9, P, 4, 9, RELU, None, 9, None), "NULL")
-    need = lib.mz_ckpt8_workspace(F32, 3, 4, 50, 100)
-    assert need > 0 and lib.mz_ckpt8_workspace(F32, 3, 0, 50, 100) == 0
+    need = lib.mz_ckpt8_workspace(F32, 3, 5000, 50, 100)
+    assert need > 0 and lib.mz_ckpt8_workspace(F32, 3, 0, 50, 100) == 0 and lib.mz_ckpt8_workspace(F32, 3, 4, 50, 100) == 0
 
-    def grad(dz=P, kind=F32, ldz=50, rows=4, N=50, codes=P, ldc=128, scales=P, bits=3, K=100, dw=P, ldw=100, db=P, work=P, nwork=need):
+    def grad(dz=P, kind=F32, ldz=50, rows=5000, N=50, codes=P, ldc=128, scales=P, bits=3, K=100, dw=P, ldw=100, db=P, work=P, nwork=need):
         return lib.mz_ckpt8_weight_grad(dz, kind, ldz, rows, N, codes, ldc, scales, bits, K, dw, ldw, db, work, nwork, None)
     _refused(grad(rows=0), "rows=0")
     _refused(grad(rows=(1 << 20) + 1), "rows")
