@@ -47,7 +47,7 @@ def weight_grad(dz: torch.Tensor, saved: QuantizedRows, want_bias: bool = True):
         raise ValueError(f"dz of shape {tuple(dz.shape)} does not match a checkpoint of shape {tuple(saved.shape)}")
     if dz.device != saved.codes.device:
         raise ValueError(f"dz is on {dz.device}, the checkpoint on {saved.codes.device}")
-    dz = rows_of(dz.detach())
+    dz = rows_of(dz.detach() if dz.requires_grad else dz)
     (R, N), K = dz.shape, saved.columns
     make = torch.empty if R > 0 else torch.zeros
     dw = make((N, K), dtype=dz.dtype, device=dz.device)
@@ -56,10 +56,12 @@ def weight_grad(dz: torch.Tensor, saved: QuantizedRows, want_bias: bool = True):
         lib, kind = _hip.lib(), TYPE[dz.dtype]
         with on_device(dz):
             need = lib.mz_ckpt8_workspace(kind, saved.scale_bits, R, N, K)
-            ws = workspace(need, dz)
-            _hip.check(lib.mz_ckpt8_weight_grad(ptr(dz), kind, row_stride(dz), R, N, ptr(saved.codes), saved.ld,
-                                                ptr(saved.scales), saved.scale_bits, K, ptr(dw), K, ptr(db), ptr(ws), need,
-                                                stream_of(dz)), "mz_ckpt8_weight_grad")
+            ws = workspace(need, dz) if need else None
+            rc = lib.mz_ckpt8_weight_grad(dz.data_ptr(), kind, row_stride(dz), R, N, saved.codes.data_ptr(), saved.ld,
+                                          saved.scales.data_ptr(), saved.scale_bits, K, dw.data_ptr(), K, ptr(db), ptr(ws), need,
+                                          stream_of(dz))
+            if rc:
+                _hip.check(rc, "mz_ckpt8_weight_grad")
     return dw, db
 
 

@@ -94,14 +94,17 @@ def quantize_rows(x: torch.Tensor, scale_bits: int = 24) -> QuantizedRows:
         raise ValueError(f"scale_bits must be 24 or 3, not {scale_bits}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x needs at least one value in a row, not shape {tuple(x.shape)}")
-    rows = rows_of(x.detach())
-    R, K = rows.shape
-    codes = rows.new_empty((R, (K + 127) // 128 * 128), dtype=torch.int8)
-    scales = rows.new_empty(R, dtype=torch.float32)
+    rows = rows_of(x.detach() if x.requires_grad else x)
+    (R, K), dev = rows.shape, rows.device
+    ldc = (K + 127) // 128 * 128
+    codes = torch.empty((R, ldc), dtype=torch.int8, device=dev)
+    scales = torch.empty(R, dtype=torch.float32, device=dev)
     if R > 0:
         with on_device(rows):
-            _hip.check(_hip.lib().mz_quant8_rows(ptr(rows), TYPE[rows.dtype], row_stride(rows), R, K, scale_bits, ptr(codes),
-                                                 codes.shape[1], ptr(scales), stream_of(rows)), "mz_quant8_rows")
+            rc = _hip.lib().mz_quant8_rows(rows.data_ptr(), TYPE[rows.dtype], row_stride(rows), R, K, scale_bits, codes.data_ptr(),
+                                           ldc, scales.data_ptr(), stream_of(rows))
+            if rc:
+                _hip.check(rc, "mz_quant8_rows")
     return QuantizedRows._of(codes, scales, x.shape, x.dtype, scale_bits)
 
 
@@ -141,7 +144,8 @@ def int8_linear(x, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, a
     if bias is not None:
         if bias.shape != (N,) or bias.device != dev:
             raise ValueError(f"bias must be {N} values on {dev}")
-        bias = bias.detach().to(torch.float32).contiguous()
+        if bias.dtype is not torch.float32 or not bias.is_contiguous():
+            bias = bias.detach().to(torch.float32).contiguous()
     check_on_gpu(weight.codes, "weight")
     K = weight.columns
     y = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype, device=dev)
@@ -156,12 +160,15 @@ def int8_linear(x, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, a
                                                  weight.ld, ptr(weight.scales), N, ptr(bias), act, ptr(y), TYPE[out_dtype],
                                                  N, ptr(ws), need, stream_of(y)), "mz_int8_forward_codes")
         else:
-            rows = rows_of(x.detach())
-            need = lib.mz_int8_workspace(rows.shape[0], K, N)
+            rows = rows_of(x)
+            R = rows.shape[0]
+            need = lib.mz_int8_workspace(R, K, N)
             ws = workspace(need, y)
-            _hip.check(lib.mz_int8_forward(ptr(rows), TYPE[rows.dtype], row_stride(rows), rows.shape[0], K, ptr(weight.codes),
-                                           weight.ld, ptr(weight.scales), N, ptr(bias), act, ptr(y), TYPE[out_dtype], N,
-                                           ptr(ws), need, stream_of(y)), "mz_int8_forward")
+            rc = lib.mz_int8_forward(rows.data_ptr(), TYPE[rows.dtype], row_stride(rows), R, K, weight.codes.data_ptr(), weight.ld,
+                                     weight.scales.data_ptr(), N, ptr(bias), act, y.data_ptr(), TYPE[out_dtype], N, ptr(ws), need,
+                                     stream_of(y))
+            if rc:
+                _hip.check(rc, "mz_int8_forward")
     return y
 
 
