@@ -28,7 +28,7 @@ using namespace mze;
 using namespace mzt8;
 
 constexpr int kCT = 256;
-constexpr int kMaxChunks = 64, kFewRows = 256, kFewChunks = 16;
+constexpr int kMaxChunks = 128, kFewRows = 256, kFewChunks = 16;
 
 enum Stats { kOwn, kChunks, kReady };  // where k_prepare's column factors come from
 
@@ -47,21 +47,23 @@ __device__ __forceinline__ float column_factor(unsigned bits, float *inverse) {
     return __uint_as_float((unsigned)(127 + e) << 23);
 }
 
-// A workgroup takes 64 packs of columns and a chunk of rows, its four waves every fourth row.
-template <class T, bool WHOLE>
+// A workgroup takes LANES packs of columns and a chunk of rows, 256 / LANES rows at a time.
+// Bound by the bytes: 8192 x 8192 bf16 40 us, 3.3 TB/s; narrow matrices by the loads' latency
+// (16384 x 64 bf16 with its product, 64 lanes of which 8 have columns / 8 lanes: 38 / 27 us).
+template <class T, bool WHOLE, int LANES>
 __global__ void __launch_bounds__(kCT)
 k_col_stats(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int chunk_rows,
             unsigned *__restrict__ part_max, float *__restrict__ part_sum) {
-    constexpr int n = Pack<T>::n;
-    __shared__ unsigned wave_max[4][64 * n];
-    __shared__ float wave_sum[4][64 * n];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, chunk = blockIdx.y, c0 = blockIdx.x * 64 * n, c = c0 + lane * n;
+    constexpr int n = Pack<T>::n, groups = kCT / LANES, width = LANES * n;
+    __shared__ unsigned group_max[kCT * n];
+    __shared__ float group_sum[kCT * n];
+    const int t = threadIdx.x, chunk = blockIdx.y, c0 = blockIdx.x * width, c = c0 + t % LANES * n;
     unsigned m[n] = {};
     float s[n] = {};
     const int end = min(R, (chunk + 1) * chunk_rows);
     if (c < N)
-#pragma unroll 4
-        for (int r = chunk * chunk_rows + wave; r < end; r += 4) {
+#pragma unroll 8
+        for (int r = chunk * chunk_rows + t / LANES; r < end; r += groups) {
             const Pack<T> p = load_pack<T, WHOLE>(dz + r * ldz, c, N);
             const float scale = scales[r];
 #pragma unroll
@@ -72,14 +74,13 @@ k_col_stats(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ sca
             }
         }
 #pragma unroll
-    for (int e = 0; e < n; ++e) wave_max[wave][lane * n + e] = m[e], wave_sum[wave][lane * n + e] = s[e];
+    for (int e = 0; e < n; ++e) group_max[t * n + e] = m[e], group_sum[t * n + e] = s[e];
     __syncthreads();
-    for (int i = threadIdx.x; i < 64 * n; i += kCT)
+    for (int i = t; i < width; i += kCT)
         if (c0 + i < N) {
             unsigned top = 0;
             float sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) top = max(top, wave_max[w][i]), sum += wave_sum[w][i];
+            for (int q = 0; q < groups; ++q) top = max(top, group_max[q * width + i]), sum += group_sum[q * width + i];
             part_max[(int64_t)chunk * N + c0 + i] = top;
             part_sum[(int64_t)chunk * N + c0 + i] = sum;
         }
@@ -232,6 +233,7 @@ __device__ void codes_block(const int8_t *__restrict__ codes, int64_t ldc, int R
     }
 }
 
+// Bound by the bytes: 8192 rows of 8192 bf16 and of 4096 codes 69 us, 370 MB, 5.4 TB/s.
 // Workgroups 0 .. split_blocks - 1: 64 columns of dz each; the others 128 columns of codes; all of them 64 rows.
 template <class T, int PLANES, bool WHOLE, Stats STATS>
 __global__ void __launch_bounds__(kCT)
@@ -245,6 +247,8 @@ k_prepare(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scale
         codes_block(codes, ldc, R, K, Rp, (blockIdx.x - split_blocks) * kCodeCols, r0, out.codes_t, lds);
 }
 
+// Bound by the matrix cores: 8192 x 4096 x 8192 with one plane 373 to 450 us (the clock follows the load), 1.2 to 1.5 PFLOP/s
+// (a library's fp16 product of 8192^3 1.50); two planes take twice that.
 template <class T, class Tl>
 __global__ void __launch_bounds__(Tl::threads)
 k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, const float *__restrict__ inverse, int K, int N,
@@ -278,7 +282,7 @@ k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, c
     });
 }
 
-// Sums of the parts of a split reduction, in a fixed order: one thread per four values of a row of dW.
+// Sums of the parts of a split reduction, in a fixed order: one thread per four values of a row of dW; bound by the bytes.
 template <class T>
 __global__ void __launch_bounds__(256)
 k_weight_join(const float *__restrict__ partial, int splits, const float *__restrict__ inverse, int K, int N, T *__restrict__ dw,
@@ -492,8 +496,14 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
         with_flag(rows_aligned<T>(dz, ldz), [&](auto whole) {
             constexpr bool W = decltype(whole)::value;
             if (l.chunks > 0) {
-                hipLaunchKernelGGL((k_col_stats<T, W>), dim3((unsigned)tiles_of(N, 64 * Pack<T>::n), (unsigned)l.chunks), dim3(kCT), 0, st,
-                                   (const T *)dz, ldz, scales, rows, N, l.chunk_rows, part_max, part_sum);
+                const auto stats = [&](auto lanes) {
+                    constexpr int L = decltype(lanes)::value;
+                    hipLaunchKernelGGL((k_col_stats<T, W, L>), dim3((unsigned)tiles_of(N, L * Pack<T>::n), (unsigned)l.chunks), dim3(kCT), 0, st,
+                                       (const T *)dz, ldz, scales, rows, N, l.chunk_rows, part_max, part_sum);
+                };
+                if (N <= 8 * Pack<T>::n) stats(std::integral_constant<int, 8>{});
+                else if (N <= 32 * Pack<T>::n) stats(std::integral_constant<int, 32>{});
+                else stats(std::integral_constant<int, 64>{});
             }
             if (l.chunks > kFewChunks)
                 hipLaunchKernelGGL(k_col_factors<T>, dim3((unsigned)tiles_of(N, 64)), dim3(64), 0, st, part_max, part_sum, l.chunks, N,

@@ -17,7 +17,7 @@ using namespace mze;
 constexpr int kQT = 256;
 // THREADS threads per row (64: four rows per workgroup).  The first HELD packs of a thread stay in registers between the
 // maximum and the codes; the rest of a longer row is read again, from cache.  Bound by the memory: 1536 x 18432 float32,
-// 142 MB with the codes, 26 us, 5.3 TB/s.
+// 142 MB with the codes, 28 us, 5.0 TB/s.
 template <class T, int THREADS, int HELD, bool WHOLE>
 __global__ void __launch_bounds__(THREADS < kQT ? kQT : THREADS)
 k_quant8(const T *__restrict__ x, int64_t ldx, int64_t rows, int K, int scale_bits, int8_t *__restrict__ codes, int64_t ldc,
@@ -63,6 +63,7 @@ k_quant8(const T *__restrict__ x, int64_t ldx, int64_t rows, int K, int scale_bi
     }
 }
 
+// Bound by the memory: 1536 x 18432 to float32, 113 MB from 28 MB of codes in cache, 22 us.
 template <class T, int THREADS, bool WHOLE, bool PAST>
 __global__ void __launch_bounds__(kQT)
 k_dequant8(const int8_t *__restrict__ codes, int64_t ldc, const float *__restrict__ scales, int64_t rows, int K,
@@ -97,6 +98,7 @@ __device__ __forceinline__ void load8(const T *row, int j, int N, float (&v)[8])
     }
 }
 
+// Both passes over an activation are one read and one write of it, bound by the memory.
 // What the backward pass needs of y = act(z): relu one bit, [not y <= 0]; tanh and sigmoid a code of 8 bits on a fixed
 // scale, -128 for a NaN.  A thread takes 8 values: a byte of bits, or 8 codes.
 template <class T, bool WHOLE>

@@ -304,6 +304,9 @@ k_scores_wave(const T *__restrict__ logits, int64_t ld, int64_t rows, Out out) {
 }
 
 // ---------------------------------------------------------------- long rows: a workgroup streams a row, or a part of it
+// One pass with a running maximum per thread; bound by the bytes: 3001 x 50001 float32 with 8 alternatives 117 us, 5.1 TB/s,
+// 4096 x 32768 bf16 without any 48 us, 5.6 TB/s (an instantiation of its own: the alternatives' registers halve the waves at
+// work).  The alternatives read a few packs again, those of the threads whose largest logit reaches the bound.
 constexpr int kCand = 1024;       // candidates for the alternatives that a workgroup can hold
 constexpr int kMaxParts = 64;     // parts of one row (one lane of the joining wave each)
 
@@ -498,7 +501,8 @@ k_scores_long(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts,
     }
 }
 
-// One wave per row: joins the sums of its parts in a fixed order and merges their lists, one lane per part.
+// One wave per row: joins the sums of its parts in a fixed order and merges their lists, one lane per part.  Bound by the
+// latency of its steps: 16 lists of 5 3.7 us, 8 lists of 20 for 64 rows 7.1 us.
 template <class T>
 __global__ void __launch_bounds__(64)
 k_scores_join(const T *__restrict__ logits, int64_t ld, int64_t rows, int parts, Out out, const Sums *__restrict__ part_sums,

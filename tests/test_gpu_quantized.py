@@ -652,7 +652,8 @@ def test_contexts_leave_float64_layers_alone():
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("bits", [3, 24])
 @pytest.mark.parametrize("R,K,N", [(1, 5, 2), (7, 65, 33), (33, 64, 31), (255, 200, 97), (257, 130, 34), (4096, 100, 70), (4097, 100, 70),
-                                   (500, 2048, 2047), (530, 2048, 2048), (90, 3000, 1500)])
+                                   (500, 2048, 2047), (530, 2048, 2048), (90, 3000, 1500),
+                                   (5000, 60, 30), (4500, 60, 60), (4500, 50, 250)])
 def test_weight_gradient_on_both_sides_of_its_variants(R, K, N, bits, dtype):
     """Rows on pairs of elements and off them, the last row at the end of its memory, garbage around the rest."""
     from muzero_amd.checkpoints import weight_grad
