@@ -782,8 +782,8 @@ int mz_policy_post(const float *policy_in, int32_t B, int32_t A, int32_t softmax
  *   top_actions i64[T][top], top_log_probs f32[T][top]   the `top` (0..32, at most V) largest logits, the lowest index
  *                     first among equals, NaN before everything; their log probabilities.
  * A logit of -inf is an illegal action (probability 0).  A row of nothing else has log probabilities -inf, entropy 0
- * and gradient 0.  A NaN or +inf makes its row's results NaN.  workspace: mz_policy_scores_workspace bytes
- * (may be 0), 16-byte aligned. */
+ * and gradient 0.  A NaN or +inf makes its row's results NaN.  T < 2^31, V <= 2^30.  workspace: mz_policy_scores_workspace
+ * bytes (may be 0), 16-byte aligned, used during the call only: calls that may run at the same time need one each. */
 int64_t mz_policy_scores_workspace(int32_t type, int64_t T, int32_t V, int32_t top);
 int mz_policy_scores(const void *logits, int32_t type, int64_t ld, const int64_t *actions, int64_t T, int32_t V,
                      int32_t top, float *log_prob, float *entropy, float *stats, int64_t *top_actions,
@@ -811,7 +811,8 @@ int mz_dequant8_rows(const int8_t *codes, int64_t ldc, const float *scales, int6
  * bias f32[N] or NULL, activation none / relu / tanh / sigmoid, y of any type.  ldw: a multiple of 128 (the columns
  * behind K zero).  The int8 form of nn.Linear + activation (build_mlp, src/neural_networks/network_builder.py:183-205).
  * mz_int8_forward_codes takes rows that are coded already (heads that share an input).
- * workspace: mz_int8_workspace / mz_int8_codes_workspace bytes (may be 0 for the latter), 16-byte aligned. */
+ * N <= 2^26, at most 2^23 tiles of 64 x 64 outputs.  workspace: mz_int8_workspace / mz_int8_codes_workspace bytes (may be
+ * 0 for the latter), 16-byte aligned, one per call that may run at the same time. */
 int64_t mz_int8_workspace(int32_t rows, int32_t K, int32_t N);
 int64_t mz_int8_codes_workspace(int32_t rows, int32_t K, int32_t N);
 int mz_int8_forward(const void *x, int32_t x_type, int64_t ldx, int32_t rows, int32_t K, const int8_t *w_codes,
@@ -826,7 +827,9 @@ int mz_int8_forward_codes(const int8_t *x_codes, int64_t ldxc, const float *x_sc
  * activation's derivative needs is kept as one bit per value (relu) or a code of 8 bits (tanh, sigmoid):
  * mz_ckpt8_act_bytes(N, activation) bytes per row.  dz may be dy itself (same stride).
  * mz_ckpt8_weight_grad: dw[N][K] = dz^T x and db[N] = column sums of dz (db may be NULL) from dz[rows][N] and the codes
- * of x[rows][K]; dz, dw and db share the type, sums are held in float32 with dz to 22 bits or exact. */
+ * of x[rows][K]; dz, dw and db share the type, sums are held in float32 with dz to 22 bits or exact.  rows <= 2^20;
+ * scale_bits says what the scales hold (3 only if every one has three significant bits).  A column of dz with an infinity
+ * or a NaN, or whose products with the scales leave float32's range, gives NaN.  workspace as above (0 bytes for few rows). */
 int64_t mz_ckpt8_act_bytes(int32_t N, int32_t activation);
 int mz_ckpt8_act_save(const void *y, int32_t type, int64_t ldy, int64_t rows, int32_t N, int32_t activation,
                       uint8_t *saved, void *stream);
