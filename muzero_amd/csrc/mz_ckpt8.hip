@@ -86,19 +86,26 @@ k_col_stats(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ sca
         }
 }
 
+// 64 columns, every wave a quarter of the chunks.
 template <class T>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(kCT)
 k_col_factors(const unsigned *__restrict__ part_max, const float *__restrict__ part_sum, int chunks, int N, float *__restrict__ factor,
               float *__restrict__ inverse, T *__restrict__ db) {
-    const int n = blockIdx.x * 64 + threadIdx.x;
-    if (n >= N) return;
+    __shared__ unsigned wave_max[4][64];
+    __shared__ float wave_sum[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n = blockIdx.x * 64 + lane;
     unsigned m = 0;
     float s = 0.0f;
+    if (n < N)
 #pragma unroll 8
-    for (int c = 0; c < chunks; ++c) {
-        m = max(m, part_max[(int64_t)c * N + n]);
-        s += part_sum[(int64_t)c * N + n];
-    }
+        for (int c = wave; c < chunks; c += 4) {
+            m = max(m, part_max[(int64_t)c * N + n]);
+            s += part_sum[(int64_t)c * N + n];
+        }
+    wave_max[wave][lane] = m, wave_sum[wave][lane] = s;
+    __syncthreads();
+    if (wave > 0 || n >= N) return;
+    for (int w = 1; w < 4; ++w) m = max(m, wave_max[w][lane]), s += wave_sum[w][lane];
     factor[n] = column_factor(m, inverse + n);
     if (db) db[n] = (T)s;
 }
@@ -506,7 +513,7 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
                 else stats(std::integral_constant<int, 64>{});
             }
             if (l.chunks > kFewChunks)
-                hipLaunchKernelGGL(k_col_factors<T>, dim3((unsigned)tiles_of(N, 64)), dim3(64), 0, st, part_max, part_sum, l.chunks, N,
+                hipLaunchKernelGGL(k_col_factors<T>, dim3((unsigned)tiles_of(N, 64)), dim3(kCT), 0, st, part_max, part_sum, l.chunks, N,
                                    prepared.factor, inverse, (T *)db);
             const auto prepare = [&](auto planes_tag) {
                 constexpr int P = decltype(planes_tag)::value;

@@ -24,7 +24,7 @@ __device__ __forceinline__ float activate(float v, int act) {
 }
 
 // The tiled product, its epilogue on the accumulators: 8192 x 4096 x 8192 bf16 224 us, 2.45 POP/s (a library's int8 product of
-// 8192^3 2.43), bound by the matrix cores; 256 x 18432 x 9216 in six parts 45 us, 3.8 TB/s of weights.
+// 8192^3 2.43), bound by the matrix cores; 256 x 18432 x 9216 in seven parts 45 us, 3.8 TB/s of weights.
 template <class T, class Tl, bool PAST>
 __global__ void __launch_bounds__(Tl::threads)
 k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs, int rows, const int8_t *__restrict__ wc,
@@ -70,7 +70,7 @@ k_int8(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict__ xs
 }
 
 // Sums of the parts of a split reduction, scales, bias, activation: one thread per four values of an output row.  Bound by
-// the bytes: 256 x 9216 from six parts 13.4 us, 4.9 TB/s.
+// the bytes: 256 x 9216 from seven parts 13.4 us, 5.6 TB/s.
 template <class T>
 __global__ void __launch_bounds__(256)
 k_int8_join(const int *__restrict__ partial, int splits, const float *__restrict__ xs, int rows, const float *__restrict__ ws, int N,

@@ -289,7 +289,7 @@ inline int64_t tiles_of(int64_t n, int64_t t) { return n > 0 ? (n + t - 1) / t :
 // 64 / 128 x 256 / 256 tiles, best number of parts in brackets):
 //     8192 x 8192, 32 steps       - / 267 / 240              2048 x 4096, 32 steps      55 / 39 / 49
 //     4096 x 4096,  4 steps      26 / 26 / 19                1024 x 4096, 32 steps      29 / 35 / 43 (3)
-//      256 x 9216, 144 steps     81 / 66 (3) / 58 (6)         256 x 9216, 72 steps      41 / 43 (3) / 47 (4)
+//      256 x 9216, 144 steps     81 / 66 (3) / 58 (7)         256 x 9216, 72 steps      41 / 43 (3) / 47 (4)
 //       64 x 9216, 144 steps     34 (3) / 52 (3) / 45 (6)     128 x 4096, 32 steps      13 / 19 (4) / 23 (6)
 //      100 x  500, 128 steps     13 (8), undivided 39         1024 x 1024, 8 steps     6.4 / 13 / 19
 inline Shape shape_of(int64_t outer, int64_t inner, int64_t steps) {
