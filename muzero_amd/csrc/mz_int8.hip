@@ -142,8 +142,10 @@ k_int8_few(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict_
 
 // The same for up to kFusedRows rows that are not coded yet, in one launch: every workgroup codes them for itself, into
 // LDS, while its first weights are on their way (a row of 9216 float32 comes from L2; a launch of the quantiser of its own
-// costs more than that).
-constexpr int kFusedRows = 4, kFusedBytes = 40960;
+// costs more than that).  Up to kSharedRows rows all waves work on one after the other; beyond, every wave has its own rows,
+// up to kOwnValues values in all: us per layer in a chain, one launch / two (which also cost 3 us more of the host):
+// 5 x 512 4.2 / 5.0, 5 x 2048 5.9 / 6.4, 16 x 168 4.8 / 5.1, 16 x 1024 6.3 / 6.1; behind it 16 x 2048 8.7 / 7.0.
+constexpr int kFusedRows = 16, kSharedRows = 4, kOwnValues = 16384, kFusedBytes = 40960;
 
 int64_t fused_stride(int64_t K) { return (K + 127) / 128 * 128 + 16; }  // rows of codes in different banks
 
@@ -165,27 +167,46 @@ k_int8_fused(const T *__restrict__ xp, int64_t ldx, int rows, int K, const int8_
 #pragma unroll
         for (int h = 0; h < 2; ++h) first[u][h] = k < kbytes ? *(const u32x4 *)(w + k + h * 16) : u32x4{};
     }
-    for (int r = 0; r < rows; ++r) {
-        unsigned m = 0;
+    if (rows <= kSharedRows) {  // all waves on one row after the other
+        for (int r = 0; r < rows; ++r) {
+            unsigned m = 0;
 #pragma unroll 4
-        for (int j = threadIdx.x * n; j < K; j += threads * n) {
-            const Pack<T> p = load_pack<T, WHOLE>(xp + r * ldx, j, K);
+            for (int j = threadIdx.x * n; j < K; j += threads * n) {
+                const Pack<T> p = load_pack<T, WHOLE>(xp + r * ldx, j, K);
 #pragma unroll
-            for (int e = 0; e < n; ++e) m = max(m, abs_bits((float)p.v[e]));
+                for (int e = 0; e < n; ++e) m = max(m, abs_bits((float)p.v[e]));
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o));
+            if (lane == 0) top[r][wave] = m;
         }
+        __syncthreads();
+        for (int r = 0; r < rows; ++r) {
+            unsigned m = 0;
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o));
-        if (lane == 0) top[r][wave] = m;
-    }
-    __syncthreads();
-    for (int r = 0; r < rows; ++r) {
-        unsigned m = 0;
-#pragma unroll
-        for (int q = 0; q < kFewWaves; ++q) m = max(m, top[r][q]);
-        const RowScale rs = row_scale(m, 24);
+            for (int q = 0; q < kFewWaves; ++q) m = max(m, top[r][q]);
+            const RowScale rs = row_scale(m, 24);
 #pragma unroll 4
-        for (int j = threadIdx.x * n; j < kbytes; j += threads * n)
-            store_codes((int8_t *)codes + r * stride + j, load_pack<T, WHOLE>(xp + r * ldx, j, K), rs.inverse);
+            for (int j = threadIdx.x * n; j < kbytes; j += threads * n)
+                store_codes((int8_t *)codes + r * stride + j, load_pack<T, WHOLE>(xp + r * ldx, j, K), rs.inverse);
+        }
+    } else {  // every wave its own rows
+        for (int r = wave; r < rows; r += kFewWaves) {
+            unsigned m = 0;
+#pragma unroll 4
+            for (int j = lane * n; j < K; j += 64 * n) {
+                const Pack<T> p = load_pack<T, WHOLE>(xp + r * ldx, j, K);
+#pragma unroll
+                for (int e = 0; e < n; ++e) m = max(m, abs_bits((float)p.v[e]));
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) m = max(m, __shfl_xor(m, o));
+            if (lane < kFewWaves) top[r][lane] = m;
+            const RowScale rs = row_scale(m, 24);
+#pragma unroll 4
+            for (int j = lane * n; j < kbytes; j += 64 * n)
+                store_codes((int8_t *)codes + r * stride + j, load_pack<T, WHOLE>(xp + r * ldx, j, K), rs.inverse);
+        }
     }
     __syncthreads();
     const uint8_t *x = codes + min(c, rows - 1) * stride + (lane >> 4) * 32;
@@ -304,7 +325,7 @@ bool few_rows(int64_t rows, int64_t N, int64_t K) { return rows <= 4 || (rows <=
 
 // One launch where x has the result's type and its codes fit a workgroup's share of LDS.
 bool fused(int32_t x_type, int32_t type, int64_t rows, int64_t K) {
-    return x_type == type && rows <= kFusedRows && rows * fused_stride(K) <= kFusedBytes;
+    return x_type == type && (rows <= kSharedRows || (rows <= kFusedRows && rows * K <= kOwnValues)) && rows * fused_stride(K) <= kFusedBytes;
 }
 
 template <class T>
