@@ -829,7 +829,7 @@ int mz_int8_forward_codes(const int8_t *x_codes, int64_t ldxc, const float *x_sc
  * mz_ckpt8_weight_grad: dw[N][K] = dz^T x and db[N] = column sums of dz (db may be NULL) from dz[rows][N] and the codes
  * of x[rows][K]; dz, dw and db share the type, sums are held in float32 with dz to 22 bits or exact.  rows <= 2^20;
  * scale_bits says what the scales hold (3 only if every one has three significant bits).  A column of dz with an infinity
- * or a NaN, or whose products with the scales leave float32's range, gives NaN.  workspace as above (0 bytes for few rows). */
+ * or a NaN, or whose products with the scales leave float32's range, gives NaN.  workspace as above (may be 0). */
 int64_t mz_ckpt8_act_bytes(int32_t N, int32_t activation);
 int mz_ckpt8_act_save(const void *y, int32_t type, int64_t ldy, int64_t rows, int32_t N, int32_t activation,
                       uint8_t *saved, void *stream);

@@ -3,7 +3,7 @@
 //     dW_nk = sum_r dz_rn s_r q_rk,     db_n = sum_r dz_rn
 // without writing x out again.
 //
-// Few rows and a small dW take one launch of their own (k_weight_grad_few).  For the rest the product runs on the fp16
+// Few rows, or a small dW, take a kernel of their own (k_weight_grad_few).  For the rest the product runs on the fp16
 // matrix instruction.  Codes are whole numbers up to 127: exact in fp16.  The row scale lies
 // along the reduction, so it goes to the other side: v_rn = dz_rn s_r, which fp16 cannot hold as it is.  Each output row n
 // is first brought into range by a power of two c_n (the largest |v_rn c_n| lies in 2^14 .. 2^15) and then held as
@@ -49,7 +49,7 @@ __device__ __forceinline__ float column_factor(unsigned bits, float *inverse) {
 
 // A workgroup takes LANES packs of columns and a chunk of rows, 256 / LANES rows at a time.
 // Bound by the bytes: 8192 x 8192 bf16 40 us, 3.3 TB/s; narrow matrices by the loads' latency
-// (16384 x 64 bf16 with its product, 64 lanes of which 8 have columns / 8 lanes: 38 / 27 us).
+// (whole gradients, bf16, 64 lanes / as many as have columns: 8192 x 9000 x 30 83 / 71 us, 8192 x 1100 x 250 47 / 40 us).
 template <class T, bool WHOLE, int LANES>
 __global__ void __launch_bounds__(kCT)
 k_col_stats(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N, int chunk_rows,
@@ -290,26 +290,34 @@ k_weight_grad(const f16 *__restrict__ codes_t, const f16 *__restrict__ planes, c
 }
 
 // Sums of the parts of a split reduction, in a fixed order: one thread per four values of a row of dW; bound by the bytes.
+// `inverse` undoes the columns' factors; part_sum holds the parts of db where the parts' kernel formed them.
 template <class T>
 __global__ void __launch_bounds__(256)
 k_weight_join(const float *__restrict__ partial, int splits, const float *__restrict__ inverse, int K, int N, T *__restrict__ dw,
-              int64_t ldw, bool aligned) {
+              int64_t ldw, bool aligned, const float *__restrict__ part_sum, T *__restrict__ db) {
     const int quads = (K + 3) / 4, n = blockIdx.y, c = blockIdx.x * 256 + threadIdx.x, k = 4 * c;
     if (c < quads) {
-        const f32x4 sum = sum_parts<f32x4>(partial, splits, (int64_t)N * quads, (int64_t)n * quads + c) * inverse[n];
+        f32x4 sum = sum_parts<f32x4>(partial, splits, (int64_t)N * quads, (int64_t)n * quads + c);
+        if (inverse) sum *= inverse[n];
         const float o[4] = {sum[0], sum[1], sum[2], sum[3]};
         store_quad<false>(dw + n * ldw, k, K, aligned, o);
     }
+    if (db && part_sum && c == 0) {
+        float sum = 0.0f;
+#pragma unroll 8
+        for (int p = 0; p < splits; ++p) sum += part_sum[(int64_t)p * N + n];
+        db[n] = (T)sum;
+    }
 }
 
-// ---------------------------------------------------------------- few rows: one launch
+// ---------------------------------------------------------------- few rows or a small dW: one launch, or two
 // A workgroup forms 32 x 64 values of dW, its eight waves every eighth 32 rows; a lane reads 2 columns of dz and 4 of the
 // codes from 8 rows, which is a fragment of the instruction already, so nothing is transposed and nothing waits for the
 // columns' factors: v = dz s is held in bfloat16 planes, which have float32's range,
 //     two    hi = bf16(v), mid = bf16(v - hi)         16 bits: 16-bit dz with scales of 3 significant bits, exact
 //     three  and lo = bf16(v - hi - mid)              24 bits, as v itself
 // (below 2^-110 the last one loses bits to its smallest value, 2^-133).
-constexpr int kFewN = 32, kFewK = 64, kFewWaves = 8;
+constexpr int kFewN = 32, kFewK = 64, kFewWaves = 8, kFewSplit = 2048;
 
 using b16x8 = __attribute__((ext_vector_type(8))) __bf16;
 
@@ -317,7 +325,7 @@ template <class T, int PLANES, bool PAIRS>
 __global__ void __launch_bounds__(64 * kFewWaves, 4)
 k_weight_grad_few(const T *__restrict__ dz, int64_t ldz, const float *__restrict__ scales, int R, int N,
                   const int8_t *__restrict__ codes, int64_t ldc, int K, T *__restrict__ dw, int64_t ldw, bool aligned,
-                  T *__restrict__ db, int tiles_k) {
+                  T *__restrict__ db, int tiles_k, int part_rows, float *__restrict__ partial, float *__restrict__ part_sum) {
     constexpr int ld = kFewK + 4;
     __shared__ __align__(16) float sums[kFewWaves][kFewN * ld];
     __shared__ float db_sums[kFewWaves][kFewN];
@@ -348,16 +356,17 @@ k_weight_grad_few(const T *__restrict__ dz, int64_t ldz, const float *__restrict
     };
     f32x4 acc[2][4] = {};
     float col[2] = {};
-    const int waves = min(kFewWaves, (R + 31) / 32);  // with rows to take
+    const int begin = blockIdx.y * part_rows, end = min(R, begin + part_rows);
+    const int waves = min(kFewWaves, (end - begin + 31) / 32);  // with rows to take
     if (wave < waves) {
-        Rows next = load(wave * 32);
-        for (int r0 = wave * 32; r0 < R; r0 += kFewWaves * 32) {
+        Rows next = load(begin + wave * 32);
+        for (int r0 = begin + wave * 32; r0 < end; r0 += kFewWaves * 32) {
             const Rows x = next;
             next = load(r0 + kFewWaves * 32);
             b16x8 plane[2][PLANES], code[4];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const bool live = r0 + 8 * g + j < R;
+                const bool live = r0 + 8 * g + j < end;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const float d = live ? (float)x.d[j].v[e] : 0.0f;
@@ -401,23 +410,48 @@ k_weight_grad_few(const T *__restrict__ dz, int64_t ldz, const float *__restrict
         if (w < waves) sum += *(const f32x4 *)&sums[w][row * ld + kq];
     if (n0 + row < N) {
         const float o[4] = {sum[0], sum[1], sum[2], sum[3]};
-        store_quad<false>(dw + (n0 + row) * ldw, k0 + kq, K, aligned, o);
+        const int Kq = (K + 3) / 4 * 4;
+        if (!partial) store_quad<false>(dw + (n0 + row) * ldw, k0 + kq, K, aligned, o);
+        else if (k0 + kq < K) *(f32x4 *)(partial + ((int64_t)blockIdx.y * N + n0 + row) * Kq + k0 + kq) = sum;
     }
     if (db && k0 == 0 && threadIdx.x < kFewN && n0 + (int)threadIdx.x < N) {
         float total = 0.0f;
 #pragma unroll
         for (int w = 0; w < kFewWaves; ++w)
             if (w < waves) total += db_sums[w][threadIdx.x];
-        db[n0 + threadIdx.x] = (T)total;
+        if (!partial) db[n0 + threadIdx.x] = (T)total;
+        else part_sum[(int64_t)blockIdx.y * N + n0 + threadIdx.x] = total;
     }
 }
 
-// Up to here the one launch wins (us, this / the kernels below; float32): 256 x 168 x 256 (rows, K, N) 5.1 / 15.0,
-// 1024 x 512 x 512 10 / 29, 2048 x 1024 x 1024 33 / 41, 4096 x 64 x 64 27 / 24 (but one launch for five, each 3 us of the
-// host), 512 x 2048 x 2048 35 / 35; behind it not: 256 x 4096 x 4096 83 / 43, 64 x 4096 x 4096 46 / 24, 16384 x 168 x 256
-// 112 / 44.  Its time is the latency of the rows' loads, 1.5 us for every 256 rows, or with many tiles the conversions,
-// which every workgroup does for itself.
-bool few_rows(int64_t R, int64_t N, int64_t K) { return R <= 4096 && N * K <= 1LL << 22 && R * N * K <= 1LL << 31; }
+// Up to here the one launch wins (us, this / the kernels above; float32): 256 x 168 x 256 (rows, K, N) 5.1 / 15.0,
+// 1024 x 512 x 512 10 / 29, 2048 x 1024 x 1024 33 / 41, 512 x 2048 x 2048 35 / 35; behind it not: 256 x 4096 x 4096 83 / 43,
+// 64 x 4096 x 4096 46 / 24.  Its time is the latency of the rows' loads, 1.5 us for every 256 rows, or with many tiles the
+// conversions, which every workgroup does for itself.
+// Any number of rows of a layer of up to 2^18 weights goes in parts of at least 512 rows, joined by a second launch, up to
+// two workgroups per compute unit: 16384 x 64 x 64 12 / 25, 16384 x 168 x 256 23 / 34, 8192 x 512 x 512 35 / 47, 10^6 x 64 x 64
+// 127 / 1116, but 65536 x 512 x 512 216 / 207 and, with 2^20 weights, 8192 x 1024 x 1024 111 / 77.  Up to kFewSplit rows the
+// second launch costs more than it gives (1536 x 168 x 64 undivided 14).
+bool few_rows(int64_t R, int64_t N, int64_t K) {
+    return (R <= 4096 && N * K <= 1LL << 22 && R * N * K <= 1LL << 31) || (N * K <= 1LL << 18 && N <= 32768);
+}
+
+struct Few {
+    int tiles_k, tiles_n, parts, part_rows;
+    int64_t off_sum, bytes;
+};
+
+Few few_layout(int64_t R, int64_t N, int64_t K) {
+    Few f;
+    f.tiles_k = (int)((K + kFewK - 1) / kFewK), f.tiles_n = (int)((N + kFewN - 1) / kFewN);
+    const int64_t tiles = (int64_t)f.tiles_k * f.tiles_n;
+    const int64_t parts = R <= kFewSplit ? 1 : std::max<int64_t>(1, std::min({R / 512, 512 / tiles, (int64_t)64}));
+    f.part_rows = (int)round_up((R + parts - 1) / parts, kFewWaves * 32);
+    f.parts = (int)((R + f.part_rows - 1) / f.part_rows);
+    f.off_sum = f.parts > 1 ? f.parts * N * round_up(K, 4) * 4 : 0;
+    f.bytes = f.parts > 1 ? f.off_sum + f.parts * N * 4 : 0;
+    return f;
+}
 
 struct Layout {
     int planes, chunks, chunk_rows;
@@ -451,7 +485,8 @@ constexpr int64_t kMaxRows = 1 << 20;  // a row of two fp16 planes is then at mo
 extern "C" {
 
 int64_t mz_ckpt8_workspace(int32_t type, int32_t scale_bits, int32_t rows, int32_t N, int32_t K) {
-    if (rows <= 0 || N <= 0 || K <= 0 || rows > kMaxRows || few_rows(rows, N, K)) return 0;
+    if (rows <= 0 || N <= 0 || K <= 0 || rows > kMaxRows) return 0;
+    if (few_rows(rows, N, K)) return few_layout(rows, N, K).bytes;
     return layout(type, scale_bits, rows, N, K).bytes;
 }
 
@@ -468,24 +503,31 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
         (((uintptr_t)dz | (uintptr_t)dw | (uintptr_t)db) & (type_bytes(type) - 1)) != 0)
         return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: bad stride or alignment (ldz=%lld ldw=%lld ldc=%lld)", (long long)ldz,
                         (long long)ldw, (long long)ldc);
+    const int64_t need = mz_ckpt8_workspace(type, scale_bits, rows, N, K);
+    if (need > 0 && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15) != 0))
+        return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: needs a 16-byte aligned workspace of %lld bytes (got %lld)", (long long)need,
+                        (long long)workspace_bytes);
     if (few_rows(rows, N, K)) {
-        const int tiles_k = (K + kFewK - 1) / kFewK, tiles_n = (N + kFewN - 1) / kFewN;
+        const Few f = few_layout(rows, N, K);
+        float *partial = f.parts > 1 ? (float *)workspace : nullptr, *part_sum = (float *)((uint8_t *)workspace + f.off_sum);
         with_type(type, [&](auto t) {
             using T = decltype(t);
-            const bool pairs = (uintptr_t)dz % (2 * sizeof(T)) == 0 && ldz % 2 == 0 && N % 2 == 0;
+            const bool pairs = (uintptr_t)dz % (2 * sizeof(T)) == 0 && ldz % 2 == 0 && N % 2 == 0, aligned = quads_aligned((T *)dw, ldw);
             const auto go = [&](auto kernel) {
-                hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles_k * tiles_n)), dim3(64 * kFewWaves), 0, (hipStream_t)stream, (const T *)dz, ldz,
-                                   scales, rows, N, codes, ldc, K, (T *)dw, ldw, quads_aligned((T *)dw, ldw), (T *)db, tiles_k);
+                hipLaunchKernelGGL(kernel, dim3((unsigned)(f.tiles_k * f.tiles_n), (unsigned)f.parts), dim3(64 * kFewWaves), 0,
+                                   (hipStream_t)stream, (const T *)dz, ldz, scales, rows, N, codes, ldc, K, (T *)dw, ldw, aligned, (T *)db,
+                                   f.tiles_k, f.part_rows, partial, part_sum);
             };
             if (type != MZ_TYPE_F32 && scale_bits == 3) pairs ? go(k_weight_grad_few<T, 2, true>) : go(k_weight_grad_few<T, 2, false>);
             else pairs ? go(k_weight_grad_few<T, 3, true>) : go(k_weight_grad_few<T, 3, false>);
+            if (f.parts > 1)
+                hipLaunchKernelGGL(k_weight_join<T>, dim3((unsigned)tiles_of(K, 1024), (unsigned)N), dim3(256), 0, (hipStream_t)stream,
+                                   (const float *)partial, f.parts, (const float *)nullptr, K, N, (T *)dw, ldw, aligned,
+                                   (const float *)part_sum, (T *)db);
         });
         return mz::check_launch("mz_ckpt8_weight_grad");
     }
     const Layout l = layout(type, scale_bits, rows, N, K);
-    if (!workspace || workspace_bytes < l.bytes || ((uintptr_t)workspace & 15) != 0)
-        return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: needs a 16-byte aligned workspace of %lld bytes (got %lld)",
-                        (long long)l.bytes, (long long)workspace_bytes);
     const int64_t tiles = (round_up(N, 64) / 64) * (round_up(K, 64) / 64);
     if (tiles > (1 << 23) || l.Rp / 64 > 65535)
         return mz::fail(MZ_ERR_ARG, "mz_ckpt8_weight_grad: rows=%d N=%d K=%d is too large for one call", rows, N, K);
@@ -537,7 +579,7 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
                                partial);
             if (l.shape.splits > 1) {
                 hipLaunchKernelGGL(k_weight_join<T>, dim3((unsigned)tiles_of(K, 1024), (unsigned)N), dim3(256), 0, st, partial,
-                                   l.shape.splits, inverse, K, N, (T *)dw, ldw, aligned);
+                                   l.shape.splits, inverse, K, N, (T *)dw, ldw, aligned, (const float *)nullptr, (T *)nullptr);
             }
         };
         if (l.shape.tile == 256) launch(Tile<OpF16, 256, 256, 4, 2>{});

@@ -654,7 +654,9 @@ def test_contexts_leave_float64_layers_alone():
 @pytest.mark.parametrize("bits", [3, 24])
 @pytest.mark.parametrize("R,K,N", [(1, 5, 2), (7, 65, 33), (33, 64, 31), (255, 200, 97), (257, 130, 34), (4096, 100, 70), (4097, 100, 70),
                                    (500, 2048, 2047), (530, 2048, 2048), (90, 3000, 1500),
-                                   (5000, 60, 30), (4500, 60, 60), (4500, 50, 250)])
+                                   (5000, 60, 30), (4500, 60, 60), (4500, 50, 250),
+                                   (5000, 9000, 30), (4500, 2300, 120), (4500, 1100, 250), (6000, 600, 500), (2048, 70, 40), (2049, 70, 40),
+                                   (40000, 33, 65), (3000, 512, 512)])
 def test_weight_gradient_on_both_sides_of_its_variants(R, K, N, bits, dtype):
     """Rows on pairs of elements and off them, the last row at the end of its memory, garbage around the rest."""
     from muzero_amd.checkpoints import weight_grad
@@ -673,4 +675,4 @@ def test_weight_gradient_on_both_sides_of_its_variants(R, K, N, bits, dtype):
         _within(dw, want, tol + HALF[dtype] * (np.abs(want) + tol) + TINY[dtype])
         _within(db, want_b, tol_b + HALF[dtype] * (np.abs(want_b) + tol_b) + TINY[dtype])
         first = dw if first is None else first
-        assert torch.equal(dw, first)
+        assert _same(dw, first)  # x may hold fp16 infinities, whose rows make everything NaN in both
