@@ -676,3 +676,37 @@ def test_weight_gradient_on_both_sides_of_its_variants(R, K, N, bits, dtype):
         _within(db, want_b, tol_b + HALF[dtype] * (np.abs(want_b) + tol_b) + TINY[dtype])
         first = dw if first is None else first
         assert _same(dw, first)  # x may hold fp16 infinities, whose rows make everything NaN in both
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,N", [(1, 1), (70, 8), (33, 9), (1000, 31), (513, 32), (257, 256), (130, 257), (9, 2047), (5, 2048), (3, 2049), (2, 30000), (2, 70008)])
+def test_rows_in_pieces(R, N, dtype):
+    """Codes, their values and kept activations for rows narrower than a wave's share up to rows of many pieces."""
+    from muzero_amd.checkpoints import _act_grad, _act_save
+    from muzero_amd.quantized import quantize_rows
+    g = torch.Generator().manual_seed(R + N)
+    x = torch.randn(R, N, generator=g).to(dtype).cuda()
+    q = quantize_rows(x)
+    codes, scales = _codes64(x, 24)
+    assert np.array_equal(q.codes[:, :N].cpu().numpy(), codes) and (q.codes[:, N:] == 0).all()
+    back = torch.from_numpy(codes.astype(np.float32)) * torch.from_numpy(scales.astype(np.float32))[:, None]
+    assert torch.equal(q.dequantize().cpu(), back.to(dtype))
+    dy = torch.randn(R, N, generator=g).to(dtype).cuda()
+    for act, y in (("relu", torch.relu(x)), ("tanh", torch.tanh(x)), ("sigmoid", torch.sigmoid(x))):
+        saved = _act_save(y, act)
+        dz = _act_grad(dy, saved, act)
+        if act == "relu":
+            assert torch.equal(dz, torch.where(y > 0, dy, torch.zeros_like(dy)))
+            continue
+        # the product with 127 or 254 is one float32 rounding away: half-way cases may go either way, one step of t
+        t = torch.from_numpy(saved.cpu().numpy().view(np.int8).astype(np.float64)) / 127
+        y64 = y.cpu().double() if act == "tanh" else 2 * y.cpu().double() - 1
+        assert float((t - y64).abs().max()) <= 0.5 / 127 + 1e-5
+        want = dy.cpu().double() * (1 - t * t) * (1.0 if act == "tanh" else 0.25)
+        _within(dz, want.numpy(), (16 * U * dy.cpu().double().abs() + HALF[dtype] * want.abs()).numpy() + TINY[dtype])
+    inplace = dy.clone()
+    from muzero_amd import _hip
+    _hip.check(_hip.lib().mz_ckpt8_act_grad(inplace.data_ptr(), _hip.TYPE_F32 if dtype == torch.float32 else _hip.TYPE_BF16 if dtype == torch.bfloat16
+                                            else _hip.TYPE_F16, N, saved.data_ptr(), R, N, _hip.ACT["sigmoid"], inplace.data_ptr(), N,
+                                            torch.cuda.current_stream().cuda_stream), "mz_ckpt8_act_grad")
+    assert torch.equal(inplace, dz)
