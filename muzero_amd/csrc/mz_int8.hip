@@ -320,8 +320,12 @@ void launch_few(const Int8Args &a, hipStream_t st) {
 
 // Few rows go by k_int8_few: up to 4 always, up to 32 where the weights are small (us, k_int8_few / tiles: 16 x 4096 x 4096
 // 5.8 / 9.1, 32 x 4096 x 4096 7.8 / 10; but 16 x 9216 x 9216 26 / 19, 32 x 9216 x 18432 73 / 31, as every workgroup reads
-// all rows of x again).
-bool few_rows(int64_t rows, int64_t N, int64_t K) { return rows <= 4 || (rows <= 32 && N * K <= 24LL * 1000 * 1000); }
+// all rows of x again); not where a few channels have long rows, which tiles in parts share among more compute units
+// (1 x 65536 x 256 37 / 11, 16 x 18432 x 16 17 / 9.7, 32 x 18432 x 256 26 / 10; but 16 x 8192 x 16 8.8 / 9.6).
+bool few_rows(int64_t rows, int64_t N, int64_t K) {
+    if (K > 12288 && N <= 1024) return false;
+    return rows <= 4 || (rows <= 32 && N * K <= 24LL * 1000 * 1000);
+}
 
 // One launch where x has the result's type and its codes fit a workgroup's share of LDS.
 bool fused(int32_t x_type, int32_t type, int64_t rows, int64_t K) {

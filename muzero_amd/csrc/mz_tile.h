@@ -292,12 +292,15 @@ inline int64_t tiles_of(int64_t n, int64_t t) { return n > 0 ? (n + t - 1) / t :
 //      256 x 9216, 144 steps     81 / 66 (3) / 58 (7)         256 x 9216, 72 steps      41 / 43 (3) / 47 (4)
 //       64 x 9216, 144 steps     34 (3) / 52 (3) / 45 (6)     128 x 4096, 32 steps      13 / 19 (4) / 23 (6)
 //      100 x  500, 128 steps     13 (8), undivided 39         1024 x 1024, 8 steps     6.4 / 13 / 19
+//       64 x 131072, 32 steps    142 / - / 175                 64 x 131072, 4 steps      21 / - / 34
 inline Shape shape_of(int64_t outer, int64_t inner, int64_t steps) {
     const int64_t large = tiles_of(outer, 256) * tiles_of(inner, 256), medium = tiles_of(outer, 256) * tiles_of(inner, 128);
-    if (large >= 200) return {256, 1};
-    if (medium >= 200) return {128, 1};
-    if (outer * inner * steps >= 240LL * 1000 * 1000 && steps >= 64)  // a long reduction: the operands are what is read
-        return {256, (int)std::max<int64_t>(1, std::min(256 / large, steps / 16))};
+    if (outer > 64) {  // else most of a larger tile would be rows that are not there
+        if (large >= 200) return {256, 1};
+        if (medium >= 200) return {128, 1};
+        if (outer * inner * steps >= 240LL * 1000 * 1000 && steps >= 64)  // a long reduction: the operands are what is read
+            return {256, (int)std::max<int64_t>(1, std::min(256 / large, steps / 16))};
+    }
     const int64_t small = tiles_of(outer, 64) * tiles_of(inner, 64);
     return {64, (int)std::max<int64_t>(1, std::min({(int64_t)32, 600 / small, steps / 16}))};
 }

@@ -114,7 +114,9 @@ def _int8_reference(x, w, b, act, bits=24):
                                        (2, 18432, 65, "none"), (300, 4097, 190, "relu"), (8, 4096, 1024, "none"), (520, 260, 520, "none"),
                                        (33, 2048, 2, "none"), (1030, 64, 1, "none"), (48, 8192, 1000, "relu"), (700, 1200, 900, "none"), (3700, 100, 3601, "none"), (3601, 384, 3700, "relu"),
                                        (2000, 130, 3700, "tanh"), (2100, 700, 3300, "none"), (200, 16500, 700, "relu"), (250, 18432, 2050, "none"),
-                                       (16, 1024, 40, "relu"), (16, 1025, 40, "none"), (7, 2300, 60, "tanh"), (15, 5, 3, "none")])
+                                       (16, 1024, 40, "relu"), (16, 1025, 40, "none"), (7, 2300, 60, "tanh"), (15, 5, 3, "none"),
+                                       (1, 20000, 16, "relu"), (3, 12289, 1024, "none"), (32, 13000, 5, "sigmoid"), (20, 12288, 90, "none"),
+                                       (64, 300, 30000, "none"), (64, 8200, 7000, "relu"), (33, 500, 20001, "none")])
 def test_int8_linear(R, K, N, act, dtype):
     from muzero_amd.quantized import int8_linear, quantize_rows
     x = _x(R, K, dtype, seed=R + K)
