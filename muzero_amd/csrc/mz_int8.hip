@@ -143,13 +143,14 @@ k_int8_few(const int8_t *__restrict__ xc, int64_t ldxc, const float *__restrict_
 // The same for up to kFusedRows rows that are not coded yet, in one launch: every workgroup codes them for itself, into
 // LDS, while its first weights are on their way (a row of 9216 float32 comes from L2; a launch of the quantiser of its own
 // costs more than that).  Up to kSharedRows rows all waves work on one after the other; beyond, every wave has its own rows,
-// up to kOwnValues values in all: us per layer in a chain, one launch / two (which also cost 3 us more of the host):
-// 5 x 512 4.2 / 5.0, 5 x 2048 5.9 / 6.4, 16 x 168 4.8 / 5.1, 16 x 1024 6.3 / 6.1; behind it 16 x 2048 8.7 / 7.0.
+// up to kOwnValues values in all (SHARED, a constant: with both in one kernel 1 x 9216 x 9216 takes 20.4 us, not 17.8).  us
+// per layer in a chain, one launch / two (which also cost 3 us more of the host): 5 x 512 4.2 / 5.0, 5 x 2048 5.9 / 6.4,
+// 16 x 168 4.8 / 5.1, 16 x 1024 6.3 / 6.1; behind it 16 x 2048 8.7 / 7.0.
 constexpr int kFusedRows = 16, kSharedRows = 4, kOwnValues = 16384, kFusedBytes = 40960;
 
 int64_t fused_stride(int64_t K) { return (K + 127) / 128 * 128 + 16; }  // rows of codes in different banks
 
-template <class T, bool WHOLE>
+template <class T, bool WHOLE, bool SHARED>
 __global__ void __launch_bounds__(64 * kFewWaves)
 k_int8_fused(const T *__restrict__ xp, int64_t ldx, int rows, int K, const int8_t *__restrict__ wc, int64_t ldw,
              const float *__restrict__ ws, int N, const float *__restrict__ bias, int act, T *__restrict__ y, int64_t ldy) {
@@ -167,7 +168,7 @@ k_int8_fused(const T *__restrict__ xp, int64_t ldx, int rows, int K, const int8_
 #pragma unroll
         for (int h = 0; h < 2; ++h) first[u][h] = k < kbytes ? *(const u32x4 *)(w + k + h * 16) : u32x4{};
     }
-    if (rows <= kSharedRows) {  // all waves on one row after the other
+    if constexpr (SHARED) {  // all waves on one row after the other
         for (int r = 0; r < rows; ++r) {
             unsigned m = 0;
 #pragma unroll 4
@@ -389,9 +390,12 @@ int mz_int8_forward(const void *x, int32_t x_type, int64_t ldx, int32_t rows, in
         with_type(type, [&](auto t) {
             using T = decltype(t);
             with_flag(rows_aligned<T>(x, ldx), [&](auto whole) {
-                hipLaunchKernelGGL((k_int8_fused<T, decltype(whole)::value>), dim3((unsigned)tiles_of(N, 16)), dim3(64 * kFewWaves),
-                                   (size_t)(rows * fused_stride(K)), (hipStream_t)stream, (const T *)x, ldx, rows, K, w_codes, ldw, w_scales, N,
-                                   bias, activation, (T *)y, ldy);
+                constexpr bool W = decltype(whole)::value;
+                const auto launch = [&](auto kernel) {
+                    hipLaunchKernelGGL(kernel, dim3((unsigned)tiles_of(N, 16)), dim3(64 * kFewWaves), (size_t)(rows * fused_stride(K)),
+                                       (hipStream_t)stream, (const T *)x, ldx, rows, K, w_codes, ldw, w_scales, N, bias, activation, (T *)y, ldy);
+                };
+                rows <= kSharedRows ? launch(k_int8_fused<T, W, true>) : launch(k_int8_fused<T, W, false>);
             });
         });
         return mz::check_launch("k_int8_fused");
