@@ -219,7 +219,7 @@ __device__ void codes_block(const int8_t *__restrict__ codes, int64_t ldc, int R
     for (int i = t; i < 64 * kCodeCols / 16; i += kCT) {
         const int r = i / (kCodeCols / 16), c = i % (kCodeCols / 16) * 16;
         u32x4 v = {};
-        if (r0 + r < R && k0 + c < ldc) v = *(const u32x4 *)(codes + (r0 + r) * ldc + k0 + c);
+        if (r0 + r < R && k0 + c < K) v = *(const u32x4 *)(codes + (r0 + r) * ldc + k0 + c);
 #pragma unroll
         for (int e = 0; e < 4; ++e) *(unsigned *)(lds + r * ld + c + 4 * e) = v[e];
     }
@@ -335,7 +335,7 @@ k_weight_grad_few(const T *__restrict__ dz, int64_t ldz, const float *__restrict
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
     const int k0 = (int)(blockIdx.x % tiles_k) * kFewK, n0 = (int)(blockIdx.x / tiles_k) * kFewN;
     // rows and columns behind the last one are read as the last one: the rows count as zero, the columns are not stored
-    const int8_t *q0 = codes + min((int64_t)(k0 + 4 * c), ldc - 4);
+    const int8_t *q0 = codes + min(k0 / 4 + c, (K - 1) / 4) * 4;
     const T *d0 = dz + min(n0 + 2 * c, PAIRS ? N - 2 : N - 1), *d1 = dz + min(n0 + 2 * c + 1, N - 1);
     struct Rows {
         unsigned q[8];

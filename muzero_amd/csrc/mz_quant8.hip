@@ -104,8 +104,8 @@ k_dequant8(const int8_t *__restrict__ codes, int64_t ldc, const float *__restric
         const float s = scales[row];
         word w[kHold];
 #pragma unroll
-        for (int h = 0; h < kHold; ++h)  // a row of codes is padded to whole packs; behind it the last one is read again
-            w[h] = *(const word *)(codes + row * ldc + min((int64_t)(at + h * LANES) * n, ldc - n));
+        for (int h = 0; h < kHold; ++h)  // a row of codes is padded to whole packs; behind K the last one is read again
+            w[h] = *(const word *)(codes + row * ldc + min(at + h * LANES, (K - 1) / n) * n);
 #pragma unroll
         for (int h = 0; h < kHold; ++h) {
             const int j = (at + h * LANES) * n;

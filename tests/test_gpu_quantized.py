@@ -712,3 +712,24 @@ def test_rows_in_pieces(R, N, dtype):
                                             else _hip.TYPE_F16, N, saved.data_ptr(), R, N, _hip.ACT["sigmoid"], inplace.data_ptr(), N,
                                             torch.cuda.current_stream().cuda_stream), "mz_ckpt8_act_grad")
     assert torch.equal(inplace, dz)
+
+
+@pytest.mark.parametrize("R,K,N", [(5, 100, 30), (40, 128, 200), (300, 130, 4200), (5000, 1000, 300)])
+def test_codes_that_are_part_of_a_wider_matrix(R, K, N):
+    """Rows of codes with a stride, the last one at the end of its memory: what lies between them is not theirs."""
+    from muzero_amd.checkpoints import weight_grad
+    from muzero_amd.quantized import QuantizedRows, int8_linear, quantize_rows
+    x = _x(R, K, torch.float32)
+    q = quantize_rows(x, scale_bits=3)
+    width = q.codes.shape[1]
+    big = torch.full((R, width + 256), 99, dtype=torch.int8, device="cuda")
+    big[:, 256:] = q.codes
+    part = QuantizedRows(big[:, 256:], q.scales, q.shape, q.dtype, 3)
+    assert part.ld == width + 256
+    assert torch.equal(part.dequantize(), q.dequantize())
+    dz = torch.randn(R, N, device="cuda")
+    assert all(torch.equal(a, b) for a, b in zip(weight_grad(dz, part), weight_grad(dz, q)))
+    w = quantize_rows(torch.randn(N, K, device="cuda"))
+    assert torch.equal(int8_linear(part, w), int8_linear(q, w))
+    v = quantize_rows(torch.randn(7, K, device="cuda"))
+    assert torch.equal(int8_linear(v, part), int8_linear(v, q))
