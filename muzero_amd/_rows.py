@@ -5,6 +5,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd import forward_ad
 
 from muzero_amd import _hip
 
@@ -13,13 +14,23 @@ MAX_ROWS, MAX_COLUMNS = (1 << 31) - 1, 1 << 30
 _NULL = contextlib.nullcontext()
 
 
-def check_tensor(t: torch.Tensor, what: str) -> None:
-    """A float32 / bfloat16 / float16 tensor on the GPU, or a TypeError / HipError that says which."""
+def check_tensor(t: torch.Tensor, what: str, forward_mode: bool = False) -> None:
+    """A float32 / bfloat16 / float16 tensor on the GPU, without a forward-mode tangent unless the caller sees to it, or an
+    error that says which."""
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{what} must be a tensor, not {type(t).__name__}")
     if t.dtype not in TYPE:
         raise TypeError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+    if not forward_mode:
+        refuse_tangent(t, what)
     check_on_gpu(t, what)
+
+
+def refuse_tangent(t: torch.Tensor, what: str) -> None:
+    """The kernels have no forward-mode derivative, and a result without a tangent would read as one that does not depend
+    on t.  (torch.no_grad() does not switch forward mode off.)"""
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:  # no call where no level is open
+        raise NotImplementedError(f"{what} carries a forward-mode tangent, for which there is no derivative here")
 
 
 def check_on_gpu(t: torch.Tensor, what: str) -> None:

@@ -25,7 +25,7 @@ from torch.autograd.function import once_differentiable
 
 from muzero_amd import _hip
 from muzero_amd._hip import ptr
-from muzero_amd._rows import TYPE, check_tensor, on_device, row_stride, rows_of, stream_of, workspace
+from muzero_amd._rows import TYPE, check_tensor, on_device, refuse_tangent, row_stride, rows_of, stream_of, workspace
 from muzero_amd.quantized import ACTIVATIONS, QuantizedRows, quantize_rows
 
 
@@ -116,6 +116,7 @@ class _CheckpointedLinear(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
+        refuse_tangent(dy, "the gradient")
         weight, codes, scales, act = ctx.saved_tensors
         K, N = ctx.x_shape[-1], dy.shape[-1]
         want_x, want_w, want_b, _ = ctx.needs_input_grad
@@ -139,8 +140,8 @@ def checkpointed_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[to
                         activation: str = "none") -> torch.Tensor:
     """act(x W^T + bias) for x [..., K], with everything the backward pass needs of x and of the result kept in 8 bits or
     fewer (nothing is kept under torch.no_grad())."""
-    check_tensor(x, "x")
-    check_tensor(weight, "weight")
+    check_tensor(x, "x", forward_mode=True)  # torch's own operators serve one under no_grad, the autograd function refuses it
+    check_tensor(weight, "weight", forward_mode=True)
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or x.shape[-1] < 1:
         raise ValueError(f"x of shape {tuple(x.shape)} does not match a weight of shape {tuple(weight.shape)}")
     if activation not in ACTIVATIONS:

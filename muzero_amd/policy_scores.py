@@ -16,11 +16,12 @@ from __future__ import annotations
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from muzero_amd import _hip
 from muzero_amd._hip import ptr
-from muzero_amd._rows import TYPE, check_tensor, on_device, rows_of, stream_of, workspace
+from muzero_amd._rows import TYPE, check_tensor, on_device, refuse_tangent, rows_of, stream_of, workspace
 
 MAX_TOP = 32
 _WHOLE = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
@@ -63,6 +64,10 @@ def _gradient(ctx, g_log_prob, g_entropy, _g_actions, g_top):
     # calls, no helpers on the way of the common case.
     logits, actions, stats, top_actions = ctx.saved_tensors
     T, V = logits.shape
+    if forward_ad._current_level >= 0:
+        for g in (g_log_prob, g_entropy, g_top):
+            if g is not None:
+                refuse_tangent(g, "the gradient")
     grad = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
     if T > 0:
         g_log_prob = None if g_log_prob is None else g_log_prob.contiguous()
@@ -103,6 +108,7 @@ def policy_scores(logits: torch.Tensor, actions: Optional[torch.Tensor] = None, 
     """Scores of every row of `logits` [..., V].  `actions` (whole numbers, shape [...]): a negative one scores 0 and
     takes no gradient (no action was played there), one of V or more scores NaN.  `top`: 0..32 alternatives.
 
+    The gradient is a reverse-mode one: logits with a forward-mode tangent are refused.
     A row with nothing but -inf has log probabilities -inf, entropy 0 and no gradient; NaN or +inf make their row NaN."""
     check_tensor(logits, "logits")
     if logits.dim() < 1 or logits.shape[-1] < 1:

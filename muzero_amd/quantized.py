@@ -17,7 +17,7 @@ import torch
 
 from muzero_amd import _hip
 from muzero_amd._hip import ptr
-from muzero_amd._rows import TYPE, check_on_gpu, check_tensor, on_device, row_stride, rows_of, stream_of, workspace
+from muzero_amd._rows import TYPE, check_on_gpu, check_tensor, on_device, refuse_tangent, row_stride, rows_of, stream_of, workspace
 
 MAX_K = 131072  # sums of K products of codes stay exact in 32 bits
 ACTIVATIONS = ("none", "linear", "relu", "tanh", "sigmoid")
@@ -88,7 +88,8 @@ class QuantizedRows:
 
 def quantize_rows(x: torch.Tensor, scale_bits: int = 24) -> QuantizedRows:
     """Codes of x [..., K], one scale per row.  scale_bits=3 rounds the scale up to 1, 1.25, 1.5 or 1.75 times a power of
-    two (what muzero_amd.checkpoints keeps)."""
+    two (what muzero_amd.checkpoints keeps).  Codes are whole numbers and carry no gradient; an x with a forward-mode tangent
+    is refused."""
     check_tensor(x, "x")
     if scale_bits not in (24, 3):
         raise ValueError(f"scale_bits must be 24 or 3, not {scale_bits}")
@@ -123,8 +124,8 @@ def _check_weight(weight: QuantizedRows, K: int) -> int:
 def int8_linear(x, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, activation: str = "none",
                 out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """act(x W^T + bias) for x [..., K] (a tensor, or QuantizedRows when several layers read the same rows).  The result
-    has x's type unless `out_dtype` says otherwise.  There is no gradient: training goes through float weights
-    (muzero_amd.checkpoints keeps their inputs in 8 bits)."""
+    has x's type unless `out_dtype` says otherwise.  There is no gradient, reverse or
+    forward mode: training goes through float weights (muzero_amd.checkpoints keeps their inputs in 8 bits)."""
     coded = isinstance(x, QuantizedRows)
     if not coded:
         check_tensor(x, "x")
@@ -144,6 +145,7 @@ def int8_linear(x, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, a
     if bias is not None:
         if bias.shape != (N,) or bias.device != dev:
             raise ValueError(f"bias must be {N} values on {dev}")
+        refuse_tangent(bias, "bias")
         if bias.dtype is not torch.float32 or not bias.is_contiguous():
             bias = bias.detach().to(torch.float32).contiguous()
     check_on_gpu(weight.codes, "weight")

@@ -733,3 +733,20 @@ def test_codes_that_are_part_of_a_wider_matrix(R, K, N):
     assert torch.equal(int8_linear(part, w), int8_linear(q, w))
     v = quantize_rows(torch.randn(7, K, device="cuda"))
     assert torch.equal(int8_linear(v, part), int8_linear(v, q))
+
+
+def test_forward_mode_through_a_checkpointed_layer():
+    """Without reverse mode the layer is torch's own operators, tangent and all; with it there is no forward-mode rule."""
+    import torch.autograd.forward_ad as fwad
+
+    from muzero_amd.checkpoints import checkpointed_linear
+    lin = torch.nn.Linear(40, 24).cuda()
+    x, t = torch.randn(5, 40, device="cuda"), torch.randn(5, 40, device="cuda")
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, t)
+        with pytest.raises(NotImplementedError):
+            checkpointed_linear(dual, lin.weight, lin.bias, "tanh")
+        with torch.no_grad():
+            got = fwad.unpack_dual(checkpointed_linear(dual, lin.weight, lin.bias, "tanh")).tangent
+            want = fwad.unpack_dual(torch.tanh(lin(dual))).tangent
+    torch.testing.assert_close(got, want)

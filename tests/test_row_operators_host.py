@@ -292,3 +292,49 @@ def test_layers_that_do_more_than_a_layer_are_left_alone():
     with eight_bit_checkpoints(own):
         assert own(5) == 5
     assert own(5) == 5
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_tangents_are_refused(grad_mode):
+    """A result without a tangent would read as one that does not depend on the input: no call takes a dual tensor and
+    drops its tangent, with reverse mode on or off."""
+    import torch.autograd.forward_ad as fwad
+
+    from muzero_amd.checkpoints import save_activations, weight_grad
+    from muzero_amd.policy_scores import policy_scores
+    from muzero_amd.quantized import QuantizedRows, int8_linear, quantize_rows
+    z = torch.zeros(2, 100)
+    coded = QuantizedRows(torch.zeros(4, 128, dtype=torch.int8), torch.zeros(4), torch.Size((4, 100)), torch.float32, 24)
+    rows = QuantizedRows(torch.zeros(2, 128, dtype=torch.int8), torch.zeros(2), torch.Size((2, 100)), torch.float32, 24)
+    with fwad.dual_level(), torch.set_grad_enabled(grad_mode):
+        dual = fwad.make_dual(z, torch.ones_like(z))
+        bias = fwad.make_dual(torch.zeros(4), torch.ones(4))
+        for call in (lambda: policy_scores(dual), lambda: policy_scores(dual[:, ::2]),
+                     lambda: quantize_rows(dual), lambda: save_activations(dual), lambda: int8_linear(dual, coded),
+                     lambda: weight_grad(dual, rows), lambda: int8_linear(rows, coded, bias)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call()
+        with pytest.raises(_hip.HipError, match="GPU"):   # a tensor without one is not refused for it
+            policy_scores(z)
+        with pytest.raises(_hip.HipError, match="GPU"):
+            policy_scores(dual.detach())
+
+
+def test_forward_mode_tangents_of_gradients_are_refused():
+    import types
+
+    import torch.autograd.forward_ad as fwad
+
+    from muzero_amd.checkpoints import _CheckpointedLinear
+    from muzero_amd.policy_scores import _gradient
+    z = torch.zeros(2, 3)
+    with fwad.dual_level():
+        dy = fwad.make_dual(z, torch.ones_like(z))
+        g = fwad.make_dual(torch.zeros(2), torch.ones(2))
+        ctx = types.SimpleNamespace(saved_tensors=(z, None, torch.zeros(2, 3), None), kind=F32, needs_input_grad=(True,) * 4)
+        for grads in ((g, None, None, None), (None, g, None, None), (None, None, None, dy)):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                _gradient(ctx, *grads)
+        ctx = types.SimpleNamespace(saved_tensors=(None, None, None, None), x_shape=(2, 5), needs_input_grad=(True,) * 4)
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
+            _CheckpointedLinear.backward(ctx, dy)
