@@ -177,7 +177,7 @@ class eight_bit_checkpoints:
     of a DynamicsNetwork -- keep 8-bit checkpoints on the GPU.  Convolutions and BatchNorm layers are left as they are, and
     so are layers with hooks or a forward of their own and everything on the CPU or in float64.  Parameters, state_dict
     keys and results of the forward pass do not change.  Contexts may be nested and overlap: a layer is as it was when the
-    last one that names it has ended."""
+    last one that names it has ended, except for a forward that somebody has given it meanwhile, which stays."""
 
     def __init__(self, *modules: torch.nn.Module):
         from muzero_amd.neural_networks.network_builder import is_dense_sequence, is_plain
@@ -225,8 +225,10 @@ class eight_bit_checkpoints:
         with _LOCK:
             for t in self._open.pop():
                 t.depth -= 1
-                if t.depth == 0 and t.before is None:
+                if t.depth > 0 or t.module.__dict__.get(t.name) is not t:  # still in use, or no longer in the method's place
+                    continue
+                if t.before is None:
                     del t.module.__dict__[t.name]
-                elif t.depth == 0:
+                else:
                     t.module.__dict__[t.name] = t.before
         return False

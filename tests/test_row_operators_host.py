@@ -338,3 +338,31 @@ def test_forward_mode_tangents_of_gradients_are_refused():
         ctx = types.SimpleNamespace(saved_tensors=(None, None, None, None), x_shape=(2, 5), needs_input_grad=(True,) * 4)
         with torch.no_grad(), pytest.raises(NotImplementedError, match="tangent"):
             _CheckpointedLinear.backward(ctx, dy)
+
+
+def test_a_context_ends_with_what_it_finds():
+    """A forward that the user sets inside a context stays; an entry that is gone keeps nothing from being put back."""
+    from muzero_amd.checkpoints import eight_bit_checkpoints
+    g, f, lat = _small_networks()
+    act = torch.tensor([0, 3, 6])
+    want = g(lat, act) + f(lat)
+    mine = lambda x: x + 1  # noqa: E731
+    with eight_bit_checkpoints(g, f):
+        f.value_mlp.forward = mine
+    assert f.value_mlp.__dict__["forward"] is mine and f.value_mlp(1) == 2 and "forward" not in f.policy_mlp.__dict__
+    del f.value_mlp.forward
+    with eight_bit_checkpoints(g, f) as ctx:
+        assert [t.name for t in ctx._open[0]].count("forward") == 3
+        del ctx._open[0][0].module.forward             # the first of the list
+        with eight_bit_checkpoints(f.value_mlp, g):    # takes it anew
+            del g.merge
+    nets = [m for net in (g, f) for m in net.modules()]
+    assert all("forward" not in m.__dict__ and "merge" not in m.__dict__ for m in nets)
+    outer, inner = eight_bit_checkpoints(f), eight_bit_checkpoints(f)
+    outer.__enter__()
+    f.policy_mlp.forward = mine
+    inner.__enter__()                                  # leaves it alone
+    outer.__exit__(None, None, None), inner.__exit__(None, None, None)
+    assert f.policy_mlp.__dict__["forward"] is mine and "forward" not in f.value_mlp.__dict__
+    del f.policy_mlp.forward
+    assert all(torch.equal(x, y) for x, y in zip(want, g(lat, act) + f(lat)))
