@@ -159,6 +159,8 @@ class _Taken:
     """Stands in for a module's method (`forward`, `merge`) while contexts are open.  Copies and pickles of the module get
     the method itself: they belong to no context."""
 
+    stands_in = True
+
     def __init__(self, module: torch.nn.Module, name: str, fn):
         self.module, self.name, self.fn, self.depth, self.before = module, name, fn, 0, module.__dict__.get(name)
 

@@ -11,6 +11,8 @@ optional max-pool) and build_mlp (Linear + activation per entry).
 """
 from __future__ import annotations
 
+import types
+
 import torch
 from torch import nn
 
@@ -115,15 +117,25 @@ def build_mlp(layers_config: list[DenseLayerConfig], input_dim: int) -> tuple[nn
 _DENSE_ACTIVATIONS = {nn.Identity: "none", nn.ReLU: "relu", nn.Tanh: "tanh", nn.Sigmoid: "sigmoid", nn.Softmax: "softmax"}
 
 
+def own_forward(module: nn.Module):
+    """The forward that somebody has given this one module, in place of its class's; None if there is none.  What stands in
+    for the class's method (`stands_in`) is none."""
+    own = module.__dict__.get("forward")
+    if isinstance(own, types.MethodType) and own.__func__ is type(module).forward and own.__self__ is module:
+        return None
+    return None if getattr(own, "stands_in", False) else own
+
+
 def is_plain(module: nn.Module, kind: type) -> bool:
     """A `kind` that does what a `kind` does: no forward of its own, no hooks."""
-    return (isinstance(module, kind) and type(module).forward is kind.forward and
+    return (isinstance(module, kind) and type(module).forward is kind.forward and own_forward(module) is None and
             not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks))
 
 
 def is_dense_sequence(module: nn.Module) -> bool:
-    """True for what build_mlp makes: plain Linear and activation modules in turn."""
-    mods = list(module) if isinstance(module, nn.Sequential) and type(module).forward is nn.Sequential.forward else []
+    """True for what build_mlp makes: plain Linear and activation modules in turn, run one after the other."""
+    plain = isinstance(module, nn.Sequential) and type(module).forward is nn.Sequential.forward and own_forward(module) is None
+    mods = list(module) if plain else []
     return len(mods) > 0 and len(mods) % 2 == 0 and all(
         is_plain(m, nn.Linear) if i % 2 == 0 else type(m) in _DENSE_ACTIVATIONS and is_plain(m, type(m)) for i, m in enumerate(mods))
 

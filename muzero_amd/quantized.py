@@ -247,7 +247,10 @@ class Int8Networks:
         self._merge()
 
     def _merge(self) -> None:
+        from muzero_amd.neural_networks.network_builder import is_plain
         g, D, A = self.dynamics_net, self.D, self.A
+        if not is_plain(g.fc_merge, torch.nn.Linear):
+            raise ValueError("fc_merge must be a Linear layer without hooks or a forward of its own")
         emb, w, b = (t.detach().to(self.device, torch.float32).contiguous()
                      for t in (g.action_embedding.weight, g.fc_merge.weight, g.fc_merge.bias))
         self.merge = _renew(self.merge, quantize_rows(w[:, :D]))

@@ -366,3 +366,32 @@ def test_a_context_ends_with_what_it_finds():
     assert f.policy_mlp.__dict__["forward"] is mine and "forward" not in f.value_mlp.__dict__
     del f.policy_mlp.forward
     assert all(torch.equal(x, y) for x, y in zip(want, g(lat, act) + f(lat)))
+
+
+def test_a_forward_of_one_inner_layer_is_its_own():
+    """Set on the instance, as a profiler or muzero_amd.neural_networks.per_call does it: on a Linear, an activation, the
+    merge layer, the sequence itself."""
+    from muzero_amd.checkpoints import eight_bit_checkpoints
+    from muzero_amd.neural_networks.network_builder import dense_pairs, is_dense_sequence, is_plain
+    from muzero_amd.quantized import Int8MLP
+    for layer in (0, 1, None):
+        seq = torch.nn.Sequential(torch.nn.Linear(3, 3), torch.nn.ReLU())
+        m = seq if layer is None else seq[layer]
+        m.forward = lambda x, f=m.forward: f(x) + 1
+        assert not is_plain(m, type(m)) and not is_dense_sequence(seq)
+        for refused in (lambda: dense_pairs(seq), lambda: Int8MLP(seq, device="cpu")):
+            with pytest.raises(ValueError):
+                refused()
+        with eight_bit_checkpoints(seq) as ctx:
+            assert ctx.sequences == []
+        del m.forward
+        m.forward = m.forward                          # the class's own method, bound: nothing of its own
+        assert is_dense_sequence(seq) and len(eight_bit_checkpoints(seq).sequences) == 1
+    g, f, lat = _small_networks()
+    g.fc_merge.forward = lambda x: torch.nn.functional.linear(x, g.fc_merge.weight)
+    act = torch.tensor([0, 3, 6])
+    want = g(lat, act)
+    with eight_bit_checkpoints(g) as ctx:
+        assert ctx.merges == [] and all(torch.equal(x, y) for x, y in zip(want, g(lat, act)))
+    with eight_bit_checkpoints(f), eight_bit_checkpoints(f) as ctx:   # what an open context put there is nobody's own
+        assert len(ctx.sequences) == 2
