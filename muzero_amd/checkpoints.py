@@ -171,6 +171,12 @@ class _Taken:
         return _bound, (getattr(type(self.module), self.name), self.module)
 
 
+def _keeps_8_bits(x: torch.Tensor) -> bool:
+    """Whether a layer inside a context keeps x in 8 bits; else it runs as it is.  Hooks that torch calls for every module
+    see a layer only if it runs as it is."""
+    return x.is_cuda and x.dtype in TYPE and not torch.nn.modules.module._has_any_global_hook()
+
+
 _LOCK = threading.Lock()  # of every module's open contexts
 
 
@@ -191,8 +197,8 @@ class eight_bit_checkpoints:
 
     @staticmethod
     def _sequence_forward(seq, x):
-        from muzero_amd.neural_networks.network_builder import dense_pairs
-        if not x.is_cuda or x.dtype not in TYPE:
+        from muzero_amd.neural_networks.network_builder import dense_pairs, is_dense_sequence
+        if not _keeps_8_bits(x) or not is_dense_sequence(seq):  # a hook may have come since the context was opened
             return type(seq).forward(seq, x)
         for i, (lin, act) in enumerate(dense_pairs(seq)):
             if act == "softmax":
@@ -203,7 +209,8 @@ class eight_bit_checkpoints:
 
     @staticmethod
     def _merge(net, merged):
-        if not merged.is_cuda or merged.dtype not in TYPE:
+        from muzero_amd.neural_networks.network_builder import is_plain
+        if not _keeps_8_bits(merged) or not is_plain(net.fc_merge, torch.nn.Linear):
             return type(net).merge(net, merged)
         return checkpointed_linear(merged, net.fc_merge.weight, net.fc_merge.bias, "relu")
 

@@ -395,3 +395,36 @@ def test_a_forward_of_one_inner_layer_is_its_own():
         assert ctx.merges == [] and all(torch.equal(x, y) for x, y in zip(want, g(lat, act)))
     with eight_bit_checkpoints(f), eight_bit_checkpoints(f) as ctx:   # what an open context put there is nobody's own
         assert len(ctx.sequences) == 2
+
+
+def test_hooks_that_come_while_a_context_is_open(monkeypatch):
+    """Such layers run as they are from then on, hooks and all, and go back to 8 bits when the hook has gone."""
+    import muzero_amd.checkpoints as ck
+    g, f, lat = _small_networks()
+    act, kept = torch.tensor([0, 3, 6]), []
+
+    def layer(x, weight, bias=None, activation="none"):
+        kept.append(activation)
+        return ck._activate_(torch.nn.functional.linear(x, weight, bias), activation)
+    monkeypatch.setattr(ck, "checkpointed_linear", layer)
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    with ck.eight_bit_checkpoints(g, f):
+        want = f(lat) + g(lat, act)
+        assert len(kept) == 3 + 3 + 2 + 1
+        seen = []
+        hooks = [m.register_forward_hook(lambda m, x, y: (seen.append(m), y + 1)[1])
+                 for m in (f.value_mlp[0], f.policy_mlp[1], g.fc_merge)]
+        kept.clear()
+        got = f(lat) + g(lat, act)
+        assert seen == [f.value_mlp[0], f.policy_mlp[1], g.fc_merge]
+        assert len(kept) == 2 and not any(torch.equal(x, y) for x, y in zip(want, got))
+        for h in hooks:
+            h.remove()
+        every = torch.nn.modules.module.register_module_forward_hook(lambda m, x, y: seen.append(m))
+        try:
+            kept.clear(), seen.clear()
+            f(lat)
+            assert f.value_mlp[0] in seen and f.policy_mlp[4] in seen and not kept
+        finally:
+            every.remove()
+        assert all(torch.equal(x, y) for x, y in zip(want, f(lat) + g(lat, act))) and len(kept) == 3 + 3 + 2 + 1
