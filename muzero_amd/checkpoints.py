@@ -96,10 +96,23 @@ def _activate_(y: torch.Tensor, activation: str) -> torch.Tensor:
     return y
 
 
+def _linear(x, weight, bias):
+    """F.linear inside an autograd function.  There autograd is off, and autocast would keep the 16-bit copies it makes of x
+    and the parameters for later layers, which would then have no gradient: its cache stays out of this call."""
+    if not torch.is_autocast_enabled(x.device.type):
+        return F.linear(x, weight, bias)
+    cached = torch.is_autocast_cache_enabled()
+    torch.set_autocast_cache_enabled(False)
+    try:
+        return F.linear(x, weight, bias)
+    finally:
+        torch.set_autocast_cache_enabled(cached)
+
+
 class _CheckpointedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, activation):
-        y = _activate_(F.linear(x, weight, bias), activation)
+        y = _activate_(_linear(x, weight, bias), activation)
         codes = scales = act = None
         if y.numel() > 0:
             if ctx.needs_input_grad[1]:

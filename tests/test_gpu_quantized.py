@@ -750,3 +750,27 @@ def test_forward_mode_through_a_checkpointed_layer():
             got = fwad.unpack_dual(checkpointed_linear(dual, lin.weight, lin.bias, "tanh")).tangent
             want = fwad.unpack_dual(torch.tanh(lin(dual))).tangent
     torch.testing.assert_close(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_layers_under_autocast(dtype):
+    """The forward pass of the layer under autocast; gradients of it and of a plain layer with the same weights beside it."""
+    from muzero_amd.checkpoints import eight_bit_checkpoints
+    _, _, f = _networks(8)
+    lat = torch.randn(32, 4, 6, 7, device="cuda")
+    params = list(f.policy_mlp.parameters())
+    with torch.autocast("cuda", dtype):
+        with eight_bit_checkpoints(f):
+            policy, _ = f(lat)
+        logits = f.policy_logits(lat)          # the same layers outside a context
+    plain = torch.autograd.grad(logits.float().square().sum(), params)
+    assert all(bool((g != 0).any()) for g in plain)
+    with torch.autocast("cuda", dtype):
+        want_policy, _ = f(lat)
+    assert torch.equal(policy, want_policy)
+    w = torch.randn(32, 7, device="cuda")
+    want = torch.autograd.grad((want_policy * w).sum(), params)
+    got = torch.autograd.grad((policy * w).sum(), params)
+    assert all(g.dtype == torch.float32 and bool(g.isfinite().all()) and bool((g != 0).any()) for g in got)
+    # the last bias: column sums of the same 16-bit dz, 32 terms in float32, rounded once to the type on each side
+    assert float((want[-1] - got[-1]).abs().max()) <= 2 * HALF[dtype] * float(want[-1].abs().max()) + 64 * U * float(w.abs().sum())

@@ -428,3 +428,18 @@ def test_hooks_that_come_while_a_context_is_open(monkeypatch):
         finally:
             every.remove()
         assert all(torch.equal(x, y) for x, y in zip(want, f(lat) + g(lat, act))) and len(kept) == 3 + 3 + 2 + 1
+
+
+def test_autocast_keeps_no_copies_without_a_gradient(monkeypatch):
+    """A layer that shares its weights with a checkpointed one in the same autocast region still has its gradient."""
+    import muzero_amd.checkpoints as ck
+    from muzero_amd.quantized import QuantizedRows
+    monkeypatch.setattr(ck, "save_activations", lambda x: QuantizedRows(
+        torch.zeros(x.shape[0], 128, dtype=torch.int8), torch.zeros(x.shape[0]), x.shape, x.dtype, 3))
+    lin, x = torch.nn.Linear(4, 3), torch.randn(5, 4, requires_grad=True)
+    with torch.autocast("cpu", torch.bfloat16):
+        y = ck._CheckpointedLinear.apply(x, lin.weight, lin.bias, "none")
+        z = lin(x)
+    assert y.dtype == z.dtype == torch.bfloat16 and torch.equal(y, z)
+    grads = torch.autograd.grad(z.sum(), (x, lin.weight, lin.bias))
+    assert all(bool((g != 0).any()) for g in grads) and torch.is_autocast_cache_enabled()
