@@ -237,7 +237,8 @@ def make_networks(dynamics: torch.nn.Module, prediction: torch.nn.Module, device
     for `res_net: []` configurations, `muzero_amd.towers.TowerNetworks` when either network has
     residual blocks or a res_final convolution (`track_running_stats`: its BatchNorm layers' running
     statistics advance with every call as in the reference; the MLP networks have none).
-    `int8`: `res_net: []` networks with their dense layers in 8-bit integers (`muzero_amd.quantized.Int8Networks`)."""
+    `int8`: `res_net: []` networks with their dense layers in 8-bit integers (`muzero_amd.quantized.Int8Networks`); they have
+    neither running statistics nor a root form, so the two arguments before it say nothing to them."""
     if int8:
         from muzero_amd.quantized import Int8Networks
         return Int8Networks(dynamics, prediction, device=device)

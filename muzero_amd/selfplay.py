@@ -23,6 +23,7 @@ from muzero_amd._hip import ptr
 from muzero_amd.engine import BatchedMCTS, _stream, make_networks
 from muzero_amd.environments.connect_four import BatchedConnectFour
 from muzero_amd.neural_networks.per_call import per_call_statistics  # noqa: F401  (re-exported: batched torch evaluation with per-game statistics)
+from muzero_amd.quantized import Int8Networks
 
 
 class DeviceHistory:
@@ -195,7 +196,7 @@ def episodes_from_records(rec, G: int):
 class SelfPlayEngine:
     def __init__(self, repr_net, dyn_net, pred_net, G: int, config, device="cuda", seed: int = 0,
                  device_rng: bool = False, env=None, track_running_stats: bool = False, root_form: bool = True,
-                 share: "SelfPlayEngine | None" = None, graph_moves: bool = False, int8: bool = False):
+                 share: "SelfPlayEngine | None" = None, graph_moves: bool = False, int8: bool | None = None):
         """`config`: TrainingDataGeneratorConfig (mcts settings, epsilon schedule, max steps).
         `env`: a batched environment (`observe`, `step`, `reset(mask)`, `num_actions`,
         `observation_space`); default: G Connect-Four games on the GPU.  Host-side simulators go
@@ -223,11 +224,14 @@ class SelfPlayEngine:
         `move` then returns the graph's own output tensors, valid until the next move (`generate` copies them).
 
         `int8`: g and f (`res_net: []`) run with their dense layers in 8-bit integers, in lock step
-        (muzero_amd.quantized.Int8Networks): for wide layers, at the accuracy of 127 steps per row.
+        (muzero_amd.quantized.Int8Networks): for wide layers, at the accuracy of 127 steps per row.  Default: what
+        `share` runs with, else float32-accurate networks.
 
         `share`: another engine over the same three modules whose device copies of the weights (h runner,
-        packed g / f) this one uses instead of packing its own; the two must issue their device work on the
-        same stream."""
+        packed g / f) this one uses instead of packing its own, in the precision they have; the two must issue their device
+        work on the same stream."""
+        if share is not None and int8 is not None and bool(int8) != isinstance(share.nets, Int8Networks):
+            raise ValueError(f"int8={int8} does not match the networks of the engine this one shares")
         self.G, self.cfg = G, config
         self.device = torch.device(device)
         m = config.mcts
@@ -242,7 +246,7 @@ class SelfPlayEngine:
             self.h = RepresentationRunner(repr_net, device=device, track_running_stats=track_running_stats)
             self._root_final = self.h.root_final() if root_form else None
             self.nets = make_networks(dyn_net, pred_net, device=device, track_running_stats=track_running_stats,
-                                      root_final=self._root_final, int8=int8)
+                                      root_final=self._root_final, int8=bool(int8))
         self.mcts = BatchedMCTS(self.nets, G, m.max_iterations, m.model_look_ahead, m.discount_factor, m.noise_frac,
                                 device=device, keep_latents=False)  # nothing here reads the children's latents
         self.history = DeviceHistory(G, repr_net.history_length, self.env.observation_space, device=device)

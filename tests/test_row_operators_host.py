@@ -443,3 +443,25 @@ def test_autocast_keeps_no_copies_without_a_gradient(monkeypatch):
     assert y.dtype == z.dtype == torch.bfloat16 and torch.equal(y, z)
     grads = torch.autograd.grad(z.sum(), (x, lin.weight, lin.bias))
     assert all(bool((g != 0).any()) for g in grads) and torch.is_autocast_cache_enabled()
+
+
+def test_an_engine_shares_networks_of_the_precision_it_asks_for():
+    import types
+
+    from muzero_amd.quantized import Int8Networks
+    from muzero_amd.selfplay import SelfPlayEngine
+
+    class Reached(Exception):
+        pass
+
+    class Config:
+        @property
+        def mcts(self):
+            raise Reached                              # the check is behind it
+    eight, full = types.SimpleNamespace(nets=object.__new__(Int8Networks)), types.SimpleNamespace(nets=object())
+    for share, int8 in ((eight, False), (full, True)):
+        with pytest.raises(ValueError, match="int8"):
+            SelfPlayEngine(None, None, None, 4, Config(), share=share, int8=int8)
+    for share, int8 in ((eight, True), (full, False), (eight, None), (full, None), (None, True), (None, False)):
+        with pytest.raises(Reached):
+            SelfPlayEngine(None, None, None, 4, Config(), share=share, int8=int8)
