@@ -41,7 +41,7 @@ def check_on_gpu(t: torch.Tensor, what: str) -> None:
 def rows_of(t: torch.Tensor) -> torch.Tensor:
     """t as [rows, columns] with adjacent columns and rows that do not overlap: a view where its strides allow one, else
     a copy."""
-    if t.is_neg():  # a view whose minus sign is not in memory yet
+    if t.is_neg():
         t = t.resolve_neg()
     if t.dim() != 2:
         cols = t.shape[-1]
@@ -52,6 +52,12 @@ def rows_of(t: torch.Tensor) -> torch.Tensor:
     if rows > MAX_ROWS or cols > MAX_COLUMNS:
         raise ValueError(f"{rows} rows of {cols} values are more than a call takes ({MAX_ROWS} of {MAX_COLUMNS})")
     return t
+
+
+def in_memory(t: torch.Tensor) -> torch.Tensor:
+    """t with adjacent values as its memory holds them: the minus sign of a view (the imaginary part of a conjugate, say)
+    is not in memory, and contiguous() leaves it out where the strides fit."""
+    return (t.resolve_neg() if t.is_neg() else t).contiguous()
 
 
 def row_stride(t: torch.Tensor) -> int:

@@ -21,7 +21,7 @@ from torch.autograd.function import once_differentiable
 
 from muzero_amd import _hip
 from muzero_amd._hip import ptr
-from muzero_amd._rows import TYPE, check_tensor, on_device, refuse_tangent, rows_of, stream_of, workspace
+from muzero_amd._rows import TYPE, check_tensor, in_memory, on_device, refuse_tangent, rows_of, stream_of, workspace
 
 MAX_TOP = 32
 _WHOLE = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
@@ -70,9 +70,9 @@ def _gradient(ctx, g_log_prob, g_entropy, _g_actions, g_top):
                 refuse_tangent(g, "the gradient")
     grad = torch.empty((T, V), dtype=logits.dtype, device=logits.device)
     if T > 0:
-        g_log_prob = None if g_log_prob is None else g_log_prob.contiguous()
-        g_entropy = None if g_entropy is None else g_entropy.contiguous()
-        g_top = None if g_top is None else g_top.contiguous()
+        g_log_prob = None if g_log_prob is None else in_memory(g_log_prob)
+        g_entropy = None if g_entropy is None else in_memory(g_entropy)
+        g_top = None if g_top is None else in_memory(g_top)
         args = (logits.data_ptr(), ctx.kind, logits.stride(0) if T > 1 else V, None if actions is None else actions.data_ptr(), T, V,
                 0 if g_top is None else g_top.shape[1], stats.data_ptr(), None if top_actions is None else top_actions.data_ptr(),
                 None if g_log_prob is None else g_log_prob.data_ptr(), None if g_entropy is None else g_entropy.data_ptr(),
@@ -123,8 +123,8 @@ def policy_scores(logits: torch.Tensor, actions: Optional[torch.Tensor] = None, 
             raise ValueError(f"actions of shape {tuple(actions.shape)} do not match logits of shape {tuple(logits.shape)}")
         if actions.device != logits.device:
             raise ValueError(f"actions are on {actions.device}, logits on {logits.device}")
-        if actions.dtype is not torch.int64 or actions.dim() != 1 or not actions.is_contiguous():
-            actions = actions.reshape(-1).to(torch.int64).contiguous()
+        if actions.dtype is not torch.int64 or actions.dim() != 1 or not actions.is_contiguous() or actions.is_neg():
+            actions = in_memory(actions.reshape(-1).to(torch.int64))
     rows = rows_of(logits)
     if torch.is_grad_enabled() and rows.requires_grad:
         log_prob, entropy, top_actions, top_log_probs = _PolicyScores.apply(rows, actions, top)

@@ -17,7 +17,7 @@ import torch
 
 from muzero_amd import _hip
 from muzero_amd._hip import ptr
-from muzero_amd._rows import TYPE, check_on_gpu, check_tensor, on_device, refuse_tangent, row_stride, rows_of, stream_of, workspace
+from muzero_amd._rows import TYPE, check_on_gpu, check_tensor, in_memory, on_device, refuse_tangent, row_stride, rows_of, stream_of, workspace
 
 MAX_K = 131072  # sums of K products of codes stay exact in 32 bits
 ACTIVATIONS = ("none", "linear", "relu", "tanh", "sigmoid")
@@ -146,8 +146,8 @@ def int8_linear(x, weight: QuantizedRows, bias: Optional[torch.Tensor] = None, a
         if bias.shape != (N,) or bias.device != dev:
             raise ValueError(f"bias must be {N} values on {dev}")
         refuse_tangent(bias, "bias")
-        if bias.dtype is not torch.float32 or not bias.is_contiguous():
-            bias = bias.detach().to(torch.float32).contiguous()
+        if bias.dtype is not torch.float32 or not bias.is_contiguous() or bias.is_neg():
+            bias = in_memory(bias.detach().to(torch.float32))
     check_on_gpu(weight.codes, "weight")
     K = weight.columns
     y = torch.empty(x.shape[:-1] + (N,), dtype=out_dtype, device=dev)

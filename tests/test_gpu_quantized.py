@@ -774,3 +774,19 @@ def test_layers_under_autocast(dtype):
     assert all(g.dtype == torch.float32 and bool(g.isfinite().all()) and bool((g != 0).any()) for g in got)
     # the last bias: column sums of the same 16-bit dz, 32 terms in float32, rounded once to the type on each side
     assert float((want[-1] - got[-1]).abs().max()) <= 2 * HALF[dtype] * float(want[-1].abs().max()) + 64 * U * float(w.abs().sum())
+
+
+def test_values_whose_sign_is_not_in_memory():
+    from muzero_amd.policy_scores import policy_scores
+    from muzero_amd.quantized import int8_linear, quantize_rows
+    w, x, bias = quantize_rows(torch.randn(24, 40, device="cuda")), torch.randn(3, 40, device="cuda"), torch.randn(24, device="cuda")
+    assert torch.equal(int8_linear(x, w, torch._neg_view(bias)), int8_linear(x, w, -bias))
+    assert torch.equal(int8_linear(torch._neg_view(x), w), int8_linear(-x, w))
+    z = torch.randn(1, 7, device="cuda", requires_grad=True)
+    a = torch.tensor([-2], device="cuda")
+    assert torch.equal(policy_scores(z, torch._neg_view(a)).log_prob, policy_scores(z, -a).log_prob)
+    s = policy_scores(z, -a)
+    turned = torch.complex(torch.zeros_like(s.log_prob), s.log_prob).conj() * 1j   # its real part is log_prob
+    got, = torch.autograd.grad(turned.real.sum(), z)
+    want, = torch.autograd.grad(policy_scores(z, -a).log_prob.sum(), z)
+    assert torch.equal(got, want)

@@ -465,3 +465,26 @@ def test_an_engine_shares_networks_of_the_precision_it_asks_for():
     for share, int8 in ((eight, True), (full, False), (eight, None), (full, None), (None, True), (None, False)):
         with pytest.raises(Reached):
             SelfPlayEngine(None, None, None, 4, Config(), share=share, int8=int8)
+
+
+def test_gradients_whose_sign_is_not_in_memory(monkeypatch):
+    """A single value is contiguous whatever its stride, so the imaginary part of a conjugate reaches a kernel as a view
+    with its minus sign left out.  What the kernel would read is read here."""
+    import ctypes
+    import types
+
+    import muzero_amd.policy_scores as ps
+    read = []
+
+    class Lib:
+        def mz_policy_scores_backward(self, *args):
+            read.extend(ctypes.cast(p, ctypes.POINTER(ctypes.c_float))[0] for p in args[9:12])
+            return 0
+    monkeypatch.setattr(ps._hip, "lib", Lib)
+    monkeypatch.setattr(ps, "stream_of", lambda t: 0)
+    one = torch._neg_view(torch.tensor([2.5]))
+    assert one.is_neg() and one.is_contiguous() and one.item() == -2.5
+    ctx = types.SimpleNamespace(saved_tensors=(torch.zeros(1, 3), torch.zeros(1, dtype=torch.int64), torch.zeros(1, 3),
+                                               torch.zeros(1, 1, dtype=torch.int64)), kind=F32)
+    ps._gradient(ctx, one, one, None, one[:, None])
+    assert read == [-2.5] * 3
