@@ -177,8 +177,8 @@ class _Taken:
     def __init__(self, module: torch.nn.Module, name: str, fn):
         self.module, self.name, self.fn, self.depth, self.before = module, name, fn, 0, module.__dict__.get(name)
 
-    def __call__(self, x):
-        return self.fn(self.module, x)
+    def __call__(self, *args, **kwargs):
+        return self.fn(self.module, *args, **kwargs)
 
     def __reduce__(self):
         return _bound, (getattr(type(self.module), self.name), self.module)
@@ -209,10 +209,11 @@ class eight_bit_checkpoints:
         self._open: list[list[_Taken]] = []
 
     @staticmethod
-    def _sequence_forward(seq, x):
+    def _sequence_forward(seq, input):  # by the name it has in torch
         from muzero_amd.neural_networks.network_builder import dense_pairs, is_dense_sequence
-        if not _keeps_8_bits(x) or not is_dense_sequence(seq):  # a hook may have come since the context was opened
-            return type(seq).forward(seq, x)
+        if not _keeps_8_bits(input) or not is_dense_sequence(seq):  # a hook may have come since the context was opened
+            return type(seq).forward(seq, input)
+        x = input
         for i, (lin, act) in enumerate(dense_pairs(seq)):
             if act == "softmax":
                 x = seq[2 * i + 1](checkpointed_linear(x, lin.weight, lin.bias))

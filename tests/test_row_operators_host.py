@@ -488,3 +488,12 @@ def test_gradients_whose_sign_is_not_in_memory(monkeypatch):
                                                torch.zeros(1, 1, dtype=torch.int64)), kind=F32)
     ps._gradient(ctx, one, one, None, one[:, None])
     assert read == [-2.5] * 3
+
+
+def test_methods_inside_a_context_take_their_arguments_by_name():
+    from muzero_amd.checkpoints import eight_bit_checkpoints
+    g, f, lat = _small_networks()
+    x, merged = lat.reshape(3, -1), torch.randn(3, g.fc_merge.in_features)
+    want = f.value_mlp(input=x), g.merge(merged=merged)
+    with eight_bit_checkpoints(g, f):
+        assert torch.equal(f.value_mlp(input=x), want[0]) and torch.equal(g.merge(merged=merged), want[1])
