@@ -210,11 +210,12 @@ class eight_bit_checkpoints:
 
     @staticmethod
     def _sequence_forward(seq, input):  # by the name it has in torch
-        from muzero_amd.neural_networks.network_builder import dense_pairs, is_dense_sequence
-        if not _keeps_8_bits(input) or not is_dense_sequence(seq):  # a hook may have come since the context was opened
+        from muzero_amd.neural_networks.network_builder import dense_pairs
+        pairs = dense_pairs(seq, strict=False) if _keeps_8_bits(input) else None
+        if pairs is None:  # a hook may have come since the context was opened
             return type(seq).forward(seq, input)
         x = input
-        for i, (lin, act) in enumerate(dense_pairs(seq)):
+        for i, (lin, act) in enumerate(pairs):
             if act == "softmax":
                 x = seq[2 * i + 1](checkpointed_linear(x, lin.weight, lin.bias))
             else:

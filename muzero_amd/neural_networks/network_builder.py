@@ -140,9 +140,11 @@ def is_dense_sequence(module: nn.Module) -> bool:
         is_plain(m, nn.Linear) if i % 2 == 0 else type(m) in _DENSE_ACTIVATIONS and is_plain(m, type(m)) for i, m in enumerate(mods))
 
 
-def dense_pairs(seq: nn.Sequential) -> list[tuple[nn.Linear, str]]:
-    """(Linear, activation name) pairs of a build_mlp sequence."""
+def dense_pairs(seq: nn.Sequential, strict: bool = True):
+    """(Linear, activation name) pairs of a build_mlp sequence; anything else is refused, or None (`strict=False`)."""
     if not is_dense_sequence(seq):
+        if not strict:
+            return None
         raise ValueError("expected a sequence of Linear layers, each followed by its activation")
     mods = list(seq)
     return [(lin, _DENSE_ACTIVATIONS[type(act)]) for lin, act in zip(mods[::2], mods[1::2])]
