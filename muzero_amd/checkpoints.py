@@ -152,7 +152,7 @@ class _CheckpointedLinear(torch.autograd.Function):
 def checkpointed_linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                         activation: str = "none") -> torch.Tensor:
     """act(x W^T + bias) for x [..., K], with everything the backward pass needs of x and of the result kept in 8 bits or
-    fewer (nothing is kept under torch.no_grad())."""
+    fewer (nothing is kept under torch.no_grad()).  At most 2^20 rows where the weight wants a gradient."""
     check_tensor(x, "x", forward_mode=True)  # torch's own operators serve one under no_grad, the autograd function refuses it
     check_tensor(weight, "weight", forward_mode=True)
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or x.shape[-1] < 1:
@@ -187,7 +187,7 @@ class _Taken:
 def _keeps_8_bits(x: torch.Tensor) -> bool:
     """Whether a layer inside a context keeps x in 8 bits; else it runs as it is.  Hooks that torch calls for every module
     see a layer only if it runs as it is."""
-    return x.is_cuda and x.dtype in TYPE and not torch.nn.modules.module._has_any_global_hook()
+    return x.is_cuda and x.dtype in TYPE and x.shape[:-1].numel() <= MAX_CHECKPOINT_ROWS and not torch.nn.modules.module._has_any_global_hook()
 
 
 _LOCK = threading.Lock()  # of every module's open contexts
@@ -196,9 +196,10 @@ _LOCK = threading.Lock()  # of every module's open contexts
 class eight_bit_checkpoints:
     """Context manager: inside it the dense layers of the given networks -- every build_mlp sequence and the merge layer
     of a DynamicsNetwork -- keep 8-bit checkpoints on the GPU.  Convolutions and BatchNorm layers are left as they are, and
-    so are layers with hooks or a forward of their own and everything on the CPU or in float64.  Parameters, state_dict
-    keys and results of the forward pass do not change.  Contexts may be nested and overlap: a layer is as it was when the
-    last one that names it has ended, except for a forward that somebody has given it meanwhile, which stays."""
+    so are layers with hooks or a forward of their own, calls with more than 2^20 rows, everything on the CPU or in float64,
+    and the part of a sequence that somebody else runs (PredictionNetwork.policy_logits).  Parameters, state_dict keys and
+    results of the forward pass do not change.  Contexts may be nested and overlap: a layer is as it was when the last one
+    that names it has ended, except for a forward that somebody has given it meanwhile, which stays."""
 
     def __init__(self, *modules: torch.nn.Module):
         from muzero_amd.neural_networks.network_builder import is_dense_sequence, is_plain

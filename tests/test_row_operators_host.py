@@ -497,3 +497,15 @@ def test_methods_inside_a_context_take_their_arguments_by_name():
     want = f.value_mlp(input=x), g.merge(merged=merged)
     with eight_bit_checkpoints(g, f):
         assert torch.equal(f.value_mlp(input=x), want[0]) and torch.equal(g.merge(merged=merged), want[1])
+
+
+def test_calls_of_more_rows_than_a_weight_gradient_takes_run_as_they_are(monkeypatch):
+    import muzero_amd.checkpoints as ck
+    seq, kept = torch.nn.Sequential(torch.nn.Linear(1, 1), torch.nn.Tanh()), []
+    monkeypatch.setattr(ck, "checkpointed_linear", lambda x, *rest: (kept.append(len(x)), x)[1])
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    most = torch.zeros(1, 1).expand(ck.MAX_CHECKPOINT_ROWS + 1, 1)
+    with ck.eight_bit_checkpoints(seq), torch.no_grad():
+        assert seq(most).shape == most.shape and kept == []
+        seq(most[1:])
+    assert kept == [ck.MAX_CHECKPOINT_ROWS]
