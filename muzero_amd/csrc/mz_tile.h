@@ -208,8 +208,12 @@ struct Tile {
         };
 #pragma unroll
         for (int b = 0; b < NO; ++b) {
+            // lanes read what other lanes of their wave wrote: LDS keeps a wave's order, the compiler has to as well
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int a = 0; a < NI; ++a) *(V *)(mine + ((lane & 15) * out_ld + 16 * a + 4 * (lane >> 4)) * 4) = pre(b, acc[a][b]);
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
             if constexpr (UNROLL) {
 #pragma unroll
                 for (int q = 0; q < lanes_per_row / 4; ++q) pass(b, q * (64 / lanes_per_row) + lane / lanes_per_row);
