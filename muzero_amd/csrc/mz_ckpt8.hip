@@ -518,8 +518,16 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
                                    (hipStream_t)stream, (const T *)dz, ldz, scales, rows, N, codes, ldc, K, (T *)dw, ldw, aligned, (T *)db,
                                    f.tiles_k, f.part_rows, partial, part_sum);
             };
-            if (type != MZ_TYPE_F32 && scale_bits == 3) pairs ? go(k_weight_grad_few<T, 2, true>) : go(k_weight_grad_few<T, 2, false>);
-            else pairs ? go(k_weight_grad_few<T, 3, true>) : go(k_weight_grad_few<T, 3, false>);
+            const auto planes = [&](auto planes_tag) {
+                constexpr int P = decltype(planes_tag)::value;
+                pairs ? go(k_weight_grad_few<T, P, true>) : go(k_weight_grad_few<T, P, false>);
+            };
+            if constexpr (sizeof(T) == 2) {
+                if (scale_bits == 3) planes(std::integral_constant<int, 2>{});
+                else planes(std::integral_constant<int, 3>{});
+            } else {
+                planes(std::integral_constant<int, 3>{});
+            }
             if (f.parts > 1)
                 hipLaunchKernelGGL(k_weight_join<T>, dim3((unsigned)tiles_of(K, 1024), (unsigned)N), dim3(256), 0, (hipStream_t)stream,
                                    (const float *)partial, f.parts, (const float *)nullptr, K, N, (T *)dw, ldw, aligned,
@@ -567,8 +575,10 @@ int mz_ckpt8_weight_grad(const void *dz, int32_t type, int64_t ldz, int32_t rows
                 else if (l.chunks <= kFewChunks) go(k_prepare<T, P, W, kChunks>);
                 else go(k_prepare<T, P, W, kReady>);
             };
-            if (l.planes == 1) prepare(std::integral_constant<int, 1>{});
-            else prepare(std::integral_constant<int, 2>{});
+            if constexpr (std::is_same_v<T, bf16>) {
+                if (l.planes == 1) return prepare(std::integral_constant<int, 1>{});
+            }
+            prepare(std::integral_constant<int, 2>{});
         });
         const auto launch = [&](auto tile) {
             using Tl = decltype(tile);

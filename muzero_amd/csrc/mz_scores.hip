@@ -662,6 +662,7 @@ dim3 grid_of(int64_t n) { return dim3((unsigned)(n < kMaxGrid ? n : kMaxGrid)); 
 // kPartBytes 8192 / 16384 / 32768: 1 x 131072 10.2 / 10.5 / 11.4.
 constexpr int kSmall = 64, kWave = 4088, kRows = 256, kManyRows = 96, kShort = 48 << 10, kWhole = 96 << 10, kFill = 512,
               kPartBytes = 16 << 10;
+static_assert((kWave + 2 * 7) / 8 <= 8 * 64 && (kWave + 2 * 3) / 4 <= 16 * 64, "8 or 16 packs a lane hold a row of kWave logits");
 
 struct Split {
     int threads, parts;
@@ -699,9 +700,11 @@ void launch_scores(const T *logits, int64_t ld, int64_t rows, Split split, const
         else if (packs <= 192) wave(integral_constant<int, 3>{});
         else if (packs <= 256) wave(integral_constant<int, 4>{});
         else if (packs <= 384) wave(integral_constant<int, 6>{});
-        else if (packs <= 512) wave(integral_constant<int, 8>{});
-        else if (packs <= 768) wave(integral_constant<int, 12>{});
-        else wave(integral_constant<int, 16>{});
+        else if (n == 8 || packs <= 512) wave(integral_constant<int, 8>{});  // all that 16-bit logits need
+        else if constexpr (n == 4) {
+            if (packs <= 768) wave(integral_constant<int, 12>{});
+            else wave(integral_constant<int, 16>{});
+        }
         return;
     }
     const int parts = split.parts;
