@@ -790,3 +790,126 @@ def test_values_whose_sign_is_not_in_memory():
     got, = torch.autograd.grad(turned.real.sum(), z)
     want, = torch.autograd.grad(policy_scores(z, -a).log_prob.sum(), z)
     assert torch.equal(got, want)
+
+
+# beyond the one-launch kernel: column factors from the block itself, from up to 16 chunks of rows, from a kernel of their own
+PLANES = [(90, 3000, 1500), (530, 2100, 2048), (5000, 9000, 30), (4100, 1030, 300)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,K,N", PLANES)
+def test_column_factors_of_any_size(R, K, N, dtype):
+    """Columns of dz from the smallest to the largest a type holds, each with a power of two of its own; zeros, subnormal
+    ones, a wide range inside one; an infinity or a NaN stays in its column, a NaN scale is everybody's."""
+    from muzero_amd.checkpoints import save_activations, weight_grad
+    from muzero_amd.quantized import QuantizedRows
+    x = _x(R, K, dtype, seed=R).nan_to_num(posinf=6e4, neginf=-6e4)
+    g = torch.Generator().manual_seed(N)
+    span = torch.logspace(-6, 3, N) if dtype == torch.float16 else torch.logspace(-33, 30, N)
+    dz = torch.randn(R, N, generator=g).clamp(-4, 4) * span[None, :]
+    dz[:, 5] = 0.0
+    dz[:, 6] = 1e-42 if dtype == torch.float32 else torch.finfo(dtype).tiny / 8
+    dz[:, 7] *= torch.logspace(0, -8, R)
+    dz = dz.to(dtype).cuda()
+    want, tol, want_b, tol_b = _grad_reference(dz, x)
+    saved = save_activations(x)
+    dw, db = weight_grad(dz, saved)
+    _within(dw, want, tol + HALF[dtype] * (np.abs(want) + tol) + TINY[dtype] + 1e-40)
+    _within(db, want_b, tol_b + HALF[dtype] * (np.abs(want_b) + tol_b) + TINY[dtype] + 1e-40)
+    assert (dw[5] == 0).all() and (db[5] == 0).all()
+    dz[3, 8], dz[R - 1, 9] = torch.inf, torch.nan
+    dw2, db2 = weight_grad(dz, saved)
+    assert dw2[8].isnan().all() and dw2[9].isnan().all() and db2[8].isinf() and db2[9].isnan()
+    keep = [n for n in range(N) if n not in (8, 9)]
+    assert torch.equal(dw2[keep], dw[keep]) and torch.equal(db2[keep], db[keep])
+    scales = saved.scales.clone()
+    scales[R // 2] = torch.nan
+    dw3, db3 = weight_grad(dz, QuantizedRows(saved.codes, scales, saved.shape, saved.dtype, 3))
+    assert dw3.isnan().all() and torch.equal(db3[keep], db[keep])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,K,N", PLANES[:1] + PLANES[-1:])
+def test_full_scales_and_strided_gradients_of_large_layers(R, K, N, dtype):
+    from muzero_amd.checkpoints import weight_grad
+    from muzero_amd.quantized import quantize_rows
+    x = _x(R, K, dtype, seed=K).nan_to_num(posinf=6e4, neginf=-6e4)
+    wide = (torch.randn(R, 2 * N + 1, generator=torch.Generator().manual_seed(R)) * 0.01).to(dtype).cuda()
+    saved = quantize_rows(x)
+    for dz in (wide[:, :N], wide[:, 1:N + 1], wide[:, : 2 * N : 2], wide[:, :N].t().contiguous().t()):
+        dw, db = weight_grad(dz, saved)
+        again = weight_grad(dz.contiguous().clone(), saved)
+        assert torch.equal(dw, again[0]) and torch.equal(db, again[1])
+    want, tol, _, _ = _grad_reference(wide[:, :N], x, bits=24)
+    _within(weight_grad(wide[:, :N], saved)[0], want, tol + HALF[dtype] * (np.abs(want) + tol) + TINY[dtype])
+
+
+@pytest.mark.parametrize("R,K,N,act,dtype", [
+    (253, 18432, 6661, "relu", torch.float32), (253, 18432, 6661, "sigmoid", torch.bfloat16),      # 256 x 256 tiles, nine parts
+    (70, 131072, 8190, "none", torch.float16),                                                      # the longest sums, in parts
+    (5201, 130, 5301, "tanh", torch.float32), (7301, 100, 7303, "relu", torch.bfloat16),            # results of 100 MB and more
+    (7301, 100, 7304, "none", torch.float16), (64, 300, 450001, "none", torch.float32)])
+def test_int8_linear_of_large_layers(R, K, N, act, dtype):
+    """Against float64 products of the codes themselves, which are exact."""
+    from muzero_amd.quantized import int8_linear, quantize_rows
+    g = torch.Generator(device="cuda").manual_seed(R)
+    x = torch.randn(R, K, generator=g, device="cuda").to(dtype)
+    w = quantize_rows(torch.randn(N, K, generator=g, device="cuda") / K ** 0.5)
+    b = torch.randn(N, generator=g, device="cuda")
+    y = int8_linear(x, w, b, act)
+    q = quantize_rows(x)
+    for lo in range(0, N, 4096):
+        part = slice(lo, min(N, lo + 4096))
+        lin = q.codes.double() @ w.codes[part].double().t().contiguous() * q.scales.double()[:, None] * w.scales[part].double()
+        pre = lin + b[part].double()
+        want = {"none": lambda v: v, "relu": lambda v: v.clamp(min=0), "tanh": torch.tanh, "sigmoid": torch.sigmoid}[act](pre)
+        tol = 4 * U * (lin.abs() + pre.abs()) + 8 * U * want.abs() + 1e-37
+        tol = tol + HALF[dtype] * (want.abs() + tol) + TINY[dtype]
+        bad = ~((y[:, part].double() - want).abs() <= tol)
+        assert not bad.any(), (lo, int(bad.sum()))
+
+
+def test_replayed_graphs_with_workspaces():
+    """A split product and a large weight gradient: two graphs, whose workspaces are theirs, and eager calls in between."""
+    from muzero_amd.checkpoints import save_activations, weight_grad
+    from muzero_amd.quantized import int8_linear, quantize_rows
+    x, dz = torch.randn(4100, 1030, device="cuda"), torch.randn(4100, 300, device="cuda")
+    long, qw = torch.randn(100, 4096, device="cuda"), quantize_rows(torch.randn(500, 4096, device="cuda"))
+
+    def step():
+        return (int8_linear(long, qw, activation="relu"),) + weight_grad(dz, save_activations(x))
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step())
+    for turn in range(3):
+        x.normal_(), dz.normal_(), long.normal_()
+        want = step()
+        for gr in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for out in outs for a, b in zip(want, out)), turn
+
+
+def test_policy_report_scores_the_recorded_moves():
+    from muzero_amd.learner import DataParallelLearner
+    h, g, f = _networks(9)
+    learner = DataParallelLearner(h, g, f, torch.optim.SGD(f.parameters(), lr=0.1), 5)
+    batch = _batch(64, seed=3)
+    with torch.no_grad():
+        policy = torch.cat([f(h(batch.history[i:i + 1]))[0] for i in range(64)]).double()   # one window at a time
+    report = learner.policy_report(batch, top=2)
+    at = torch.arange(64, device="cuda")
+    # the network in float32, one window at a time or all together, differs by roundings of sums of at most 512 terms
+    torch.testing.assert_close(report.log_prob.double(), policy[at, batch.actions[:, 0]].log(), rtol=0, atol=1e-3)
+    torch.testing.assert_close(report.entropy.double(), -(policy * policy.log()).sum(1), rtol=0, atol=1e-3)
+    torch.testing.assert_close(report.top_log_probs.double().exp(), policy.topk(2, dim=1).values, rtol=0, atol=1e-3)
+    assert torch.equal(report.top_actions[:, 0], policy.argmax(1))
