@@ -757,6 +757,11 @@ int mz_tower_tail_forward(const mz_tower *h_tower, const float *Y, int32_t B, in
 int mz_action_table(const float *embedding, const float *merge_weight, const float *merge_bias,
                     int32_t D, int32_t A, float *table, void *stream);
 
+/* y[rows[r]][:] = x[r][:] for B rows of D floats (row strides ldx, ldy); entries of rows i32[B] outside 0..y_rows-1 are
+ * skipped.  Which of several rows with the same target is kept is not said; x and y must not overlap. */
+int mz_scatter_rows(const float *x, int64_t ldx, const int32_t *rows, int32_t B, int32_t D, float *y, int64_t ldy,
+                    int64_t y_rows, void *stream);
+
 /* Policy post-processing on f32[B][A] rows: `softmax_times` softmax passes (expand_node's
  * softmax of the network's already-normalised policy, src/search/expansion.py:26-27) into
  * policy_out (may alias policy_in, or NULL) and the first maximum of the INPUT row into

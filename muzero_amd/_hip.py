@@ -195,6 +195,7 @@ _SIGS = {
     "mz_tower_forward": (C.c_int, [C.POINTER(Tower), _P, C.c_int64, _P, _P, C.c_int64, _P, _P, C.c_int64, _P,
                                    _P, C.c_int64, C.c_int32, C.c_int32, _P]),
     "mz_action_table": (C.c_int, [_P, _P, _P, C.c_int32, C.c_int32, _P, _P]),
+    "mz_scatter_rows": (C.c_int, [_P, C.c_int64, _P, C.c_int32, C.c_int32, _P, C.c_int64, C.c_int64, _P]),
     "mz_policy_post": (C.c_int, [_P, C.c_int32, C.c_int32, C.c_int32, _P, _P, _P]),
     "mz_policy_scores_workspace": (C.c_int64, [C.c_int32, C.c_int64, C.c_int32, C.c_int32]),
     "mz_policy_scores": (C.c_int, [_P, C.c_int32, C.c_int64, _P, C.c_int64, C.c_int32, C.c_int32, _P, _P, _P, _P, _P, _P, C.c_int64,

@@ -220,6 +220,17 @@ k_act_grad(const T *dy, int64_t ldy, const uint8_t *__restrict__ saved, int64_t 
     });
 }
 
+// Rows to where they belong, one wave each.
+__global__ void __launch_bounds__(kQT)
+k_scatter_rows(const float *__restrict__ x, int64_t ldx, const int32_t *__restrict__ rows, int64_t B, int D, float *__restrict__ y,
+               int64_t ldy, int64_t y_rows) {
+    for (int64_t r = (int64_t)blockIdx.x * (kQT / 64) + (threadIdx.x >> 6); r < B; r += (int64_t)gridDim.x * (kQT / 64)) {
+        const int64_t to = rows[r];
+        if (to < 0 || to >= y_rows) continue;
+        for (int c = threadIdx.x & 63; c < D; c += 64) y[to * ldy + c] = x[r * ldx + c];
+    }
+}
+
 // Workgroups for `rows` rows, `per` of them each, up to this many (a grid holds fewer than 2^32 threads); more rows are
 // taken in turns.
 dim3 row_grid(int64_t rows, int per) {
@@ -292,6 +303,17 @@ int mz_dequant8_rows(const int8_t *codes, int64_t ldc, const float *scales, int6
         });
     });
     return mz::check_launch("k_dequant8");
+}
+
+int mz_scatter_rows(const float *x, int64_t ldx, const int32_t *rows, int32_t B, int32_t D, float *y, int64_t ldy, int64_t y_rows,
+                    void *stream) {
+    MZ_TRY(check_rows("mz_scatter_rows", x, MZ_TYPE_F32, ldx, B, D));
+    MZ_TRY(check_rows("mz_scatter_rows", y, MZ_TYPE_F32, ldy, B, D));
+    if (B == 0) return MZ_OK;
+    if (!rows) return mz::fail(MZ_ERR_ARG, "mz_scatter_rows: NULL argument");
+    hipLaunchKernelGGL(k_scatter_rows, row_grid(B, kQT / 64), dim3(kQT), 0, (hipStream_t)stream, x, ldx, rows, (int64_t)B, D, y, ldy,
+                       y_rows);
+    return mz::check_launch("k_scatter_rows");
 }
 
 int64_t mz_ckpt8_act_bytes(int32_t N, int32_t activation) {

@@ -281,9 +281,15 @@ class Int8Networks:
             out = next_latent.view(-1, self.D)
             if next_rows is None:
                 out[:B] = nxt
-            else:  # rows below 0 are skipped: they put back what row 0, a root's and no child's, holds
-                at = next_rows.clamp(min=0).long()
-                out[at] = torch.where((next_rows >= 0)[:, None], nxt, out[at])
+            else:  # rows below 0 are skipped
+                next_rows = next_rows.reshape(-1).to(torch.int32).contiguous()
+                if next_rows.numel() != B or next_rows.device != nxt.device:
+                    raise ValueError(f"next_rows must be {B} rows on {nxt.device}")
+                if out.dtype != torch.float32 or out.device != nxt.device or (self.D > 1 and out.stride(1) != 1):
+                    raise ValueError(f"next_latent must be float32 with adjacent values in a row, on {nxt.device}")
+                with on_device(nxt):
+                    _hip.check(_hip.lib().mz_scatter_rows(ptr(nxt), self.D, ptr(next_rows), B, self.D, ptr(out), row_stride(out),
+                                                          out.shape[0], stream_of(nxt)), "mz_scatter_rows")
 
     @torch.no_grad()
     def prediction(self, latent, B, *, ld=None, rows=None, softmax_times=0, policy=None, value=None, argmax=None) -> None:

@@ -913,3 +913,33 @@ def test_policy_report_scores_the_recorded_moves():
     torch.testing.assert_close(report.entropy.double(), -(policy * policy.log()).sum(1), rtol=0, atol=1e-3)
     torch.testing.assert_close(report.top_log_probs.double().exp(), policy.topk(2, dim=1).values, rtol=0, atol=1e-3)
     assert torch.equal(report.top_actions[:, 0], policy.argmax(1))
+
+
+def test_skipped_rows_leave_row_0_to_whom_it_belongs():
+    """next_rows of Int8Networks: any row may be written, row 0 too, beside rows that are skipped, or nothing at all."""
+    from muzero_amd.engine import make_networks
+    _, g, f = _networks(11)
+    nets = make_networks(g, f, int8=True)
+    B, D = 4096, 168
+    lat, act = torch.randn(B, D, device="cuda"), torch.randint(0, 7, (B,), device="cuda", dtype=torch.int32)
+    want = torch.empty(B, D, device="cuda")
+    nets.dynamics(lat, B, action=act, next_latent=want)
+    for keep in (torch.arange(B) % 3 == 0, torch.arange(B) == B - 1, torch.arange(B) < 0, torch.arange(B) >= 0):
+        keep = keep.cuda()
+        rows = torch.where(keep, torch.arange(B, device="cuda").flip(0) if bool(keep[-1]) else torch.arange(B, device="cuda"), -5).int()
+        out = torch.full((B, D), 9.0, device="cuda")
+        nets.dynamics(lat, B, action=act, next_latent=out, next_rows=rows)
+        ref = torch.full((B, D), 9.0, device="cuda")
+        ref[rows[keep].long()] = want[keep]
+        assert torch.equal(out, ref)
+    rows[0], rows[1] = B, 2 ** 31 - 1                  # behind the last row: skipped as well
+    nets.dynamics(lat, B, action=act, next_latent=out, next_rows=rows)
+    ref[:2] = out[:2]
+    assert torch.equal(out, ref)
+    wide = torch.full((B, D + 3), 9.0, device="cuda")
+    nets.dynamics(lat, B, action=act, next_latent=wide[:, :D], next_rows=torch.arange(B, device="cuda"))
+    assert torch.equal(wide[:, :D], want) and (wide[:, D:] == 9.0).all()
+    for bad in (dict(next_latent=out, next_rows=rows[1:]), dict(next_latent=out, next_rows=rows.cpu()),
+                dict(next_latent=out.half(), next_rows=rows)):
+        with pytest.raises(ValueError):
+            nets.dynamics(lat, B, action=act, **bad)

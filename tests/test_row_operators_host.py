@@ -509,3 +509,18 @@ def test_calls_of_more_rows_than_a_weight_gradient_takes_run_as_they_are(monkeyp
         assert seq(most).shape == most.shape and kept == []
         seq(most[1:])
     assert kept == [ck.MAX_CHECKPOINT_ROWS]
+
+
+def test_scatter_rows_refusals():
+    f = _hip.lib().mz_scatter_rows
+
+    def call(x=P, ldx=8, rows=P, B=4, D=8, y=P, ldy=8):
+        return f(x, ldx, rows, B, D, y, ldy, 10, None)
+    _refused(call(B=-1), "rows=-1")
+    _refused(call(D=0), "K=0")
+    for name in ("x", "rows", "y"):
+        _refused(call(**{name: None}), "NULL")
+    _refused(call(ldx=7), "stride 7")
+    _refused(call(ldy=7), "stride 7")
+    _refused(call(y=P + 2), "misaligned")
+    assert call(B=0, x=None, rows=None, y=None) == 0
