@@ -830,11 +830,12 @@ int mz_int8_forward_codes(const int8_t *x_codes, int64_t ldxc, const float *x_sc
 
 /* 8-bit activation checkpoints.  A dense layer's input is kept as row codes (mz_quant8_rows with scale_bits 3); what its
  * activation's derivative needs is kept as one bit per value (relu) or a code of 8 bits (tanh, sigmoid):
- * mz_ckpt8_act_bytes(N, activation) bytes per row.  dz may be dy itself (same stride).
+ * mz_ckpt8_act_bytes(N, activation) bytes per row.  The code of tanh t is rne(127 t), of sigmoid s rne(254 s - 127) (both
+ * -128 for a NaN); the derivative is formed from it, 0 for a code of +-127.  dz may be dy itself (same stride).
  * mz_ckpt8_weight_grad: dw[N][K] = dz^T x and db[N] = column sums of dz (db may be NULL) from dz[rows][N] and the codes
  * of x[rows][K]; dz, dw and db share the type, sums are held in float32 with dz to 22 bits or exact.  rows <= 2^20;
  * scale_bits says what the scales hold (3 only if every one has three significant bits).  A column of dz with an infinity
- * or a NaN, or whose products with the scales leave float32's range, gives NaN.  workspace as above (may be 0). */
+ * or a NaN, or whose products with the scales reach 3.39e38 (bfloat16's largest value), gives NaN.  workspace as above (may be 0). */
 int64_t mz_ckpt8_act_bytes(int32_t N, int32_t activation);
 int mz_ckpt8_act_save(const void *y, int32_t type, int64_t ldy, int64_t rows, int32_t N, int32_t activation,
                       uint8_t *saved, void *stream);

@@ -88,7 +88,8 @@ k_int8_join(const int *__restrict__ partial, int splits, const float *__restrict
 // A few rows (at most 16 NB): bound by reading the weights once.  A workgroup takes 16 output channels and all rows, its
 // eight waves every eighth 128 bytes of the reduction; a lane reads 32 consecutive bytes of one channel and of NB rows of x
 // and feeds them to the instructions straight from registers: weights are used once, so LDS would only add a barrier.
-// The waves' sums meet in LDS.  1 x 9216 x 9216: 18 us, 4.7 TB/s (64 x 64 tiles, the reduction in four: 18 + the quantiser;
+// The waves' sums meet in LDS.  1 x 9216 x 9216: 18 us, 4.7 TB/s, where the last level still holds the weights of the
+// call before; 22 us, 3.8 TB/s, for twelve weights in turn (64 x 64 tiles, the reduction in four: 18 + the quantiser;
 // 1 x 4096 x 4096: 4.5 against 8.6).  32 channels per workgroup: 23 us.
 constexpr int kFewWaves = 8;
 
@@ -328,7 +329,9 @@ bool few_rows(int64_t rows, int64_t N, int64_t K) {
     return rows <= 4 || (rows <= 32 && N * K <= 24LL * 1000 * 1000);
 }
 
-// One launch where x has the result's type and its codes fit a workgroup's share of LDS.
+// One launch where x has the result's type and its codes fit a workgroup's share of LDS; asked before few_rows, for long rows
+// of a few channels too (whole calls, us, one launch / rows coded by a call of their own and tiles: 1 x 12288 x 256 12.3 / 20,
+// 1 x 20480 x 256 14.5 / 24, 1 x 32768 x 1024 22.3 / 23.8; at the end of its range, 1 x 40832 x 256, 26.3 / 23.8).
 bool fused(int32_t x_type, int32_t type, int64_t rows, int64_t K) {
     return x_type == type && (rows <= kSharedRows || (rows <= kFusedRows && rows * K <= kOwnValues)) && rows * fused_stride(K) <= kFusedBytes;
 }
@@ -341,7 +344,7 @@ void launch_shape(const Int8Args &a, hipStream_t st) {
         return;
     }
     const Shape s = shape_of_int8(a.rows, a.N, a.K);
-    const bool past = past_caches((int64_t)a.rows * a.N * (int64_t)sizeof(T));  // such outputs have 256 x 256 tiles
+    const bool past = past_caches((int64_t)a.rows * a.N * (int64_t)sizeof(T));  // 256 x 256 tiles, but for up to 64 rows
     if (s.tile == 256 && past) launch_tiles<T, Tile<OpI8, 256, 256, 4, 2>, true>(a, s.splits, st);
     else if (s.tile == 256) launch_tiles<T, Tile<OpI8, 256, 256, 4, 2>>(a, s.splits, st);
     else if (s.tile == 128) launch_tiles<T, Tile<OpI8, 128, 256, 2, 4>>(a, s.splits, st);

@@ -208,7 +208,8 @@ struct Span {
 // No barrier and no second read; bound by the bytes with many rows and by the load's latency with few.  us for 20000 rows
 // (fp16, without / with 5 alternatives), and in brackets for a workgroup per row: 1000 logits 12.7 / 18.9, 2048 21.6 / 32.6
 // (58.9 / 109), 3000 34 / 53 (68 / 119), 4000 68 / 113 (72 / 122); 256 rows of 2048 3.9 / 5.6 (4.3 / 6.8), of 4000 4.7 / 6.9
-// (4.6 / 7.2).  2048 half-precision logits without alternatives are 3.8 TB/s, the rate of reading.
+// (4.6 / 7.2).  2048 half-precision logits without alternatives are 3.8 TB/s, against
+// 5.1 to 5.6 of a kernel that only reads: from 4 packs a lane on, the packs' registers leave 3 waves per SIMD, 1 or 2 for 8.
 template <class T, int P>
 __global__ void __launch_bounds__(256)
 k_scores_wave(const T *__restrict__ logits, int64_t ld, int64_t rows, Out out) {
