@@ -282,6 +282,8 @@ class Int8Networks:
             if next_rows is None:
                 out[:B] = nxt
             else:  # rows below 0 are skipped
+                if next_rows.dtype == torch.int64:  # what 32 bits do not hold names no row
+                    next_rows = next_rows.clamp(-1, (1 << 31) - 1)
                 next_rows = next_rows.reshape(-1).to(torch.int32).contiguous()
                 if next_rows.numel() != B or next_rows.device != nxt.device:
                     raise ValueError(f"next_rows must be {B} rows on {nxt.device}")

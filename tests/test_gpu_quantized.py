@@ -943,3 +943,15 @@ def test_skipped_rows_leave_row_0_to_whom_it_belongs():
                 dict(next_latent=out.half(), next_rows=rows)):
         with pytest.raises(ValueError):
             nets.dynamics(lat, B, action=act, **bad)
+
+
+def test_rows_that_32_bits_do_not_hold_are_none():
+    from muzero_amd.engine import make_networks
+    _, g, f = _networks(12)
+    nets = make_networks(g, f, int8=True)
+    lat, act = torch.randn(6, 168, device="cuda"), torch.arange(6, device="cuda", dtype=torch.int32)
+    want, out = torch.empty(6, 168, device="cuda"), torch.full((6, 168), 9.0, device="cuda")
+    nets.dynamics(lat, 6, action=act, next_latent=want)
+    rows = torch.tensor([3, (1 << 32) + 5, -(1 << 32) + 4, 6, 1, 2 ** 31], device="cuda")
+    nets.dynamics(lat, 6, action=act, next_latent=out, next_rows=rows)
+    assert torch.equal(out[3], want[0]) and torch.equal(out[1], want[4]) and (out[[0, 2, 4, 5]] == 9.0).all()
